@@ -126,6 +126,51 @@ int ps_cuda_matmul_f32(ps_cuda_ctx *ctx, float *dst, const void *src0, int64_t n
 /* GGMLBackend::softmax (ggml_wrapper.cpp:57-69 -> powerserve_compute_forward_soft_max, ggml.c:15060-15089): scale 1, no mask */
 int ps_cuda_softmax(ps_cuda_ctx *ctx, float *dst, const float *x, int64_t ne0, int64_t n_rows);
 
+/* ---------------------------------------------------------------------------------------------- serving operators
+ * What a step over many conversations needs beside the table above; for every context (layer-list ones too), on caches of the caller's or
+ * the context's own (ps_cuda_kv_k / ps_cuda_kv_v, type PS_TYPE_F32).  They have no counterpart in the reference, so no bits to reproduce: sums run in 32 bits
+ * or more, in an order that depends on the shapes alone.  `caches` is a HOST array, read before the call returns; all pointers in it
+ * and all other arguments are device pointers.  A context's calls run one after another; so must graphs that were captured from its
+ * stream, which share its workspace.  A captured call's lengths are those of the capture; a workspace that would have to grow is
+ * refused in a capture (PS_CUDA_ERR_UNSUPPORTED: make the call once before).  Arrays may not overlap unless said so. */
+#define PS_CUDA_TREE_TOKENS 256 /* tokens that a sequence may bring to one ps_cuda_attn_tree call */
+typedef struct {                /* one sequence's cache in one layer */
+    void    *k;                 /* rows [n_ctx][n_kv_heads * head_size] */
+    void    *v;                 /* transposed [n_kv_heads * head_size][n_ctx] */
+    float   *weight;            /* [n_kv_heads][n_ctx]: attention weight that each slot has gathered (attn_tree: NULL = not kept) */
+    float   *weight_to;         /* kv_evict: the weights of the slots that stay; `weight` itself or another array */
+    int32_t *pos;               /* kv_evict: [n_kv_heads][n_ctx] position of the token in each slot (NULL: none are kept for their position) */
+    int32_t *pos_to;            /* kv_evict: `pos` itself or another array */
+    const uint8_t *hidden;      /* attn_tree: [n_ctx], not 0 = no token sees the slot, which may hold anything (NULL = all are seen) */
+    int32_t n_ctx, n_kv;        /* slots that there are; slots that are filled, those of the call's tokens included */
+    int32_t n_tok;              /* attn_tree: tokens that the sequence brings (0: it takes no part); their K / V lie in the last n_tok filled slots */
+    int32_t n_keep;             /* kv_evict: slots that stay, <= n_kv */
+} ps_cuda_cache;
+/* Attention of a step's tokens - one a sequence, a chunk, or a tree of drafted ones - over the sequences' caches:
+ * out[t][h] = sum_j p_j v_j with p = soft-max of scale * q[t][h] . k_j over the slots that the token sees: all that are filled and not hidden, of
+ * the step's own those that tree_mask gives it (per sequence n_tok x n_tok bytes, row t = the tokens that token t sees, one sequence after another;
+ * NULL: itself and the ones before).  A token that sees nothing gets zeros.  weight[g][j] += the sum of p_j over the sequence's tokens and the
+ * heads of kv head g.  q and out: [tokens][n_heads * head_size] fp32, sequence after sequence; out may be q's memory only if it IS q.  What a slot
+ * that some token sees holds must be finite.  head_size: multiples of 32 up to 256; at most 32 heads a kv head. */
+int ps_cuda_attn_tree(ps_cuda_ctx *ctx, float *out, const float *q, const ps_cuda_cache *caches, int n_seqs, int cache_type, int64_t head_size,
+                      int64_t n_heads, int64_t n_kv_heads, const uint8_t *tree_mask, float scale);
+/* Eviction: every kv head of every cache keeps n_keep slots - those whose position is below n_sink or among the n_recent latest, then those of
+ * the largest weight, the lower slot where weights are equal (were there more safe ones than n_keep: the same order among them; a weight that is no number comes last).
+ * The i-th kept slot at n_keep or behind moves into the i-th freed one before n_keep (K, V, weight, position), slots that stay are not
+ * touched, what lies at n_keep and behind is left as it was: the cache then has n_keep filled slots, in no order.  hidden must be NULL. */
+int ps_cuda_kv_evict(ps_cuda_ctx *ctx, const ps_cuda_cache *caches, int n_sets, int cache_type, int64_t head_size, int64_t n_kv_heads, int n_sink, int n_recent);
+typedef struct { /* one row's settings (SamplerChain's order, src/sampler/sampler_chain.cpp:19-51; min-p after top-p) */
+    float   temperature;        /* not above 0: the largest logit (the lowest token that has it), probability 1 */
+    int32_t top_k;              /* 1 .. vocab - 1: only the top_k largest logits, lower tokens first where equal; otherwise all */
+    float   top_p;              /* below 1: of those, largest first, the fewest whose mass is at least top_p of theirs (never none) */
+    float   min_p;              /* above 0: of those, the ones that weigh at least min_p (at most 1) of the largest */
+} ps_cuda_sampler;
+/* ids[r] = the first token, in the vocabulary's order, at which the running sum of the kept tokens' exp(logit / temperature) is over u[r] (in [0, 1)) times
+ * their whole sum; probs[r] (may be NULL) its share of that sum.  A logit that is no number counts as -inf; -1 and probability 0 for a row that has
+ * nothing else.  logits: rows row_stride floats apart; samplers [rows] and u [rows] on the device.  vocab <= 262144. */
+int ps_cuda_sample(ps_cuda_ctx *ctx, int32_t *ids, float *probs, const float *logits, int64_t row_stride, int64_t vocab, int64_t rows,
+                   const ps_cuda_sampler *samplers, const float *u);
+
 /* ---------------------------------------------------------------------------------------------- KV cache
  * Device implementation of the position bookkeeping of KVCacheInterface (src/core/kv_cache.hpp:97-163) that
  * Platform::get/reset_kv_position (src/backend/platform.cpp:34-50) and LlamaModel::forward (:84-86,109) use. */

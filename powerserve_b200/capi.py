@@ -94,6 +94,12 @@ class ArchWeights(C.Structure):
                 ("token_embed", Tensor)]
 
 
+BF16, TREE_TOKENS = 30, 256
+# ps_cuda_cache and ps_cuda_sampler: tables of them are numpy arrays of these records (device addresses in the pointer fields)
+CACHE = np.dtype([("k", "u8"), ("v", "u8"), ("weight", "u8"), ("weight_to", "u8"), ("pos", "u8"), ("pos_to", "u8"), ("hidden", "u8"),
+                  ("n_ctx", "i4"), ("n_kv", "i4"), ("n_tok", "i4"), ("n_keep", "i4")])
+SAMPLER = np.dtype([("temperature", "f4"), ("top_k", "i4"), ("top_p", "f4"), ("min_p", "f4")])
+
 COMPUTE_BF16, COMPUTE_F32 = 0, 1
 MIXER_ATTENTION, MLP_NONE, MLP_ROUTED = 1, 0, 1
 MIXER_LATENT, MLP_DENSE = 2, 2
@@ -152,6 +158,9 @@ def load_library() -> C.CDLL:
         "ps_cuda_copy_4d": (ci, [vp, vp, C.POINTER(i64), C.POINTER(i64), vp, C.POINTER(i64), C.POINTER(i64)]),
         "ps_cuda_matmul_f32": (ci, [vp, fp, vp, i64, i64, i64, i64, i64, vp, i64, i64, i64, i64]),
         "ps_cuda_softmax": (ci, [vp, fp, fp, i64, i64]),
+        "ps_cuda_attn_tree": (ci, [vp, vp, vp, vp, ci, ci, i64, i64, i64, vp, C.c_float]),
+        "ps_cuda_kv_evict": (ci, [vp, vp, ci, ci, i64, i64, ci, ci]),
+        "ps_cuda_sample": (ci, [vp, vp, vp, vp, i64, i64, i64, vp, vp]),
         "ps_cuda_kv_position": (ci, [vp]),
         "ps_cuda_kv_reset": (ci, [vp]),
         "ps_cuda_kv_truncate": (ci, [vp, ci]),
@@ -202,6 +211,13 @@ def load_library() -> C.CDLL:
 
 def exported_symbols() -> List[str]:
     return list(load_library()._ps_signatures.keys())
+
+
+def _dev(a) -> Optional[int]:
+    """device address of a DeviceBuffer, a tensor of another library (data_ptr), or an address"""
+    if a is None or isinstance(a, int):
+        return a
+    return a.ptr if hasattr(a, "ptr") else a.data_ptr()
 
 
 def _i32(a: Sequence[int]) -> np.ndarray:
@@ -444,6 +460,23 @@ class CudaBackend:
 
     def softmax(self, out, x, ne0, n_rows):
         self._ck(self.L.ps_cuda_softmax(self.h, out.ptr, x.ptr, ne0, n_rows))
+
+    # ---- serving operators (arrays: DeviceBuffers, tensors with data_ptr, or addresses; they belong to this context's stream while a call uses them)
+    def attn_tree(self, out, q, caches: np.ndarray, n_heads: int, n_kv_heads: int, head_size: int, scale: float, tree_mask=None, cache_type: int = F32):
+        """attention of a step's tokens over the caches (a CACHE array) of their sequences"""
+        if caches.dtype != CACHE or not caches.flags.c_contiguous:
+            raise PsCudaError("attn_tree: caches is a contiguous array of capi.CACHE records")
+        self._ck(self.L.ps_cuda_attn_tree(self.h, _dev(out), _dev(q), caches.ctypes.data, caches.size, cache_type, head_size, n_heads, n_kv_heads, _dev(tree_mask), scale))
+
+    def kv_evict(self, caches: np.ndarray, n_kv_heads: int, head_size: int, n_sink: int = 0, n_recent: int = 0, cache_type: int = F32):
+        """cuts every cache to its n_keep slots of the largest gathered weight, beside the first and latest positions"""
+        if caches.dtype != CACHE or not caches.flags.c_contiguous:
+            raise PsCudaError("kv_evict: caches is a contiguous array of capi.CACHE records")
+        self._ck(self.L.ps_cuda_kv_evict(self.h, caches.ctypes.data, caches.size, cache_type, head_size, n_kv_heads, n_sink, n_recent))
+
+    def sample(self, ids, probs, logits, vocab: int, rows: int, samplers, u, row_stride: Optional[int] = None):
+        """a token of each row of logits by the row's settings (SAMPLER records on the device) and random number"""
+        self._ck(self.L.ps_cuda_sample(self.h, _dev(ids), _dev(probs), _dev(logits), vocab if row_stride is None else row_stride, vocab, rows, _dev(samplers), _dev(u)))
 
     def read_device(self, dev_ptr: int, n_floats: int, dtype=np.float32) -> np.ndarray:
         out = np.empty(n_floats, dtype=dtype)

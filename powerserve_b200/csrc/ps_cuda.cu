@@ -8,6 +8,7 @@
 #include "ps_mk.cuh"
 #include "ps_step.cuh"
 #include "ps_arch.h"
+#include "ps_serve.h"
 
 #include <dlfcn.h>
 
@@ -214,6 +215,8 @@ struct ps_cuda_ctx {
     // layer-list model (ps_cuda_create_arch): weights, workspace and kernels live in the executor (ps_arch.cu); the context keeps
     // what every model family shares - stream, staging, cache sets / sessions, positions, logits read-back, sampling
     PsArch *arch = nullptr;
+    void *serve_ws = nullptr;   // what the serving operators work in; earlier, smaller ones stay in `owned` (a captured graph may hold them)
+    size_t serve_ws_bytes = 0;
     std::vector<size_t> kv_k_bytes, kv_v_bytes; // per layer: bytes of the K rows / V^T rows of ONE cache set
 };
 
@@ -1588,7 +1591,41 @@ namespace {
 } // namespace
 
 
-// ====================================================================================================================
+// ---------------------------------------------------------------------------------------------- serving operators (ps_serve.cu)
+namespace {
+int serve_workspace(void *user, size_t bytes, void **p) {
+    ps_cuda_ctx *ctx = static_cast<ps_cuda_ctx *>(user);
+    if (bytes > ctx->serve_ws_bytes) {
+        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+        PS_CK(cudaStreamIsCapturing(ctx->stream, &st));
+        if (st != cudaStreamCaptureStatusNone) return fail(ctx, PS_CUDA_ERR_UNSUPPORTED, "the call needs more workspace than a capture can ask for: make it once before");
+        const size_t want = std::max(bytes, ctx->serve_ws_bytes + ctx->serve_ws_bytes / 2);
+        void *mem = nullptr;
+        if (int rc = dev_alloc_yield(ctx, &mem, want)) return rc;
+        ctx->serve_ws = mem;
+        ctx->serve_ws_bytes = want;
+    }
+    *p = ctx->serve_ws;
+    return 0;
+}
+// one call of a serving operator: the context's lock, its device (the caller's comes back), its error text
+template <typename F> int serve(ps_cuda_ctx *ctx, F call) {
+    if (!ctx) return fail(nullptr, PS_CUDA_ERR_INVALID, "null context");
+    std::lock_guard<std::mutex> lock(ctx->mu);
+    PsServeCall c{};
+    c.stream = ctx->stream; c.n_sm = ctx->n_sm; c.err_dev = ctx->err_dev; c.workspace = serve_workspace; c.user = ctx;
+    int rc = 0;
+    const cudaError_t e = on_device(ctx->device, [&] { // (it may run in another thread: no exception leaves it)
+        try { rc = call(&c); } catch (...) { rc = fail(ctx, PS_CUDA_ERR_OOM, "out of host memory"); }
+        return cudaSuccess;
+    });
+    if (e != cudaSuccess) return fail(ctx, PS_CUDA_ERR_CUDA, "device %d: %s", ctx->device, cudaGetErrorString(e));
+    ctx->n_launch += c.launches;
+    return rc && c.msg[0] ? fail(ctx, rc, "%s", c.msg) : rc;
+}
+bool fits_int(int64_t v) { return v >= INT32_MIN && v <= INT32_MAX; }
+} // namespace
+
 extern "C" {
 
 int ps_cuda_abi_version(void) { return PS_CUDA_ABI_VERSION; }
@@ -2178,6 +2215,26 @@ int ps_cuda_softmax(ps_cuda_ctx *ctx, float *dst, const float *x, int64_t ne0, i
     ps_k_softmax_ext<<<(unsigned)n_rows, 256, (size_t)ne0 * 4, ctx->stream>>>(dst, x, nullptr, nullptr, ne0, 1, 1.0f);
     PS_LAUNCH_CK();
     return 0;
+}
+
+// ---------------------------------------------------------------------------------------------- serving operators (ps_serve.cu)
+
+int ps_cuda_attn_tree(ps_cuda_ctx *ctx, float *out, const float *q, const ps_cuda_cache *caches, int n_seqs, int cache_type, int64_t head_size, int64_t n_heads,
+                      int64_t n_kv_heads, const uint8_t *tree_mask, float scale) {
+    return serve(ctx, [&](PsServeCall *c) {
+        if (!fits_int(head_size) || !fits_int(n_heads) || !fits_int(n_kv_heads)) return fail(ctx, PS_CUDA_ERR_INVALID, "attn_tree: head geometry");
+        return ps_serve_attn_tree(c, out, q, caches, n_seqs, cache_type, (int)head_size, (int)n_heads, (int)n_kv_heads, tree_mask, scale);
+    });
+}
+int ps_cuda_kv_evict(ps_cuda_ctx *ctx, const ps_cuda_cache *caches, int n_sets, int cache_type, int64_t head_size, int64_t n_kv_heads, int n_sink, int n_recent) {
+    return serve(ctx, [&](PsServeCall *c) {
+        if (!fits_int(head_size) || !fits_int(n_kv_heads)) return fail(ctx, PS_CUDA_ERR_INVALID, "kv_evict: head geometry");
+        return ps_serve_kv_evict(c, caches, n_sets, cache_type, (int)head_size, (int)n_kv_heads, n_sink, n_recent);
+    });
+}
+int ps_cuda_sample(ps_cuda_ctx *ctx, int32_t *ids, float *probs, const float *logits, int64_t row_stride, int64_t vocab, int64_t rows, const ps_cuda_sampler *samplers,
+                   const float *u) {
+    return serve(ctx, [&](PsServeCall *c) { return ps_serve_sample(c, ids, probs, logits, row_stride, vocab, rows, samplers, u); });
 }
 
 // ---------------------------------------------------------------------------------------------- KV cache

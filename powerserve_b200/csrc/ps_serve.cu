@@ -1,0 +1,226 @@
+// ps_serve.cu - host side of the serving operators (ps_serve.h): what they accept, how they are cut into launches, and what they work in.
+#include "ps_serve.h"
+
+#include "ps_serve_attn.cuh"
+#include "ps_serve_evict.cuh"
+#include "ps_serve_sample.cuh"
+
+#include <algorithm>
+#include <cstdarg>
+#include <cstdio>
+
+namespace {
+
+int fail(PsServeCall *c, int code, const char *fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(c->msg, sizeof c->msg, fmt, ap);
+    va_end(ap);
+    return code;
+}
+
+#define SV_CK(call)                                                                                                    \
+    do {                                                                                                               \
+        const cudaError_t e_ = (call);                                                                                 \
+        if (e_ != cudaSuccess) return fail(c, PS_CUDA_ERR_CUDA, "%s failed: %s", #call, cudaGetErrorString(e_));       \
+    } while (0)
+#define SV_LAUNCHED(what)                                                                                              \
+    do {                                                                                                               \
+        const cudaError_t e_ = cudaGetLastError();                                                                     \
+        if (e_ != cudaSuccess) return fail(c, PS_CUDA_ERR_CUDA, what ": launch failed: %s", cudaGetErrorString(e_));   \
+        c->launches++;                                                                                                 \
+    } while (0)
+
+bool aligned(const void *p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+size_t up(size_t v) { return (v + 255) & ~(size_t)255; }
+
+int check_caches(PsServeCall *c, const char *what, const ps_cuda_cache *caches, int n, int cache_type, int head_size, int n_kv_heads) {
+    if (n < 0 || (n > 0 && !caches)) return fail(c, PS_CUDA_ERR_INVALID, "%s: no caches", what);
+    if (cache_type != PS_TYPE_F32 && cache_type != PS_TYPE_BF16) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "%s: cache type %d (float32 and bfloat16 are there)", what, cache_type);
+    if (head_size <= 0 || head_size % 32 || head_size > 256) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "%s: head size %d (multiples of 32 up to 256)", what, head_size);
+    if (n_kv_heads <= 0 || n_kv_heads > 1024) return fail(c, PS_CUDA_ERR_INVALID, "%s: %d kv heads", what, n_kv_heads);
+    const size_t es = cache_type == PS_TYPE_F32 ? 4 : 2;
+    for (int i = 0; i < n; i++) {
+        const ps_cuda_cache &s = caches[i];
+        if (s.n_ctx <= 0 || s.n_kv < 0 || s.n_kv > s.n_ctx) return fail(c, PS_CUDA_ERR_INVALID, "%s: cache %d holds %d of %d slots", what, i, s.n_kv, s.n_ctx);
+        if (s.n_kv && (!s.k || !s.v)) return fail(c, PS_CUDA_ERR_INVALID, "%s: cache %d has no rows", what, i);
+        if (!aligned(s.k, es) || !aligned(s.v, es) || !aligned(s.weight, 4) || !aligned(s.weight_to, 4) || !aligned(s.pos, 4) || !aligned(s.pos_to, 4))
+            return fail(c, PS_CUDA_ERR_INVALID, "%s: cache %d: an array that is not aligned to its elements", what, i);
+    }
+    return 0;
+}
+
+// Splits of the launch: as many CTAs as the GPU takes at once, none of fewer than `least` tiles
+int split_tiles(const ps_cuda_cache *caches, int n, int per_split, int target, int least) {
+    int64_t tiles = 0;
+    for (int i = 0; i < n; i++) tiles += caches[i].n_tok > 0 ? (caches[i].n_kv + SV_TILE - 1) / SV_TILE : 0;
+    int tps = (int)std::max<int64_t>(least, tiles * per_split / std::max(target, 1));
+    for (;; tps++) { // (the last splits are short: a few more tiles for each until all fit)
+        int64_t ctas = 0;
+        for (int i = 0; i < n; i++)
+            if (caches[i].n_tok > 0) ctas += ((caches[i].n_kv + SV_TILE - 1) / SV_TILE + tps - 1) / tps;
+        if (ctas * per_split <= target || ctas <= n) return tps;
+    }
+}
+
+} // namespace
+
+int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda_cache *caches, int n_seqs, int cache_type, int head_size, int n_heads, int n_kv_heads,
+                       const uint8_t *tree_mask, float scale) {
+    if (int rc = check_caches(c, "attn_tree", caches, n_seqs, cache_type, head_size, n_kv_heads)) return rc;
+    if (n_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > 32) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "attn_tree: %d heads over %d kv heads", n_heads, n_kv_heads);
+    const int R = n_heads / n_kv_heads, hs = head_size;
+    int64_t tokens = 0;
+    for (int i = 0; i < n_seqs; i++) {
+        const ps_cuda_cache &s = caches[i];
+        if (s.n_tok < 0 || s.n_tok > s.n_kv) return fail(c, PS_CUDA_ERR_INVALID, "attn_tree: sequence %d brings %d tokens, its cache holds %d", i, s.n_tok, s.n_kv);
+        if (s.n_tok > PS_CUDA_TREE_TOKENS) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "attn_tree: sequence %d brings %d tokens (at most %d)", i, s.n_tok, PS_CUDA_TREE_TOKENS);
+        tokens += s.n_tok;
+    }
+    if (tokens == 0) return 0;
+    if (tokens > INT32_MAX / 1024) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "attn_tree: %lld tokens in one call", (long long)tokens);
+    if (!out || !q) return fail(c, PS_CUDA_ERR_INVALID, "attn_tree: null argument");
+    if (!aligned(out, 4) || !aligned(q, 4)) return fail(c, PS_CUDA_ERR_INVALID, "attn_tree: an array that is not aligned to its elements");
+
+    int tok0 = 0;
+    for (int first = 0; first < n_seqs;) {
+        // sequences of a launch: as many as the table takes, and as their scores leave the workspace at a size
+        int n = 0;
+        size_t scores = 0;
+        int most_tok = 0, most_kv = 0;
+        bool weights = false;
+        while (first + n < n_seqs && n < SV_SEQS) {
+            const ps_cuda_cache &s = caches[first + n];
+            const size_t more = s.weight && s.n_tok ? up(4 * (size_t)n_kv_heads * s.n_kv * ((s.n_tok * R + 3) & ~3)) : 0;
+            if (n && scores + more > ((size_t)1 << 30)) break;
+            scores += more;
+            weights |= more != 0;
+            most_tok = std::max(most_tok, s.n_tok);
+            most_kv = std::max(most_kv, s.n_kv);
+            n++;
+        }
+        SvAttn a{};
+        a.q = q; a.out = out; a.hs = hs; a.n_heads = n_heads; a.G = n_kv_heads; a.R = R; a.scale = scale * SV_LOG2E; a.err = c->err_dev; a.n_seqs = n;
+        const int row_tiles = (most_tok * R + 15) / 16;
+        if (most_tok) {
+            a.tps = split_tiles(caches + first, n, n_kv_heads * row_tiles, c->n_sm * 4, 1);
+            size_t bytes = scores;
+            int units = 0;
+            bool joined = false;
+            for (int i = 0; i < n; i++) {
+                const ps_cuda_cache &s = caches[first + i];
+                SvSeq &d = a.seq[i];
+                d.k = s.k; d.v = s.v; d.weight = s.n_tok ? s.weight : nullptr; d.hidden = s.hidden; d.n_ctx = s.n_ctx; d.n_kv = s.n_kv; d.n_tok = s.n_tok; d.tok0 = tok0;
+                d.mask = tree_mask;
+                if (tree_mask) tree_mask += (size_t)s.n_tok * s.n_tok;
+                tok0 += s.n_tok;
+                const int tiles = s.n_tok ? (s.n_kv + SV_TILE - 1) / SV_TILE : 0;
+                d.splits = (tiles + a.tps - 1) / a.tps;
+                d.unit0 = units;
+                units += d.splits;
+                joined |= d.splits > 1;
+                bytes += up(4 * (size_t)d.splits * n_kv_heads * s.n_tok * R * (hs + 2));
+            }
+            void *mem = nullptr;
+            if (int rc = c->workspace(c->user, bytes, &mem)) return rc;
+            char *at = static_cast<char *>(mem);
+            for (int i = 0; i < n; i++) {
+                SvSeq &d = a.seq[i];
+                if (d.weight) {
+                    d.scores = reinterpret_cast<float *>(at);
+                    at += up(4 * (size_t)n_kv_heads * d.n_kv * ((d.n_tok * R + 3) & ~3));
+                }
+                d.part = reinterpret_cast<float *>(at);
+                at += up(4 * (size_t)d.splits * n_kv_heads * d.n_tok * R * (hs + 2));
+            }
+            const size_t smem = sv_attn_smem(hs);
+            const dim3 grid(units, n_kv_heads, row_tiles);
+            if (cache_type == PS_TYPE_F32) {
+                SV_CK(cudaFuncSetAttribute(sv_k_attn<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+                sv_k_attn<float><<<grid, 128, smem, c->stream>>>(a);
+            } else {
+                SV_CK(cudaFuncSetAttribute(sv_k_attn<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+                sv_k_attn<__nv_bfloat16><<<grid, 128, smem, c->stream>>>(a);
+            }
+            SV_LAUNCHED("attn_tree");
+            if (joined || weights) {
+                const int row_blocks = joined ? (most_tok * R + 7) / 8 : 0, slot_blocks = weights ? (most_kv + SV_FIN_SLOTS - 1) / SV_FIN_SLOTS : 0;
+                sv_k_finish<<<dim3(row_blocks + slot_blocks, n_kv_heads, n), 256, 4 * (size_t)most_tok * R, c->stream>>>(a, row_blocks);
+                SV_LAUNCHED("attn_tree");
+            }
+        }
+        first += n;
+    }
+    return 0;
+}
+
+int ps_serve_kv_evict(PsServeCall *c, const ps_cuda_cache *caches, int n_sets, int cache_type, int head_size, int n_kv_heads, int n_sink, int n_recent) {
+    if (int rc = check_caches(c, "kv_evict", caches, n_sets, cache_type, head_size, n_kv_heads)) return rc;
+    if (n_sink < 0 || n_recent < 0) return fail(c, PS_CUDA_ERR_INVALID, "kv_evict: %d first and %d latest positions", n_sink, n_recent);
+    for (int i = 0; i < n_sets; i++) {
+        const ps_cuda_cache &s = caches[i];
+        if (s.n_keep < 0 || s.n_keep > s.n_kv) return fail(c, PS_CUDA_ERR_INVALID, "kv_evict: cache %d keeps %d of %d slots", i, s.n_keep, s.n_kv);
+        if (s.n_kv && (!s.weight || !s.weight_to)) return fail(c, PS_CUDA_ERR_INVALID, "kv_evict: cache %d has no gathered weights", i);
+        if ((s.pos != nullptr) != (s.pos_to != nullptr)) return fail(c, PS_CUDA_ERR_INVALID, "kv_evict: cache %d: pos and pos_to go together", i);
+        if (!s.pos && (n_sink || n_recent)) return fail(c, PS_CUDA_ERR_INVALID, "kv_evict: cache %d has no positions to keep the first or latest of", i);
+        if (s.hidden) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "kv_evict: cache %d has hidden slots (every kv head moves its own)", i);
+    }
+    for (int first = 0; first < n_sets; first += SV_SETS) {
+        const int n = std::min(n_sets - first, SV_SETS);
+        SvEvict a{};
+        a.G = n_kv_heads; a.hs = head_size; a.n_sink = n_sink; a.n_recent = n_recent;
+        size_t bytes = 0;
+        int most = 0;
+        for (int i = 0; i < n; i++) {
+            const ps_cuda_cache &s = caches[first + i];
+            SvSet &d = a.set[i];
+            d.k = s.k; d.v = s.v; d.weight = s.weight; d.weight_to = s.weight_to; d.pos = s.pos; d.pos_to = s.pos_to; d.n_ctx = s.n_ctx; d.n_kv = s.n_kv; d.n_keep = s.n_keep;
+            d.moves = std::min(s.n_keep, s.n_kv - s.n_keep);
+            most = std::max(most, d.moves);
+            bytes += up(4 * (size_t)n_kv_heads * (1 + 2 * (size_t)d.moves));
+        }
+        void *mem = nullptr;
+        if (int rc = c->workspace(c->user, bytes, &mem)) return rc;
+        char *at = static_cast<char *>(mem);
+        for (int i = 0; i < n; i++) {
+            a.set[i].list = reinterpret_cast<int32_t *>(at);
+            at += up(4 * (size_t)n_kv_heads * (1 + 2 * (size_t)a.set[i].moves));
+        }
+        sv_k_select<<<dim3(n_kv_heads, n), SV_SEL_THREADS, 0, c->stream>>>(a);
+        SV_LAUNCHED("kv_evict");
+        if (most) {
+            const dim3 grid((most + 31) / 32, n_kv_heads, n);
+            if (cache_type == PS_TYPE_F32) sv_k_move<uint32_t><<<grid, 256, 0, c->stream>>>(a);
+            else sv_k_move<uint16_t><<<grid, 256, 0, c->stream>>>(a);
+            SV_LAUNCHED("kv_evict");
+        }
+    }
+    return 0;
+}
+
+int ps_serve_sample(PsServeCall *c, int32_t *ids, float *probs, const float *logits, int64_t row_stride, int64_t vocab, int64_t rows, const ps_cuda_sampler *samplers, const float *u) {
+    if (rows < 0 || vocab <= 0 || vocab > 1 << 18 || row_stride < vocab)
+        return fail(c, PS_CUDA_ERR_INVALID, "sample: %lld rows of %lld tokens (1 to 262144), %lld apart", (long long)rows, (long long)vocab, (long long)row_stride);
+    if (rows == 0) return 0;
+    if (!ids || !logits || !samplers || !u) return fail(c, PS_CUDA_ERR_INVALID, "sample: null argument");
+    if (!aligned(ids, 4) || !aligned(probs, 4) || !aligned(logits, 4) || !aligned(samplers, 4) || !aligned(u, 4)) return fail(c, PS_CUDA_ERR_INVALID, "sample: an array that is not aligned to its elements");
+    SvSample a{};
+    a.logits = logits; a.samplers = samplers; a.u = u; a.ids = ids; a.probs = probs; a.row_stride = row_stride; a.vocab = (int)vocab;
+    const int C = SV_SMP_CLUSTER;
+    a.chunk = (int)((vocab + C - 1) / C + 31) & ~31;
+    const size_t smem = 4 * (size_t)a.chunk;
+    for (int64_t r0 = 0; r0 < rows; r0 += 1 << 20) {
+        const int n = (int)std::min<int64_t>(rows - r0, 1 << 20);
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = C; at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.gridDim = dim3(n * C); cfg.blockDim = dim3(SV_SMP_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = c->stream; cfg.attrs = at; cfg.numAttrs = 1;
+        SV_CK(cudaFuncSetAttribute(sv_k_sample<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        SV_CK(cudaLaunchKernelEx(&cfg, sv_k_sample<true>, a));
+        SV_LAUNCHED("sample");
+        a.logits += (int64_t)n * row_stride; a.samplers += n; a.u += n; a.ids += n;
+        if (a.probs) a.probs += n;
+    }
+    return 0;
+}

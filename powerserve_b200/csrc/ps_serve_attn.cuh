@@ -1,0 +1,208 @@
+// ps_serve_attn.cuh - attention of a step's tokens over the caches of several sequences.
+//
+//   z[t][h][j] = scale q[t][h] . k[j][g(h)],   p = soft-max over the slots j that token t sees,   out[t][h] = sum_j p[t][h][j] v[g(h)][j]
+//   weight[g][j] += sum over tokens t and heads h of g of p[t][h][j]
+//
+// A sequence's query rows of one kv head (n_tok tokens x the heads that share it) go together, so that its K rows and V^T columns are read once.
+// The slots are cut into splits; a split leaves its rows' running maximum, sum and unnormalised output in the workspace, and sv_k_finish joins
+// them.  Where weights are gathered, the scores (32 bits) go to the workspace too, [slot][row], and sv_k_finish sums exp(z - log-sum) over the rows.
+#pragma once
+#include "ps_ptx.cuh"
+
+#include <cuda_bf16.h>
+
+#define SV_SEQS 64      // sequences of a launch: their table is a kernel parameter
+#define SV_TILE 64      // slots of a tile
+#define SV_LOG2E 1.4426950408889634f
+#define SV_NONE (-INFINITY)
+
+struct SvSeq {
+    const void *k, *v;
+    float *weight;
+    const uint8_t *hidden, *mask;
+    float *scores;          // [kv head][n_kv][rp], or null
+    float *part;            // [split][kv head][row][hs]; then [split][kv head][row] pairs of maximum and sum
+    int n_ctx, n_kv, n_tok, tok0;
+    int splits, unit0;      // unit0: number of the sequence's first split among all of the launch
+};
+struct SvAttn {
+    SvSeq seq[SV_SEQS];
+    const float *q;
+    float *out;
+    int n_seqs, hs, n_heads, G, R, tps; // R: heads that share a kv head; tps: tiles of a split
+    float scale;                        // times log2 e
+    int *err;
+};
+
+PS_D float sv_ld(const float *p, int64_t i) { return p[i]; }
+PS_D float sv_ld(const __nv_bfloat16 *p, int64_t i) { return __bfloat162float(p[i]); }
+PS_D int sv_rp(int rows) { return (rows + 3) & ~3; }
+PS_D int sv_find(const SvAttn &a, int unit) {
+    int s = 0;
+    while (s + 1 < a.n_seqs && unit >= a.seq[s + 1].unit0) s++;
+    return s;
+}
+// slot j, token t: back = j - (n_kv - n_tok) is the slot's number among the step's own tokens (negative: the past)
+PS_D bool sv_sees(const SvSeq &s, int t, int back) { return back < 0 || (s.mask ? s.mask[t * s.n_tok + back] != 0 : back <= t); }
+
+// ---------------------------------------------------------------------------------------------------- any head size
+// Sixteen query rows, 32 slots at a time, everything in 32-bit arithmetic on the CUDA cores.  Thread (slot, row group) takes four scores; a warp
+// takes the soft-max of four rows; then a thread owns channels d, d + 128 of all sixteen rows.
+template <typename T>
+__global__ void __launch_bounds__(128) sv_k_attn(const __grid_constant__ SvAttn a) {
+    extern __shared__ float sv_sm[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hs = a.hs;
+    const int si = sv_find(a, blockIdx.x), split = blockIdx.x - a.seq[si].unit0, g = blockIdx.y;
+    const SvSeq &s = a.seq[si];
+    const int rows = s.n_tok * a.R, r0 = blockIdx.z * 16;
+    if (r0 >= rows) return;
+    const int kp = hs + 1;
+    float *sq = sv_sm, *sk = sq + 16 * hs, *sv = sk + 32 * kp, *sp = sv + hs * 33, *sc = sp + 16 * 33;
+    const T *kc = static_cast<const T *>(s.k) + (int64_t)g * hs, *vc = static_cast<const T *>(s.v) + (int64_t)g * hs * s.n_ctx;
+    const int64_t kvd = (int64_t)a.G * hs;
+    for (int i = tid; i < 16 * hs; i += 128) {
+        const int r = r0 + i / hs, t = r / a.R, h = g * a.R + r % a.R;
+        sq[i] = r < rows ? a.q[((int64_t)(s.tok0 + t) * a.n_heads + h) * hs + i % hs] * a.scale : 0.f;
+    }
+    float acc[2][16], m[4], l[4];
+#pragma unroll
+    for (int r = 0; r < 16; r++) acc[0][r] = acc[1][r] = 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; r++) { m[r] = SV_NONE; l[r] = 0.f; }
+    const int j_end = min(s.n_kv, (split + 1) * a.tps * SV_TILE), past = s.n_kv - s.n_tok, rp = sv_rp(rows);
+    for (int j0 = split * a.tps * SV_TILE; j0 < j_end; j0 += 32) {
+        __syncthreads();
+        // what a slot that is hidden, or behind the last one, holds may be anything: it is not read into the products
+        for (int i = tid; i < 32 * hs; i += 128) {
+            const int j = j0 + i / hs, d = i % hs;
+            sk[(i / hs) * kp + d] = j < j_end && !(s.hidden && s.hidden[j]) ? sv_ld(kc, j * kvd + d) : 0.f;
+        }
+        for (int i = tid; i < 32 * hs; i += 128) {
+            const int j = j0 + (i & 31), d = i >> 5;
+            sv[d * 33 + (i & 31)] = j < j_end && !(s.hidden && s.hidden[j]) ? sv_ld(vc, (int64_t)d * s.n_ctx + j) : 0.f;
+        }
+        __syncthreads();
+        const int j = j0 + lane;
+        const bool in = j < j_end && !(s.hidden && s.hidden[j]);
+        float z[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int d = 0; d < hs; d++) {
+            const float kv = sk[lane * kp + d];
+#pragma unroll
+            for (int r = 0; r < 4; r++) z[r] = fmaf(sq[(warp * 4 + r) * hs + d], kv, z[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int row = r0 + warp * 4 + r;
+            if (!in || row >= rows || !sv_sees(s, row / a.R, j - past)) z[r] = SV_NONE;
+            if (s.scores && row < rows && j < j_end) s.scores[((int64_t)g * s.n_kv + j) * rp + row] = z[r];
+            float mx = z[r];
+#pragma unroll
+            for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            const float mn = fmaxf(m[r], mx), ref = mn == SV_NONE ? 0.f : mn, f = exp2f(m[r] - ref), p = exp2f(z[r] - ref);
+            float sum = p;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            l[r] = l[r] * f + sum;
+            m[r] = mn;
+            sp[(warp * 4 + r) * 33 + lane] = p;
+            if (lane == 0) sc[warp * 4 + r] = f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const int d = tid + 128 * c;
+            if (d >= hs) break;
+#pragma unroll
+            for (int r = 0; r < 16; r++) acc[c][r] *= sc[r];
+            for (int jj = 0; jj < 32; jj++) {
+                const float v = sv[d * 33 + jj];
+#pragma unroll
+                for (int r = 0; r < 16; r++) acc[c][r] = fmaf(sp[r * 33 + jj], v, acc[c][r]);
+            }
+        }
+    }
+    __syncthreads();
+    float *ml = s.part + (int64_t)s.splits * a.G * rows * hs;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int row = r0 + warp * 4 + r;
+        if (lane == 0 && row < rows) {
+            reinterpret_cast<float2 *>(ml)[((int64_t)split * a.G + g) * rows + row] = make_float2(m[r], l[r]);
+            sc[warp * 4 + r] = s.splits == 1 ? (l[r] > 0.f ? 1.f / l[r] : 0.f) : 1.f;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+        const int d = tid + 128 * c;
+        if (d >= hs) break;
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            const int row = r0 + r;
+            if (row >= rows) break;
+            if (s.splits == 1) a.out[((int64_t)(s.tok0 + row / a.R) * a.n_heads + g * a.R + row % a.R) * hs + d] = acc[c][r] * sc[r];
+            else s.part[(((int64_t)split * a.G + g) * rows + row) * hs + d] = acc[c][r];
+        }
+    }
+}
+inline size_t sv_attn_smem(int hs) { return 4 * ((size_t)16 * hs + 32 * (hs + 1) + (size_t)hs * 33 + 16 * 33 + 16); }
+
+// ---------------------------------------------------------------------------------------------------- joining the splits
+// y < G: a warp takes an output row of kv head y (skipped for a sequence with one split).  y >= G, x: 256 slots of a sequence's kv head y - G: their weights.
+#define SV_FIN_SLOTS 256
+__global__ void __launch_bounds__(256) sv_k_finish(const __grid_constant__ SvAttn a, int row_blocks) {
+    extern __shared__ float sv_lse[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hs = a.hs, g = blockIdx.y;
+    const SvSeq &s = a.seq[blockIdx.z];
+    const int rows = s.n_tok * a.R;
+    const float2 *ml = reinterpret_cast<const float2 *>(s.part + (int64_t)s.splits * a.G * rows * hs);
+    if ((int)blockIdx.x < row_blocks) {
+        const int row = blockIdx.x * 8 + warp;
+        if (row >= rows || s.splits == 1) return;
+        float mx = SV_NONE;
+        for (int i = lane; i < s.splits; i += 32) mx = fmaxf(mx, ml[((int64_t)i * a.G + g) * rows + row].x);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float ref = mx == SV_NONE ? 0.f : mx;
+        float l = 0.f, acc[8] = {};
+        for (int i = 0; i < s.splits; i++) {
+            const int64_t at = ((int64_t)i * a.G + g) * rows + row;
+            const float2 p = ml[at];
+            const float f = exp2f(p.x - ref);
+            l = fmaf(p.y, f, l);
+#pragma unroll
+            for (int c = 0; c < 8; c++)
+                if (c * 32 < hs) acc[c] = fmaf(s.part[at * hs + c * 32 + lane], f, acc[c]);
+        }
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        float *to = a.out + ((int64_t)(s.tok0 + row / a.R) * a.n_heads + g * a.R + row % a.R) * hs;
+#pragma unroll
+        for (int c = 0; c < 8; c++)
+            if (c * 32 < hs) to[c * 32 + lane] = acc[c] * inv;
+        return;
+    }
+    const int j0 = (blockIdx.x - row_blocks) * SV_FIN_SLOTS;
+    if (!s.scores || j0 >= s.n_kv) return;
+    for (int row = tid; row < rows; row += 256) {
+        float mx = SV_NONE, l = 0.f;
+        for (int i = 0; i < s.splits; i++) mx = fmaxf(mx, ml[((int64_t)i * a.G + g) * rows + row].x);
+        for (int i = 0; i < s.splits; i++) {
+            const float2 p = ml[((int64_t)i * a.G + g) * rows + row];
+            if (p.y > 0.f) l = fmaf(p.y, exp2f(p.x - mx), l);
+        }
+        sv_lse[row] = l > 0.f ? mx + log2f(l) : INFINITY; // (a row that sees nothing adds nothing)
+    }
+    __syncthreads();
+    const int rp = sv_rp(rows);
+    int per = 1;                                          // lanes of a slot: a power of two
+    while (per < 32 && per * 4 < rp) per *= 2;
+    for (int jb = j0; jb < min(j0 + SV_FIN_SLOTS, s.n_kv); jb += 256 / per) {
+        const int j = jb + tid / per;
+        const float *z = s.scores + ((int64_t)g * s.n_kv + j) * rp;
+        float sum = 0.f;
+        if (j < s.n_kv)
+            for (int row = tid % per; row < rows; row += per) sum += exp2f(z[row] - sv_lse[row]);
+        for (int o = per / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (tid % per == 0 && j < s.n_kv) s.weight[(int64_t)g * s.n_ctx + j] += sum;
+    }
+}
