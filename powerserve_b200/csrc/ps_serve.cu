@@ -2,12 +2,14 @@
 #include "ps_serve.h"
 
 #include "ps_serve_attn.cuh"
+#include "ps_serve_attn_tc.cuh"
 #include "ps_serve_evict.cuh"
 #include "ps_serve_sample.cuh"
 
 #include <algorithm>
 #include <cstdarg>
 #include <cstdio>
+#include <type_traits>
 
 namespace {
 
@@ -101,9 +103,12 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
         }
         SvAttn a{};
         a.q = q; a.out = out; a.hs = hs; a.n_heads = n_heads; a.G = n_kv_heads; a.R = R; a.scale = scale * SV_LOG2E; a.err = c->err_dev; a.n_seqs = n;
-        const int row_tiles = (most_tok * R + 15) / 16;
+        const bool tc = hs == 64 || hs == 128;
+        const int tile_rows = tc ? SV_TC_ROWS : 16, row_tiles = (most_tok * R + tile_rows - 1) / tile_rows;
+        a.out_vec = aligned(out, 16);
         if (most_tok) {
-            a.tps = split_tiles(caches + first, n, n_kv_heads * row_tiles, c->n_sm * 4, 1);
+            a.tps = split_tiles(caches + first, n, n_kv_heads * row_tiles, tc ? c->n_sm : c->n_sm * 4, 1);
+            if (tc) a.tps = std::min(a.tps, SV_TC_TILES);
             size_t bytes = scores;
             int units = 0;
             bool joined = false;
@@ -117,6 +122,9 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
                 const int tiles = s.n_tok ? (s.n_kv + SV_TILE - 1) / SV_TILE : 0;
                 d.splits = (tiles + a.tps - 1) / a.tps;
                 d.unit0 = units;
+                const bool f32 = cache_type == PS_TYPE_F32;
+                d.k_mode = aligned(s.k, f32 ? 32 : 16) ? 2 : aligned(s.k, 16) ? 1 : 0;
+                d.v_mode = s.n_ctx % 8 == 0 && aligned(s.v, f32 ? 32 : 16) ? 2 : f32 && s.n_ctx % 8 == 0 && aligned(s.v, 16) ? 1 : 0;
                 units += d.splits;
                 joined |= d.splits > 1;
                 bytes += up(4 * (size_t)d.splits * n_kv_heads * s.n_tok * R * (hs + 2));
@@ -133,12 +141,23 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
                 d.part = reinterpret_cast<float *>(at);
                 at += up(4 * (size_t)d.splits * n_kv_heads * d.n_tok * R * (hs + 2));
             }
-            const size_t smem = sv_attn_smem(hs);
             const dim3 grid(units, n_kv_heads, row_tiles);
-            if (cache_type == PS_TYPE_F32) {
+            if (tc) {
+                auto launch = [&](auto kern, size_t smem) -> int {
+                    SV_CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+                    kern<<<grid, SV_TC_THREADS, smem, c->stream>>>(a);
+                    return 0;
+                };
+                const bool f32 = cache_type == PS_TYPE_F32;
+                const int rc = hs == 64 ? (f32 ? launch(sv_k_attn_tc<float, 64>, SvTc<float, 64>::SMEM) : launch(sv_k_attn_tc<__nv_bfloat16, 64>, SvTc<__nv_bfloat16, 64>::SMEM))
+                                        : (f32 ? launch(sv_k_attn_tc<float, 128>, SvTc<float, 128>::SMEM) : launch(sv_k_attn_tc<__nv_bfloat16, 128>, SvTc<__nv_bfloat16, 128>::SMEM));
+                if (rc) return rc;
+            } else if (cache_type == PS_TYPE_F32) {
+                const size_t smem = sv_attn_smem(hs);
                 SV_CK(cudaFuncSetAttribute(sv_k_attn<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
                 sv_k_attn<float><<<grid, 128, smem, c->stream>>>(a);
             } else {
+                const size_t smem = sv_attn_smem(hs);
                 SV_CK(cudaFuncSetAttribute(sv_k_attn<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
                 sv_k_attn<__nv_bfloat16><<<grid, 128, smem, c->stream>>>(a);
             }

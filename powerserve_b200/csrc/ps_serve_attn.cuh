@@ -23,6 +23,7 @@ struct SvSeq {
     float *scores;          // [kv head][n_kv][rp], or null
     float *part;            // [split][kv head][row][hs]; then [split][kv head][row] pairs of maximum and sum
     int n_ctx, n_kv, n_tok, tok0;
+    int k_mode, v_mode;     // head sizes 64 and 128: how rows can be read (sv_get)
     int splits, unit0;      // unit0: number of the sequence's first split among all of the launch
 };
 struct SvAttn {
@@ -30,6 +31,7 @@ struct SvAttn {
     const float *q;
     float *out;
     int n_seqs, hs, n_heads, G, R, tps; // R: heads that share a kv head; tps: tiles of a split
+    int out_vec;                        // out is aligned to 16 bytes
     float scale;                        // times log2 e
     int *err;
 };
