@@ -93,7 +93,7 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
         bool weights = false;
         while (first + n < n_seqs && n < SV_SEQS) {
             const ps_cuda_cache &s = caches[first + n];
-            const size_t more = s.weight && s.n_tok ? up(4 * (size_t)n_kv_heads * s.n_kv * ((s.n_tok * R + 3) & ~3)) : 0;
+            const size_t more = s.weight && s.n_tok ? up(16 * (size_t)n_kv_heads * sv_quads(s.n_kv) * sv_rp(s.n_tok * R)) : 0;
             if (n && scores + more > ((size_t)1 << 30)) break;
             scores += more;
             weights |= more != 0;
@@ -123,8 +123,8 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
                 d.splits = (tiles + a.tps - 1) / a.tps;
                 d.unit0 = units;
                 const bool f32 = cache_type == PS_TYPE_F32;
-                d.k_mode = aligned(s.k, f32 ? 32 : 16) ? 2 : aligned(s.k, 16) ? 1 : 0;
-                d.v_mode = s.n_ctx % 8 == 0 && aligned(s.v, f32 ? 32 : 16) ? 2 : f32 && s.n_ctx % 8 == 0 && aligned(s.v, 16) ? 1 : 0;
+                d.k_mode = aligned(s.k, 16);
+                d.v_mode = aligned(s.v, 16) && s.n_ctx % (f32 ? 4 : 8) == 0;
                 units += d.splits;
                 joined |= d.splits > 1;
                 bytes += up(4 * (size_t)d.splits * n_kv_heads * s.n_tok * R * (hs + 2));
@@ -136,21 +136,24 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
                 SvSeq &d = a.seq[i];
                 if (d.weight) {
                     d.scores = reinterpret_cast<float *>(at);
-                    at += up(4 * (size_t)n_kv_heads * d.n_kv * ((d.n_tok * R + 3) & ~3));
+                    at += up(16 * (size_t)n_kv_heads * sv_quads(d.n_kv) * sv_rp(d.n_tok * R));
                 }
                 d.part = reinterpret_cast<float *>(at);
                 at += up(4 * (size_t)d.splits * n_kv_heads * d.n_tok * R * (hs + 2));
             }
             const dim3 grid(units, n_kv_heads, row_tiles);
             if (tc) {
-                auto launch = [&](auto kern, size_t smem) -> int {
-                    SV_CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-                    kern<<<grid, SV_TC_THREADS, smem, c->stream>>>(a);
+                const int most_rows = most_tok * R;
+                auto launch = [&](auto kern, auto shape) -> int {
+                    using C = decltype(shape);
+                    const int stages = C::stages(most_rows, 220 * 1024), smem = C::smem(most_rows, stages); // (7 KB for what the kernel declares)
+                    SV_CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+                    kern<<<grid, SV_TC_THREADS, smem, c->stream>>>(a, stages, C::q_bytes(most_rows));
                     return 0;
                 };
                 const bool f32 = cache_type == PS_TYPE_F32;
-                const int rc = hs == 64 ? (f32 ? launch(sv_k_attn_tc<float, 64>, SvTc<float, 64>::SMEM) : launch(sv_k_attn_tc<__nv_bfloat16, 64>, SvTc<__nv_bfloat16, 64>::SMEM))
-                                        : (f32 ? launch(sv_k_attn_tc<float, 128>, SvTc<float, 128>::SMEM) : launch(sv_k_attn_tc<__nv_bfloat16, 128>, SvTc<__nv_bfloat16, 128>::SMEM));
+                const int rc = hs == 64 ? (f32 ? launch(sv_k_attn_tc<float, 64>, SvTc<float, 64>()) : launch(sv_k_attn_tc<__nv_bfloat16, 64>, SvTc<__nv_bfloat16, 64>()))
+                                        : (f32 ? launch(sv_k_attn_tc<float, 128>, SvTc<float, 128>()) : launch(sv_k_attn_tc<__nv_bfloat16, 128>, SvTc<__nv_bfloat16, 128>()));
                 if (rc) return rc;
             } else if (cache_type == PS_TYPE_F32) {
                 const size_t smem = sv_attn_smem(hs);

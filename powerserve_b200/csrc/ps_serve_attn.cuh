@@ -5,7 +5,7 @@
 //
 // A sequence's query rows of one kv head (n_tok tokens x the heads that share it) go together, so that its K rows and V^T columns are read once.
 // The slots are cut into splits; a split leaves its rows' running maximum, sum and unnormalised output in the workspace, and sv_k_finish joins
-// them.  Where weights are gathered, the scores (32 bits) go to the workspace too, [slot][row], and sv_k_finish sums exp(z - log-sum) over the rows.
+// them.  Where weights are gathered, the scores (32 bits) go to the workspace too, and sv_k_finish sums exp(z - log-sum) over the rows.
 #pragma once
 #include "ps_ptx.cuh"
 
@@ -20,10 +20,10 @@ struct SvSeq {
     const void *k, *v;
     float *weight;
     const uint8_t *hidden, *mask;
-    float *scores;          // [kv head][n_kv][rp], or null
+    float *scores;          // [kv head][quad of slots][rp][4], or null: quads up to a whole tile, -inf where a row does not see the slot
     float *part;            // [split][kv head][row][hs]; then [split][kv head][row] pairs of maximum and sum
     int n_ctx, n_kv, n_tok, tok0;
-    int k_mode, v_mode;     // head sizes 64 and 128: how rows can be read (sv_get)
+    int k_mode, v_mode;     // head sizes 64 and 128: rows begin at 16-byte boundaries
     int splits, unit0;      // unit0: number of the sequence's first split among all of the launch
 };
 struct SvAttn {
@@ -38,7 +38,8 @@ struct SvAttn {
 
 PS_D float sv_ld(const float *p, int64_t i) { return p[i]; }
 PS_D float sv_ld(const __nv_bfloat16 *p, int64_t i) { return __bfloat162float(p[i]); }
-PS_D int sv_rp(int rows) { return (rows + 3) & ~3; }
+PS_HD int sv_rp(int rows) { return (rows + 3) & ~3; }
+PS_HD int64_t sv_quads(int n_kv) { return (int64_t)((n_kv + SV_TILE - 1) / SV_TILE) * (SV_TILE / 4); }
 PS_D int sv_find(const SvAttn &a, int unit) {
     int s = 0;
     while (s + 1 < a.n_seqs && unit >= a.seq[s + 1].unit0) s++;
@@ -96,7 +97,7 @@ __global__ void __launch_bounds__(128) sv_k_attn(const __grid_constant__ SvAttn 
         for (int r = 0; r < 4; r++) {
             const int row = r0 + warp * 4 + r;
             if (!in || row >= rows || !sv_sees(s, row / a.R, j - past)) z[r] = SV_NONE;
-            if (s.scores && row < rows && j < j_end) s.scores[((int64_t)g * s.n_kv + j) * rp + row] = z[r];
+            if (s.scores && row < rows && j < j_end) s.scores[(((int64_t)g * sv_quads(s.n_kv) + j / 4) * rp + row) * 4 + j % 4] = z[r];
             float mx = z[r];
 #pragma unroll
             for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -196,15 +197,24 @@ __global__ void __launch_bounds__(256) sv_k_finish(const __grid_constant__ SvAtt
     }
     __syncthreads();
     const int rp = sv_rp(rows);
-    int per = 1;                                          // lanes of a slot: a power of two
-    while (per < 32 && per * 4 < rp) per *= 2;
-    for (int jb = j0; jb < min(j0 + SV_FIN_SLOTS, s.n_kv); jb += 256 / per) {
-        const int j = jb + tid / per;
-        const float *z = s.scores + ((int64_t)g * s.n_kv + j) * rp;
-        float sum = 0.f;
-        if (j < s.n_kv)
-            for (int row = tid % per; row < rows; row += per) sum += exp2f(z[row] - sv_lse[row]);
-        for (int o = per / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (tid % per == 0 && j < s.n_kv) s.weight[(int64_t)g * s.n_ctx + j] += sum;
+    int per = 1;                                          // lanes of a quad of slots: a power of two
+    while (per < 32 && per < rows) per *= 2;
+    for (int b = 0; b < SV_FIN_SLOTS / 4; b += 256 / per) {
+        const int j = j0 + 4 * (b + tid / per);
+        const bool in = b + tid / per < SV_FIN_SLOTS / 4 && j < s.n_kv;
+        float sum[4] = {};
+        if (in) {
+            const float4 *z = reinterpret_cast<const float4 *>(s.scores) + ((int64_t)g * sv_quads(s.n_kv) + j / 4) * rp;
+            for (int row = tid % per; row < rows; row += per) {
+                const float4 v = z[row];
+                const float lse = sv_lse[row];
+                sum[0] += exp2f(v.x - lse); sum[1] += exp2f(v.y - lse); sum[2] += exp2f(v.z - lse); sum[3] += exp2f(v.w - lse);
+            }
+        }
+        for (int o = per / 2; o; o >>= 1)
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], o);
+        if (tid % per == 0 && in)
+            for (int e = 0; e < min(4, s.n_kv - j); e++) s.weight[(int64_t)g * s.n_ctx + j + e] += sum[e];
     }
 }

@@ -1,24 +1,28 @@
 // ps_serve_attn_tc.cuh - ps_serve_attn.cuh's attention for head sizes 64 and 128, on the fifth-generation tensor cores, to float32's precision.
 //
-// Operands.  A number x is cut into two fp16 parts, hi = fp16(x 2^e) and lo = fp16(x 2^e - hi), with 2^e from the largest of its group so that the
+// Operands.  A number x is cut into two fp16 parts, the upper eleven bits of x 2^e and the others, rounded, with 2^e from the largest of its group so that the
 // group fits fp16's range from the top: what is lost is below 2^-22 of x, or 2^-39 of the group's largest.  Three MMAs (lo hi, hi lo, hi hi) replace the
-// 32-bit products; the missing lo lo is below 2^-22 of the product.  bfloat16 caches have no lo part: two MMAs.  Groups: a query row; 16 slots' K rows;
-// hs / 4 channels of a tile of V.  The weights p of the soft-max, at most 1, are cut after a factor 2^15.
+// 32-bit products; the missing lo lo is below 2^-22 of the product.  bfloat16 caches have no lo part: two MMAs.  Groups: a query row; eight slots' K rows;
+// hs / 8 channels of a tile of V.  The weights p of the soft-max, at most 1, are cut after a factor 2^15.
 // A tile's output leaves the tensor memory after every tile and is added up in registers, with rounding: the accumulator, which truncates, sees the
-// twelve MMAs of one tile, and groups' and rows' factors may differ from tile to tile.
+// MMAs of one tile alone.  So groups' factors and a row's maximum may differ from tile to tile, and the soft-max of a tile knows of no other tile.
 //
-// A CTA takes up to 128 query rows (the MMAs' M side: one row, one lane of tensor memory, one thread of the soft-max) of one kv head over one split.
-// Roles: warps 0-3 soft-max; 4-11 output (a row's channels in two halves); 12-15 load K rows, 16-19 V columns: from memory to registers a tile ahead,
-// into parts, to shared memory in the K-major no-swizzle layout; 20 issues MMAs.  Tensor memory: two tiles of scores, of weights (both parts), of outputs.
-// Bound by memory: a tile of 64 slots at head size 128 is 64 KB, some 2 850 cycles of an SM's share of the bandwidth; its MMAs take some 1 500.
+// A CTA takes up to 128 query rows (the MMAs' M side: one row, one lane of tensor memory) of one kv head over one split.  Warps 0-3 and 4-7: soft-max of
+// the even and of the odd tiles; 8-15: output, a row's channels in two halves; 16-23: converters; 24: MMAs; 25-27: copies.
+// Tiles of K and of V go through one ring of shared-memory stages: asynchronous 16-byte copies bring a stage as it lies in memory (bulk copies of rows of 256 and
+// 512 bytes took 65 cycles each, 12 400 a tile), the converters cut it
+// into parts in its place (eight rows, read by one warp, become the same eight rows' parts in the K-major no-swizzle layout, in the same bytes),
+// the MMAs read it.  Rows are 16 bytes apart from the next so that neither reading nor writing meets a bank twice.
+// Bound by memory: at head size 128 a tile of 64 slots is 64 KB, some 2 850 cycles of an SM's share of the bandwidth.
 #pragma once
 #include "ps_serve_attn.cuh"
 
 #include <cuda_fp16.h>
 
-#define SV_TC_THREADS 672
+#define SV_TC_THREADS 896
 #define SV_TC_ROWS 128
 #define SV_TC_TILES 256  // most tiles of a split (a word of live slots for each)
+#define SV_TC_STAGES 6   // most stages of the ring
 
 PS_D void sv_bar_wait(uint64_t *bar, uint32_t parity, bool &ok, int *err, int site) {
     if (ok && !ps_tc_wait_warp(bar, parity)) { *err = site; ok = false; }
@@ -34,400 +38,429 @@ PS_D uint32_t sv_pack(float a, float b) { // fp16 of a (low half) and b
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
     return r;
 }
-PS_D void sv_cut(float a, float b, uint32_t &hi, uint32_t &lo) {
-    hi = sv_pack(a, b);
-    const float2 h = __half22float2(*reinterpret_cast<__half2 *>(&hi));
-    lo = sv_pack(a - h.x, b - h.y);
+PS_D void sv_cut(float a, float b, uint32_t &hi, uint32_t &lo) { // hi: the upper eleven bits, as they are (no conversion back); lo: the others, rounded
+    const float ha = __uint_as_float(__float_as_uint(a) & 0xffffe000u), hb = __uint_as_float(__float_as_uint(b) & 0xffffe000u);
+    hi = sv_pack(ha, hb);
+    lo = sv_pack(a - ha, b - hb);
 }
 PS_D float sv_ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+PS_D void sv_tm_ld16(uint32_t (&v)[16], uint32_t at) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]),
+                   "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(at)
+                 : "memory");
+}
+PS_D void sv_tm_st8(uint32_t at, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+template <int N> PS_D void sv_regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> PS_D void sv_regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 // eight elements of a cache as they lie in memory
-struct SvRaw32 { float v[8]; };
-struct SvRaw16 { uint4 v; };
-PS_D void sv_get(SvRaw32 &r, const float *p, int mode, uint32_t live) { // mode 2: 32 bytes at once, 1: twice 16, 0: one by one, the live ones
-    if (mode == 2) {
-        asm volatile("ld.global.nc.L1::no_allocate.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                     : "=f"(r.v[0]), "=f"(r.v[1]), "=f"(r.v[2]), "=f"(r.v[3]), "=f"(r.v[4]), "=f"(r.v[5]), "=f"(r.v[6]), "=f"(r.v[7]) : "l"(p));
-    } else if (mode == 1) {
-        const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-        r.v[0] = a.x; r.v[1] = a.y; r.v[2] = a.z; r.v[3] = a.w; r.v[4] = b.x; r.v[5] = b.y; r.v[6] = b.z; r.v[7] = b.w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) r.v[i] = live >> i & 1 ? __ldg(p + i) : 0.f;
-    }
+struct SvRaw32 { float4 a, b; };
+struct SvRaw16 { uint4 a; };
+PS_D void sv_get(SvRaw32 &r, const uint8_t *p) {
+    r.a = *reinterpret_cast<const float4 *>(p);
+    r.b = *reinterpret_cast<const float4 *>(p + 16);
 }
-PS_D void sv_get(SvRaw16 &r, const __nv_bfloat16 *p, int mode, uint32_t live) {
-    if (mode) r.v = __ldg(reinterpret_cast<const uint4 *>(p));
-    else {
-        uint32_t w[4] = {};
-        const uint16_t *u = reinterpret_cast<const uint16_t *>(p);
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (live >> i & 1) w[i / 2] |= (uint32_t)__ldg(u + i) << (16 * (i & 1));
-        r.v = make_uint4(w[0], w[1], w[2], w[3]);
-    }
+PS_D void sv_get(SvRaw16 &r, const uint8_t *p) { r.a = *reinterpret_cast<const uint4 *>(p); }
+PS_D float sv_at(const SvRaw32 &r, int i) {
+    const float4 &q = i < 4 ? r.a : r.b;
+    return i % 4 == 0 ? q.x : i % 4 == 1 ? q.y : i % 4 == 2 ? q.z : q.w;
 }
-PS_D void sv_zero(SvRaw32 &r) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) r.v[i] = 0.f;
-}
-PS_D void sv_zero(SvRaw16 &r) { r.v = make_uint4(0, 0, 0, 0); }
-PS_D float sv_at(const SvRaw32 &r, int i) { return r.v[i]; }
 PS_D float sv_at(const SvRaw16 &r, int i) {
-    const uint32_t w = i < 2 ? r.v.x : i < 4 ? r.v.y : i < 6 ? r.v.z : r.v.w;
+    const uint32_t w = i < 2 ? r.a.x : i < 4 ? r.a.y : i < 6 ? r.a.z : r.a.w;
     return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
-}
-template <typename R> PS_D void sv_keep(R &r, uint32_t live);
-template <> PS_D void sv_keep<SvRaw32>(SvRaw32 &r, uint32_t live) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) r.v[i] = live >> i & 1 ? r.v[i] : 0.f;
-}
-template <> PS_D void sv_keep<SvRaw16>(SvRaw16 &r, uint32_t live) {
-    uint32_t *w = &r.v.x;
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-        if (!(live >> i & 1)) w[i / 2] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
 }
 
 template <typename T, int D> struct SvTc {
     static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int PARTS = F32 ? 2 : 1;
-    static constexpr int KPART = SV_TILE * D * 2;                     // bytes of one part of a tile of K or of V
-    static constexpr int STAGE = PARTS * KPART;
-    static constexpr int Q = 2 * SV_TC_ROWS * D * 2;                  // both parts of the queries
-    static constexpr int SMEM = Q + 4 * STAGE + 1024;
-    static constexpr int ITS = D / 16;                                // eights that a loading thread holds
+    static constexpr int K_ROW = D * (int)sizeof(T) + 16, V_ROW = SV_TILE * (int)sizeof(T) + 16; // bytes from row to row of a stage
+    static constexpr int K_LO = D * 16, V_LO = SV_TILE * 16;                                     // from a group's hi part to its lo part
+    static constexpr int STAGE = (SV_TILE * K_ROW > D * V_ROW ? SV_TILE * K_ROW : D * V_ROW);
+    static constexpr int Q_GROUP = D * 32;                                                       // both parts of eight query rows
+    static constexpr int V_GROUPS = D / 64;                                                      // groups of eight channels that a converter takes
     using Raw = typename std::conditional<F32, SvRaw32, SvRaw16>::type;
+    static int q_bytes(int rows) { return (std::min(rows, SV_TC_ROWS) + 7) / 8 * Q_GROUP; }
+    // stages beside the queries; the MMAs read 128 query rows whatever there are, and what follows them in shared memory is read for rows that nobody looks at
+    static int stages(int rows, int smem) { return std::min(SV_TC_STAGES, (smem - 128 - q_bytes(rows)) / STAGE); }
+    static int smem(int rows, int n) { return std::max(q_bytes(rows) + n * STAGE, SV_TC_ROWS / 8 * Q_GROUP) + 128; }
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_constant__ SvAttn a) {
+__global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_constant__ SvAttn a, int stages, int q_bytes) {
     using C = SvTc<T, D>;
-    using Raw = typename C::Raw;
-    extern __shared__ __align__(1024) uint8_t sv_tc_raw[];
-    __shared__ __align__(8) uint64_t full_k[2], full_v[2], s_full[2], s_empty[2], p_full[2], o_full[2], o_empty[2], done;
+    extern __shared__ __align__(128) uint8_t sv_tc_raw[];
+    __shared__ __align__(8) uint64_t raw_full[SV_TC_STAGES], ready[SV_TC_STAGES], unused[SV_TC_STAGES], s_full[2], p_full[2], o_full[2], o_empty[2], done;
     __shared__ uint32_t tmem_smem;
-    __shared__ float s_alpha[2][SV_TC_ROWS], s_kinv[2][4], s_vinv[2][4], s_qinv[SV_TC_ROWS], s_sum[SV_TC_ROWS];
+    __shared__ float s_top[2][SV_TC_ROWS], s_sum[2][SV_TC_ROWS], s_qinv[SV_TC_ROWS];
+    __shared__ __align__(16) float s_kinv[8][8], s_vinv[8][8];
     __shared__ uint64_t s_live[SV_TC_TILES];
-    uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)sv_tc_raw + 1023) & ~(uintptr_t)1023);
-    uint8_t *sm_q = smem, *sm_k = smem + C::Q, *sm_v = sm_k + 2 * C::STAGE;
+    uint8_t *sm_q = reinterpret_cast<uint8_t *>(((uintptr_t)sv_tc_raw + 127) & ~(uintptr_t)127), *sm_ring = sm_q + q_bytes;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    const int si = sv_find(a, blockIdx.x), split = blockIdx.x - a.seq[si].unit0, g = blockIdx.y;
+    const int si = __shfl_sync(0xffffffffu, sv_find(a, blockIdx.x), 0), split = blockIdx.x - a.seq[si].unit0, g = blockIdx.y;
     const SvSeq &s = a.seq[si];
     const int all_rows = s.n_tok * a.R, r0 = blockIdx.z * SV_TC_ROWS, rows = min(all_rows - r0, SV_TC_ROWS);
     if (rows <= 0) return;
     const int j0 = split * a.tps * SV_TILE, j_end = min(s.n_kv, j0 + a.tps * SV_TILE), tiles = (j_end - j0 + SV_TILE - 1) / SV_TILE, past = s.n_kv - s.n_tok;
 
-    if (tid == 0) {
-        for (int b = 0; b < 2; b++) {
-            ps_mbar_init(&full_k[b], 4); ps_mbar_init(&full_v[b], 4); ps_mbar_init(&s_full[b], 1); ps_mbar_init(&s_empty[b], 4);
-            ps_mbar_init(&p_full[b], 4); ps_mbar_init(&o_full[b], 1); ps_mbar_init(&o_empty[b], 8);
+    // ===== copies: K 0, then for every tile the K of the next and its own V
+    int st = 0;             // stage and round of the ring, for the roles that go through it
+    uint32_t round = 0;
+    auto step = [&] {
+        if (++st == stages) { st = 0; round ^= 1; }
+    };
+    int put_n = 0;
+    auto put = [&](bool is_v, int t) -> bool { // by each of the three warps, its share of the rows
+        if (put_n >= stages && !ps_tc_wait_warp(&unused[st], round ^ 1)) { *a.err = 11; return false; }
+        const int j = j0 + t * SV_TILE;
+        if (is_v ? s.v_mode : s.k_mode) {
+            const int count = is_v ? D : min(SV_TILE, j_end - j), step_rows = is_v ? C::V_ROW : C::K_ROW, lanes = (step_rows - 16) / 16; // lanes of a row: 16 bytes each
+            const int64_t ld = (is_v ? (int64_t)s.n_ctx : (int64_t)a.G * D) * (int64_t)sizeof(T);
+            const uint8_t *src = is_v ? reinterpret_cast<const uint8_t *>(static_cast<const T *>(s.v) + (int64_t)g * D * s.n_ctx + j)
+                                      : reinterpret_cast<const uint8_t *>(static_cast<const T *>(s.k) + (int64_t)j * a.G * D + (int64_t)g * D);
+            const int in_row = (lane % lanes) * 16, rows_at_once = 32 / lanes, last = is_v ? (s.n_ctx - j) * (int)sizeof(T) : INT32_MAX; // (a row of V is read up to its own end)
+            const uint32_t to = ps_smem_u32(sm_ring + st * C::STAGE) + in_row;
+            if (in_row < last)
+#pragma unroll 4
+                for (int i = (warp - 25) * rows_at_once + lane / lanes; i < count; i += 3 * rows_at_once)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * step_rows), "l"(src + i * ld + in_row) : "memory");
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ps_smem_u32(&raw_full[st])) : "memory");
+        } else ps_mbar_arrive(&raw_full[st]);
+        __syncwarp();
+        put_n++;
+        step();
+        return true;
+    };
+    int put_t = 0;          // next of the pairs (K of t + 1, V of t); the first K is put alone
+    if (warp >= 25) {
+        if (tid == 25 * 32) {
+            for (int b = 0; b < SV_TC_STAGES; b++) { ps_mbar_init(&raw_full[b], 96); ps_mbar_init(&ready[b], 8); ps_mbar_init(&unused[b], 1); }
+            for (int b = 0; b < 2; b++) { ps_mbar_init(&s_full[b], 1); ps_mbar_init(&p_full[b], 4); ps_mbar_init(&o_full[b], 1); ps_mbar_init(&o_empty[b], 8); }
+            ps_mbar_init(&done, 1);
+            ps_fence_barrier_init();
         }
-        ps_mbar_init(&done, 1);
-        ps_fence_barrier_init();
+        ps_bar_sync(1, 96);
+        put(false, 0);      // (the ring is empty: these do not wait)
+        while (put_t < tiles && put_n + 2 <= stages) {
+            if (put_t + 1 < tiles) put(false, put_t + 1);
+            put(true, put_t++);
+        }
     }
-    if (warp == 20) {
+    if (warp == 24) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(ps_smem_u32(&tmem_smem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     // live slots of a tile: in the split and not hidden
-    auto in_split = [&](int t) -> uint64_t {
-        const int n = j_end - j0 - t * SV_TILE;
-        return n >= SV_TILE ? ~0ull : (1ull << n) - 1;
-    };
-    if (s.hidden)
-        for (int t = warp; t < tiles; t += SV_TC_THREADS / 32) {
+    if (s.hidden && warp < 24)
+        for (int t = warp; t < tiles; t += 24) {
             const int j = j0 + t * SV_TILE + lane;
             const uint32_t lo = __ballot_sync(0xffffffffu, j < j_end && !s.hidden[min(j, j_end - 1)]), hi = __ballot_sync(0xffffffffu, j + 32 < j_end && !s.hidden[min(j + 32, j_end - 1)]);
             if (lane == 0) s_live[t] = (uint64_t)hi << 32 | lo;
         }
-    auto live_of = [&](int t) -> uint64_t { return s.hidden ? s_live[t] : in_split(t); };
+    auto live_of = [&](int t) -> uint64_t {
+        if (s.hidden) return s_live[t];
+        const int n = j_end - j0 - t * SV_TILE;
+        return n >= SV_TILE ? ~0ull : (1ull << n) - 1;
+    };
     // queries: a half-warp (quarter-warp for head size 64) per row
-    for (int i = tid; i < rows * (D / 8); i += SV_TC_THREADS) { // (rows * D / 8 is a multiple of D / 8: the lanes of a row are there together)
-        const int r = i / (D / 8), c = i % (D / 8), row = r0 + r;
-        const float *q = a.q + ((int64_t)(s.tok0 + row / a.R) * a.n_heads + g * a.R + row % a.R) * D + c * 8;
-        const unsigned mates = (D == 128 ? 0xffffu : 0xffu) << (lane & (D == 128 ? 16 : 24));
-        float x[8], inv;
-        uint32_t mx = 0;
+    if (warp < 24)
+        for (int i = tid; i < rows * (D / 8); i += 768) { // (rows * D / 8 and 768 are multiples of D / 8: the lanes of a row are there together)
+            const int r = i / (D / 8), c = i % (D / 8), row = r0 + r;
+            const float *q = a.q + ((int64_t)(s.tok0 + row / a.R) * a.n_heads + g * a.R + row % a.R) * D + c * 8;
+            const unsigned mates = (D == 128 ? 0xffffu : 0xffu) << (lane & (D == 128 ? 16 : 24));
+            float x[8], inv;
+            uint32_t mx = 0;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            x[e] = q[e] * a.scale;
-            mx = max(mx, __float_as_uint(x[e]) & 0x7fffffffu);
+            for (int e = 0; e < 8; e++) {
+                x[e] = q[e] * a.scale;
+                mx = max(mx, __float_as_uint(x[e]) & 0x7fffffffu);
+            }
+#pragma unroll
+            for (int o = D / 16; o; o >>= 1) mx = max(mx, __shfl_xor_sync(mates, mx, o));
+            const float f = sv_scale(mx, inv);
+            uint4 hi, lo;
+            sv_cut(x[0] * f, x[1] * f, hi.x, lo.x);
+            sv_cut(x[2] * f, x[3] * f, hi.y, lo.y);
+            sv_cut(x[4] * f, x[5] * f, hi.z, lo.z);
+            sv_cut(x[6] * f, x[7] * f, hi.w, lo.w);
+            uint8_t *to = sm_q + (r >> 3) * C::Q_GROUP + c * 128 + (r & 7) * 16;
+            *reinterpret_cast<uint4 *>(to) = hi;
+            *reinterpret_cast<uint4 *>(to + D * 16) = lo;
+            if (c == 0) s_qinv[r] = inv;
         }
-#pragma unroll
-        for (int o = D / 16; o; o >>= 1) mx = max(mx, __shfl_xor_sync(mates, mx, o));
-        const float f = sv_scale(mx, inv);
-        uint4 hi, lo;
-        sv_cut(x[0] * f, x[1] * f, hi.x, lo.x);
-        sv_cut(x[2] * f, x[3] * f, hi.y, lo.y);
-        sv_cut(x[4] * f, x[5] * f, hi.z, lo.z);
-        sv_cut(x[6] * f, x[7] * f, hi.w, lo.w);
-        *reinterpret_cast<uint4 *>(sm_q + c * (SV_TC_ROWS * 16) + r * 16) = hi;
-        *reinterpret_cast<uint4 *>(sm_q + C::Q / 2 + c * (SV_TC_ROWS * 16) + r * 16) = lo;
-        if (c == 0) s_qinv[r] = inv;
-    }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     ps_tc_fence_before();
     __syncthreads();
     ps_tc_fence_after();
-    const uint32_t tm = tmem_smem, tm_s = tm, tm_p = tm + 2 * SV_TILE, tm_o = tm + 4 * SV_TILE; // columns: scores 2 x 64, weights 2 x (32 + 32), outputs 2 x D
-    bool ok = true;
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem_smem, 0), tm_s = tm, tm_p = tm + 2 * SV_TILE, tm_o = tm + 4 * SV_TILE; // columns: scores 2 x 64, weights 2 x (32 + 32), outputs 2 x D
+    // A barrier is waited on only by who must have passed it before it can complete again (a phase that was missed would never end): groups' and rows' factors
+    // come with the MMAs' barrier, whose issuer has waited for those who wrote them.
+    // Registers: 72 a thread at the launch, 504 over the seven warpgroups; 2 x 72 (soft-max) + 2 x 88 (output) + 2 x 72 (converters) + 40 (MMAs, copies) = 504
 
-    if (warp >= 12 && warp < 20) {
-        // ===== loaders: K by warps 12-15 (16 slots each), V by warps 16-19 (D / 4 channels each).  A thread's eights: lane % 8 picks one of eight rows (slots of
-        // K, channels of V), lane / 8 one of four neighbouring eights of the row: a warp's load is 8 rows x 128 bytes, its store eight times 128 bytes
-        const bool is_v = warp >= 16;
-        const int w = warp & 3, sub = lane & 7, quad = lane >> 3;
-        const int64_t ld = is_v ? s.n_ctx : (int64_t)a.G * D;
-        const T *base = static_cast<const T *>(is_v ? s.v : s.k) + (is_v ? ((int64_t)g * D + w * (D / 4) + sub) * ld : (int64_t)g * D);
-        const int mode = is_v ? s.v_mode : s.k_mode;
-        uint8_t *sm = is_v ? sm_v : sm_k;
-        uint64_t *full = is_v ? full_v : full_k, *empty = is_v ? o_empty : s_empty;
-        Raw raw[C::ITS];
-        auto load = [&](int t) {
+    if (warp >= 24) {
+        sv_regs_less<40>();
+        if (warp >= 25) {
+            bool fine = true;
+            for (; put_t < tiles && fine; put_t++) {
+                if (put_t + 1 < tiles) fine = put(false, put_t + 1);
+                fine = fine && put(true, put_t);
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory"); // (what is in flight ends before the CTA does, even when a wait gave up)
+        } else {
+            // ===== MMAs.  Small products first, while the truncating accumulator is small
+            const uint32_t idesc_s = (1u << 4) | ((uint32_t)(SV_TILE >> 3) << 17) | ((uint32_t)(SV_TC_ROWS >> 4) << 24);
+            const uint32_t idesc_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(SV_TC_ROWS >> 4) << 24);
+            const uint64_t dq = ps_tc_smem_desc(ps_smem_u32(sm_q), 128, C::Q_GROUP), dk = ps_tc_smem_desc(ps_smem_u32(sm_ring), 128, 8 * C::K_ROW), dv = ps_tc_smem_desc(ps_smem_u32(sm_ring), 128, 8 * C::V_ROW);
+            auto scores = [&](int t) -> bool { // (the soft-max of tile t - 2 is done with these scores: its weights have been waited for)
+                if (!ps_tc_wait_warp(&ready[st], round)) { *a.err = 12; return false; }
+                ps_tc_fence_after();
+                const uint64_t kb = dk + (uint64_t)(st * (C::STAGE >> 4));
+                const uint32_t to = tm_s + (t & 1) * SV_TILE;
+                if (ps_elect_one()) {
+#pragma unroll
+                    for (int p = 0; p < C::PARTS + 1; p++) // lo hi, hi lo, hi hi (bfloat16 caches: lo hi, hi hi)
+#pragma unroll
+                        for (int j = 0; j < D / 16; j++) ps_tc_mma_f16(to, dq + (p == 0 ? (D * 16) >> 4 : 0) + j * 16, kb + (C::F32 && p == 1 ? C::K_LO >> 4 : 0) + j * 16, idesc_s, (p | j) != 0);
+                    ps_tc_commit(&unused[st]);
+                    ps_tc_commit(&s_full[t & 1]);
+                }
+                __syncwarp();
+                step();
+                return true;
+            };
+            bool fine = scores(0);
+            for (int t = 0; t < tiles && fine; t++) {
+                const int b = t & 1;
+                if (t + 1 < tiles && !scores(t + 1)) break;
+                if (!ps_tc_wait_warp(&ready[st], round)) { *a.err = 14; break; }
+                if (!ps_tc_wait_warp(&p_full[b], (t >> 1) & 1)) { *a.err = 15; break; } // (the soft-max has waited for the output of tile t - 2)
+                ps_tc_fence_after();
+                const uint64_t vb = dv + (uint64_t)(st * (C::STAGE >> 4));
+                const uint32_t to = tm_o + b * D, pa = tm_p + b * SV_TILE;
+                if (ps_elect_one()) {
+#pragma unroll
+                    for (int p = 0; p < C::PARTS + 1; p++)
+#pragma unroll
+                        for (int j = 0; j < SV_TILE / 16; j++)
+                            ps_tc_mma_f16_ta(to, pa + (p == 0 ? SV_TILE / 2 : 0) + j * 8, vb + (C::F32 && p == 1 ? C::V_LO >> 4 : 0) + j * 16, idesc_o, (p | j) != 0);
+                    ps_tc_commit(&unused[st]);
+                    ps_tc_commit(&o_full[b]);
+                }
+                __syncwarp();
+                step();
+            }
+            if (ps_elect_one()) ps_tc_commit(&done); // MMAs in flight end before the tensor memory is given back
+            __syncwarp();
+            if (!ps_tc_wait_warp(&done, 0)) *a.err = 16;
+        }
+    } else if (warp >= 16) {
+        // ===== converters.  lane % 8 picks one of eight rows (slots of K, channels of V), lane / 8 one of four neighbouring eights of the row
+        const int w = warp - 16, sub = lane & 7, quad = lane >> 3;
+        auto convert = [&](bool is_v, int t) -> bool {
+            if (!ps_tc_wait_warp(&raw_full[st], round)) { *a.err = 17; return false; }
+            constexpr int ITS = D / 32; // eights of a thread
+            const int mode = is_v ? s.v_mode : s.k_mode, j = j0 + t * SV_TILE;
             const uint64_t live = live_of(t);
-            const int j = j0 + t * SV_TILE;
+            uint8_t *group = sm_ring + st * C::STAGE + (is_v ? w * C::V_GROUPS * 8 * C::V_ROW : w * 8 * C::K_ROW);
+            // eight i of the thread: K: 32 elements further along the row; V: the row's second half, then the next group of channels
+            typename C::Raw raw[ITS];
+            if (mode) {
+                const uint8_t *from = group + sub * (is_v ? C::V_ROW : C::K_ROW) + quad * (8 * (int)sizeof(T));
 #pragma unroll
-            for (int i = 0; i < C::ITS; i++) {
-                if (is_v) { // i: channel group (of eight), half of the tile
-                    const int chunk = quad + 4 * (i & 1);
-                    const uint32_t m = (uint32_t)(live >> (8 * chunk)) & 0xffu;
-                    if (m) sv_get(raw[i], base + (int64_t)(i >> 1) * 8 * ld + j + 8 * chunk, mode, m);
-                    else sv_zero(raw[i]);
-                } else {    // i: slot group (of eight), four eights of the row
-                    const int slot = w * 16 + (i / (D / 32)) * 8 + sub;
-                    if (live >> slot & 1) sv_get(raw[i], base + (int64_t)(j + slot) * ld + ((i % (D / 32)) * 4 + quad) * 8, mode, 0xffu);
-                    else sv_zero(raw[i]);
+                for (int i = 0; i < ITS; i++) sv_get(raw[i], from + (is_v ? (i >> 1) * 8 * C::V_ROW + (i & 1) * (32 * (int)sizeof(T)) : i * (32 * (int)sizeof(T))));
+            } else { // rows that no bulk copy can read: element by element
+#pragma unroll
+                for (int i = 0; i < ITS; i++) {
+                    T x[8];
+                    const int slot = is_v ? (quad + 4 * (i & 1)) * 8 : w * 8 + sub;
+                    const T *src = is_v ? static_cast<const T *>(s.v) + ((int64_t)g * D + (w * C::V_GROUPS + (i >> 1)) * 8 + sub) * s.n_ctx + j + slot
+                                        : static_cast<const T *>(s.k) + (int64_t)(j + slot) * a.G * D + (int64_t)g * D + (i * 4 + quad) * 8;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        x[e] = T(0.f);
+                        if (live >> (is_v ? slot + e : slot) & 1) x[e] = src[e];
+                    }
+                    memcpy(&raw[i], x, sizeof raw[i]);
                 }
             }
-        };
-        load(0);
-        for (int t = 0; t < tiles && ok; t++) {
-            const int b = t & 1;
-            if (is_v) {
-                const uint64_t live = live_of(t);
-                if (live != ~0ull) {
+            float x[ITS][8], top = 0.f;
+            if (live == ~0ull) {
 #pragma unroll
-                    for (int i = 0; i < C::ITS; i++) sv_keep(raw[i], (uint32_t)(live >> (8 * (quad + 4 * (i & 1)))) & 0xffu);
+                for (int i = 0; i < ITS; i++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[i][e] = sv_at(raw[i], e);
+            } else { // what a slot that is not live holds, or was not copied, may be anything
+#pragma unroll
+                for (int i = 0; i < ITS; i++) {
+                    const uint32_t m = is_v ? (uint32_t)(live >> (8 * (quad + 4 * (i & 1)))) : live >> (w * 8 + sub) & 1 ? 0xffu : 0u;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[i][e] = m >> e & 1 ? sv_at(raw[i], e) : 0.f;
                 }
             }
-            uint32_t mx = 0;
 #pragma unroll
-            for (int i = 0; i < C::ITS; i++)
+            for (int i = 0; i < ITS; i++)
 #pragma unroll
-                for (int e = 0; e < 8; e++) mx = max(mx, __float_as_uint(sv_at(raw[i], e)) & 0x7fffffffu);
-            mx = __reduce_max_sync(0xffffffffu, mx);
+                for (int e = 0; e < 8; e += 2) top = fmaxf(fmaxf(top, fabsf(x[i][e])), fabsf(x[i][e + 1]));
             float inv;
-            const float f = sv_scale(mx, inv);
-            if (t >= 2) sv_bar_wait(&empty[b], ((t >> 1) - 1) & 1, ok, a.err, 11);
-            if (!ok) break;
-            uint8_t *to = sm + b * C::STAGE;
+            const float f = sv_scale(__reduce_max_sync(0xffffffffu, __float_as_uint(top)), inv); // (and all lanes have read)
+            uint8_t *to = group + sub * 16 + quad * 128;
+            const int lo_at = is_v ? C::V_LO : C::K_LO;
 #pragma unroll
-            for (int i = 0; i < C::ITS; i++) {
+            for (int i = 0; i < ITS; i++) {
                 uint4 hi, lo;
-                sv_cut(sv_at(raw[i], 0) * f, sv_at(raw[i], 1) * f, hi.x, lo.x);
-                sv_cut(sv_at(raw[i], 2) * f, sv_at(raw[i], 3) * f, hi.y, lo.y);
-                sv_cut(sv_at(raw[i], 4) * f, sv_at(raw[i], 5) * f, hi.z, lo.z);
-                sv_cut(sv_at(raw[i], 6) * f, sv_at(raw[i], 7) * f, hi.w, lo.w);
-                const int at = is_v ? (quad + 4 * (i & 1)) * (D * 16) + (w * (D / 4) + (i >> 1) * 8 + sub) * 16
-                                    : ((i % (D / 32)) * 4 + quad) * (SV_TILE * 16) + (w * 16 + (i / (D / 32)) * 8 + sub) * 16;
-                *reinterpret_cast<uint4 *>(to + at) = hi;
-                if (C::F32) *reinterpret_cast<uint4 *>(to + C::KPART + at) = lo;
+                sv_cut(x[i][0] * f, x[i][1] * f, hi.x, lo.x);
+                sv_cut(x[i][2] * f, x[i][3] * f, hi.y, lo.y);
+                sv_cut(x[i][4] * f, x[i][5] * f, hi.z, lo.z);
+                sv_cut(x[i][6] * f, x[i][7] * f, hi.w, lo.w);
+                uint8_t *p = to + (is_v ? (i >> 1) * 8 * C::V_ROW + (i & 1) * 512 : i * 512);
+                *reinterpret_cast<uint4 *>(p) = hi;
+                if (C::F32) *reinterpret_cast<uint4 *>(p + lo_at) = lo;
             }
-            if (lane == 0) (is_v ? s_vinv : s_kinv)[b][w] = inv;
+            if (lane == 0) (is_v ? s_vinv : s_kinv)[t & 7][w] = inv; // (who reads tile t - 8's is done: the ring's stages span three tiles, and what comes after MMAs two more)
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) ps_mbar_arrive(&full[b]);
-            if (t + 1 < tiles) load(t + 1);
-        }
-    } else if (warp == 20) {
-        // ===== MMAs.  Small products first, while the truncating accumulator is small
-        const uint32_t idesc_s = (1u << 4) | ((uint32_t)(SV_TILE >> 3) << 17) | ((uint32_t)(SV_TC_ROWS >> 4) << 24);
-        const uint32_t idesc_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(SV_TC_ROWS >> 4) << 24);
-        const uint64_t dq = ps_tc_smem_desc(ps_smem_u32(sm_q), SV_TC_ROWS * 16, 128), dk = ps_tc_smem_desc(ps_smem_u32(sm_k), SV_TILE * 16, 128), dv = ps_tc_smem_desc(ps_smem_u32(sm_v), D * 16, 128);
-        auto scores = [&](int t) {
-            const int b = t & 1;
-            sv_bar_wait(&full_k[b], (t >> 1) & 1, ok, a.err, 12);
-            if (t >= 2) sv_bar_wait(&s_empty[b], ((t >> 1) - 1) & 1, ok, a.err, 13);
-            if (!ok) return;
-            ps_tc_fence_after();
-            if (ps_elect_one()) {
-                const uint64_t kb = dk + (uint64_t)(b * (C::STAGE >> 4));
-                const uint32_t to = tm_s + b * SV_TILE;
-#pragma unroll
-                for (int p = 0; p < C::PARTS + 1; p++) // lo hi, hi lo, hi hi (bfloat16 caches: lo hi, hi hi)
-#pragma unroll
-                    for (int j = 0; j < D / 16; j++)
-                        ps_tc_mma_f16(to, dq + (p == 0 ? (C::Q / 2) >> 4 : 0) + j * ((2 * SV_TC_ROWS * 16) >> 4), kb + (C::F32 && p == 1 ? C::KPART >> 4 : 0) + j * ((2 * SV_TILE * 16) >> 4), idesc_s, (p | j) != 0);
-                ps_tc_commit(&s_full[b]);
-            }
-            __syncwarp();
+            if (lane == 0) ps_mbar_arrive(&ready[st]);
+            step();
+            return true;
         };
-        if (tiles > 0) scores(0);
-        for (int t = 0; t < tiles && ok; t++) {
-            const int b = t & 1;
-            if (t + 1 < tiles) scores(t + 1);
-            sv_bar_wait(&full_v[b], (t >> 1) & 1, ok, a.err, 14);
-            sv_bar_wait(&p_full[b], (t >> 1) & 1, ok, a.err, 15); // (the soft-max has waited for the output of tile t - 2)
-            if (!ok) break;
-            ps_tc_fence_after();
-            if (ps_elect_one()) {
-                const uint64_t vb = dv + (uint64_t)(b * (C::STAGE >> 4));
-                const uint32_t to = tm_o + b * D, pa = tm_p + b * SV_TILE;
-#pragma unroll
-                for (int p = 0; p < C::PARTS + 1; p++)
-#pragma unroll
-                    for (int j = 0; j < SV_TILE / 16; j++)
-                        ps_tc_mma_f16_ta(to, pa + (p == 0 ? SV_TILE / 2 : 0) + j * 8, vb + (C::F32 && p == 1 ? C::KPART >> 4 : 0) + j * ((2 * D * 16) >> 4), idesc_o, (p | j) != 0);
-                ps_tc_commit(&o_full[b]);
-            }
-            __syncwarp();
-        }
-        if (ps_elect_one()) ps_tc_commit(&done); // MMAs in flight end before the tensor memory is given back
-        __syncwarp();
-        if (!ps_tc_wait_warp(&done, 0)) *a.err = 16;
-    } else if (warp < 4) {
-        // ===== soft-max: thread = row
-        const int r = warp * 32 + lane, row = r0 + r;
-        const bool mine = r < rows, any = warp * 32 < rows; // (any: of the warp)
-        const uint32_t lane_at = (uint32_t)(warp * 32) << 16;
+        bool fine = convert(false, 0);
+        for (int i = 0; i < 2 * tiles && fine; i++) // K of the next tile, V of this one
+            if (i & 1 || i / 2 + 1 < tiles) fine = convert(i & 1, i / 2 + 1 - (i & 1));
+    } else if (warp < 8) {
+        // ===== soft-max of every other tile: thread = row
+        const int r = (warp & 3) * 32 + lane, row = r0 + r, tok = row / a.R, rp = sv_rp(all_rows);
+        const bool mine = r < rows, any = (warp & 3) * 32 < rows; // (any: of the warp)
+        const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
         const float qinv = mine ? s_qinv[r] : 0.f;
-        const int tok = row / a.R;
-        const int rp = sv_rp(all_rows);
-        float m = SV_NONE, l = 0.f;
-        for (int t = 0; t < tiles && ok; t++) {
+        bool ok = true;
+        for (int t = warp >> 2; t < tiles; t += 2) {
             const int b = t & 1, j = j0 + t * SV_TILE;
             uint64_t see = live_of(t);
-            if (j + SV_TILE > past && any) { // of the step's own slots those that this token sees
+            if (j + SV_TILE > past && mine) // of the step's own slots those that this token sees
                 for (int c = max(0, past - j); c < min(SV_TILE, j_end - j); c++)
-                    if (mine && !sv_sees(s, tok, j + c - past)) see &= ~(1ull << c);
-            }
-            sv_bar_wait(&full_k[b], (t >> 1) & 1, ok, a.err, 17); // (the groups' factors)
+                    if (!sv_sees(s, tok, j + c - past)) see &= ~(1ull << c);
+            const bool whole = __all_sync(0xffffffffu, see == ~0ull);
             sv_bar_wait(&s_full[b], (t >> 1) & 1, ok, a.err, 18);
             if (!ok) break;
             ps_tc_fence_after();
-            __syncwarp();
-            uint32_t v[SV_TILE];
-            if (any) {
-#pragma unroll
-                for (int c = 0; c < SV_TILE; c += 32)
-                    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                                 : "=r"(v[c]), "=r"(v[c + 1]), "=r"(v[c + 2]), "=r"(v[c + 3]), "=r"(v[c + 4]), "=r"(v[c + 5]), "=r"(v[c + 6]), "=r"(v[c + 7]), "=r"(v[c + 8]), "=r"(v[c + 9]),
-                                   "=r"(v[c + 10]), "=r"(v[c + 11]), "=r"(v[c + 12]), "=r"(v[c + 13]), "=r"(v[c + 14]), "=r"(v[c + 15]), "=r"(v[c + 16]), "=r"(v[c + 17]), "=r"(v[c + 18]),
-                                   "=r"(v[c + 19]), "=r"(v[c + 20]), "=r"(v[c + 21]), "=r"(v[c + 22]), "=r"(v[c + 23]), "=r"(v[c + 24]), "=r"(v[c + 25]), "=r"(v[c + 26]), "=r"(v[c + 27]),
-                                   "=r"(v[c + 28]), "=r"(v[c + 29]), "=r"(v[c + 30]), "=r"(v[c + 31])
-                                 : "r"(tm_s + b * SV_TILE + c + lane_at)
-                                 : "memory");
-                ps_tc_ld_wait();
-            }
-            float f[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++) f[k] = qinv * s_kinv[b][k];
-            ps_tc_fence_before();
-            __syncwarp();
-            if (lane == 0) ps_mbar_arrive(&s_empty[b]);
+            // sixteen slots at a time, twice (loops, not copies: the code of all roles has to fit the instruction caches)
             float mx = SV_NONE;
-            if (any) {
-                const bool whole = __all_sync(0xffffffffu, see == ~0ull);
+            if (any)
+#pragma unroll 1
+                for (int k = 0; k < 4; k++) {
+                    uint32_t v[16];
+                    sv_tm_ld16(v, tm_s + b * SV_TILE + 16 * k + lane_at);
+                    const float2 ki = *reinterpret_cast<const float2 *>(&s_kinv[t & 7][2 * k]);
+                    const float f0 = fmaxf(qinv * ki.x, 0x1p-126f), f1 = fmaxf(qinv * ki.y, 0x1p-126f); // (never zero: -inf times it is -inf)
+                    ps_tc_ld_wait();
+                    if (!whole) {
+                        const uint32_t bits = (uint32_t)(see >> (16 * k));
 #pragma unroll
-                for (int c = 0; c < SV_TILE; c++) {
-                    float z = __uint_as_float(v[c]) * f[c / 16];
-                    if (!whole) z = see >> c & 1 ? z : SV_NONE;
-                    v[c] = __float_as_uint(z);
-                    mx = fmaxf(mx, z);
-                }
-                if (s.scores && mine) {
-                    float *to = s.scores + ((int64_t)g * s.n_kv + j) * rp + row;
-                    const int n = min(SV_TILE, j_end - j);
+                        for (int c = 0; c < 16; c++)
+                            if (!(bits >> c & 1)) v[c] = __float_as_uint(SV_NONE);
+                    }
+                    float t0 = SV_NONE, t1 = SV_NONE;
 #pragma unroll
-                    for (int c = 0; c < SV_TILE; c++)
-                        if (c < n) to[(int64_t)c * rp] = __uint_as_float(v[c]);
+                    for (int c = 0; c < 8; c += 2) {
+                        t0 = fmaxf(fmaxf(t0, __uint_as_float(v[c])), __uint_as_float(v[c + 1]));
+                        t1 = fmaxf(fmaxf(t1, __uint_as_float(v[c + 8])), __uint_as_float(v[c + 9]));
+                    }
+                    mx = fmaxf(fmaxf(mx, t0 * f0), t1 * f1);
+                    if (s.scores && mine) {
+                        float4 *to = reinterpret_cast<float4 *>(s.scores) + ((int64_t)g * sv_quads(s.n_kv) + j / 4 + 4 * k) * rp + row;
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            const float f = c < 2 ? f0 : f1;
+                            to[(int64_t)c * rp] = make_float4(__uint_as_float(v[4 * c]) * f, __uint_as_float(v[4 * c + 1]) * f, __uint_as_float(v[4 * c + 2]) * f, __uint_as_float(v[4 * c + 3]) * f);
+                        }
+                    }
+                    __syncwarp();
                 }
-            }
-            const float mn = fmaxf(m, mx), ref = mn == SV_NONE ? 0.f : mn, alpha = sv_ex2(m - ref);
-            m = mn;
-            if (t >= 2) sv_bar_wait(&o_empty[b], ((t >> 1) - 1) & 1, ok, a.err, 19); // (its weights are used up, and its factors)
+            if (t >= 2) sv_bar_wait(&o_empty[b], ((t >> 1) - 1) & 1, ok, a.err, 19); // (tile t - 2's weights are used up, and its maximum and sum)
             if (!ok) break;
-            s_alpha[b][r] = alpha;
-            __syncwarp();
+            // the weights are 2^15 p, and so is their sum
+            const float shift = mx == SV_NONE ? 15.f : 15.f - mx;
+            float sum = 0.f, sum1 = 0.f;
             if (any) {
-                float sum = 0.f;
+#pragma unroll 1
+                for (int k = 0; k < 4; k++) {
+                    uint32_t v[16], hi[8], lo[8];
+                    sv_tm_ld16(v, tm_s + b * SV_TILE + 16 * k + lane_at);
+                    const float2 ki = *reinterpret_cast<const float2 *>(&s_kinv[t & 7][2 * k]);
+                    const float f0 = fmaxf(qinv * ki.x, 0x1p-126f), f1 = fmaxf(qinv * ki.y, 0x1p-126f);
+                    ps_tc_ld_wait();
+                    if (!whole) {
+                        const uint32_t bits = (uint32_t)(see >> (16 * k));
 #pragma unroll
-                for (int c = 0; c < SV_TILE; c += 16) {
-                    uint32_t hi[8], lo[8];
+                        for (int c = 0; c < 16; c++)
+                            if (!(bits >> c & 1)) v[c] = __float_as_uint(SV_NONE);
+                    }
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        const float p0 = sv_ex2(__uint_as_float(v[c + 2 * e]) - ref), p1 = sv_ex2(__uint_as_float(v[c + 2 * e + 1]) - ref);
-                        sum += p0 + p1;
-                        sv_cut(p0 * 32768.f, p1 * 32768.f, hi[e], lo[e]);
+                        const float f = e < 4 ? f0 : f1;
+                        const float p0 = sv_ex2(fmaf(__uint_as_float(v[2 * e]), f, shift)), p1 = sv_ex2(fmaf(__uint_as_float(v[2 * e + 1]), f, shift));
+                        sum += p0;
+                        sum1 += p1;
+                        sv_cut(p0, p1, hi[e], lo[e]);
                     }
-                    const uint32_t to = tm_p + b * SV_TILE + c / 2 + lane_at;
-                    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(to), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]), "r"(hi[4]), "r"(hi[5]), "r"(hi[6]),
-                                 "r"(hi[7]) : "memory");
-                    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(to + SV_TILE / 2), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]), "r"(lo[4]), "r"(lo[5]),
-                                 "r"(lo[6]), "r"(lo[7]) : "memory");
+                    sv_tm_st8(tm_p + b * SV_TILE + 8 * k + lane_at, hi);
+                    sv_tm_st8(tm_p + b * SV_TILE + SV_TILE / 2 + 8 * k + lane_at, lo);
                 }
-                l = fmaf(l, alpha, sum);
+                s_top[b][r] = mx;
+                s_sum[b][r] = sum + sum1;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             }
             ps_tc_fence_before();
             __syncwarp();
             if (lane == 0) ps_mbar_arrive(&p_full[b]);
         }
-        if (mine) {
-            s_sum[r] = l;
-            reinterpret_cast<float2 *>(s.part + (int64_t)s.splits * a.G * all_rows * D)[((int64_t)split * a.G + g) * all_rows + row] = make_float2(m, l);
-        }
-    }
-    float acc[D / 2];
-    if (warp >= 4 && warp < 12) {
-        // ===== output: thread = row, half of the channels
-        const int half = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
+    } else {
+        // ===== output: thread = row, half of the channels; the row's maximum and sum so far
+        sv_regs_more<88>();
+        const int half = (warp - 8) >> 2, r = (warp & 3) * 32 + lane, row = r0 + r;
         const bool any = (warp & 3) * 32 < rows;
         const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
+        float acc[D / 2], m = SV_NONE, l = 0.f;
+        bool ok = true;
 #pragma unroll
         for (int c = 0; c < D / 2; c++) acc[c] = 0.f;
-        for (int t = 0; t < tiles && ok; t++) {
+        for (int t = 0; t < tiles; t++) {
             const int b = t & 1;
-            sv_bar_wait(&full_v[b], (t >> 1) & 1, ok, a.err, 20);
-            sv_bar_wait(&p_full[b], (t >> 1) & 1, ok, a.err, 21);
             sv_bar_wait(&o_full[b], (t >> 1) & 1, ok, a.err, 22);
             if (!ok) break;
             ps_tc_fence_after();
             if (any) {
-                const float alpha = s_alpha[b][r];
-                const float f[2] = {s_vinv[b][half * 2], s_vinv[b][half * 2 + 1]};
+                const float top = s_top[b][r], mn = fmaxf(m, top), ref = mn == SV_NONE ? 0.f : mn, fo = sv_ex2(m - ref), fn = sv_ex2(top - ref);
+                const float4 vi = *reinterpret_cast<const float4 *>(&s_vinv[t & 7][4 * half]);
+                const float f[4] = {fn * vi.x, fn * vi.y, fn * vi.z, fn * vi.w};
+                l = fmaf(l, fo, s_sum[b][r] * fn);
+                m = mn;
+                if (__any_sync(0xffffffffu, fo != 1.f)) {
+#pragma unroll
+                    for (int c = 0; c < D / 2; c++) acc[c] *= fo;
+                }
 #pragma unroll
                 for (int c = 0; c < D / 2; c += 16) {
                     uint32_t v[16];
-                    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
-                                   "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-                                 : "r"(tm_o + b * D + half * (D / 2) + c + lane_at)
-                                 : "memory");
+                    sv_tm_ld16(v, tm_o + b * D + half * (D / 2) + c + lane_at);
                     ps_tc_ld_wait();
 #pragma unroll
-                    for (int e = 0; e < 16; e++) acc[c + e] = fmaf(acc[c + e], alpha, __uint_as_float(v[e]) * f[(c + e) / (D / 4)]);
+                    for (int e = 0; e < 16; e++) acc[c + e] = fmaf(__uint_as_float(v[e]), f[(c + e) / (D / 8)], acc[c + e]);
                 }
             }
             ps_tc_fence_before();
             __syncwarp();
             if (lane == 0) ps_mbar_arrive(&o_empty[b]);
         }
-    }
-    ps_tc_fence_before();
-    __syncthreads();
-    if (warp == 20) {
-        ps_tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm) : "memory");
-    }
-    if (warp >= 4 && warp < 12) {
-        const int half = (warp - 4) >> 2, r = (warp & 3) * 32 + lane, row = r0 + r;
         if (r < rows) {
-            const float l = s_sum[r], f = (s.splits == 1 ? (l > 0.f ? 1.f / l : 0.f) : 1.f) * (1.f / 32768.f);
+            if (half == 0) reinterpret_cast<float2 *>(s.part + (int64_t)s.splits * a.G * all_rows * D)[((int64_t)split * a.G + g) * all_rows + row] = make_float2(m, l * (1.f / 32768.f));
+            const float f = s.splits == 1 ? (l > 0.f ? 1.f / l : 0.f) : 1.f / 32768.f;
             float *to = s.splits == 1 ? a.out + ((int64_t)(s.tok0 + row / a.R) * a.n_heads + g * a.R + row % a.R) * D : s.part + (((int64_t)split * a.G + g) * all_rows + row) * D;
             to += half * (D / 2);
             if (a.out_vec || s.splits > 1) {
@@ -438,5 +471,11 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
                 for (int c = 0; c < D / 2; c++) to[c] = acc[c] * f;
             }
         }
+    }
+    ps_tc_fence_before();
+    __syncthreads();
+    if (warp == 24) {
+        ps_tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm) : "memory");
     }
 }
