@@ -106,6 +106,7 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
         const bool tc = hs == 64 || hs == 128;
         const int tile_rows = tc ? SV_TC_ROWS : 16, row_tiles = (most_tok * R + tile_rows - 1) / tile_rows;
         a.out_vec = aligned(out, 16);
+        a.q_vec = aligned(q, 16);
         if (most_tok) {
             a.tps = split_tiles(caches + first, n, n_kv_heads * row_tiles, tc ? c->n_sm : c->n_sm * 4, 1);
             if (tc) a.tps = std::min(a.tps, SV_TC_TILES);
@@ -143,17 +144,14 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
             }
             const dim3 grid(units, n_kv_heads, row_tiles);
             if (tc) {
-                const int most_rows = most_tok * R;
-                auto launch = [&](auto kern, auto shape) -> int {
-                    using C = decltype(shape);
-                    const int stages = C::stages(most_rows, 220 * 1024), smem = C::smem(most_rows, stages); // (7 KB for what the kernel declares)
+                auto launch = [&](auto kern, int smem) -> int {
                     SV_CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-                    kern<<<grid, SV_TC_THREADS, smem, c->stream>>>(a, stages, C::q_bytes(most_rows));
+                    kern<<<grid, SV_TC_THREADS, smem, c->stream>>>(a);
                     return 0;
                 };
                 const bool f32 = cache_type == PS_TYPE_F32;
-                const int rc = hs == 64 ? (f32 ? launch(sv_k_attn_tc<float, 64>, SvTc<float, 64>()) : launch(sv_k_attn_tc<__nv_bfloat16, 64>, SvTc<__nv_bfloat16, 64>()))
-                                        : (f32 ? launch(sv_k_attn_tc<float, 128>, SvTc<float, 128>()) : launch(sv_k_attn_tc<__nv_bfloat16, 128>, SvTc<__nv_bfloat16, 128>()));
+                const int rc = hs == 64 ? (f32 ? launch(sv_k_attn_tc<float, 64>, SvTc<float, 64>::SMEM) : launch(sv_k_attn_tc<__nv_bfloat16, 64>, SvTc<__nv_bfloat16, 64>::SMEM))
+                                        : (f32 ? launch(sv_k_attn_tc<float, 128>, SvTc<float, 128>::SMEM) : launch(sv_k_attn_tc<__nv_bfloat16, 128>, SvTc<__nv_bfloat16, 128>::SMEM));
                 if (rc) return rc;
             } else if (cache_type == PS_TYPE_F32) {
                 const size_t smem = sv_attn_smem(hs);

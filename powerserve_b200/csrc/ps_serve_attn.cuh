@@ -31,7 +31,7 @@ struct SvAttn {
     const float *q;
     float *out;
     int n_seqs, hs, n_heads, G, R, tps; // R: heads that share a kv head; tps: tiles of a split
-    int out_vec;                        // out is aligned to 16 bytes
+    int q_vec, out_vec;                 // aligned to 16 bytes
     float scale;                        // times log2 e
     int *err;
 };

@@ -4,11 +4,12 @@
 // group fits fp16's range from the top: what is lost is below 2^-22 of x, or 2^-39 of the group's largest.  Three MMAs (lo hi, hi lo, hi hi) replace the
 // 32-bit products; the missing lo lo is below 2^-22 of the product.  bfloat16 caches have no lo part: two MMAs.  Groups: a query row; eight slots' K rows;
 // hs / 8 channels of a tile of V.  The weights p of the soft-max, at most 1, are cut after a factor 2^15.
+// The queries' parts stay in tensor memory (in shared memory they took the room of two stages).
 // A tile's output leaves the tensor memory after every tile and is added up in registers, with rounding: the accumulator, which truncates, sees the
 // MMAs of one tile alone.  So groups' factors and a row's maximum may differ from tile to tile, and the soft-max of a tile knows of no other tile.
 //
 // A CTA takes up to 128 query rows (the MMAs' M side: one row, one lane of tensor memory) of one kv head over one split.  Warps 0-3 and 4-7: soft-max of
-// the even and of the odd tiles; 8-15: output, a row's channels in two halves; 16-23: converters; 24: MMAs; 25-27: copies.
+// the even and of the odd tiles; 8-15: output, a row's channels in two halves; 16-23: converters; 24, 25: MMAs; 26, 27: copies.
 // Tiles of K and of V go through one ring of shared-memory stages: asynchronous 16-byte copies bring a stage as it lies in memory (bulk copies of rows of 256 and
 // 512 bytes took 65 cycles each, 12 400 a tile), the converters cut it
 // into parts in its place (eight rows, read by one warp, become the same eight rows' parts in the K-major no-swizzle layout, in the same bytes),
@@ -83,25 +84,22 @@ template <typename T, int D> struct SvTc {
     static constexpr int K_ROW = D * (int)sizeof(T) + 16, V_ROW = SV_TILE * (int)sizeof(T) + 16; // bytes from row to row of a stage
     static constexpr int K_LO = D * 16, V_LO = SV_TILE * 16;                                     // from a group's hi part to its lo part
     static constexpr int STAGE = (SV_TILE * K_ROW > D * V_ROW ? SV_TILE * K_ROW : D * V_ROW);
-    static constexpr int Q_GROUP = D * 32;                                                       // both parts of eight query rows
     static constexpr int V_GROUPS = D / 64;                                                      // groups of eight channels that a converter takes
     using Raw = typename std::conditional<F32, SvRaw32, SvRaw16>::type;
-    static int q_bytes(int rows) { return (std::min(rows, SV_TC_ROWS) + 7) / 8 * Q_GROUP; }
-    // stages beside the queries; the MMAs read 128 query rows whatever there are, and what follows them in shared memory is read for rows that nobody looks at
-    static int stages(int rows, int smem) { return std::min(SV_TC_STAGES, (smem - 128 - q_bytes(rows)) / STAGE); }
-    static int smem(int rows, int n) { return std::max(q_bytes(rows) + n * STAGE, SV_TC_ROWS / 8 * Q_GROUP) + 128; }
+    static constexpr int SMEM = SV_TC_STAGES * STAGE + 128;
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_constant__ SvAttn a, int stages, int q_bytes) {
+__global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_constant__ SvAttn a) {
     using C = SvTc<T, D>;
     extern __shared__ __align__(128) uint8_t sv_tc_raw[];
     __shared__ __align__(8) uint64_t raw_full[SV_TC_STAGES], ready[SV_TC_STAGES], unused[SV_TC_STAGES], s_full[2], p_full[2], o_full[2], o_empty[2], done;
     __shared__ uint32_t tmem_smem;
-    __shared__ float s_top[2][SV_TC_ROWS], s_sum[2][SV_TC_ROWS], s_qinv[SV_TC_ROWS];
+    __shared__ float s_top[2][SV_TC_ROWS], s_sum[2][SV_TC_ROWS], s_qtop[2][SV_TC_ROWS];
     __shared__ __align__(16) float s_kinv[8][8], s_vinv[8][8];
     __shared__ uint64_t s_live[SV_TC_TILES];
-    uint8_t *sm_q = reinterpret_cast<uint8_t *>(((uintptr_t)sv_tc_raw + 127) & ~(uintptr_t)127), *sm_ring = sm_q + q_bytes;
+    uint8_t *sm_ring = reinterpret_cast<uint8_t *>(((uintptr_t)sv_tc_raw + 127) & ~(uintptr_t)127);
+    constexpr int stages = SV_TC_STAGES;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int si = __shfl_sync(0xffffffffu, sv_find(a, blockIdx.x), 0), split = blockIdx.x - a.seq[si].unit0, g = blockIdx.y;
     const SvSeq &s = a.seq[si];
@@ -116,7 +114,7 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
         if (++st == stages) { st = 0; round ^= 1; }
     };
     int put_n = 0;
-    auto put = [&](bool is_v, int t) -> bool { // by each of the three warps, its share of the rows
+    auto put = [&](bool is_v, int t) -> bool { // by both warps, each its share of the rows
         if (put_n >= stages && !ps_tc_wait_warp(&unused[st], round ^ 1)) { *a.err = 11; return false; }
         const int j = j0 + t * SV_TILE;
         if (is_v ? s.v_mode : s.k_mode) {
@@ -128,7 +126,7 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
             const uint32_t to = ps_smem_u32(sm_ring + st * C::STAGE) + in_row;
             if (in_row < last)
 #pragma unroll 4
-                for (int i = (warp - 25) * rows_at_once + lane / lanes; i < count; i += 3 * rows_at_once)
+                for (int i = (warp - 26) * rows_at_once + lane / lanes; i < count; i += 2 * rows_at_once)
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * step_rows), "l"(src + i * ld + in_row) : "memory");
             asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ps_smem_u32(&raw_full[st])) : "memory");
         } else ps_mbar_arrive(&raw_full[st]);
@@ -138,14 +136,14 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
         return true;
     };
     int put_t = 0;          // next of the pairs (K of t + 1, V of t); the first K is put alone
-    if (warp >= 25) {
-        if (tid == 25 * 32) {
-            for (int b = 0; b < SV_TC_STAGES; b++) { ps_mbar_init(&raw_full[b], 96); ps_mbar_init(&ready[b], 8); ps_mbar_init(&unused[b], 1); }
+    if (warp >= 26) {
+        if (tid == 26 * 32) {
+            for (int b = 0; b < SV_TC_STAGES; b++) { ps_mbar_init(&raw_full[b], 64); ps_mbar_init(&ready[b], 8); ps_mbar_init(&unused[b], 1); }
             for (int b = 0; b < 2; b++) { ps_mbar_init(&s_full[b], 1); ps_mbar_init(&p_full[b], 4); ps_mbar_init(&o_full[b], 1); ps_mbar_init(&o_empty[b], 8); }
-            ps_mbar_init(&done, 1);
+            ps_mbar_init(&done, 2);
             ps_fence_barrier_init();
         }
-        ps_bar_sync(1, 96);
+        ps_bar_sync(1, 64);
         put(false, 0);      // (the ring is empty: these do not wait)
         while (put_t < tiles && put_n + 2 <= stages) {
             if (put_t + 1 < tiles) put(false, put_t + 1);
@@ -168,44 +166,57 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
         const int n = j_end - j0 - t * SV_TILE;
         return n >= SV_TILE ? ~0ull : (1ull << n) - 1;
     };
-    // queries: a half-warp (quarter-warp for head size 64) per row
-    if (warp < 24)
-        for (int i = tid; i < rows * (D / 8); i += 768) { // (rows * D / 8 and 768 are multiples of D / 8: the lanes of a row are there together)
-            const int r = i / (D / 8), c = i % (D / 8), row = r0 + r;
-            const float *q = a.q + ((int64_t)(s.tok0 + row / a.R) * a.n_heads + g * a.R + row % a.R) * D + c * 8;
-            const unsigned mates = (D == 128 ? 0xffffu : 0xffu) << (lane & (D == 128 ? 16 : 24));
-            float x[8], inv;
-            uint32_t mx = 0;
+    // queries: warps 0-3 the first half of the channels, 4-7 the second, a thread its half of a row
+    float4 qv[D / 8];
+    if (warp < 8) {
+        const int r = (warp & 3) * 32 + lane, row = r0 + r;
+        const float *q = a.q + ((int64_t)(s.tok0 + row / a.R) * a.n_heads + g * a.R + row % a.R) * D + (warp >> 2) * (D / 2);
+        float top = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                x[e] = q[e] * a.scale;
-                mx = max(mx, __float_as_uint(x[e]) & 0x7fffffffu);
+        for (int i = 0; i < D / 8; i++) {
+            qv[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < rows) {
+                if (a.q_vec) qv[i] = __ldg(reinterpret_cast<const float4 *>(q) + i);
+                else qv[i] = make_float4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
             }
-#pragma unroll
-            for (int o = D / 16; o; o >>= 1) mx = max(mx, __shfl_xor_sync(mates, mx, o));
-            const float f = sv_scale(mx, inv);
-            uint4 hi, lo;
-            sv_cut(x[0] * f, x[1] * f, hi.x, lo.x);
-            sv_cut(x[2] * f, x[3] * f, hi.y, lo.y);
-            sv_cut(x[4] * f, x[5] * f, hi.z, lo.z);
-            sv_cut(x[6] * f, x[7] * f, hi.w, lo.w);
-            uint8_t *to = sm_q + (r >> 3) * C::Q_GROUP + c * 128 + (r & 7) * 16;
-            *reinterpret_cast<uint4 *>(to) = hi;
-            *reinterpret_cast<uint4 *>(to + D * 16) = lo;
-            if (c == 0) s_qinv[r] = inv;
+            qv[i].x *= a.scale; qv[i].y *= a.scale; qv[i].z *= a.scale; qv[i].w *= a.scale;
+            top = fmaxf(fmaxf(fmaxf(top, fabsf(qv[i].x)), fabsf(qv[i].y)), fmaxf(fabsf(qv[i].z), fabsf(qv[i].w)));
         }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        s_qtop[warp >> 2][r] = top;
+    }
     ps_tc_fence_before();
     __syncthreads();
     ps_tc_fence_after();
-    const uint32_t tm = __shfl_sync(0xffffffffu, tmem_smem, 0), tm_s = tm, tm_p = tm + 2 * SV_TILE, tm_o = tm + 4 * SV_TILE; // columns: scores 2 x 64, weights 2 x (32 + 32), outputs 2 x D
+    // columns of tensor memory: scores 2 x 64, weights 2 x (32 + 32), output D, queries D / 2 + D / 2
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem_smem, 0), tm_s = tm, tm_p = tm + 2 * SV_TILE, tm_o = tm + 4 * SV_TILE, tm_q = tm_o + D;
+    float qinv = 1.f;
+    if (warp < 8) {
+        const int r = (warp & 3) * 32 + lane;
+        const float f = sv_scale(__float_as_uint(fmaxf(s_qtop[0][r], s_qtop[1][r])), qinv);
+#pragma unroll
+        for (int i = 0; i < D / 8; i += 4) {
+            uint32_t hi[8], lo[8];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                sv_cut(qv[i + e].x * f, qv[i + e].y * f, hi[2 * e], lo[2 * e]);
+                sv_cut(qv[i + e].z * f, qv[i + e].w * f, hi[2 * e + 1], lo[2 * e + 1]);
+            }
+            const uint32_t to = tm_q + (warp >> 2) * (D / 4) + 2 * i + ((uint32_t)((warp & 3) * 32) << 16);
+            sv_tm_st8(to, hi);
+            sv_tm_st8(to + D / 2, lo);
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+    }
+    ps_tc_fence_before();
+    __syncthreads();
+    ps_tc_fence_after();
     // A barrier is waited on only by who must have passed it before it can complete again (a phase that was missed would never end): groups' and rows' factors
     // come with the MMAs' barrier, whose issuer has waited for those who wrote them.
     // Registers: 72 a thread at the launch, 504 over the seven warpgroups; 2 x 72 (soft-max) + 2 x 88 (output) + 2 x 72 (converters) + 40 (MMAs, copies) = 504
 
     if (warp >= 24) {
         sv_regs_less<40>();
-        if (warp >= 25) {
+        if (warp >= 26) {
             bool fine = true;
             for (; put_t < tiles && fine; put_t++) {
                 if (put_t + 1 < tiles) fine = put(false, put_t + 1);
@@ -213,47 +224,40 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
             }
             asm volatile("cp.async.wait_all;" ::: "memory"); // (what is in flight ends before the CTA does, even when a wait gave up)
         } else {
-            // ===== MMAs.  Small products first, while the truncating accumulator is small
-            const uint32_t idesc_s = (1u << 4) | ((uint32_t)(SV_TILE >> 3) << 17) | ((uint32_t)(SV_TC_ROWS >> 4) << 24);
-            const uint32_t idesc_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(SV_TC_ROWS >> 4) << 24);
-            const uint64_t dq = ps_tc_smem_desc(ps_smem_u32(sm_q), 128, C::Q_GROUP), dk = ps_tc_smem_desc(ps_smem_u32(sm_ring), 128, 8 * C::K_ROW), dv = ps_tc_smem_desc(ps_smem_u32(sm_ring), 128, 8 * C::V_ROW);
-            auto scores = [&](int t) -> bool { // (the soft-max of tile t - 2 is done with these scores: its weights have been waited for)
-                if (!ps_tc_wait_warp(&ready[st], round)) { *a.err = 12; return false; }
+            // ===== MMAs, scores by warp 24, outputs by warp 25: neither's waits hold up the other's.  Small products first, while the truncating accumulator is small
+            const bool pv = warp == 25;
+            const uint32_t idesc = (1u << 4) | ((uint32_t)((pv ? D : SV_TILE) >> 3) << 17) | ((uint32_t)(SV_TC_ROWS >> 4) << 24);
+            const uint64_t desc = ps_tc_smem_desc(ps_smem_u32(sm_ring), 128, 8 * (pv ? C::V_ROW : C::K_ROW));
+            int item = pv ? min(2, 2 * tiles - 1) : 0; // number of the tile's K or V among what goes through the ring
+            for (int t = 0; t < tiles; t++) {
+                const int b = t & 1, at = item % stages;
+                if (!ps_tc_wait_warp(&ready[at], (item / stages) & 1)) { *a.err = 12; break; }
+                if (pv) { // (there is one output: the tile before has to be out of it)
+                    if (!ps_tc_wait_warp(&p_full[b], (t >> 1) & 1)) { *a.err = 15; break; }
+                    if (t && !ps_tc_wait_warp(&o_empty[b ^ 1], ((t - 1) >> 1) & 1)) { *a.err = 13; break; }
+                } else if (t >= 2 && !ps_tc_wait_warp(&p_full[b], ((t >> 1) - 1) & 1)) { *a.err = 14; break; } // (the scores of tile t - 2 have been read)
                 ps_tc_fence_after();
-                const uint64_t kb = dk + (uint64_t)(st * (C::STAGE >> 4));
-                const uint32_t to = tm_s + (t & 1) * SV_TILE;
+                const uint64_t d = desc + (uint64_t)(at * (C::STAGE >> 4));
                 if (ps_elect_one()) {
+                    if (pv) {
+                        const uint32_t pa = tm_p + b * SV_TILE;
 #pragma unroll
-                    for (int p = 0; p < C::PARTS + 1; p++) // lo hi, hi lo, hi hi (bfloat16 caches: lo hi, hi hi)
+                        for (int p = 0; p < C::PARTS + 1; p++)
 #pragma unroll
-                        for (int j = 0; j < D / 16; j++) ps_tc_mma_f16(to, dq + (p == 0 ? (D * 16) >> 4 : 0) + j * 16, kb + (C::F32 && p == 1 ? C::K_LO >> 4 : 0) + j * 16, idesc_s, (p | j) != 0);
-                    ps_tc_commit(&unused[st]);
-                    ps_tc_commit(&s_full[t & 1]);
+                            for (int j = 0; j < SV_TILE / 16; j++)
+                                ps_tc_mma_f16_ta(tm_o, pa + (p == 0 ? SV_TILE / 2 : 0) + j * 8, d + (C::F32 && p == 1 ? C::V_LO >> 4 : 0) + j * 16, idesc, (p | j) != 0);
+                    } else {
+                        const uint32_t to = tm_s + b * SV_TILE;
+#pragma unroll
+                        for (int p = 0; p < C::PARTS + 1; p++) // lo hi, hi lo, hi hi (bfloat16 caches: lo hi, hi hi)
+#pragma unroll
+                            for (int j = 0; j < D / 16; j++) ps_tc_mma_f16_ta(to, tm_q + (p == 0 ? D / 2 : 0) + j * 8, d + (C::F32 && p == 1 ? C::K_LO >> 4 : 0) + j * 16, idesc, (p | j) != 0);
+                    }
+                    ps_tc_commit(&unused[at]);
+                    ps_tc_commit(pv ? &o_full[b] : &s_full[b]);
                 }
                 __syncwarp();
-                step();
-                return true;
-            };
-            bool fine = scores(0);
-            for (int t = 0; t < tiles && fine; t++) {
-                const int b = t & 1;
-                if (t + 1 < tiles && !scores(t + 1)) break;
-                if (!ps_tc_wait_warp(&ready[st], round)) { *a.err = 14; break; }
-                if (!ps_tc_wait_warp(&p_full[b], (t >> 1) & 1)) { *a.err = 15; break; } // (the soft-max has waited for the output of tile t - 2)
-                ps_tc_fence_after();
-                const uint64_t vb = dv + (uint64_t)(st * (C::STAGE >> 4));
-                const uint32_t to = tm_o + b * D, pa = tm_p + b * SV_TILE;
-                if (ps_elect_one()) {
-#pragma unroll
-                    for (int p = 0; p < C::PARTS + 1; p++)
-#pragma unroll
-                        for (int j = 0; j < SV_TILE / 16; j++)
-                            ps_tc_mma_f16_ta(to, pa + (p == 0 ? SV_TILE / 2 : 0) + j * 8, vb + (C::F32 && p == 1 ? C::V_LO >> 4 : 0) + j * 16, idesc_o, (p | j) != 0);
-                    ps_tc_commit(&unused[st]);
-                    ps_tc_commit(&o_full[b]);
-                }
-                __syncwarp();
-                step();
+                item += pv ? (t + 2 < tiles ? 2 : 1) : t ? 2 : 1;
             }
             if (ps_elect_one()) ps_tc_commit(&done); // MMAs in flight end before the tensor memory is given back
             __syncwarp();
@@ -337,7 +341,6 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
         const int r = (warp & 3) * 32 + lane, row = r0 + r, tok = row / a.R, rp = sv_rp(all_rows);
         const bool mine = r < rows, any = (warp & 3) * 32 < rows; // (any: of the warp)
         const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
-        const float qinv = mine ? s_qinv[r] : 0.f;
         bool ok = true;
         for (int t = warp >> 2; t < tiles; t += 2) {
             const int b = t & 1, j = j0 + t * SV_TILE;
@@ -448,7 +451,7 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
 #pragma unroll
                 for (int c = 0; c < D / 2; c += 16) {
                     uint32_t v[16];
-                    sv_tm_ld16(v, tm_o + b * D + half * (D / 2) + c + lane_at);
+                    sv_tm_ld16(v, tm_o + half * (D / 2) + c + lane_at);
                     ps_tc_ld_wait();
 #pragma unroll
                     for (int e = 0; e < 16; e++) acc[c + e] = fmaf(__uint_as_float(v[e]), f[(c + e) / (D / 8)], acc[c + e]);
