@@ -226,9 +226,11 @@ int ps_serve_sample(PsServeCall *c, int32_t *ids, float *probs, const float *log
     if (!aligned(ids, 4) || !aligned(probs, 4) || !aligned(logits, 4) || !aligned(samplers, 4) || !aligned(u, 4)) return fail(c, PS_CUDA_ERR_INVALID, "sample: an array that is not aligned to its elements");
     SvSample a{};
     a.logits = logits; a.samplers = samplers; a.u = u; a.ids = ids; a.probs = probs; a.row_stride = row_stride; a.vocab = (int)vocab;
-    const int C = SV_SMP_CLUSTER;
+    // few rows: as many CTAs a row as a cluster can have, so that the GPU is at work; many: eight
+    const int C = rows * 16 <= c->n_sm ? 16 : 8;
     a.chunk = (int)((vocab + C - 1) / C + 31) & ~31;
-    const size_t smem = 4 * (size_t)a.chunk;
+    a.vec = aligned(logits, 16) && row_stride % 4 == 0;
+    const size_t smem = sizeof(SvSmpShared) + 4 * (size_t)a.chunk;
     for (int64_t r0 = 0; r0 < rows; r0 += 1 << 20) {
         const int n = (int)std::min<int64_t>(rows - r0, 1 << 20);
         cudaLaunchConfig_t cfg{};
@@ -236,8 +238,9 @@ int ps_serve_sample(PsServeCall *c, int32_t *ids, float *probs, const float *log
         at[0].id = cudaLaunchAttributeClusterDimension;
         at[0].val.clusterDim.x = C; at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
         cfg.gridDim = dim3(n * C); cfg.blockDim = dim3(SV_SMP_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = c->stream; cfg.attrs = at; cfg.numAttrs = 1;
-        SV_CK(cudaFuncSetAttribute(sv_k_sample<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        SV_CK(cudaLaunchKernelEx(&cfg, sv_k_sample<true>, a));
+        SV_CK(cudaFuncSetAttribute(sv_k_sample, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        SV_CK(cudaFuncSetAttribute(sv_k_sample, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        SV_CK(cudaLaunchKernelEx(&cfg, sv_k_sample, a));
         SV_LAUNCHED("sample");
         a.logits += (int64_t)n * row_stride; a.samplers += n; a.u += n; a.ids += n;
         if (a.probs) a.probs += n;
