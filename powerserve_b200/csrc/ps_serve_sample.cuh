@@ -571,8 +571,15 @@ __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_sample(const __grid_co
     const bool filters = r.use_k || r.use_p || r.min_w;
     bool listed = false;
     if (filters) {
+        const bool least = r.min_w >= SV_ONE >> (int)SV_SMP_SPAN; // min-p takes out all that is not listed
         unsigned long long whole = 0;
-        if (r.use_p && !r.use_k) whole = sv_block<false>(sh, sv_all(r, sh, x)); // (top-p needs the mass of all)
+        // Top-p needs the mass of all.  Beside such a min-p it is enough, nearly always, to know it to a thousandth: where what min-p leaves is less than top_p of it,
+        // top-p takes out nothing more
+        bool roughly = r.use_p && !r.use_k && least;
+        const bool exactly = r.use_p && !r.use_k && !least;
+        const float rs = (float)r.log2w.s;
+        float rough = 0.f, rough_in = 0.f;
+        if (exactly) whole = sv_block<false>(sh, sv_all(r, sh, x));
         for (int i = r.w0; i < r.w1; i += 128) {
             float v[4];
 #pragma unroll
@@ -585,6 +592,14 @@ __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_sample(const __grid_co
                 if (in && at < SV_SMP_CAP) sh.lists[warp][at] = (uint16_t)(i + 32 * e + lane);
                 r.listed += __popc(ball);
             }
+            if (roughly)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float w;
+                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"((v[e] - r.log2w.top) * rs));
+                    rough += w;
+                    rough_in += v[e] >= r.cut ? w : 0.f;
+                }
         }
         const bool over = r.listed > SV_SMP_CAP;
         if (over) r.listed = SV_SMP_CAP;
@@ -599,16 +614,33 @@ __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_sample(const __grid_co
         uint32_t total = 0;
         bool over_any = false;
         {
-            const unsigned long long(*m)[16] = mail.post(cta, whole);
+            unsigned long long in = 0;
+            if (roughly) { // (no number, as with an infinite logit: the exact mass is asked for)
+                whole = sv_block<false>(sh, (unsigned long long)(rough * 16777216.f));
+                in = sv_block<false>(sh, (unsigned long long)(rough_in * 16777216.f) + 1);
+                const bool odd = __syncthreads_or(!(rough < 1e9f)) != 0;
+                if (odd) in = 1ull << 60;
+            }
+            const unsigned long long(*m)[16] = mail.post(cta, whole, in);
+            unsigned long long all_in = 0;
             whole = 0;
             for (int o = 0; o < C; o++) {
                 if (o < mail.rank) at += (uint32_t)m[0][o];
                 total += (uint32_t)m[0][o];
                 over_any |= m[0][o] >= SV_SMP_OVER;
                 whole += m[1][o];
+                all_in += m[2][o];
+            }
+            if (roughly) {
+                if (1.002 * (double)all_in < (double)fmaxf(r.p.top_p, 0.f) * (double)whole) r.use_p = false;
+                else {
+                    const unsigned long long mine = sv_block<false>(sh, sv_all(r, sh, x));
+                    const unsigned long long(*n)[16] = mail.post(mine);
+                    whole = 0;
+                    for (int o = 0; o < C; o++) whole += n[0][o];
+                }
             }
         }
-        const bool least = r.min_w >= SV_ONE >> (int)SV_SMP_SPAN;  // min-p takes out all that is not listed
         const bool known = r.use_k ? total >= (uint32_t)r.p.top_k || (least && !r.use_p) : least; // what the filters leave is listed, and the mass that top-p asks for known
         if (known && total <= SV_SMP_BINS) {
             SvSmpShared *to = mail.cl.map_shared_rank(&sh, 0);
