@@ -165,7 +165,13 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
             SV_LAUNCHED("attn_tree");
             if (joined || weights) {
                 const int row_blocks = joined ? (most_tok * R + 7) / 8 : 0, slot_blocks = weights ? (most_kv + SV_FIN_SLOTS - 1) / SV_FIN_SLOTS : 0;
-                sv_k_finish<<<dim3(row_blocks + slot_blocks, n_kv_heads, n), 256, 4 * (size_t)most_tok * R, c->stream>>>(a, row_blocks);
+                cudaLaunchConfig_t cfg{};
+                cudaLaunchAttribute attr[1];
+                attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+                attr[0].val.programmaticStreamSerializationAllowed = 1;
+                cfg.gridDim = dim3(row_blocks + slot_blocks, n_kv_heads, n); cfg.blockDim = dim3(256); cfg.dynamicSmemBytes = 4 * (size_t)most_tok * R; cfg.stream = c->stream;
+                cfg.attrs = attr; cfg.numAttrs = 1;
+                SV_CK(cudaLaunchKernelEx(&cfg, sv_k_finish, a, row_blocks));
                 SV_LAUNCHED("attn_tree");
             }
         }
@@ -190,14 +196,26 @@ int ps_serve_kv_evict(PsServeCall *c, const ps_cuda_cache *caches, int n_sets, i
         SvEvict a{};
         a.G = n_kv_heads; a.hs = head_size; a.n_sink = n_sink; a.n_recent = n_recent;
         size_t bytes = 0;
-        int most = 0;
+        int most = 0, most_kv = 0, most_gone = 0;
+        bool vec = true;
+        const size_t es = cache_type == PS_TYPE_F32 ? 4 : 2;
         for (int i = 0; i < n; i++) {
             const ps_cuda_cache &s = caches[first + i];
             SvSet &d = a.set[i];
             d.k = s.k; d.v = s.v; d.weight = s.weight; d.weight_to = s.weight_to; d.pos = s.pos; d.pos_to = s.pos_to; d.n_ctx = s.n_ctx; d.n_kv = s.n_kv; d.n_keep = s.n_keep;
             d.moves = std::min(s.n_keep, s.n_kv - s.n_keep);
             most = std::max(most, d.moves);
+            most_kv = std::max(most_kv, s.n_kv);
+            most_gone = std::max(most_gone, s.n_kv - s.n_keep);
+            vec &= aligned(s.k, 16);
             bytes += up(4 * (size_t)n_kv_heads * (1 + 2 * (size_t)d.moves));
+        }
+        const dim3 heads(n_kv_heads, n);
+        if (most_gone <= SV_FEW) { // one by one costs a pass over the weights each: some 1 025 slots of 256 heads 16 us for one, 21 for eight; the select and its moves 25 for nine (from Python)
+            if (es == 4) sv_k_evict_few<uint32_t><<<heads, 256, 0, c->stream>>>(a);
+            else sv_k_evict_few<uint16_t><<<heads, 256, 0, c->stream>>>(a);
+            SV_LAUNCHED("kv_evict");
+            continue;
         }
         void *mem = nullptr;
         if (int rc = c->workspace(c->user, bytes, &mem)) return rc;
@@ -206,12 +224,19 @@ int ps_serve_kv_evict(PsServeCall *c, const ps_cuda_cache *caches, int n_sets, i
             a.set[i].list = reinterpret_cast<int32_t *>(at);
             at += up(4 * (size_t)n_kv_heads * (1 + 2 * (size_t)a.set[i].moves));
         }
-        sv_k_select<<<dim3(n_kv_heads, n), SV_SEL_THREADS, 0, c->stream>>>(a);
+        const int keys = most_kv <= SV_KEYS ? most_kv : 0;
+        SV_CK(cudaFuncSetAttribute(sv_k_select, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * SV_KEYS));
+        sv_k_select<<<heads, SV_SEL_THREADS, 4 * (size_t)keys, c->stream>>>(a, keys);
         SV_LAUNCHED("kv_evict");
         if (most) {
-            const dim3 grid((most + 31) / 32, n_kv_heads, n);
-            if (cache_type == PS_TYPE_F32) sv_k_move<uint32_t><<<grid, 256, 0, c->stream>>>(a);
-            else sv_k_move<uint16_t><<<grid, 256, 0, c->stream>>>(a);
+            cudaLaunchConfig_t cfg{};
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[0].val.programmaticStreamSerializationAllowed = 1;
+            cfg.gridDim = dim3((most + SV_MOVES - 1) / SV_MOVES * (1 + SV_V_PARTS), n_kv_heads, n); cfg.blockDim = dim3(256); cfg.stream = c->stream; cfg.attrs = attr; cfg.numAttrs = 1;
+            // (rows of head sizes that are multiples of 32 begin at 16-byte boundaries where the cache does)
+            SV_CK(es == 4 ? vec ? cudaLaunchKernelEx(&cfg, sv_k_move<uint32_t, 4>, a) : cudaLaunchKernelEx(&cfg, sv_k_move<uint32_t, 1>, a)
+                          : vec ? cudaLaunchKernelEx(&cfg, sv_k_move<uint16_t, 8>, a) : cudaLaunchKernelEx(&cfg, sv_k_move<uint16_t, 1>, a));
             SV_LAUNCHED("kv_evict");
         }
     }

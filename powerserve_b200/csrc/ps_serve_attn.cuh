@@ -155,6 +155,7 @@ inline size_t sv_attn_smem(int hs) { return 4 * ((size_t)16 * hs + 32 * (hs + 1)
 #define SV_FIN_SLOTS 256
 __global__ void __launch_bounds__(256) sv_k_finish(const __grid_constant__ SvAttn a, int row_blocks) {
     extern __shared__ float sv_lse[];
+    ps_grid_dep_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hs = a.hs, g = blockIdx.y;
     const SvSeq &s = a.seq[blockIdx.z];
     const int rows = s.n_tok * a.R;
@@ -162,21 +163,39 @@ __global__ void __launch_bounds__(256) sv_k_finish(const __grid_constant__ SvAtt
     if ((int)blockIdx.x < row_blocks) {
         const int row = blockIdx.x * 8 + warp;
         if (row >= rows || s.splits == 1) return;
+        // a lane a split: maxima and sums are asked for at once, then eight splits' outputs at a time
+        const int64_t at = (int64_t)g * rows + row, step = (int64_t)a.G * rows;
         float mx = SV_NONE;
-        for (int i = lane; i < s.splits; i += 32) mx = fmaxf(mx, ml[((int64_t)i * a.G + g) * rows + row].x);
+        for (int i = lane; i < s.splits; i += 32) mx = fmaxf(mx, ml[i * step + at].x);
 #pragma unroll
         for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         const float ref = mx == SV_NONE ? 0.f : mx;
         float l = 0.f, acc[8] = {};
-        for (int i = 0; i < s.splits; i++) {
-            const int64_t at = ((int64_t)i * a.G + g) * rows + row;
-            const float2 p = ml[at];
-            const float f = exp2f(p.x - ref);
-            l = fmaf(p.y, f, l);
+        for (int i0 = 0; i0 < s.splits; i0 += 32) {
+            float f = 0.f;
+            if (i0 + lane < s.splits) {
+                const float2 p = ml[(i0 + lane) * step + at];
+                f = exp2f(p.x - ref);
+                l = fmaf(p.y, f, l);
+            }
+            for (int i = 0; i < min(32, s.splits - i0); i += 8) {
+                float v[8][8];
 #pragma unroll
-            for (int c = 0; c < 8; c++)
-                if (c * 32 < hs) acc[c] = fmaf(s.part[at * hs + c * 32 + lane], f, acc[c]);
+                for (int e = 0; e < 8; e++)
+#pragma unroll
+                    for (int c = 0; c < 8; c++)
+                        if (c * 32 < hs && i0 + i + e < s.splits) v[e][c] = s.part[((i0 + i + e) * step + at) * hs + c * 32 + lane];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float fe = __shfl_sync(0xffffffffu, f, i + e);
+#pragma unroll
+                    for (int c = 0; c < 8; c++)
+                        if (c * 32 < hs && i0 + i + e < s.splits) acc[c] = fmaf(v[e][c], fe, acc[c]);
+                }
+            }
         }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
         const float inv = l > 0.f ? 1.f / l : 0.f;
         float *to = a.out + ((int64_t)(s.tok0 + row / a.R) * a.n_heads + g * a.R + row % a.R) * hs;
 #pragma unroll
@@ -186,14 +205,18 @@ __global__ void __launch_bounds__(256) sv_k_finish(const __grid_constant__ SvAtt
     }
     const int j0 = (blockIdx.x - row_blocks) * SV_FIN_SLOTS;
     if (!s.scores || j0 >= s.n_kv) return;
-    for (int row = tid; row < rows; row += 256) {
+    for (int row = warp; row < rows; row += 8) {
         float mx = SV_NONE, l = 0.f;
-        for (int i = 0; i < s.splits; i++) mx = fmaxf(mx, ml[((int64_t)i * a.G + g) * rows + row].x);
-        for (int i = 0; i < s.splits; i++) {
+        for (int i = lane; i < s.splits; i += 32) mx = fmaxf(mx, ml[((int64_t)i * a.G + g) * rows + row].x);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        for (int i = lane; i < s.splits; i += 32) {
             const float2 p = ml[((int64_t)i * a.G + g) * rows + row];
             if (p.y > 0.f) l = fmaf(p.y, exp2f(p.x - mx), l);
         }
-        sv_lse[row] = l > 0.f ? mx + log2f(l) : INFINITY; // (a row that sees nothing adds nothing)
+#pragma unroll
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (lane == 0) sv_lse[row] = l > 0.f ? mx + log2f(l) : INFINITY; // (a row that sees nothing adds nothing)
     }
     __syncthreads();
     const int rp = sv_rp(rows);

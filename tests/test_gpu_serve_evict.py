@@ -74,6 +74,15 @@ def test_first_and_latest_positions(be, same, order, n_sink, n_recent):
     check(be, [500, 2100, 31], [301, 2000, 30], 3, 64, n_sink=n_sink, n_recent=n_recent, same=same, order=order, seed=n_recent % 97)
 
 
+@pytest.mark.parametrize("gone", [2, 3, 5, 7, 8, 9])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_few_go(be, gone, dtype):
+    """what goes lies before the new end, behind it, and on both sides"""
+    lens = [gone, gone + 1, 40, 300, 1026, 2049]
+    check(be, lens, [n - gone for n in lens], 5, 64, dtype=dtype, n_sink=2, n_recent=9, order=True, seed=gone)
+    check(be, lens, [n - gone for n in lens], 3, 128, dtype=dtype, n_recent=1, same=True, seed=gone, weights=lambda shape, r: r.integers(0, 4, shape))
+
+
 @pytest.mark.parametrize("same", [False, True])
 def test_without_positions(be, same):
     check(be, [700, 5], [350, 2], 2, 128, pos=False, same=same)

@@ -67,7 +67,7 @@ int main() {
     expect("caches below zero", I, "no caches", [&](PsServeCall *c) { return ps_serve_attn_tree(c, mem, mem, &good, -1, 0, 32, 4, 2, nullptr, 1.f); });
     expect("nobody", 0, nullptr, [&](PsServeCall *c) { return ps_serve_attn_tree(c, mem, mem, nullptr, 0, 0, 32, 4, 2, nullptr, 1.f); });
 
-    evict("a call that is right asks for memory", PS_CUDA_ERR_OOM, nullptr, none, 1, 1);
+    evict("a call that is right asks for memory", PS_CUDA_ERR_OOM, nullptr, [](ps_cuda_cache &s) { s.n_ctx = s.n_kv = 100; }, 1, 1);
     evict("keeps more than there are", I, "keeps", [](ps_cuda_cache &s) { s.n_keep = 13; });
     evict("keeps below zero", I, "keeps", [](ps_cuda_cache &s) { s.n_keep = -1; });
     evict("no weights", I, "gathered", [](ps_cuda_cache &s) { s.weight = nullptr; });
