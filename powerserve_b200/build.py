@@ -16,7 +16,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libps_cuda.so")
 SOURCES = ["ps_cuda.cu", "ps_arch.cu", "ps_serve.cu"]
 HEADERS = ["ps_step.cuh", "ps_tc.cuh", "ps_mk.cuh", "ps_rw.cuh", "ps_decode.cuh", "ps_kernels.cuh", "ps_math.cuh", "ps_mv32.cuh", "ps_ptx.cuh", "ps_arch.h", "ps_arch_kernels.cuh",
-           "ps_arch_decode.cuh", "ps_arch_tc.cuh", "ps_arch_recur.cuh", "ps_serve.h", "ps_serve_attn.cuh", "ps_serve_attn_tc.cuh", "ps_serve_evict.cuh", "ps_serve_sample.cuh",
+           "ps_arch_decode.cuh", "ps_arch_tc.cuh", "ps_arch_recur.cuh", "ps_serve.h", "ps_serve_attn.cuh", "ps_serve_attn_tc.cuh", "ps_serve_attn_few.cuh", "ps_serve_evict.cuh", "ps_serve_sample.cuh",
            os.path.join("..", "..", "include", "ps_cuda.h")]
 
 COMMON_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-cudart", "shared"]
@@ -48,7 +48,7 @@ def _unit_stale(src: str) -> bool:
         return True
     t = os.path.getmtime(o)
     mine = {"ps_arch.cu": ["ps_arch.h", "ps_arch_kernels.cuh", "ps_arch_decode.cuh", "ps_arch_tc.cuh", "ps_arch_recur.cuh", "ps_ptx.cuh", os.path.join("..", "..", "include", "ps_cuda.h")],
-            "ps_serve.cu": ["ps_serve.h", "ps_serve_attn.cuh", "ps_serve_attn_tc.cuh", "ps_serve_evict.cuh", "ps_serve_sample.cuh", "ps_ptx.cuh", "ps_math.cuh", os.path.join("..", "..", "include", "ps_cuda.h")]}.get(src, HEADERS)
+            "ps_serve.cu": ["ps_serve.h", "ps_serve_attn.cuh", "ps_serve_attn_tc.cuh", "ps_serve_attn_few.cuh", "ps_serve_evict.cuh", "ps_serve_sample.cuh", "ps_ptx.cuh", "ps_math.cuh", os.path.join("..", "..", "include", "ps_cuda.h")]}.get(src, HEADERS)
     deps = [os.path.join(CSRC, f) for f in [src] + mine] + [os.path.abspath(__file__)]
     return any(os.path.getmtime(os.path.normpath(d)) > t for d in deps if os.path.exists(os.path.normpath(d)))
 

@@ -3,6 +3,7 @@
 
 #include "ps_serve_attn.cuh"
 #include "ps_serve_attn_tc.cuh"
+#include "ps_serve_attn_few.cuh"
 #include "ps_serve_evict.cuh"
 #include "ps_serve_sample.cuh"
 
@@ -103,12 +104,12 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
         }
         SvAttn a{};
         a.q = q; a.out = out; a.hs = hs; a.n_heads = n_heads; a.G = n_kv_heads; a.R = R; a.scale = scale * SV_LOG2E; a.err = c->err_dev; a.n_seqs = n;
-        const bool tc = hs == 64 || hs == 128;
+        const bool own = hs == 64 || hs == 128, few = own && most_tok * R <= SV_FEW_ROWS, tc = own && !few;
         const int tile_rows = tc ? SV_TC_ROWS : 16, row_tiles = (most_tok * R + tile_rows - 1) / tile_rows;
         a.out_vec = aligned(out, 16);
         a.q_vec = aligned(q, 16);
         if (most_tok) {
-            a.tps = split_tiles(caches + first, n, n_kv_heads * row_tiles, tc ? c->n_sm : c->n_sm * 4, 1);
+            a.tps = split_tiles(caches + first, n, n_kv_heads * row_tiles, tc ? c->n_sm : c->n_sm * (few ? 8 : 4), few ? 2 : 1);
             if (tc) a.tps = std::min(a.tps, SV_TC_TILES);
             size_t bytes = scores;
             int units = 0;
@@ -128,6 +129,7 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
                 d.v_mode = aligned(s.v, 16) && s.n_ctx % (f32 ? 4 : 8) == 0;
                 units += d.splits;
                 joined |= d.splits > 1;
+                if (d.weight) bytes += up(4 * (size_t)n_kv_heads * s.n_tok * R);
                 bytes += up(4 * (size_t)d.splits * n_kv_heads * s.n_tok * R * (hs + 2));
             }
             void *mem = nullptr;
@@ -138,12 +140,18 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
                 if (d.weight) {
                     d.scores = reinterpret_cast<float *>(at);
                     at += up(16 * (size_t)n_kv_heads * sv_quads(d.n_kv) * sv_rp(d.n_tok * R));
+                    d.lse = reinterpret_cast<float *>(at);
+                    at += up(4 * (size_t)n_kv_heads * d.n_tok * R);
                 }
                 d.part = reinterpret_cast<float *>(at);
                 at += up(4 * (size_t)d.splits * n_kv_heads * d.n_tok * R * (hs + 2));
             }
             const dim3 grid(units, n_kv_heads, row_tiles);
-            if (tc) {
+            if (few) {
+                const bool f32 = cache_type == PS_TYPE_F32;
+                auto kern = hs == 64 ? (f32 ? sv_k_attn_few<float, 64> : sv_k_attn_few<__nv_bfloat16, 64>) : (f32 ? sv_k_attn_few<float, 128> : sv_k_attn_few<__nv_bfloat16, 128>);
+                kern<<<grid, 128, 0, c->stream>>>(a);
+            } else if (tc) {
                 auto launch = [&](auto kern, int smem) -> int {
                     SV_CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
                     kern<<<grid, SV_TC_THREADS, smem, c->stream>>>(a);
@@ -163,17 +171,20 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
                 sv_k_attn<__nv_bfloat16><<<grid, 128, smem, c->stream>>>(a);
             }
             SV_LAUNCHED("attn_tree");
-            if (joined || weights) {
-                const int row_blocks = joined ? (most_tok * R + 7) / 8 : 0, slot_blocks = weights ? (most_kv + SV_FIN_SLOTS - 1) / SV_FIN_SLOTS : 0;
+            auto after = [&](auto kern, dim3 g, size_t smem) -> int { // (its start overlaps the end of the kernel before)
                 cudaLaunchConfig_t cfg{};
                 cudaLaunchAttribute attr[1];
                 attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
                 attr[0].val.programmaticStreamSerializationAllowed = 1;
-                cfg.gridDim = dim3(row_blocks + slot_blocks, n_kv_heads, n); cfg.blockDim = dim3(256); cfg.dynamicSmemBytes = 4 * (size_t)most_tok * R; cfg.stream = c->stream;
-                cfg.attrs = attr; cfg.numAttrs = 1;
-                SV_CK(cudaLaunchKernelEx(&cfg, sv_k_finish, a, row_blocks));
+                cfg.gridDim = g; cfg.blockDim = dim3(256); cfg.dynamicSmemBytes = smem; cfg.stream = c->stream; cfg.attrs = attr; cfg.numAttrs = 1;
+                SV_CK(cudaLaunchKernelEx(&cfg, kern, a));
                 SV_LAUNCHED("attn_tree");
-            }
+                return 0;
+            };
+            if (joined || weights)
+                if (int rc = after(sv_k_join, dim3((most_tok * R + 7) / 8, n_kv_heads, n), 0)) return rc;
+            if (weights)
+                if (int rc = after(sv_k_weights, dim3((most_kv + SV_FIN_SLOTS - 1) / SV_FIN_SLOTS, n_kv_heads, n), 4 * (size_t)most_tok * R)) return rc;
         }
         first += n;
     }

@@ -4,8 +4,8 @@
 //   weight[g][j] += sum over tokens t and heads h of g of p[t][h][j]
 //
 // A sequence's query rows of one kv head (n_tok tokens x the heads that share it) go together, so that its K rows and V^T columns are read once.
-// The slots are cut into splits; a split leaves its rows' running maximum, sum and unnormalised output in the workspace, and sv_k_finish joins
-// them.  Where weights are gathered, the scores (32 bits) go to the workspace too, and sv_k_finish sums exp(z - log-sum) over the rows.
+// The slots are cut into splits; a split leaves its rows' running maximum, sum and unnormalised output in the workspace, and sv_k_join joins
+// them.  Where weights are gathered, the scores (32 bits) go to the workspace too, and sv_k_weights sums exp(z - log-sum) over the rows.
 #pragma once
 #include "ps_ptx.cuh"
 
@@ -22,6 +22,7 @@ struct SvSeq {
     const uint8_t *hidden, *mask;
     float *scores;          // [kv head][quad of slots][rp][4], or null: quads up to a whole tile, -inf where a row does not see the slot
     float *part;            // [split][kv head][row][hs]; then [split][kv head][row] pairs of maximum and sum
+    float *lse;             // [kv head][row] log2 of the row's sum, for the weights; or null
     int n_ctx, n_kv, n_tok, tok0;
     int k_mode, v_mode;     // head sizes 64 and 128: rows begin at 16-byte boundaries
     int splits, unit0;      // unit0: number of the sequence's first split among all of the launch
@@ -151,93 +152,98 @@ __global__ void __launch_bounds__(128) sv_k_attn(const __grid_constant__ SvAttn 
 inline size_t sv_attn_smem(int hs) { return 4 * ((size_t)16 * hs + 32 * (hs + 1) + (size_t)hs * 33 + 16 * 33 + 16); }
 
 // ---------------------------------------------------------------------------------------------------- joining the splits
-// y < G: a warp takes an output row of kv head y (skipped for a sequence with one split).  y >= G, x: 256 slots of a sequence's kv head y - G: their weights.
+// A warp a row of kv head y: a lane a split takes maxima and sums at once, then eight splits' outputs are under way at a time.  (By the last of the CTAs above
+// to come it took longer: one CTA for all of a head's rows, 16 splits of 48 rows 30 us; 5 so.)
+__global__ void __launch_bounds__(256) sv_k_join(const __grid_constant__ SvAttn a) {
+    ps_grid_dep_wait();
+    ps_grid_dep_launch();
+    const int tid = threadIdx.x, lane = tid & 31, hs = a.hs, g = blockIdx.y;
+    const SvSeq &s = a.seq[blockIdx.z];
+    const int rows = s.n_tok * a.R, row = blockIdx.x * 8 + (tid >> 5);
+    if (row >= rows || (s.splits == 1 && !s.lse)) return;
+    const float2 *ml = reinterpret_cast<const float2 *>(s.part + (int64_t)s.splits * a.G * rows * hs);
+    const int64_t at = (int64_t)g * rows + row, step = (int64_t)a.G * rows;
+    float mx = SV_NONE;
+    for (int i = lane; i < s.splits; i += 32) mx = fmaxf(mx, ml[i * step + at].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float ref = mx == SV_NONE ? 0.f : mx;
+    float l = 0.f, acc[8] = {};
+    for (int i0 = 0; i0 < s.splits; i0 += 32) {
+        float f = 0.f;
+        if (i0 + lane < s.splits) {
+            const float2 p = ml[(i0 + lane) * step + at];
+            f = exp2f(p.x - ref);
+            l = fmaf(p.y, f, l);
+        }
+        if (s.splits == 1) break;
+        for (int i = 0; i < min(32, s.splits - i0); i += 8) {
+            float v[8][8];
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+#pragma unroll
+                for (int c = 0; c < 8; c++)
+                    if (c * 32 < hs && i0 + i + e < s.splits) v[e][c] = s.part[((i0 + i + e) * step + at) * hs + c * 32 + lane];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float fe = __shfl_sync(0xffffffffu, f, i + e);
+#pragma unroll
+                for (int c = 0; c < 8; c++)
+                    if (c * 32 < hs && i0 + i + e < s.splits) acc[c] = fmaf(v[e][c], fe, acc[c]);
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (s.lse && lane == 0) s.lse[at] = l > 0.f ? mx + log2f(l) : INFINITY; // (a row that sees nothing adds nothing)
+    if (s.splits == 1) return;
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    float *to = a.out + ((int64_t)(s.tok0 + row / a.R) * a.n_heads + g * a.R + row % a.R) * hs;
+#pragma unroll
+    for (int c = 0; c < 8; c++)
+        if (c * 32 < hs) to[c * 32 + lane] = acc[c] * inv;
+}
+
+// x: 256 slots of a sequence's kv head y: their weights.  Lanes take rows, four slots each; two such quads are under way at a time
 #define SV_FIN_SLOTS 256
-__global__ void __launch_bounds__(256) sv_k_finish(const __grid_constant__ SvAttn a, int row_blocks) {
+__global__ void __launch_bounds__(256) sv_k_weights(const __grid_constant__ SvAttn a) {
     extern __shared__ float sv_lse[];
     ps_grid_dep_wait();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hs = a.hs, g = blockIdx.y;
+    const int tid = threadIdx.x, g = blockIdx.y;
     const SvSeq &s = a.seq[blockIdx.z];
-    const int rows = s.n_tok * a.R;
-    const float2 *ml = reinterpret_cast<const float2 *>(s.part + (int64_t)s.splits * a.G * rows * hs);
-    if ((int)blockIdx.x < row_blocks) {
-        const int row = blockIdx.x * 8 + warp;
-        if (row >= rows || s.splits == 1) return;
-        // a lane a split: maxima and sums are asked for at once, then eight splits' outputs at a time
-        const int64_t at = (int64_t)g * rows + row, step = (int64_t)a.G * rows;
-        float mx = SV_NONE;
-        for (int i = lane; i < s.splits; i += 32) mx = fmaxf(mx, ml[i * step + at].x);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const float ref = mx == SV_NONE ? 0.f : mx;
-        float l = 0.f, acc[8] = {};
-        for (int i0 = 0; i0 < s.splits; i0 += 32) {
-            float f = 0.f;
-            if (i0 + lane < s.splits) {
-                const float2 p = ml[(i0 + lane) * step + at];
-                f = exp2f(p.x - ref);
-                l = fmaf(p.y, f, l);
-            }
-            for (int i = 0; i < min(32, s.splits - i0); i += 8) {
-                float v[8][8];
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-#pragma unroll
-                    for (int c = 0; c < 8; c++)
-                        if (c * 32 < hs && i0 + i + e < s.splits) v[e][c] = s.part[((i0 + i + e) * step + at) * hs + c * 32 + lane];
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float fe = __shfl_sync(0xffffffffu, f, i + e);
-#pragma unroll
-                    for (int c = 0; c < 8; c++)
-                        if (c * 32 < hs && i0 + i + e < s.splits) acc[c] = fmaf(v[e][c], fe, acc[c]);
-                }
-            }
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        const float inv = l > 0.f ? 1.f / l : 0.f;
-        float *to = a.out + ((int64_t)(s.tok0 + row / a.R) * a.n_heads + g * a.R + row % a.R) * hs;
-#pragma unroll
-        for (int c = 0; c < 8; c++)
-            if (c * 32 < hs) to[c * 32 + lane] = acc[c] * inv;
-        return;
-    }
-    const int j0 = (blockIdx.x - row_blocks) * SV_FIN_SLOTS;
+    const int rows = s.n_tok * a.R, j0 = blockIdx.x * SV_FIN_SLOTS;
     if (!s.scores || j0 >= s.n_kv) return;
-    for (int row = warp; row < rows; row += 8) {
-        float mx = SV_NONE, l = 0.f;
-        for (int i = lane; i < s.splits; i += 32) mx = fmaxf(mx, ml[((int64_t)i * a.G + g) * rows + row].x);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        for (int i = lane; i < s.splits; i += 32) {
-            const float2 p = ml[((int64_t)i * a.G + g) * rows + row];
-            if (p.y > 0.f) l = fmaf(p.y, exp2f(p.x - mx), l);
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        if (lane == 0) sv_lse[row] = l > 0.f ? mx + log2f(l) : INFINITY; // (a row that sees nothing adds nothing)
-    }
+    for (int row = tid; row < rows; row += 256) sv_lse[row] = s.lse[(int64_t)g * rows + row];
     __syncthreads();
     const int rp = sv_rp(rows);
     int per = 1;                                          // lanes of a quad of slots: a power of two
     while (per < 32 && per < rows) per *= 2;
-    for (int b = 0; b < SV_FIN_SLOTS / 4; b += 256 / per) {
-        const int j = j0 + 4 * (b + tid / per);
-        const bool in = b + tid / per < SV_FIN_SLOTS / 4 && j < s.n_kv;
-        float sum[4] = {};
-        if (in) {
-            const float4 *z = reinterpret_cast<const float4 *>(s.scores) + ((int64_t)g * sv_quads(s.n_kv) + j / 4) * rp;
-            for (int row = tid % per; row < rows; row += per) {
-                const float4 v = z[row];
-                const float lse = sv_lse[row];
-                sum[0] += exp2f(v.x - lse); sum[1] += exp2f(v.y - lse); sum[2] += exp2f(v.z - lse); sum[3] += exp2f(v.w - lse);
-            }
+    const int at_once = 256 / per;
+    const float4 *z0 = reinterpret_cast<const float4 *>(s.scores) + ((int64_t)g * sv_quads(s.n_kv) + j0 / 4) * rp;
+    for (int b = 0; b < SV_FIN_SLOTS / 4; b += 2 * at_once) {
+        const int qa = b + tid / per, qb = qa + at_once;
+        const bool ina = qa < SV_FIN_SLOTS / 4 && j0 + 4 * qa < s.n_kv, inb = qb < SV_FIN_SLOTS / 4 && j0 + 4 * qb < s.n_kv;
+        float sa[4] = {}, sb[4] = {};
+#pragma unroll 4
+        for (int row = tid % per; row < rows; row += per) {
+            const float4 none = make_float4(SV_NONE, SV_NONE, SV_NONE, SV_NONE);
+            const float4 va = ina ? __ldcs(z0 + (int64_t)qa * rp + row) : none, vb = inb ? __ldcs(z0 + (int64_t)qb * rp + row) : none;
+            const float lse = sv_lse[row];
+            sa[0] += exp2f(va.x - lse); sa[1] += exp2f(va.y - lse); sa[2] += exp2f(va.z - lse); sa[3] += exp2f(va.w - lse);
+            sb[0] += exp2f(vb.x - lse); sb[1] += exp2f(vb.y - lse); sb[2] += exp2f(vb.z - lse); sb[3] += exp2f(vb.w - lse);
         }
         for (int o = per / 2; o; o >>= 1)
 #pragma unroll
-            for (int e = 0; e < 4; e++) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], o);
-        if (tid % per == 0 && in)
-            for (int e = 0; e < min(4, s.n_kv - j); e++) s.weight[(int64_t)g * s.n_ctx + j + e] += sum[e];
+            for (int e = 0; e < 4; e++) {
+                sa[e] += __shfl_xor_sync(0xffffffffu, sa[e], o);
+                sb[e] += __shfl_xor_sync(0xffffffffu, sb[e], o);
+            }
+        if (tid % per == 0) {
+            float *w = s.weight + (int64_t)g * s.n_ctx + j0;
+            for (int e = 0; e < 4; e++) {
+                if (ina && j0 + 4 * qa + e < s.n_kv) w[4 * qa + e] += sa[e];
+                if (inb && j0 + 4 * qb + e < s.n_kv) w[4 * qb + e] += sb[e];
+            }
+        }
     }
 }
