@@ -66,6 +66,30 @@ int split_tiles(const ps_cuda_cache *caches, int n, int per_split, int target, i
     }
 }
 
+// Tiles of a split for the kernel of few rows, of which `slots` CTAs run at once: the least of an estimate in tiles' time.  A CTA costs its tiles and one more to begin and end;
+// CTAs that do not all run at once end half a CTA apart; joining splits costs one and a half.  64 sequences, 8 kv heads, head size 128, us with four / eight / sixteen
+// CTAs an SM asked for: lengths 256 to 2 041 145 / 124 / 126, all 2 041 294 / 254 / 237; head size 64, all at once without splits, 104 / 117 / 122
+int split_few(const ps_cuda_cache *caches, int n, int heads, int slots) {
+    int most = 1, best = 1;
+    for (int i = 0; i < n; i++)
+        if (caches[i].n_tok > 0) most = std::max(most, (caches[i].n_kv + SV_TILE - 1) / SV_TILE);
+    double least = 1e30;
+    for (int tps = 2, last = 0; !last; tps = std::max(tps + 1, tps * 5 / 4)) {
+        if (tps >= most) { tps = most; last = 1; }
+        double ctas = 0, tiles = 0;
+        for (int i = 0; i < n; i++)
+            if (caches[i].n_tok > 0) {
+                const int t = (caches[i].n_kv + SV_TILE - 1) / SV_TILE;
+                ctas += (double)heads * ((t + tps - 1) / tps);
+                tiles += (double)heads * t;
+            }
+        const double longest = std::min(tps, most) + 1.0;
+        const double cost = (ctas <= slots ? longest : (tiles + ctas) / slots + 0.5 * longest) + (tps < most ? 1.5 : 0.0);
+        if (cost < least) { least = cost; best = tps; }
+    }
+    return best;
+}
+
 } // namespace
 
 int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda_cache *caches, int n_seqs, int cache_type, int head_size, int n_heads, int n_kv_heads,
@@ -109,7 +133,7 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
         a.out_vec = aligned(out, 16);
         a.q_vec = aligned(q, 16);
         if (most_tok) {
-            a.tps = split_tiles(caches + first, n, n_kv_heads * row_tiles, tc ? c->n_sm : c->n_sm * (few ? 8 : 4), few ? 2 : 1);
+            a.tps = few ? split_few(caches + first, n, n_kv_heads, c->n_sm * (hs == 128 && cache_type == PS_TYPE_F32 ? 3 : 4)) : split_tiles(caches + first, n, n_kv_heads * row_tiles, tc ? c->n_sm : c->n_sm * 4, 1);
             if (tc) a.tps = std::min(a.tps, SV_TC_TILES);
             size_t bytes = scores;
             int units = 0;

@@ -80,7 +80,7 @@ PS_D uint32_t sv_turn(uint32_t x) { // an 8 x 8 matrix of halves, transposed
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(128, 3) sv_k_attn_few(const __grid_constant__ SvAttn a) {
+__global__ void __launch_bounds__(128, sizeof(T) == 4 && D == 128 ? 3 : 4) sv_k_attn_few(const __grid_constant__ SvAttn a) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int KS = D / 16, HALF = D / 64; // steps of the first product; items of 64 channels
     __shared__ uint4 s_q[KS][32];             // the queries' fragments: hi, hi, lo, lo

@@ -8,12 +8,12 @@
 // A tile's output leaves the tensor memory after every tile and is added up in registers, with rounding: the accumulator, which truncates, sees the
 // MMAs of one tile alone.  So groups' factors and a row's maximum may differ from tile to tile, and the soft-max of a tile knows of no other tile.
 //
-// A CTA takes up to 128 query rows (the MMAs' M side: one row, one lane of tensor memory) of one kv head over one split.  Warps 0-3 and 4-7: soft-max of
-// the even and of the odd tiles; 8-15: output, a row's channels in two halves; 16-23: converters; 24, 25: MMAs; 26, 27: copies.
-// Tiles of K and of V go through one ring of shared-memory stages: asynchronous 16-byte copies bring a stage as it lies in memory (bulk copies of rows of 256 and
-// 512 bytes took 65 cycles each, 12 400 a tile), the converters cut it
-// into parts in its place (eight rows, read by one warp, become the same eight rows' parts in the K-major no-swizzle layout, in the same bytes),
-// the MMAs read it.  Rows are 16 bytes apart from the next so that neither reading nor writing meets a bank twice.
+// A CTA takes up to 128 query rows (the MMAs' M side: one row, one lane of tensor memory) of one kv head over one split.  Warps 0-3 and 4-7: soft-max of a
+// tile's first and last 32 slots; 8-15: output, a row's channels in two halves; 16-23: copies and conversion; 24, 25: MMAs (26, 27 make the warpgroup whole).
+// Tiles of K and of V go through one ring of shared-memory stages.  A converter warp brings the rows that it will cut, three stages (nine small ones) ahead, as they lie
+// in memory, by asynchronous 16-byte copies, cuts them into parts in their place (eight rows become the same eight rows' parts in the K-major
+// no-swizzle layout, in the same bytes), and the MMAs read them.  Rows are 16 bytes apart from the next so that neither reading nor writing meets a bank twice.
+// (Bulk copies of rows of 256 and 512 bytes took 65 cycles each, 12 400 a tile; two warps that only copied 60 for 512 bytes, 3 500 a tile.)
 // Bound by memory: at head size 128 a tile of 64 slots is 64 KB, some 2 850 cycles of an SM's share of the bandwidth.
 #pragma once
 #include "ps_serve_attn.cuh"
@@ -23,7 +23,6 @@
 #define SV_TC_THREADS 896
 #define SV_TC_ROWS 128
 #define SV_TC_TILES 256  // most tiles of a split (a word of live slots for each)
-#define SV_TC_STAGES 6   // most stages of the ring
 
 PS_D void sv_bar_wait(uint64_t *bar, uint32_t parity, bool &ok, int *err, int site) {
     if (ok && !ps_tc_wait_warp(bar, parity)) { *err = site; ok = false; }
@@ -86,20 +85,22 @@ template <typename T, int D> struct SvTc {
     static constexpr int STAGE = (SV_TILE * K_ROW > D * V_ROW ? SV_TILE * K_ROW : D * V_ROW);
     static constexpr int V_GROUPS = D / 64;                                                      // groups of eight channels that a converter takes
     using Raw = typename std::conditional<F32, SvRaw32, SvRaw16>::type;
-    static constexpr int SMEM = SV_TC_STAGES * STAGE + 128;
+    static constexpr int STAGES = 12 * STAGE < 216 * 1024 ? 12 : 6;                               // of the ring
+    static constexpr int AHEAD = STAGES - 3;                                                     // items that the copies are ahead of the conversion
+    static constexpr int SMEM = STAGES * STAGE + 128;
 };
 
 template <typename T, int D>
 __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_constant__ SvAttn a) {
     using C = SvTc<T, D>;
     extern __shared__ __align__(128) uint8_t sv_tc_raw[];
-    __shared__ __align__(8) uint64_t raw_full[SV_TC_STAGES], ready[SV_TC_STAGES], unused[SV_TC_STAGES], s_full[2], p_full[2], o_full[2], o_empty[2], done;
+    __shared__ __align__(8) uint64_t ready[C::STAGES], unused[C::STAGES], s_full[2], s_free[2], p_full[2], o_full[2], o_empty[2], done;
     __shared__ uint32_t tmem_smem;
-    __shared__ float s_top[2][SV_TC_ROWS], s_sum[2][SV_TC_ROWS], s_qtop[2][SV_TC_ROWS];
+    __shared__ float s_top[2][SV_TC_ROWS], s_sum[2][2][SV_TC_ROWS], s_half[2][2][SV_TC_ROWS], s_qtop[2][SV_TC_ROWS];
     __shared__ __align__(16) float s_kinv[8][8], s_vinv[8][8];
     __shared__ uint64_t s_live[SV_TC_TILES];
     uint8_t *sm_ring = reinterpret_cast<uint8_t *>(((uintptr_t)sv_tc_raw + 127) & ~(uintptr_t)127);
-    constexpr int stages = SV_TC_STAGES;
+    constexpr int stages = C::STAGES;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int si = __shfl_sync(0xffffffffu, sv_find(a, blockIdx.x), 0), split = blockIdx.x - a.seq[si].unit0, g = blockIdx.y;
     const SvSeq &s = a.seq[si];
@@ -107,49 +108,44 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
     if (rows <= 0) return;
     const int j0 = split * a.tps * SV_TILE, j_end = min(s.n_kv, j0 + a.tps * SV_TILE), tiles = (j_end - j0 + SV_TILE - 1) / SV_TILE, past = s.n_kv - s.n_tok;
 
-    // ===== copies: K 0, then for every tile the K of the next and its own V
-    int st = 0;             // stage and round of the ring, for the roles that go through it
-    uint32_t round = 0;
-    auto step = [&] {
-        if (++st == stages) { st = 0; round ^= 1; }
-    };
-    int put_n = 0;
-    auto put = [&](bool is_v, int t) -> bool { // by both warps, each its share of the rows
-        if (put_n >= stages && !ps_tc_wait_warp(&unused[st], round ^ 1)) { *a.err = 11; return false; }
-        const int j = j0 + t * SV_TILE;
-        if (is_v ? s.v_mode : s.k_mode) {
-            const int count = is_v ? D : min(SV_TILE, j_end - j), step_rows = is_v ? C::V_ROW : C::K_ROW, lanes = (step_rows - 16) / 16; // lanes of a row: 16 bytes each
-            const int64_t ld = (is_v ? (int64_t)s.n_ctx : (int64_t)a.G * D) * (int64_t)sizeof(T);
-            const uint8_t *src = is_v ? reinterpret_cast<const uint8_t *>(static_cast<const T *>(s.v) + (int64_t)g * D * s.n_ctx + j)
-                                      : reinterpret_cast<const uint8_t *>(static_cast<const T *>(s.k) + (int64_t)j * a.G * D + (int64_t)g * D);
-            const int in_row = (lane % lanes) * 16, rows_at_once = 32 / lanes, last = is_v ? (s.n_ctx - j) * (int)sizeof(T) : INT32_MAX; // (a row of V is read up to its own end)
-            const uint32_t to = ps_smem_u32(sm_ring + st * C::STAGE) + in_row;
-            if (in_row < last)
-#pragma unroll 4
-                for (int i = (warp - 26) * rows_at_once + lane / lanes; i < count; i += 2 * rows_at_once)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * step_rows), "l"(src + i * ld + in_row) : "memory");
-            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ps_smem_u32(&raw_full[st])) : "memory");
-        } else ps_mbar_arrive(&raw_full[st]);
-        __syncwarp();
-        put_n++;
-        step();
-        return true;
-    };
-    int put_t = 0;          // next of the pairs (K of t + 1, V of t); the first K is put alone
-    if (warp >= 26) {
-        if (tid == 26 * 32) {
-            for (int b = 0; b < SV_TC_STAGES; b++) { ps_mbar_init(&raw_full[b], 64); ps_mbar_init(&ready[b], 8); ps_mbar_init(&unused[b], 1); }
-            for (int b = 0; b < 2; b++) { ps_mbar_init(&s_full[b], 1); ps_mbar_init(&p_full[b], 4); ps_mbar_init(&o_full[b], 1); ps_mbar_init(&o_empty[b], 8); }
-            ps_mbar_init(&done, 2);
-            ps_fence_barrier_init();
-        }
-        ps_bar_sync(1, 64);
-        put(false, 0);      // (the ring is empty: these do not wait)
-        while (put_t < tiles && put_n + 2 <= stages) {
-            if (put_t + 1 < tiles) put(false, put_t + 1);
-            put(true, put_t++);
-        }
+    // What goes through the ring, by number: K 0, then for every tile the K of the next and its own V
+    auto is_value = [&](int i) { return i == 2 * tiles - 1 || (i && i % 2 == 0); };
+    auto tile_of = [&](int i) { return i == 2 * tiles - 1 ? tiles - 1 : is_value(i) ? i / 2 - 1 : (i + 1) / 2; };
+    if (tid == 0) {
+        for (int b = 0; b < stages; b++) { ps_mbar_init(&ready[b], 8); ps_mbar_init(&unused[b], 1); }
+        for (int b = 0; b < 2; b++) { ps_mbar_init(&s_full[b], 1); ps_mbar_init(&s_free[b], 8); ps_mbar_init(&p_full[b], 8); ps_mbar_init(&o_full[b], 1); ps_mbar_init(&o_empty[b], 8); }
+        ps_mbar_init(&done, 2);
+        ps_fence_barrier_init();
     }
+    // Copies: a converter brings the rows that it will cut, sixteen bytes a lane; one group of copies an item
+    auto bring = [&](int i) {
+        const int w = warp - 16;
+        if (i < 2 * tiles) {
+            const bool is_v = is_value(i);
+            const int t = tile_of(i), j = j0 + t * SV_TILE;
+            const uint32_t to = ps_smem_u32(sm_ring + (i % stages) * C::STAGE);
+            if (is_v && s.v_mode) {
+                constexpr int LANES = SV_TILE * (int)sizeof(T) / 16, AT_ONCE = 32 / LANES;  // lanes of a row, rows at once
+                const int row = w * (D / 8) + lane / LANES, col = lane % LANES;
+                const T *src = static_cast<const T *>(s.v) + ((int64_t)g * D + row) * s.n_ctx + j + col * (16 / (int)sizeof(T));
+                if (j + col * (16 / (int)sizeof(T)) < s.n_ctx) // (a row of V is read up to its own end)
+#pragma unroll
+                    for (int r = 0; r < D / 8; r += AT_ONCE)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (row + r) * C::V_ROW + col * 16), "l"(src + (int64_t)r * s.n_ctx) : "memory");
+            } else if (!is_v && s.k_mode) {
+                constexpr int LANES = D * (int)sizeof(T) / 16, AT_ONCE = 32 / LANES;
+                const int row = w * 8 + lane / LANES, col = lane % LANES;
+                const int64_t ld = (int64_t)a.G * D;
+                const T *src = static_cast<const T *>(s.k) + (int64_t)(j + row) * ld + (int64_t)g * D + col * (16 / (int)sizeof(T));
+#pragma unroll
+                for (int r = 0; r < 8; r += AT_ONCE)
+                    if (j + row + r < j_end) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (row + r) * C::K_ROW + col * 16), "l"(src + r * ld) : "memory");
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if (warp >= 16 && warp < 24)
+        for (int i = 0; i < C::AHEAD; i++) bring(i); // (the ring is empty)
     if (warp == 24) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(ps_smem_u32(&tmem_smem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -187,8 +183,8 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
     ps_tc_fence_before();
     __syncthreads();
     ps_tc_fence_after();
-    // columns of tensor memory: scores 2 x 64, weights 2 x (32 + 32), output D, queries D / 2 + D / 2
-    const uint32_t tm = __shfl_sync(0xffffffffu, tmem_smem, 0), tm_s = tm, tm_p = tm + 2 * SV_TILE, tm_o = tm + 4 * SV_TILE, tm_q = tm_o + D;
+    // columns of tensor memory: scores 2 x 64, weights 2 x (32 + 32), outputs 128 (head size 64: two), queries D / 2 + D / 2
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem_smem, 0), tm_s = tm, tm_p = tm + 2 * SV_TILE, tm_o = tm + 4 * SV_TILE, tm_q = tm_o + 128;
     float qinv = 1.f;
     if (warp < 8) {
         const int r = (warp & 3) * 32 + lane;
@@ -216,26 +212,19 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
 
     if (warp >= 24) {
         sv_regs_less<40>();
-        if (warp >= 26) {
-            bool fine = true;
-            for (; put_t < tiles && fine; put_t++) {
-                if (put_t + 1 < tiles) fine = put(false, put_t + 1);
-                fine = fine && put(true, put_t);
-            }
-            asm volatile("cp.async.wait_all;" ::: "memory"); // (what is in flight ends before the CTA does, even when a wait gave up)
-        } else {
+        if (warp < 26) {
             // ===== MMAs, scores by warp 24, outputs by warp 25: neither's waits hold up the other's.  Small products first, while the truncating accumulator is small
             const bool pv = warp == 25;
             const uint32_t idesc = (1u << 4) | ((uint32_t)((pv ? D : SV_TILE) >> 3) << 17) | ((uint32_t)(SV_TC_ROWS >> 4) << 24);
             const uint64_t desc = ps_tc_smem_desc(ps_smem_u32(sm_ring), 128, 8 * (pv ? C::V_ROW : C::K_ROW));
-            int item = pv ? min(2, 2 * tiles - 1) : 0; // number of the tile's K or V among what goes through the ring
+            int item = pv ? min(2, 2 * tiles - 1) : 0;
             for (int t = 0; t < tiles; t++) {
                 const int b = t & 1, at = item % stages;
                 if (!ps_tc_wait_warp(&ready[at], (item / stages) & 1)) { *a.err = 12; break; }
-                if (pv) { // (there is one output: the tile before has to be out of it)
+                if (pv) { // (head size 128: there is one output, and the tile before has to be out of it)
                     if (!ps_tc_wait_warp(&p_full[b], (t >> 1) & 1)) { *a.err = 15; break; }
-                    if (t && !ps_tc_wait_warp(&o_empty[b ^ 1], ((t - 1) >> 1) & 1)) { *a.err = 13; break; }
-                } else if (t >= 2 && !ps_tc_wait_warp(&p_full[b], ((t >> 1) - 1) & 1)) { *a.err = 14; break; } // (the scores of tile t - 2 have been read)
+                    if (D == 128 && t && !ps_tc_wait_warp(&o_empty[b ^ 1], ((t - 1) >> 1) & 1)) { *a.err = 13; break; }
+                } else if (t >= 2 && !ps_tc_wait_warp(&s_free[b], ((t >> 1) - 1) & 1)) { *a.err = 14; break; } // (the scores of tile t - 2 have been read)
                 ps_tc_fence_after();
                 const uint64_t d = desc + (uint64_t)(at * (C::STAGE >> 4));
                 if (ps_elect_one()) {
@@ -245,7 +234,7 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
                         for (int p = 0; p < C::PARTS + 1; p++)
 #pragma unroll
                             for (int j = 0; j < SV_TILE / 16; j++)
-                                ps_tc_mma_f16_ta(tm_o, pa + (p == 0 ? SV_TILE / 2 : 0) + j * 8, d + (C::F32 && p == 1 ? C::V_LO >> 4 : 0) + j * 16, idesc, (p | j) != 0);
+                                ps_tc_mma_f16_ta(tm_o + (D == 64 ? b * D : 0), pa + (p == 0 ? SV_TILE / 2 : 0) + j * 8, d + (C::F32 && p == 1 ? C::V_LO >> 4 : 0) + j * 16, idesc, (p | j) != 0);
                     } else {
                         const uint32_t to = tm_s + b * SV_TILE;
 #pragma unroll
@@ -266,8 +255,13 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
     } else if (warp >= 16) {
         // ===== converters.  lane % 8 picks one of eight rows (slots of K, channels of V), lane / 8 one of four neighbouring eights of the row
         const int w = warp - 16, sub = lane & 7, quad = lane >> 3;
-        auto convert = [&](bool is_v, int t) -> bool {
-            if (!ps_tc_wait_warp(&raw_full[st], round)) { *a.err = 17; return false; }
+        for (int item = 0; item < 2 * tiles; item++) {
+            const bool is_v = is_value(item);
+            const int t = tile_of(item), st = item % stages, ahead = item + C::AHEAD;
+            if (ahead >= stages && ahead < 2 * tiles && !ps_tc_wait_warp(&unused[ahead % stages], (ahead / stages - 1) & 1)) { *a.err = 11; break; }
+            bring(ahead);
+            asm volatile("cp.async.wait_group %0;" ::"n"(C::AHEAD) : "memory");
+            __syncwarp();
             constexpr int ITS = D / 32; // eights of a thread
             const int mode = is_v ? s.v_mode : s.k_mode, j = j0 + t * SV_TILE;
             const uint64_t live = live_of(t);
@@ -330,93 +324,81 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) ps_mbar_arrive(&ready[st]);
-            step();
-            return true;
-        };
-        bool fine = convert(false, 0);
-        for (int i = 0; i < 2 * tiles && fine; i++) // K of the next tile, V of this one
-            if (i & 1 || i / 2 + 1 < tiles) fine = convert(i & 1, i / 2 + 1 - (i & 1));
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory"); // (what is in flight ends before the CTA does, even when a wait gave up)
     } else if (warp < 8) {
-        // ===== soft-max of every other tile: thread = row
-        const int r = (warp & 3) * 32 + lane, row = r0 + r, tok = row / a.R, rp = sv_rp(all_rows);
+        // ===== soft-max: thread = row, warps 0-3 take a tile's first 32 slots, 4-7 the others
+        const int r = (warp & 3) * 32 + lane, row = r0 + r, tok = row / a.R, rp = sv_rp(all_rows), half = warp >> 2;
         const bool mine = r < rows, any = (warp & 3) * 32 < rows; // (any: of the warp)
         const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
         bool ok = true;
-        for (int t = warp >> 2; t < tiles; t += 2) {
-            const int b = t & 1, j = j0 + t * SV_TILE;
-            uint64_t see = live_of(t);
-            if (j + SV_TILE > past && mine) // of the step's own slots those that this token sees
-                for (int c = max(0, past - j); c < min(SV_TILE, j_end - j); c++)
-                    if (!sv_sees(s, tok, j + c - past)) see &= ~(1ull << c);
-            const bool whole = __all_sync(0xffffffffu, see == ~0ull);
+        for (int t = 0; t < tiles; t++) {
+            const int b = t & 1, j = j0 + t * SV_TILE + 32 * half;
+            uint32_t see = (uint32_t)(live_of(t) >> (32 * half));
+            if (j + 32 > past && mine) // of the step's own slots those that this token sees
+                for (int c = max(0, past - j); c < min(32, j_end - j); c++)
+                    if (!sv_sees(s, tok, j + c - past)) see &= ~(1u << c);
+            const bool whole = __all_sync(0xffffffffu, see == ~0u);
             sv_bar_wait(&s_full[b], (t >> 1) & 1, ok, a.err, 18);
-            if (!ok) break;
             ps_tc_fence_after();
-            // sixteen slots at a time, twice (loops, not copies: the code of all roles has to fit the instruction caches)
+            __syncwarp();
+            uint32_t v[32];
             float mx = SV_NONE;
-            if (any)
-#pragma unroll 1
-                for (int k = 0; k < 4; k++) {
-                    uint32_t v[16];
-                    sv_tm_ld16(v, tm_s + b * SV_TILE + 16 * k + lane_at);
-                    const float2 ki = *reinterpret_cast<const float2 *>(&s_kinv[t & 7][2 * k]);
-                    const float f0 = fmaxf(qinv * ki.x, 0x1p-126f), f1 = fmaxf(qinv * ki.y, 0x1p-126f); // (never zero: -inf times it is -inf)
-                    ps_tc_ld_wait();
-                    if (!whole) {
-                        const uint32_t bits = (uint32_t)(see >> (16 * k));
+            if (any && ok) {
+                uint32_t (&va)[16] = *reinterpret_cast<uint32_t (*)[16]>(v), (&vb)[16] = *reinterpret_cast<uint32_t (*)[16]>(v + 16);
+                sv_tm_ld16(va, tm_s + b * SV_TILE + 32 * half + lane_at);
+                sv_tm_ld16(vb, tm_s + b * SV_TILE + 32 * half + 16 + lane_at);
+                const float4 ki = *reinterpret_cast<const float4 *>(&s_kinv[t & 7][4 * half]);
+                // (never zero: -inf times it is -inf)
+                const float f[4] = {fmaxf(qinv * ki.x, 0x1p-126f), fmaxf(qinv * ki.y, 0x1p-126f), fmaxf(qinv * ki.z, 0x1p-126f), fmaxf(qinv * ki.w, 0x1p-126f)};
+                ps_tc_ld_wait();
 #pragma unroll
-                        for (int c = 0; c < 16; c++)
-                            if (!(bits >> c & 1)) v[c] = __float_as_uint(SV_NONE);
-                    }
-                    float t0 = SV_NONE, t1 = SV_NONE;
+                for (int c = 0; c < 32; c++) v[c] = __float_as_uint(__uint_as_float(v[c]) * f[c / 8]);
+                if (!whole) {
 #pragma unroll
-                    for (int c = 0; c < 8; c += 2) {
-                        t0 = fmaxf(fmaxf(t0, __uint_as_float(v[c])), __uint_as_float(v[c + 1]));
-                        t1 = fmaxf(fmaxf(t1, __uint_as_float(v[c + 8])), __uint_as_float(v[c + 9]));
-                    }
-                    mx = fmaxf(fmaxf(mx, t0 * f0), t1 * f1);
-                    if (s.scores && mine) {
-                        float4 *to = reinterpret_cast<float4 *>(s.scores) + ((int64_t)g * sv_quads(s.n_kv) + j / 4 + 4 * k) * rp + row;
-#pragma unroll
-                        for (int c = 0; c < 4; c++) {
-                            const float f = c < 2 ? f0 : f1;
-                            to[(int64_t)c * rp] = make_float4(__uint_as_float(v[4 * c]) * f, __uint_as_float(v[4 * c + 1]) * f, __uint_as_float(v[4 * c + 2]) * f, __uint_as_float(v[4 * c + 3]) * f);
-                        }
-                    }
-                    __syncwarp();
+                    for (int c = 0; c < 32; c++)
+                        if (!(see >> c & 1)) v[c] = __float_as_uint(SV_NONE);
                 }
-            if (t >= 2) sv_bar_wait(&o_empty[b], ((t >> 1) - 1) & 1, ok, a.err, 19); // (tile t - 2's weights are used up, and its maximum and sum)
-            if (!ok) break;
-            // the weights are 2^15 p, and so is their sum
-            const float shift = mx == SV_NONE ? 15.f : 15.f - mx;
-            float sum = 0.f, sum1 = 0.f;
-            if (any) {
-#pragma unroll 1
-                for (int k = 0; k < 4; k++) {
-                    uint32_t v[16], hi[8], lo[8];
-                    sv_tm_ld16(v, tm_s + b * SV_TILE + 16 * k + lane_at);
-                    const float2 ki = *reinterpret_cast<const float2 *>(&s_kinv[t & 7][2 * k]);
-                    const float f0 = fmaxf(qinv * ki.x, 0x1p-126f), f1 = fmaxf(qinv * ki.y, 0x1p-126f);
-                    ps_tc_ld_wait();
-                    if (!whole) {
-                        const uint32_t bits = (uint32_t)(see >> (16 * k));
+                float t0 = SV_NONE, t1 = SV_NONE;
 #pragma unroll
-                        for (int c = 0; c < 16; c++)
-                            if (!(bits >> c & 1)) v[c] = __float_as_uint(SV_NONE);
-                    }
+                for (int c = 0; c < 16; c += 2) {
+                    t0 = fmaxf(fmaxf(t0, __uint_as_float(v[c])), __uint_as_float(v[c + 1]));
+                    t1 = fmaxf(fmaxf(t1, __uint_as_float(v[c + 16])), __uint_as_float(v[c + 17]));
+                }
+                mx = fmaxf(t0, t1);
+            }
+            s_half[b][half][r] = mx;
+            ps_tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ps_mbar_arrive(&s_free[b]); // the scores are in registers: those of tile t + 2 may come
+            if (t >= 2) sv_bar_wait(&o_empty[b], ((t >> 1) - 1) & 1, ok, a.err, 19); // (tile t - 2's weights are used up, and its maximum and sum)
+            ok = ps_bar_all(1 + (warp & 3), 64, ok); // the two warps of the same rows go on together, or give up together
+            if (!ok) break;
+            if (any) {
+                if (s.scores && mine) {
+                    float4 *to = reinterpret_cast<float4 *>(s.scores) + ((int64_t)g * sv_quads(s.n_kv) + j / 4) * rp + row;
+#pragma unroll
+                    for (int c = 0; c < 32; c += 4) to[(int64_t)(c / 4) * rp] = make_float4(__uint_as_float(v[c]), __uint_as_float(v[c + 1]), __uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
+                }
+                mx = fmaxf(mx, s_half[b][half ^ 1][r]);
+                // the weights are 2^15 p, and so is their sum
+                const float shift = mx == SV_NONE ? 15.f : 15.f - mx;
+                float sum = 0.f, sum1 = 0.f;
+#pragma unroll
+                for (int c = 0; c < 32; c += 16) {
+                    uint32_t hi[8], lo[8];
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        const float f = e < 4 ? f0 : f1;
-                        const float p0 = sv_ex2(fmaf(__uint_as_float(v[2 * e]), f, shift)), p1 = sv_ex2(fmaf(__uint_as_float(v[2 * e + 1]), f, shift));
+                        const float p0 = sv_ex2(__uint_as_float(v[c + 2 * e]) + shift), p1 = sv_ex2(__uint_as_float(v[c + 2 * e + 1]) + shift);
                         sum += p0;
                         sum1 += p1;
                         sv_cut(p0, p1, hi[e], lo[e]);
                     }
-                    sv_tm_st8(tm_p + b * SV_TILE + 8 * k + lane_at, hi);
-                    sv_tm_st8(tm_p + b * SV_TILE + SV_TILE / 2 + 8 * k + lane_at, lo);
+                    sv_tm_st8(tm_p + b * SV_TILE + 16 * half + c / 2 + lane_at, hi);
+                    sv_tm_st8(tm_p + b * SV_TILE + SV_TILE / 2 + 16 * half + c / 2 + lane_at, lo);
                 }
-                s_top[b][r] = mx;
-                s_sum[b][r] = sum + sum1;
+                s_top[b][r] = mx; // (both warps write the same)
+                s_sum[b][half][r] = sum + sum1;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             }
             ps_tc_fence_before();
@@ -442,7 +424,7 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
                 const float top = s_top[b][r], mn = fmaxf(m, top), ref = mn == SV_NONE ? 0.f : mn, fo = sv_ex2(m - ref), fn = sv_ex2(top - ref);
                 const float4 vi = *reinterpret_cast<const float4 *>(&s_vinv[t & 7][4 * half]);
                 const float f[4] = {fn * vi.x, fn * vi.y, fn * vi.z, fn * vi.w};
-                l = fmaf(l, fo, s_sum[b][r] * fn);
+                l = fmaf(l, fo, (s_sum[b][0][r] + s_sum[b][1][r]) * fn);
                 m = mn;
                 if (__any_sync(0xffffffffu, fo != 1.f)) {
 #pragma unroll
@@ -451,7 +433,7 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
 #pragma unroll
                 for (int c = 0; c < D / 2; c += 16) {
                     uint32_t v[16];
-                    sv_tm_ld16(v, tm_o + half * (D / 2) + c + lane_at);
+                    sv_tm_ld16(v, tm_o + (D == 64 ? b * D : 0) + half * (D / 2) + c + lane_at);
                     ps_tc_ld_wait();
 #pragma unroll
                     for (int e = 0; e < 16; e++) acc[c + e] = fmaf(__uint_as_float(v[e]), f[(c + e) / (D / 8)], acc[c + e]);
