@@ -10,7 +10,7 @@
 //
 // A CTA takes up to 128 query rows (the MMAs' M side: one row, one lane of tensor memory) of one kv head over one split.  Warps 0-3 and 4-7: soft-max of a
 // tile's first and last 32 slots; 8-15: output, a row's channels in two halves; 16-23: copies and conversion; 24, 25: MMAs (26, 27 make the warpgroup whole).
-// Tiles of K and of V go through one ring of shared-memory stages.  A converter warp brings the rows that it will cut, three stages (nine small ones) ahead, as they lie
+// Tiles of K and of V go through rings of three shared-memory stages each (six small ones).  A converter warp brings the rows that it will cut, two tiles ahead, as they lie
 // in memory, by asynchronous 16-byte copies, cuts them into parts in their place (eight rows become the same eight rows' parts in the K-major
 // no-swizzle layout, in the same bytes), and the MMAs read them.  Rows are 16 bytes apart from the next so that neither reading nor writing meets a bank twice.
 // (Bulk copies of rows of 256 and 512 bytes took 65 cycles each, 12 400 a tile; two warps that only copied 60 for 512 bytes, 3 500 a tile.)
@@ -82,24 +82,23 @@ template <typename T, int D> struct SvTc {
     static constexpr int PARTS = F32 ? 2 : 1;
     static constexpr int K_ROW = D * (int)sizeof(T) + 16, V_ROW = SV_TILE * (int)sizeof(T) + 16; // bytes from row to row of a stage
     static constexpr int K_LO = D * 16, V_LO = SV_TILE * 16;                                     // from a group's hi part to its lo part
-    static constexpr int STAGE = (SV_TILE * K_ROW > D * V_ROW ? SV_TILE * K_ROW : D * V_ROW);
+    static constexpr int K_STAGE = SV_TILE * K_ROW, V_STAGE = D * V_ROW;
+    static constexpr int STAGES = 6 * (K_STAGE + V_STAGE) < 216 * 1024 ? 6 : 3;                  // of K's ring and of V's
+    static constexpr int SMEM = STAGES * (K_STAGE + V_STAGE) + 128;
     static constexpr int V_GROUPS = D / 64;                                                      // groups of eight channels that a converter takes
     using Raw = typename std::conditional<F32, SvRaw32, SvRaw16>::type;
-    static constexpr int STAGES = 12 * STAGE < 216 * 1024 ? 12 : 6;                               // of the ring
-    static constexpr int AHEAD = STAGES - 3;                                                     // items that the copies are ahead of the conversion
-    static constexpr int SMEM = STAGES * STAGE + 128;
 };
 
 template <typename T, int D>
 __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_constant__ SvAttn a) {
     using C = SvTc<T, D>;
     extern __shared__ __align__(128) uint8_t sv_tc_raw[];
-    __shared__ __align__(8) uint64_t ready[C::STAGES], unused[C::STAGES], s_full[2], s_free[2], p_full[2], o_full[2], o_empty[2], done;
+    __shared__ __align__(8) uint64_t ready[2][C::STAGES], unused[2][C::STAGES], s_full[2], s_free[2], p_full[2], o_full[2], o_empty[2], done;
     __shared__ uint32_t tmem_smem;
     __shared__ float s_top[2][SV_TC_ROWS], s_sum[2][2][SV_TC_ROWS], s_half[2][2][SV_TC_ROWS], s_qtop[2][SV_TC_ROWS];
     __shared__ __align__(16) float s_kinv[8][8], s_vinv[8][8];
     __shared__ uint64_t s_live[SV_TC_TILES];
-    uint8_t *sm_ring = reinterpret_cast<uint8_t *>(((uintptr_t)sv_tc_raw + 127) & ~(uintptr_t)127);
+    uint8_t *sm_k = reinterpret_cast<uint8_t *>(((uintptr_t)sv_tc_raw + 127) & ~(uintptr_t)127), *sm_v = sm_k + C::STAGES * C::K_STAGE;
     constexpr int stages = C::STAGES;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int si = __shfl_sync(0xffffffffu, sv_find(a, blockIdx.x), 0), split = blockIdx.x - a.seq[si].unit0, g = blockIdx.y;
@@ -108,44 +107,44 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
     if (rows <= 0) return;
     const int j0 = split * a.tps * SV_TILE, j_end = min(s.n_kv, j0 + a.tps * SV_TILE), tiles = (j_end - j0 + SV_TILE - 1) / SV_TILE, past = s.n_kv - s.n_tok;
 
-    // What goes through the ring, by number: K 0, then for every tile the K of the next and its own V
-    auto is_value = [&](int i) { return i == 2 * tiles - 1 || (i && i % 2 == 0); };
-    auto tile_of = [&](int i) { return i == 2 * tiles - 1 ? tiles - 1 : is_value(i) ? i / 2 - 1 : (i + 1) / 2; };
     if (tid == 0) {
-        for (int b = 0; b < stages; b++) { ps_mbar_init(&ready[b], 8); ps_mbar_init(&unused[b], 1); }
+        for (int b = 0; b < stages; b++)
+            for (int v = 0; v < 2; v++) { ps_mbar_init(&ready[v][b], 4); ps_mbar_init(&unused[v][b], 1); }
         for (int b = 0; b < 2; b++) { ps_mbar_init(&s_full[b], 1); ps_mbar_init(&s_free[b], 8); ps_mbar_init(&p_full[b], 8); ps_mbar_init(&o_full[b], 1); ps_mbar_init(&o_empty[b], 8); }
         ps_mbar_init(&done, 2);
         ps_fence_barrier_init();
     }
-    // Copies: a converter brings the rows that it will cut, sixteen bytes a lane; one group of copies an item
-    auto bring = [&](int i) {
-        const int w = warp - 16;
-        if (i < 2 * tiles) {
-            const bool is_v = is_value(i);
-            const int t = tile_of(i), j = j0 + t * SV_TILE;
-            const uint32_t to = ps_smem_u32(sm_ring + (i % stages) * C::STAGE);
-            if (is_v && s.v_mode) {
-                constexpr int LANES = SV_TILE * (int)sizeof(T) / 16, AT_ONCE = 32 / LANES;  // lanes of a row, rows at once
-                const int row = w * (D / 8) + lane / LANES, col = lane % LANES;
-                const T *src = static_cast<const T *>(s.v) + ((int64_t)g * D + row) * s.n_ctx + j + col * (16 / (int)sizeof(T));
-                if (j + col * (16 / (int)sizeof(T)) < s.n_ctx) // (a row of V is read up to its own end)
+    // Copies: a converter (of K: warps 16-19, of V: 20-23) brings the quarter of a tile's rows that it will cut, sixteen bytes a lane; one group of copies a tile
+    auto bring = [&](int t) {
+        const int w = warp & 3, j = j0 + t * SV_TILE, at = t % stages;
+        if (t < tiles) {
+            if (warp >= 20) {
+                if (s.v_mode) {
+                    constexpr int LANES = SV_TILE * (int)sizeof(T) / 16, AT_ONCE = 32 / LANES;  // lanes of a row, rows at once
+                    const int row = w * (D / 4) + lane / LANES, col = lane % LANES;
+                    const uint32_t to = ps_smem_u32(sm_v + at * C::V_STAGE) + row * C::V_ROW + col * 16;
+                    const T *src = static_cast<const T *>(s.v) + ((int64_t)g * D + row) * s.n_ctx + j + col * (16 / (int)sizeof(T));
+                    const int64_t step = (int64_t)AT_ONCE * s.n_ctx;
+                    if (j + col * (16 / (int)sizeof(T)) < s.n_ctx) // (a row of V is read up to its own end)
 #pragma unroll
-                    for (int r = 0; r < D / 8; r += AT_ONCE)
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (row + r) * C::V_ROW + col * 16), "l"(src + (int64_t)r * s.n_ctx) : "memory");
-            } else if (!is_v && s.k_mode) {
+                        for (int r = 0; r < D / 4 / AT_ONCE; r++, src += step) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + r * AT_ONCE * C::V_ROW), "l"(src) : "memory");
+                }
+            } else if (s.k_mode) {
                 constexpr int LANES = D * (int)sizeof(T) / 16, AT_ONCE = 32 / LANES;
-                const int row = w * 8 + lane / LANES, col = lane % LANES;
-                const int64_t ld = (int64_t)a.G * D;
+                const int row = w * 16 + lane / LANES, col = lane % LANES;
+                const uint32_t to = ps_smem_u32(sm_k + at * C::K_STAGE) + row * C::K_ROW + col * 16;
+                const int64_t ld = (int64_t)a.G * D, step = AT_ONCE * ld;
                 const T *src = static_cast<const T *>(s.k) + (int64_t)(j + row) * ld + (int64_t)g * D + col * (16 / (int)sizeof(T));
+                const int n = j_end - j - row;
 #pragma unroll
-                for (int r = 0; r < 8; r += AT_ONCE)
-                    if (j + row + r < j_end) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (row + r) * C::K_ROW + col * 16), "l"(src + r * ld) : "memory");
+                for (int r = 0; r < 16 / AT_ONCE; r++, src += step)
+                    if (r * AT_ONCE < n) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + r * AT_ONCE * C::K_ROW), "l"(src) : "memory");
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     if (warp >= 16 && warp < 24)
-        for (int i = 0; i < C::AHEAD; i++) bring(i); // (the ring is empty)
+        for (int t = 0; t < stages - 1; t++) bring(t); // (the rings are empty)
     if (warp == 24) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(ps_smem_u32(&tmem_smem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -216,17 +215,16 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
             // ===== MMAs, scores by warp 24, outputs by warp 25: neither's waits hold up the other's.  Small products first, while the truncating accumulator is small
             const bool pv = warp == 25;
             const uint32_t idesc = (1u << 4) | ((uint32_t)((pv ? D : SV_TILE) >> 3) << 17) | ((uint32_t)(SV_TC_ROWS >> 4) << 24);
-            const uint64_t desc = ps_tc_smem_desc(ps_smem_u32(sm_ring), 128, 8 * (pv ? C::V_ROW : C::K_ROW));
-            int item = pv ? min(2, 2 * tiles - 1) : 0;
+            const uint64_t desc = ps_tc_smem_desc(ps_smem_u32(pv ? sm_v : sm_k), 128, 8 * (pv ? C::V_ROW : C::K_ROW));
             for (int t = 0; t < tiles; t++) {
-                const int b = t & 1, at = item % stages;
-                if (!ps_tc_wait_warp(&ready[at], (item / stages) & 1)) { *a.err = 12; break; }
+                const int b = t & 1, at = t % stages;
+                if (!ps_tc_wait_warp(&ready[pv][at], (t / stages) & 1)) { *a.err = 12; break; }
                 if (pv) { // (head size 128: there is one output, and the tile before has to be out of it)
                     if (!ps_tc_wait_warp(&p_full[b], (t >> 1) & 1)) { *a.err = 15; break; }
                     if (D == 128 && t && !ps_tc_wait_warp(&o_empty[b ^ 1], ((t - 1) >> 1) & 1)) { *a.err = 13; break; }
                 } else if (t >= 2 && !ps_tc_wait_warp(&s_free[b], ((t >> 1) - 1) & 1)) { *a.err = 14; break; } // (the scores of tile t - 2 have been read)
                 ps_tc_fence_after();
-                const uint64_t d = desc + (uint64_t)(at * (C::STAGE >> 4));
+                const uint64_t d = desc + (uint64_t)(at * ((pv ? C::V_STAGE : C::K_STAGE) >> 4));
                 if (ps_elect_one()) {
                     if (pv) {
                         const uint32_t pa = tm_p + b * SV_TILE;
@@ -242,30 +240,31 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
 #pragma unroll
                             for (int j = 0; j < D / 16; j++) ps_tc_mma_f16_ta(to, tm_q + (p == 0 ? D / 2 : 0) + j * 8, d + (C::F32 && p == 1 ? C::K_LO >> 4 : 0) + j * 16, idesc, (p | j) != 0);
                     }
-                    ps_tc_commit(&unused[at]);
+                    ps_tc_commit(&unused[pv][at]);
                     ps_tc_commit(pv ? &o_full[b] : &s_full[b]);
                 }
                 __syncwarp();
-                item += pv ? (t + 2 < tiles ? 2 : 1) : t ? 2 : 1;
             }
             if (ps_elect_one()) ps_tc_commit(&done); // MMAs in flight end before the tensor memory is given back
             __syncwarp();
             if (!ps_tc_wait_warp(&done, 0)) *a.err = 16;
         }
     } else if (warp >= 16) {
-        // ===== converters.  lane % 8 picks one of eight rows (slots of K, channels of V), lane / 8 one of four neighbouring eights of the row
-        const int w = warp - 16, sub = lane & 7, quad = lane >> 3;
-        for (int item = 0; item < 2 * tiles; item++) {
-            const bool is_v = is_value(item);
-            const int t = tile_of(item), st = item % stages, ahead = item + C::AHEAD;
-            if (ahead >= stages && ahead < 2 * tiles && !ps_tc_wait_warp(&unused[ahead % stages], (ahead / stages - 1) & 1)) { *a.err = 11; break; }
-            bring(ahead);
-            asm volatile("cp.async.wait_group %0;" ::"n"(C::AHEAD) : "memory");
+        // ===== converters.  lane % 8 picks one of eight rows (slots of K, channels of V), lane / 8 one of four neighbouring eights of the row; a warp's quarter of a tile in
+        // two parts, of which each has a factor of its own
+        const int sub = lane & 7, quad = lane >> 3;
+        const bool is_v = warp >= 20;
+        for (int t = 0; t < tiles; t++) {
+            const int st = t % stages;
+            asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 2) : "memory");
             __syncwarp();
+#pragma unroll 1
+            for (int part = 0; part < 2; part++) {
+            const int w = 2 * (warp & 3) + part;
             constexpr int ITS = D / 32; // eights of a thread
             const int mode = is_v ? s.v_mode : s.k_mode, j = j0 + t * SV_TILE;
             const uint64_t live = live_of(t);
-            uint8_t *group = sm_ring + st * C::STAGE + (is_v ? w * C::V_GROUPS * 8 * C::V_ROW : w * 8 * C::K_ROW);
+            uint8_t *group = is_v ? sm_v + st * C::V_STAGE + w * C::V_GROUPS * 8 * C::V_ROW : sm_k + st * C::K_STAGE + w * 8 * C::K_ROW;
             // eight i of the thread: K: 32 elements further along the row; V: the row's second half, then the next group of channels
             typename C::Raw raw[ITS];
             if (mode) {
@@ -321,9 +320,13 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
                 if (C::F32) *reinterpret_cast<uint4 *>(p + lo_at) = lo;
             }
             if (lane == 0) (is_v ? s_vinv : s_kinv)[t & 7][w] = inv; // (who reads tile t - 8's is done: the ring's stages span three tiles, and what comes after MMAs two more)
+            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) ps_mbar_arrive(&ready[st]);
+            if (lane == 0) ps_mbar_arrive(&ready[is_v][st]);
+            // (what is asked for now has a tile's time to come)
+            if (t && t + stages - 1 < tiles && !ps_tc_wait_warp(&unused[is_v][(t - 1) % stages], ((t - 1) / stages) & 1)) { *a.err = 11; break; }
+            bring(t + stages - 1);
         }
         asm volatile("cp.async.wait_all;" ::: "memory"); // (what is in flight ends before the CTA does, even when a wait gave up)
     } else if (warp < 8) {
