@@ -142,7 +142,7 @@ typedef struct {                /* one sequence's cache in one layer */
     int32_t *pos;               /* kv_evict: [n_kv_heads][n_ctx] position of the token in each slot (NULL: none are kept for their position) */
     int32_t *pos_to;            /* kv_evict: `pos` itself or another array */
     const uint8_t *hidden;      /* attn_tree: [n_ctx], not 0 = no token sees the slot, which may hold anything (NULL = all are seen) */
-    int32_t n_ctx, n_kv;        /* slots that there are; slots that are filled, those of the call's tokens included */
+    int32_t n_ctx, n_kv;        /* slots that there are (at most 2^30); slots that are filled, those of the call's tokens included */
     int32_t n_tok;              /* attn_tree: tokens that the sequence brings (0: it takes no part); their K / V lie in the last n_tok filled slots */
     int32_t n_keep;             /* kv_evict: slots that stay, <= n_kv */
 } ps_cuda_cache;
@@ -150,8 +150,8 @@ typedef struct {                /* one sequence's cache in one layer */
  * out[t][h] = sum_j p_j v_j with p = soft-max of scale * q[t][h] . k_j over the slots that the token sees: all that are filled and not hidden, of
  * the step's own those that tree_mask gives it (per sequence n_tok x n_tok bytes, row t = the tokens that token t sees, one sequence after another;
  * NULL: itself and the ones before).  A token that sees nothing gets zeros.  weight[g][j] += the sum of p_j over the sequence's tokens and the
- * heads of kv head g.  q and out: [tokens][n_heads * head_size] fp32, sequence after sequence; out may be q's memory only if it IS q.  What a
- * filled slot that is not hidden holds must be finite.  head_size: multiples of 32 up to 256; at most 32 heads a kv head. */
+ * heads of kv head g.  q and out: [tokens][n_heads * head_size] fp32, sequence after sequence; out may be q's memory only if it IS q; sequences may share K and V (a common
+ * beginning), not weights.  What a filled slot that is not hidden holds must be finite.  head_size: multiples of 32 up to 256; at most 32 heads a kv head. */
 int ps_cuda_attn_tree(ps_cuda_ctx *ctx, float *out, const float *q, const ps_cuda_cache *caches, int n_seqs, int cache_type, int64_t head_size,
                       int64_t n_heads, int64_t n_kv_heads, const uint8_t *tree_mask, float scale);
 /* Eviction: every kv head of every cache keeps n_keep slots - those whose position is below n_sink or among the n_recent latest, then those of
@@ -238,6 +238,10 @@ const float *ps_cuda_logits_dev(ps_cuda_ctx *ctx);
  * last forward pass, descending (equal logits by ascending token id), with their token ids.  2 k words cross PCIe instead of
  * the vocabulary's logits; the rest of the sampler chain (temperature, soft-max, top-p, stochastic pick) runs on k entries. */
 int ps_cuda_sample_topk(ps_cuda_ctx *ctx, int row, int k, float *logits_out, int32_t *tokens_out);
+
+/* ps_cuda_sample on the first `rows` rows of the last forward pass's logits (whose logits_host may have been NULL), all arrays the HOST's: a
+ * server's step draws the next token of every session with its own settings, and only ids (and probabilities, if probs is not NULL) come back */
+int ps_cuda_sample_last(ps_cuda_ctx *ctx, int rows, const ps_cuda_sampler *samplers, const float *u, int32_t *ids, float *probs);
 
 /* ---------------------------------------------------------------------------------------------- tensor parallelism
  * One process per GPU.  A context created with desc.tp_size = N > 1 owns rows [rank * rows / N, (rank + 1) * rows / N) of

@@ -161,6 +161,7 @@ def load_library() -> C.CDLL:
         "ps_cuda_attn_tree": (ci, [vp, vp, vp, vp, ci, ci, i64, i64, i64, vp, C.c_float]),
         "ps_cuda_kv_evict": (ci, [vp, vp, ci, ci, i64, i64, ci, ci]),
         "ps_cuda_sample": (ci, [vp, vp, vp, vp, i64, i64, i64, vp, vp]),
+        "ps_cuda_sample_last": (ci, [vp, ci, vp, vp, vp, vp]),
         "ps_cuda_kv_position": (ci, [vp]),
         "ps_cuda_kv_reset": (ci, [vp]),
         "ps_cuda_kv_truncate": (ci, [vp, ci]),
@@ -660,6 +661,16 @@ class CudaModel:
         vals, ids = np.empty(k, np.float32), np.empty(k, np.int32)
         self.be._ck(self.be.L.ps_cuda_sample_topk(self.be.h, row, k, vals.ctypes.data_as(C.POINTER(C.c_float)), ids.ctypes.data_as(C.POINTER(C.c_int32))))
         return vals, ids
+
+    def sample(self, settings, u):
+        """a token of each of the first len(u) rows of the last forward pass, on the device: (ids, probabilities).  settings: SAMPLER records or
+        (temperature, top_k, top_p, min_p), one for each row or one for all; u: a random number in [0, 1) for each row"""
+        u = np.ascontiguousarray(u, np.float32).reshape(-1)
+        s = np.asarray(settings) if isinstance(settings, np.ndarray) else np.array([tuple(r) for r in ([settings] if np.ndim(settings) == 1 else settings)], SAMPLER)
+        s = np.ascontiguousarray(np.broadcast_to(s.astype(SAMPLER, casting="no").reshape(-1), u.shape))
+        ids, probs = np.empty(len(u), np.int32), np.empty(len(u), np.float32)
+        self.be._ck(self.be.L.ps_cuda_sample_last(self.be.h, len(u), s.ctypes.data, u.ctypes.data, ids.ctypes.data, probs.ctypes.data))
+        return ids, probs
 
     def prefill(self, prompt, batch_size: int = 128):
         """ModelTokenIterator's prefill loop (src/model/model.hpp:147-160): prompt[:-1] in chunks, lm_head = false."""

@@ -217,6 +217,8 @@ struct ps_cuda_ctx {
     PsArch *arch = nullptr;
     void *serve_ws = nullptr;   // what the serving operators work in; earlier, smaller ones stay in `owned` (a captured graph may hold them)
     size_t serve_ws_bytes = 0;
+    uint8_t *smp_dev = nullptr, *h_smp = nullptr; // ps_cuda_sample_last: settings, random numbers, ids and probabilities of smp_rows rows, 28 bytes each
+    int smp_rows = 0;
     std::vector<size_t> kv_k_bytes, kv_v_bytes; // per layer: bytes of the K rows / V^T rows of ONE cache set
 };
 
@@ -1898,6 +1900,7 @@ void ps_cuda_destroy(ps_cuda_ctx *ctx) {
     if (ctx->h_ids) cudaFreeHost(ctx->h_ids);
     if (ctx->h_err) cudaFreeHost(ctx->h_err);
     if (ctx->h_logits) cudaFreeHost(ctx->h_logits);
+    if (ctx->h_smp) cudaFreeHost(ctx->h_smp);
     if (ctx->g_step) cudaGraphExecDestroy(ctx->g_step);
     if (ctx->g_fwd) cudaGraphExecDestroy(ctx->g_fwd);
     for (int p = 0; p < PS_TP_MAX; p++)
@@ -3214,6 +3217,39 @@ int ps_cuda_sample_topk(ps_cuda_ctx *ctx, int row, int k, float *logits_out, int
     memcpy(logits_out, ctx->h_ids + k, (size_t)k * 4);
     ctx->d2h += (int64_t)k * 8;
     return 0;
+}
+
+int ps_cuda_sample_last(ps_cuda_ctx *ctx, int rows, const ps_cuda_sampler *samplers, const float *u, int32_t *ids, float *probs) {
+    return serve(ctx, [&](PsServeCall *c) {
+        if (!ctx->logits_last || rows < 0 || rows > std::max(ctx->logits_rows, 1)) return fail(ctx, PS_CUDA_ERR_INVALID, "sample_last: %d rows, the last pass left %d", rows, ctx->logits_last ? std::max(ctx->logits_rows, 1) : 0);
+        if (rows == 0) return 0;
+        if (!samplers || !u || !ids) return fail(ctx, PS_CUDA_ERR_INVALID, "sample_last: null argument");
+        if (rows > ctx->smp_rows) {
+            void *dev = nullptr, *host = nullptr;
+            if (int rc = dev_alloc_yield(ctx, &dev, 28 * (size_t)rows)) return rc;
+            PS_CK(cudaHostAlloc(&host, 28 * (size_t)rows, cudaHostAllocDefault));
+            if (ctx->h_smp) PS_CK(cudaFreeHost(ctx->h_smp)); // (every call waits for its copies)
+            ctx->smp_dev = static_cast<uint8_t *>(dev);
+            ctx->h_smp = static_cast<uint8_t *>(host);
+            ctx->smp_rows = rows;
+        }
+        // settings, random numbers | ids, probabilities
+        const size_t up = 20 * (size_t)rows, down = (probs ? 8 : 4) * (size_t)rows;
+        memcpy(ctx->h_smp, samplers, 16 * (size_t)rows);
+        memcpy(ctx->h_smp + 16 * (size_t)rows, u, 4 * (size_t)rows);
+        PS_CK(cudaMemcpyAsync(ctx->smp_dev, ctx->h_smp, up, cudaMemcpyHostToDevice, ctx->stream));
+        uint8_t *out = ctx->smp_dev + up;
+        if (int rc = ps_serve_sample(c, reinterpret_cast<int32_t *>(out), probs ? reinterpret_cast<float *>(out + 4 * (size_t)rows) : nullptr, ctx->logits_last, ctx->d.vocab_size, ctx->d.vocab_size, rows,
+                                     reinterpret_cast<const ps_cuda_sampler *>(ctx->smp_dev), reinterpret_cast<const float *>(ctx->smp_dev + 16 * (size_t)rows)))
+            return rc;
+        PS_CK(cudaMemcpyAsync(ctx->h_smp + up, out, down, cudaMemcpyDeviceToHost, ctx->stream));
+        if (int rc = sync_and_check(ctx)) return rc;
+        memcpy(ids, ctx->h_smp + up, 4 * (size_t)rows);
+        if (probs) memcpy(probs, ctx->h_smp + up + 4 * (size_t)rows, 4 * (size_t)rows);
+        ctx->h2d += (int64_t)up;
+        ctx->d2h += (int64_t)down;
+        return 0;
+    });
 }
 
 const float *ps_cuda_logits_dev(ps_cuda_ctx *ctx) { return ctx->logits_last ? ctx->logits_last : ctx->logits; }

@@ -46,6 +46,7 @@ int check_caches(PsServeCall *c, const char *what, const ps_cuda_cache *caches, 
     for (int i = 0; i < n; i++) {
         const ps_cuda_cache &s = caches[i];
         if (s.n_ctx <= 0 || s.n_kv < 0 || s.n_kv > s.n_ctx) return fail(c, PS_CUDA_ERR_INVALID, "%s: cache %d holds %d of %d slots", what, i, s.n_kv, s.n_ctx);
+        if (s.n_ctx > 1 << 30) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "%s: cache %d has %d slots (at most 2^30)", what, i, s.n_ctx);
         if (s.n_kv && (!s.k || !s.v)) return fail(c, PS_CUDA_ERR_INVALID, "%s: cache %d has no rows", what, i);
         if (!aligned(s.k, es) || !aligned(s.v, es) || !aligned(s.weight, 4) || !aligned(s.weight_to, 4) || !aligned(s.pos, 4) || !aligned(s.pos_to, 4))
             return fail(c, PS_CUDA_ERR_INVALID, "%s: cache %d: an array that is not aligned to its elements", what, i);
@@ -101,6 +102,9 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
     for (int i = 0; i < n_seqs; i++) {
         const ps_cuda_cache &s = caches[i];
         if (s.n_tok < 0 || s.n_tok > s.n_kv) return fail(c, PS_CUDA_ERR_INVALID, "attn_tree: sequence %d brings %d tokens, its cache holds %d", i, s.n_tok, s.n_kv);
+        if (s.weight && s.n_tok)
+            for (int o = 0; o < i && i < 4096; o++) // (beyond that many the caller is taken at their word)
+                if (caches[o].weight == s.weight && caches[o].n_tok) return fail(c, PS_CUDA_ERR_INVALID, "attn_tree: sequences %d and %d gather their weights in the same array", o, i);
         if (s.n_tok > PS_CUDA_TREE_TOKENS) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "attn_tree: sequence %d brings %d tokens (at most %d)", i, s.n_tok, PS_CUDA_TREE_TOKENS);
         tokens += s.n_tok;
     }
@@ -224,6 +228,8 @@ int ps_serve_kv_evict(PsServeCall *c, const ps_cuda_cache *caches, int n_sets, i
         if (s.n_kv && (!s.weight || !s.weight_to)) return fail(c, PS_CUDA_ERR_INVALID, "kv_evict: cache %d has no gathered weights", i);
         if ((s.pos != nullptr) != (s.pos_to != nullptr)) return fail(c, PS_CUDA_ERR_INVALID, "kv_evict: cache %d: pos and pos_to go together", i);
         if (!s.pos && (n_sink || n_recent)) return fail(c, PS_CUDA_ERR_INVALID, "kv_evict: cache %d has no positions to keep the first or latest of", i);
+        for (int o = 0; o < i && i < 4096 && s.n_kv; o++)
+            if (caches[o].n_kv && (caches[o].k == s.k || caches[o].v == s.v || caches[o].weight_to == s.weight_to)) return fail(c, PS_CUDA_ERR_INVALID, "kv_evict: caches %d and %d are the same", o, i);
         if (s.hidden) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "kv_evict: cache %d has hidden slots (every kv head moves its own)", i);
     }
     for (int first = 0; first < n_sets; first += SV_SETS) {

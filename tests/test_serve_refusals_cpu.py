@@ -48,6 +48,7 @@ int main() {
     attn("more filled than there are", I, "holds", [](ps_cuda_cache &s) { s.n_kv = 17; });
     attn("filled below zero", I, "holds", [](ps_cuda_cache &s) { s.n_kv = -1; s.n_tok = 0; });
     attn("no slots at all", I, "holds", [](ps_cuda_cache &s) { s.n_ctx = 0; });
+    attn("more slots than are taken", U, "slots", [](ps_cuda_cache &s) { s.n_ctx = (1 << 30) + 1; });
     attn("tokens below zero", I, "brings", [](ps_cuda_cache &s) { s.n_tok = -1; });
     attn("more tokens than filled", I, "brings", [](ps_cuda_cache &s) { s.n_tok = 13; });
     attn("too many tokens", U, "brings", [](ps_cuda_cache &s) { s.n_ctx = s.n_kv = 1000; s.n_tok = PS_CUDA_TREE_TOKENS + 1; });
@@ -65,6 +66,9 @@ int main() {
     attn("no output", I, "null", none, 32, 4, 2, 0, nullptr);
     expect("no caches", I, "no caches", [&](PsServeCall *c) { return ps_serve_attn_tree(c, mem, mem, nullptr, 1, 0, 32, 4, 2, nullptr, 1.f); });
     expect("caches below zero", I, "no caches", [&](PsServeCall *c) { return ps_serve_attn_tree(c, mem, mem, &good, -1, 0, 32, 4, 2, nullptr, 1.f); });
+    ps_cuda_cache two[2] = {good, good};
+    expect("weights gathered twice", I, "same array", [&](PsServeCall *c) { return ps_serve_attn_tree(c, mem, mem, two, 2, 0, 32, 4, 2, nullptr, 1.f); });
+    expect("a cache cut twice", I, "the same", [&](PsServeCall *c) { return ps_serve_kv_evict(c, two, 2, 0, 32, 2, 0, 0); });
     expect("nobody", 0, nullptr, [&](PsServeCall *c) { return ps_serve_attn_tree(c, mem, mem, nullptr, 0, 0, 32, 4, 2, nullptr, 1.f); });
 
     evict("a call that is right asks for memory", PS_CUDA_ERR_OOM, nullptr, [](ps_cuda_cache &s) { s.n_ctx = s.n_kv = 100; }, 1, 1);
