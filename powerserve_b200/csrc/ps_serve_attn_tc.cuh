@@ -38,11 +38,22 @@ PS_D uint32_t sv_pack(float a, float b) { // fp16 of a (low half) and b
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
     return r;
 }
-PS_D void sv_cut(float a, float b, uint32_t &hi, uint32_t &lo) { // hi: the upper eleven bits, as they are (no conversion back); lo: the others, rounded
+// two floats at a time: the kernel below is bound by the instructions that it issues
+using sv_f2 = unsigned long long;
+PS_D sv_f2 sv_two(float a, float b) { sv_f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+PS_D void sv_one(sv_f2 x, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+PS_D sv_f2 sv_mul2(sv_f2 a, sv_f2 b) { sv_f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+PS_D sv_f2 sv_add2(sv_f2 a, sv_f2 b) { sv_f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+PS_D sv_f2 sv_fma2(sv_f2 a, sv_f2 b, sv_f2 c) { sv_f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+PS_D void sv_cut2(sv_f2 x, uint32_t &hi, uint32_t &lo) { // hi: the upper eleven bits, as they are (no conversion back); lo: the others, rounded
+    float a, b;
+    sv_one(x, a, b);
     const float ha = __uint_as_float(__float_as_uint(a) & 0xffffe000u), hb = __uint_as_float(__float_as_uint(b) & 0xffffe000u);
     hi = sv_pack(ha, hb);
-    lo = sv_pack(a - ha, b - hb);
+    sv_one(sv_fma2(sv_two(ha, hb), sv_two(-1.f, -1.f), x), a, b);
+    lo = sv_pack(a, b);
 }
+PS_D void sv_cut(float a, float b, uint32_t &hi, uint32_t &lo) { sv_cut2(sv_two(a, b), hi, lo); }
 PS_D float sv_ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -68,6 +79,16 @@ PS_D void sv_get(SvRaw32 &r, const uint8_t *p) {
     r.b = *reinterpret_cast<const float4 *>(p + 16);
 }
 PS_D void sv_get(SvRaw16 &r, const uint8_t *p) { r.a = *reinterpret_cast<const uint4 *>(p); }
+PS_D void sv_keep(SvRaw32 &r, uint32_t m) { // zero where the bit is not set
+    r.a.x = m & 1 ? r.a.x : 0.f; r.a.y = m & 2 ? r.a.y : 0.f; r.a.z = m & 4 ? r.a.z : 0.f; r.a.w = m & 8 ? r.a.w : 0.f;
+    r.b.x = m & 16 ? r.b.x : 0.f; r.b.y = m & 32 ? r.b.y : 0.f; r.b.z = m & 64 ? r.b.z : 0.f; r.b.w = m & 128 ? r.b.w : 0.f;
+}
+PS_D void sv_keep(SvRaw16 &r, uint32_t m) {
+    uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] &= (m >> (2 * i) & 1 ? 0x0000ffffu : 0u) | (m >> (2 * i) & 2 ? 0xffff0000u : 0u);
+    r.a = make_uint4(w[0], w[1], w[2], w[3]);
+}
 PS_D float sv_at(const SvRaw32 &r, int i) {
     const float4 &q = i < 4 ? r.a : r.b;
     return i % 4 == 0 ? q.x : i % 4 == 1 ? q.y : i % 4 == 2 ? q.z : q.w;
@@ -115,30 +136,44 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
         ps_fence_barrier_init();
     }
     // Copies: a converter (of K: warps 16-19, of V: 20-23) brings the quarter of a tile's rows that it will cut, sixteen bytes a lane; one group of copies a tile
+    constexpr int COPIES = D * (int)sizeof(T) / 32, K_LANES = D * (int)sizeof(T) / 16, V_LANES = SV_TILE * (int)sizeof(T) / 16; // lanes of a row
+    const T *src = nullptr;
+    int64_t step = 0, tile_step = 0;
+    uint32_t ring_at = 0;
+    if (warp >= 20 && s.v_mode) {
+        const int row = (warp & 3) * (D / 4) + lane / V_LANES, col = lane % V_LANES;
+        src = static_cast<const T *>(s.v) + ((int64_t)g * D + row) * s.n_ctx + j0 + col * (16 / (int)sizeof(T));
+        step = (int64_t)(32 / V_LANES) * s.n_ctx;
+        tile_step = SV_TILE;
+        ring_at = ps_smem_u32(sm_v) + row * C::V_ROW + col * 16;
+    } else if (warp < 20 && s.k_mode) {
+        const int row = (warp & 3) * 16 + lane / K_LANES, col = lane % K_LANES;
+        const int64_t ld = (int64_t)a.G * D;
+        src = static_cast<const T *>(s.k) + (int64_t)(j0 + row) * ld + (int64_t)g * D + col * (16 / (int)sizeof(T));
+        step = (32 / K_LANES) * ld;
+        tile_step = SV_TILE * ld;
+        ring_at = ps_smem_u32(sm_k) + row * C::K_ROW + col * 16;
+    }
     auto bring = [&](int t) {
-        const int w = warp & 3, j = j0 + t * SV_TILE, at = t % stages;
-        if (t < tiles) {
+        const int at = t % stages, n = j_end - j0 - t * SV_TILE;
+        auto copy = [](uint32_t to, const T *p) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(p) : "memory"); };
+        if (t < tiles && src) {
+            const T *p = src + t * tile_step;
             if (warp >= 20) {
-                if (s.v_mode) {
-                    constexpr int LANES = SV_TILE * (int)sizeof(T) / 16, AT_ONCE = 32 / LANES;  // lanes of a row, rows at once
-                    const int row = w * (D / 4) + lane / LANES, col = lane % LANES;
-                    const uint32_t to = ps_smem_u32(sm_v + at * C::V_STAGE) + row * C::V_ROW + col * 16;
-                    const T *src = static_cast<const T *>(s.v) + ((int64_t)g * D + row) * s.n_ctx + j + col * (16 / (int)sizeof(T));
-                    const int64_t step = (int64_t)AT_ONCE * s.n_ctx;
-                    if (j + col * (16 / (int)sizeof(T)) < s.n_ctx) // (a row of V is read up to its own end)
+                const uint32_t to = ring_at + at * C::V_STAGE;
+                if (n >= SV_TILE || t * SV_TILE + j0 + (lane % V_LANES) * (16 / (int)sizeof(T)) < s.n_ctx) // (a row of V is read up to its own end)
 #pragma unroll
-                        for (int r = 0; r < D / 4 / AT_ONCE; r++, src += step) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + r * AT_ONCE * C::V_ROW), "l"(src) : "memory");
+                    for (int r = 0; r < COPIES; r++, p += step) copy(to + r * (32 / V_LANES) * C::V_ROW, p);
+            } else {
+                const uint32_t to = ring_at + at * C::K_STAGE;
+                if (n >= SV_TILE) {
+#pragma unroll
+                    for (int r = 0; r < COPIES; r++, p += step) copy(to + r * (32 / K_LANES) * C::K_ROW, p);
+                } else {
+                    const int row = (warp & 3) * 16 + lane / K_LANES;
+#pragma unroll 1
+                    for (int r = 0; r < COPIES && row + r * (32 / K_LANES) < n; r++, p += step) copy(to + r * (32 / K_LANES) * C::K_ROW, p);
                 }
-            } else if (s.k_mode) {
-                constexpr int LANES = D * (int)sizeof(T) / 16, AT_ONCE = 32 / LANES;
-                const int row = w * 16 + lane / LANES, col = lane % LANES;
-                const uint32_t to = ps_smem_u32(sm_k + at * C::K_STAGE) + row * C::K_ROW + col * 16;
-                const int64_t ld = (int64_t)a.G * D, step = AT_ONCE * ld;
-                const T *src = static_cast<const T *>(s.k) + (int64_t)(j + row) * ld + (int64_t)g * D + col * (16 / (int)sizeof(T));
-                const int n = j_end - j - row;
-#pragma unroll
-                for (int r = 0; r < 16 / AT_ONCE; r++, src += step)
-                    if (r * AT_ONCE < n) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + r * AT_ONCE * C::K_ROW), "l"(src) : "memory");
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -252,82 +287,83 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
     } else if (warp >= 16) {
         // ===== converters.  lane % 8 picks one of eight rows (slots of K, channels of V), lane / 8 one of four neighbouring eights of the row; a warp's quarter of a tile in
         // two parts, of which each has a factor of its own
-        const int sub = lane & 7, quad = lane >> 3;
-        const bool is_v = warp >= 20;
-        for (int t = 0; t < tiles; t++) {
-            const int st = t % stages;
-            asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 2) : "memory");
-            __syncwarp();
+        auto convert = [&](auto of_v) {
+            constexpr bool V = decltype(of_v)::value;
+            constexpr int ITS = D / 32, ROW = V ? C::V_ROW : C::K_ROW, LO = V ? C::V_LO : C::K_LO; // ITS: eights of a thread
+            const int sub = lane & 7, quad = lane >> 3, mode = V ? s.v_mode : s.k_mode, first = V ? 2 * C::V_GROUPS * (warp & 3) : 2 * (warp & 3);
+            uint8_t *ring = V ? sm_v : sm_k;
+            for (int t = 0; t < tiles; t++) {
+                const int st = t % stages;
+                const uint64_t live = live_of(t);
+                asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 2) : "memory");
+                __syncwarp();
 #pragma unroll 1
-            for (int part = 0; part < 2; part++) {
-            const int w = 2 * (warp & 3) + part;
-            constexpr int ITS = D / 32; // eights of a thread
-            const int mode = is_v ? s.v_mode : s.k_mode, j = j0 + t * SV_TILE;
-            const uint64_t live = live_of(t);
-            uint8_t *group = is_v ? sm_v + st * C::V_STAGE + w * C::V_GROUPS * 8 * C::V_ROW : sm_k + st * C::K_STAGE + w * 8 * C::K_ROW;
-            // eight i of the thread: K: 32 elements further along the row; V: the row's second half, then the next group of channels
-            typename C::Raw raw[ITS];
-            if (mode) {
-                const uint8_t *from = group + sub * (is_v ? C::V_ROW : C::K_ROW) + quad * (8 * (int)sizeof(T));
+                for (int part = 0; part < 2; part++) {
+                    uint8_t *group = ring + st * (V ? C::V_STAGE : C::K_STAGE) + (first + (V ? C::V_GROUPS * part : part)) * 8 * ROW;
+                    // eight i of the thread: K: 32 elements further along the row; V: the row's second half, then the next group of channels
+                    typename C::Raw raw[ITS];
+                    if (mode) {
+                        const uint8_t *from = group + sub * ROW + quad * (8 * (int)sizeof(T));
 #pragma unroll
-                for (int i = 0; i < ITS; i++) sv_get(raw[i], from + (is_v ? (i >> 1) * 8 * C::V_ROW + (i & 1) * (32 * (int)sizeof(T)) : i * (32 * (int)sizeof(T))));
-            } else { // rows that no bulk copy can read: element by element
+                        for (int i = 0; i < ITS; i++) sv_get(raw[i], from + (V ? (i >> 1) * 8 * ROW + (i & 1) * (32 * (int)sizeof(T)) : i * (32 * (int)sizeof(T))));
+                    } else { // rows that no wide copy can read: element by element
+                        const int w = 2 * (warp & 3) + part, j = j0 + t * SV_TILE;
 #pragma unroll
-                for (int i = 0; i < ITS; i++) {
-                    T x[8];
-                    const int slot = is_v ? (quad + 4 * (i & 1)) * 8 : w * 8 + sub;
-                    const T *src = is_v ? static_cast<const T *>(s.v) + ((int64_t)g * D + (w * C::V_GROUPS + (i >> 1)) * 8 + sub) * s.n_ctx + j + slot
-                                        : static_cast<const T *>(s.k) + (int64_t)(j + slot) * a.G * D + (int64_t)g * D + (i * 4 + quad) * 8;
+                        for (int i = 0; i < ITS; i++) {
+                            T x[8];
+                            const int slot = V ? (quad + 4 * (i & 1)) * 8 : w * 8 + sub;
+                            const T *src = V ? static_cast<const T *>(s.v) + ((int64_t)g * D + (w * C::V_GROUPS + (i >> 1)) * 8 + sub) * s.n_ctx + j + slot
+                                             : static_cast<const T *>(s.k) + (int64_t)(j + slot) * a.G * D + (int64_t)g * D + (i * 4 + quad) * 8;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        x[e] = T(0.f);
-                        if (live >> (is_v ? slot + e : slot) & 1) x[e] = src[e];
+                            for (int e = 0; e < 8; e++) {
+                                x[e] = T(0.f);
+                                if (live >> (V ? slot + e : slot) & 1) x[e] = src[e];
+                            }
+                            memcpy(&raw[i], x, sizeof raw[i]);
+                        }
                     }
-                    memcpy(&raw[i], x, sizeof raw[i]);
+                    if (live != ~0ull) { // what a slot that is not live holds, or was not copied, may be anything
+#pragma unroll
+                        for (int i = 0; i < ITS; i++) sv_keep(raw[i], V ? (uint32_t)(live >> (8 * (quad + 4 * (i & 1)))) : live >> (16 * (warp & 3) + 8 * part + sub) & 1 ? 0xffu : 0u);
+                    }
+                    float top = 0.f;
+#pragma unroll
+                    for (int i = 0; i < ITS; i++)
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) top = fmaxf(fmaxf(top, fabsf(sv_at(raw[i], e))), fabsf(sv_at(raw[i], e + 1)));
+                    float inv;
+                    const float f1 = sv_scale(__reduce_max_sync(0xffffffffu, __float_as_uint(top)), inv); // (and all lanes have read)
+                    const sv_f2 f = sv_two(f1, f1);
+                    uint8_t *to = group + sub * 16 + quad * 128;
+#pragma unroll
+                    for (int i = 0; i < ITS; i++) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const sv_f2 x = sv_mul2(sv_two(sv_at(raw[i], 2 * e), sv_at(raw[i], 2 * e + 1)), f);
+                            if (C::F32) sv_cut2(x, hi[e], lo[e]);
+                            else { // (eight bits: hi is all of it)
+                                float x0, x1;
+                                sv_one(x, x0, x1);
+                                hi[e] = sv_pack(x0, x1);
+                            }
+                        }
+                        uint8_t *p = to + (V ? (i >> 1) * 8 * ROW + (i & 1) * 512 : i * 512);
+                        *reinterpret_cast<uint4 *>(p) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        if (C::F32) *reinterpret_cast<uint4 *>(p + LO) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
+                    if (lane == 0) (V ? s_vinv : s_kinv)[t & 7][2 * (warp & 3) + part] = inv; // (who reads tile t - 8's is done: the ring's stages span three tiles, and what comes after MMAs two more)
                 }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) ps_mbar_arrive(&ready[V][st]);
+                // (what is asked for now has a tile's time to come)
+                if (t && t + stages - 1 < tiles && !ps_tc_wait_warp(&unused[V][(t - 1) % stages], ((t - 1) / stages) & 1)) { *a.err = 11; break; }
+                bring(t + stages - 1);
             }
-            float x[ITS][8], top = 0.f;
-            if (live == ~0ull) {
-#pragma unroll
-                for (int i = 0; i < ITS; i++)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[i][e] = sv_at(raw[i], e);
-            } else { // what a slot that is not live holds, or was not copied, may be anything
-#pragma unroll
-                for (int i = 0; i < ITS; i++) {
-                    const uint32_t m = is_v ? (uint32_t)(live >> (8 * (quad + 4 * (i & 1)))) : live >> (w * 8 + sub) & 1 ? 0xffu : 0u;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[i][e] = m >> e & 1 ? sv_at(raw[i], e) : 0.f;
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < ITS; i++)
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) top = fmaxf(fmaxf(top, fabsf(x[i][e])), fabsf(x[i][e + 1]));
-            float inv;
-            const float f = sv_scale(__reduce_max_sync(0xffffffffu, __float_as_uint(top)), inv); // (and all lanes have read)
-            uint8_t *to = group + sub * 16 + quad * 128;
-            const int lo_at = is_v ? C::V_LO : C::K_LO;
-#pragma unroll
-            for (int i = 0; i < ITS; i++) {
-                uint4 hi, lo;
-                sv_cut(x[i][0] * f, x[i][1] * f, hi.x, lo.x);
-                sv_cut(x[i][2] * f, x[i][3] * f, hi.y, lo.y);
-                sv_cut(x[i][4] * f, x[i][5] * f, hi.z, lo.z);
-                sv_cut(x[i][6] * f, x[i][7] * f, hi.w, lo.w);
-                uint8_t *p = to + (is_v ? (i >> 1) * 8 * C::V_ROW + (i & 1) * 512 : i * 512);
-                *reinterpret_cast<uint4 *>(p) = hi;
-                if (C::F32) *reinterpret_cast<uint4 *>(p + lo_at) = lo;
-            }
-            if (lane == 0) (is_v ? s_vinv : s_kinv)[t & 7][w] = inv; // (who reads tile t - 8's is done: the ring's stages span three tiles, and what comes after MMAs two more)
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) ps_mbar_arrive(&ready[is_v][st]);
-            // (what is asked for now has a tile's time to come)
-            if (t && t + stages - 1 < tiles && !ps_tc_wait_warp(&unused[is_v][(t - 1) % stages], ((t - 1) / stages) & 1)) { *a.err = 11; break; }
-            bring(t + stages - 1);
-        }
+        };
+        if (warp >= 20) convert(std::true_type{});
+        else convert(std::false_type{});
         asm volatile("cp.async.wait_all;" ::: "memory"); // (what is in flight ends before the CTA does, even when a wait gave up)
     } else if (warp < 8) {
         // ===== soft-max: thread = row, warps 0-3 take a tile's first 32 slots, 4-7 the others
@@ -346,29 +382,26 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
             ps_tc_fence_after();
             __syncwarp();
             uint32_t v[32];
-            float mx = SV_NONE;
+            float mx = SV_NONE, f[4];
             if (any && ok) {
                 uint32_t (&va)[16] = *reinterpret_cast<uint32_t (*)[16]>(v), (&vb)[16] = *reinterpret_cast<uint32_t (*)[16]>(v + 16);
                 sv_tm_ld16(va, tm_s + b * SV_TILE + 32 * half + lane_at);
                 sv_tm_ld16(vb, tm_s + b * SV_TILE + 32 * half + 16 + lane_at);
                 const float4 ki = *reinterpret_cast<const float4 *>(&s_kinv[t & 7][4 * half]);
                 // (never zero: -inf times it is -inf)
-                const float f[4] = {fmaxf(qinv * ki.x, 0x1p-126f), fmaxf(qinv * ki.y, 0x1p-126f), fmaxf(qinv * ki.z, 0x1p-126f), fmaxf(qinv * ki.w, 0x1p-126f)};
+                f[0] = fmaxf(qinv * ki.x, 0x1p-126f); f[1] = fmaxf(qinv * ki.y, 0x1p-126f); f[2] = fmaxf(qinv * ki.z, 0x1p-126f); f[3] = fmaxf(qinv * ki.w, 0x1p-126f);
                 ps_tc_ld_wait();
-#pragma unroll
-                for (int c = 0; c < 32; c++) v[c] = __float_as_uint(__uint_as_float(v[c]) * f[c / 8]);
                 if (!whole) {
 #pragma unroll
                     for (int c = 0; c < 32; c++)
                         if (!(see >> c & 1)) v[c] = __float_as_uint(SV_NONE);
                 }
-                float t0 = SV_NONE, t1 = SV_NONE;
+                float top[4] = {SV_NONE, SV_NONE, SV_NONE, SV_NONE};
 #pragma unroll
-                for (int c = 0; c < 16; c += 2) {
-                    t0 = fmaxf(fmaxf(t0, __uint_as_float(v[c])), __uint_as_float(v[c + 1]));
-                    t1 = fmaxf(fmaxf(t1, __uint_as_float(v[c + 16])), __uint_as_float(v[c + 17]));
-                }
-                mx = fmaxf(t0, t1);
+                for (int c = 0; c < 8; c += 2)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) top[e] = fmaxf(fmaxf(top[e], __uint_as_float(v[8 * e + c])), __uint_as_float(v[8 * e + c + 1]));
+                mx = fmaxf(fmaxf(top[0] * f[0], top[1] * f[1]), fmaxf(top[2] * f[2], top[3] * f[3]));
             }
             s_half[b][half][r] = mx;
             ps_tc_fence_before();
@@ -381,27 +414,32 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
                 if (s.scores && mine) {
                     float4 *to = reinterpret_cast<float4 *>(s.scores) + ((int64_t)g * sv_quads(s.n_kv) + j / 4) * rp + row;
 #pragma unroll
-                    for (int c = 0; c < 32; c += 4) to[(int64_t)(c / 4) * rp] = make_float4(__uint_as_float(v[c]), __uint_as_float(v[c + 1]), __uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
+                    for (int c = 0; c < 32; c += 4) to[(int64_t)(c / 4) * rp] = make_float4(__uint_as_float(v[c]) * f[c / 8], __uint_as_float(v[c + 1]) * f[c / 8], __uint_as_float(v[c + 2]) * f[c / 8], __uint_as_float(v[c + 3]) * f[c / 8]);
                 }
                 mx = fmaxf(mx, s_half[b][half ^ 1][r]);
                 // the weights are 2^15 p, and so is their sum
                 const float shift = mx == SV_NONE ? 15.f : 15.f - mx;
-                float sum = 0.f, sum1 = 0.f;
+                const sv_f2 shift2 = sv_two(shift, shift);
+                sv_f2 sum = 0ull;
 #pragma unroll
                 for (int c = 0; c < 32; c += 16) {
                     uint32_t hi[8], lo[8];
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        const float p0 = sv_ex2(__uint_as_float(v[c + 2 * e]) + shift), p1 = sv_ex2(__uint_as_float(v[c + 2 * e + 1]) + shift);
-                        sum += p0;
-                        sum1 += p1;
-                        sv_cut(p0, p1, hi[e], lo[e]);
+                        const float fe = f[(c + 2 * e) / 8];
+                        float p0, p1;
+                        sv_one(sv_fma2(sv_two(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1])), sv_two(fe, fe), shift2), p0, p1);
+                        const sv_f2 p = sv_two(sv_ex2(p0), sv_ex2(p1));
+                        sum = sv_add2(sum, p);
+                        sv_cut2(p, hi[e], lo[e]);
                     }
                     sv_tm_st8(tm_p + b * SV_TILE + 16 * half + c / 2 + lane_at, hi);
                     sv_tm_st8(tm_p + b * SV_TILE + SV_TILE / 2 + 16 * half + c / 2 + lane_at, lo);
                 }
                 s_top[b][r] = mx; // (both warps write the same)
-                s_sum[b][half][r] = sum + sum1;
+                float sum0, sum1;
+                sv_one(sum, sum0, sum1);
+                s_sum[b][half][r] = sum0 + sum1;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             }
             ps_tc_fence_before();
@@ -414,24 +452,28 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
         const int half = (warp - 8) >> 2, r = (warp & 3) * 32 + lane, row = r0 + r;
         const bool any = (warp & 3) * 32 < rows;
         const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
-        float acc[D / 2], m = SV_NONE, l = 0.f;
+        sv_f2 acc[D / 4];
+        float m = SV_NONE, l = 0.f;
         bool ok = true;
 #pragma unroll
-        for (int c = 0; c < D / 2; c++) acc[c] = 0.f;
+        for (int c = 0; c < D / 4; c++) acc[c] = 0ull;
         for (int t = 0; t < tiles; t++) {
             const int b = t & 1;
             sv_bar_wait(&o_full[b], (t >> 1) & 1, ok, a.err, 22);
             if (!ok) break;
             ps_tc_fence_after();
             if (any) {
-                const float top = s_top[b][r], mn = fmaxf(m, top), ref = mn == SV_NONE ? 0.f : mn, fo = sv_ex2(m - ref), fn = sv_ex2(top - ref);
+                // (what has been added up changes its reference when a maximum is 2^8 above it, or the first there is: seldom)
+                const float top = s_top[b][r];
+                const bool up = top > m + 8.f;
+                const float mn = up ? top : m, ref = mn == SV_NONE ? 0.f : mn, fo = up ? sv_ex2(m - ref) : 1.f, fn = sv_ex2(top - ref);
                 const float4 vi = *reinterpret_cast<const float4 *>(&s_vinv[t & 7][4 * half]);
-                const float f[4] = {fn * vi.x, fn * vi.y, fn * vi.z, fn * vi.w};
+                const sv_f2 f[4] = {sv_two(fn * vi.x, fn * vi.x), sv_two(fn * vi.y, fn * vi.y), sv_two(fn * vi.z, fn * vi.z), sv_two(fn * vi.w, fn * vi.w)};
                 l = fmaf(l, fo, (s_sum[b][0][r] + s_sum[b][1][r]) * fn);
                 m = mn;
-                if (__any_sync(0xffffffffu, fo != 1.f)) {
+                if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
-                    for (int c = 0; c < D / 2; c++) acc[c] *= fo;
+                    for (int c = 0; c < D / 4; c++) acc[c] = sv_mul2(acc[c], sv_two(fo, fo));
                 }
 #pragma unroll
                 for (int c = 0; c < D / 2; c += 16) {
@@ -439,7 +481,7 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
                     sv_tm_ld16(v, tm_o + (D == 64 ? b * D : 0) + half * (D / 2) + c + lane_at);
                     ps_tc_ld_wait();
 #pragma unroll
-                    for (int e = 0; e < 16; e++) acc[c + e] = fmaf(__uint_as_float(v[e]), f[(c + e) / (D / 8)], acc[c + e]);
+                    for (int e = 0; e < 16; e += 2) acc[(c + e) / 2] = sv_fma2(sv_two(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), f[(c + e) / (D / 8)], acc[(c + e) / 2]);
                 }
             }
             ps_tc_fence_before();
@@ -451,12 +493,13 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
             const float f = s.splits == 1 ? (l > 0.f ? 1.f / l : 0.f) : 1.f / 32768.f;
             float *to = s.splits == 1 ? a.out + ((int64_t)(s.tok0 + row / a.R) * a.n_heads + g * a.R + row % a.R) * D : s.part + (((int64_t)split * a.G + g) * all_rows + row) * D;
             to += half * (D / 2);
-            if (a.out_vec || s.splits > 1) {
 #pragma unroll
-                for (int c = 0; c < D / 2; c += 4) *reinterpret_cast<float4 *>(to + c) = make_float4(acc[c] * f, acc[c + 1] * f, acc[c + 2] * f, acc[c + 3] * f);
-            } else {
-#pragma unroll
-                for (int c = 0; c < D / 2; c++) to[c] = acc[c] * f;
+            for (int c = 0; c < D / 2; c += 4) {
+                float x[4];
+                sv_one(sv_mul2(acc[c / 2], sv_two(f, f)), x[0], x[1]);
+                sv_one(sv_mul2(acc[c / 2 + 1], sv_two(f, f)), x[2], x[3]);
+                if (a.out_vec || s.splits > 1) *reinterpret_cast<float4 *>(to + c) = make_float4(x[0], x[1], x[2], x[3]);
+                else { to[c] = x[0]; to[c + 1] = x[1]; to[c + 2] = x[2]; to[c + 3] = x[3]; }
             }
         }
     }
