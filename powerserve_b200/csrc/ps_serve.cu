@@ -185,9 +185,12 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
                     kern<<<grid, SV_TC_THREADS, smem, c->stream>>>(a);
                     return 0;
                 };
-                const bool f32 = cache_type == PS_TYPE_F32;
-                const int rc = hs == 64 ? (f32 ? launch(sv_k_attn_tc<float, 64>, SvTc<float, 64>::SMEM) : launch(sv_k_attn_tc<__nv_bfloat16, 64>, SvTc<__nv_bfloat16, 64>::SMEM))
-                                        : (f32 ? launch(sv_k_attn_tc<float, 128>, SvTc<float, 128>::SMEM) : launch(sv_k_attn_tc<__nv_bfloat16, 128>, SvTc<__nv_bfloat16, 128>::SMEM));
+                auto pick = [&](auto w) -> int { // (with weights the soft-max needs more registers)
+                    constexpr bool W = decltype(w)::value;
+                    if (cache_type == PS_TYPE_F32) return hs == 64 ? launch(sv_k_attn_tc<float, 64, W>, SvTc<float, 64>::SMEM) : launch(sv_k_attn_tc<float, 128, W>, SvTc<float, 128>::SMEM);
+                    return hs == 64 ? launch(sv_k_attn_tc<__nv_bfloat16, 64, W>, SvTc<__nv_bfloat16, 64>::SMEM) : launch(sv_k_attn_tc<__nv_bfloat16, 128, W>, SvTc<__nv_bfloat16, 128>::SMEM);
+                };
+                const int rc = weights ? pick(std::true_type{}) : pick(std::false_type{});
                 if (rc) return rc;
             } else if (cache_type == PS_TYPE_F32) {
                 const size_t smem = sv_attn_smem(hs);

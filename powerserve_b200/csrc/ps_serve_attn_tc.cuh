@@ -110,7 +110,7 @@ template <typename T, int D> struct SvTc {
     using Raw = typename std::conditional<F32, SvRaw32, SvRaw16>::type;
 };
 
-template <typename T, int D>
+template <typename T, int D, bool W>
 __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_constant__ SvAttn a) {
     using C = SvTc<T, D>;
     extern __shared__ __align__(128) uint8_t sv_tc_raw[];
@@ -195,6 +195,15 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
         if (s.hidden) return s_live[t];
         const int n = j_end - j0 - t * SV_TILE;
         return n >= SV_TILE ? ~0ull : (1ull << n) - 1;
+    };
+    // which of a tile's 32 slots from `half` on token `tok` sees
+    auto see_of = [&](int t, int half, int tok, bool mine) -> uint32_t {
+        const int j = j0 + t * SV_TILE + 32 * half;
+        uint32_t see = (uint32_t)(live_of(t) >> (32 * half));
+        if (j + 32 > past && mine) // of the step's own slots those that this token sees
+            for (int c = max(0, past - j); c < min(32, j_end - j); c++)
+                if (!sv_sees(s, tok, j + c - past)) see &= ~(1u << c);
+        return see;
     };
     // queries: warps 0-3 the first half of the channels, 4-7 the second, a thread its half of a row
     float4 qv[D / 8];
@@ -372,11 +381,8 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
         const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
         bool ok = true;
         for (int t = 0; t < tiles; t++) {
-            const int b = t & 1, j = j0 + t * SV_TILE + 32 * half;
-            uint32_t see = (uint32_t)(live_of(t) >> (32 * half));
-            if (j + 32 > past && mine) // of the step's own slots those that this token sees
-                for (int c = max(0, past - j); c < min(32, j_end - j); c++)
-                    if (!sv_sees(s, tok, j + c - past)) see &= ~(1u << c);
+            const int b = t & 1;
+            const uint32_t see = see_of(t, half, tok, mine);
             const bool whole = __all_sync(0xffffffffu, see == ~0u);
             sv_bar_wait(&s_full[b], (t >> 1) & 1, ok, a.err, 18);
             ps_tc_fence_after();
@@ -411,11 +417,6 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
             ok = ps_bar_all(1 + (warp & 3), 64, ok); // the two warps of the same rows go on together, or give up together
             if (!ok) break;
             if (any) {
-                if (s.scores && mine) {
-                    float4 *to = reinterpret_cast<float4 *>(s.scores) + ((int64_t)g * sv_quads(s.n_kv) + j / 4) * rp + row;
-#pragma unroll
-                    for (int c = 0; c < 32; c += 4) to[(int64_t)(c / 4) * rp] = make_float4(__uint_as_float(v[c]) * f[c / 8], __uint_as_float(v[c + 1]) * f[c / 8], __uint_as_float(v[c + 2]) * f[c / 8], __uint_as_float(v[c + 3]) * f[c / 8]);
-                }
                 mx = fmaxf(mx, s_half[b][half ^ 1][r]);
                 // the weights are 2^15 p, and so is their sum
                 const float shift = mx == SV_NONE ? 15.f : 15.f - mx;
@@ -445,6 +446,11 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
             ps_tc_fence_before();
             __syncwarp();
             if (lane == 0) ps_mbar_arrive(&p_full[b]);
+            if (W && s.scores && mine) { // (nothing waits for them)
+                float4 *to = reinterpret_cast<float4 *>(s.scores) + ((int64_t)g * sv_quads(s.n_kv) + (j0 + t * SV_TILE + 32 * half) / 4) * rp + row;
+#pragma unroll
+                for (int c = 0; c < 32; c += 4, to += rp) *to = make_float4(__uint_as_float(v[c]) * f[c / 8], __uint_as_float(v[c + 1]) * f[c / 8], __uint_as_float(v[c + 2]) * f[c / 8], __uint_as_float(v[c + 3]) * f[c / 8]);
+            }
         }
     } else {
         // ===== output: thread = row, half of the channels; the row's maximum and sum so far
