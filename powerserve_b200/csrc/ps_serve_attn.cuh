@@ -39,6 +39,11 @@ struct SvAttn {
 
 PS_D float sv_ld(const float *p, int64_t i) { return p[i]; }
 PS_D float sv_ld(const __nv_bfloat16 *p, int64_t i) { return __bfloat162float(p[i]); }
+PS_D float sv_ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 PS_HD int sv_rp(int rows) { return (rows + 3) & ~3; }
 PS_HD int64_t sv_quads(int n_kv) { return (int64_t)((n_kv + SV_TILE - 1) / SV_TILE) * (SV_TILE / 4); }
 PS_D int sv_find(const SvAttn &a, int unit) {
@@ -204,46 +209,68 @@ __global__ void __launch_bounds__(256) sv_k_join(const __grid_constant__ SvAttn 
         if (c * 32 < hs) to[c * 32 + lane] = acc[c] * inv;
 }
 
-// x: 256 slots of a sequence's kv head y: their weights.  Lanes take rows, four slots each; two such quads are under way at a time
+// x: 256 slots of a sequence's kv head y: their weights.  PER lanes take rows, four slots each, two such quads at a time; then the lanes exchange halves of their eight sums
+// until each has sums of its own (nine shuffles for 32 lanes instead of forty), the old weights are there by then.  Bound by memory: two sequences of 32 700 slots, 128 rows
+// of each of 8 kv heads, 268 MB
 #define SV_FIN_SLOTS 256
+template <int PER> PS_D void sv_weights(const SvSeq &s, const float *lse, int rows, int g, int j0) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = lane % PER, rp = sv_rp(rows);
+    constexpr int AT = 32 / PER, N = PER >= 8 ? 1 : 8 / PER; // quads of a warp; sums that a lane ends with
+    const float4 *z0 = reinterpret_cast<const float4 *>(s.scores) + ((int64_t)g * sv_quads(s.n_kv) + j0 / 4) * rp;
+    float *w0 = s.weight + (int64_t)g * s.n_ctx + j0;
+    const int n = s.n_kv - j0;
+    int first = 0; // number of the first sum that the lane ends with: quad, slot
+#pragma unroll
+    for (int o = PER / 2, half = 4; o && half; o /= 2, half /= 2) first += at & o ? half : 0;
+    const bool writes = PER <= 8 || at % (PER > 8 ? PER / 8 : 1) == 0;
+    for (int b = warp * 2 * AT; b < SV_FIN_SLOTS / 4 && 4 * b < n; b += 16 * AT) {
+        const int q[2] = {b + lane / PER, b + AT + lane / PER};
+        const bool in[2] = {q[0] < SV_FIN_SLOTS / 4 && 4 * q[0] < n, q[1] < SV_FIN_SLOTS / 4 && 4 * q[1] < n};
+        float old[N], v[8] = {};
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            const int i = first + e, slot = 4 * (i >= 4 ? q[1] : q[0]) + i % 4;
+            old[e] = writes && (i >= 4 ? in[1] : in[0]) && slot < n ? w0[slot] : 0.f;
+        }
+#pragma unroll 4
+        for (int row = at; row < rows; row += PER) {
+            const float4 none = make_float4(SV_NONE, SV_NONE, SV_NONE, SV_NONE);
+            const float4 a = in[0] ? __ldcs(z0 + (int64_t)q[0] * rp + row) : none, c = in[1] ? __ldcs(z0 + (int64_t)q[1] * rp + row) : none;
+            const float l = lse[row];
+            v[0] += sv_ex2(a.x - l); v[1] += sv_ex2(a.y - l); v[2] += sv_ex2(a.z - l); v[3] += sv_ex2(a.w - l);
+            v[4] += sv_ex2(c.x - l); v[5] += sv_ex2(c.y - l); v[6] += sv_ex2(c.z - l); v[7] += sv_ex2(c.w - l);
+        }
+#pragma unroll
+        for (int o = PER / 2, half = 4; o; o /= 2, half /= 2) {
+            if (half) {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (e < half) {
+                        const float keep = at & o ? v[e + half] : v[e], give = at & o ? v[e] : v[e + half];
+                        v[e] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+                    }
+            } else v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+        }
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            const int i = first + e, slot = 4 * (i >= 4 ? q[1] : q[0]) + i % 4;
+            if (writes && (i >= 4 ? in[1] : in[0]) && slot < n) w0[slot] = old[e] + v[e];
+        }
+    }
+}
 __global__ void __launch_bounds__(256) sv_k_weights(const __grid_constant__ SvAttn a) {
     extern __shared__ float sv_lse[];
     ps_grid_dep_wait();
-    const int tid = threadIdx.x, g = blockIdx.y;
+    const int g = blockIdx.y, j0 = blockIdx.x * SV_FIN_SLOTS;
     const SvSeq &s = a.seq[blockIdx.z];
-    const int rows = s.n_tok * a.R, j0 = blockIdx.x * SV_FIN_SLOTS;
+    const int rows = s.n_tok * a.R;
     if (!s.scores || j0 >= s.n_kv) return;
-    for (int row = tid; row < rows; row += 256) sv_lse[row] = s.lse[(int64_t)g * rows + row];
+    for (int row = threadIdx.x; row < rows; row += 256) sv_lse[row] = s.lse[(int64_t)g * rows + row];
     __syncthreads();
-    const int rp = sv_rp(rows);
-    int per = 1;                                          // lanes of a quad of slots: a power of two
-    while (per < 32 && per < rows) per *= 2;
-    const int at_once = 256 / per;
-    const float4 *z0 = reinterpret_cast<const float4 *>(s.scores) + ((int64_t)g * sv_quads(s.n_kv) + j0 / 4) * rp;
-    for (int b = 0; b < SV_FIN_SLOTS / 4; b += 2 * at_once) {
-        const int qa = b + tid / per, qb = qa + at_once;
-        const bool ina = qa < SV_FIN_SLOTS / 4 && j0 + 4 * qa < s.n_kv, inb = qb < SV_FIN_SLOTS / 4 && j0 + 4 * qb < s.n_kv;
-        float sa[4] = {}, sb[4] = {};
-#pragma unroll 4
-        for (int row = tid % per; row < rows; row += per) {
-            const float4 none = make_float4(SV_NONE, SV_NONE, SV_NONE, SV_NONE);
-            const float4 va = ina ? __ldcs(z0 + (int64_t)qa * rp + row) : none, vb = inb ? __ldcs(z0 + (int64_t)qb * rp + row) : none;
-            const float lse = sv_lse[row];
-            sa[0] += exp2f(va.x - lse); sa[1] += exp2f(va.y - lse); sa[2] += exp2f(va.z - lse); sa[3] += exp2f(va.w - lse);
-            sb[0] += exp2f(vb.x - lse); sb[1] += exp2f(vb.y - lse); sb[2] += exp2f(vb.z - lse); sb[3] += exp2f(vb.w - lse);
-        }
-        for (int o = per / 2; o; o >>= 1)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                sa[e] += __shfl_xor_sync(0xffffffffu, sa[e], o);
-                sb[e] += __shfl_xor_sync(0xffffffffu, sb[e], o);
-            }
-        if (tid % per == 0) {
-            float *w = s.weight + (int64_t)g * s.n_ctx + j0;
-            for (int e = 0; e < 4; e++) {
-                if (ina && j0 + 4 * qa + e < s.n_kv) w[4 * qa + e] += sa[e];
-                if (inb && j0 + 4 * qb + e < s.n_kv) w[4 * qb + e] += sb[e];
-            }
-        }
-    }
+    if (rows > 16) sv_weights<32>(s, sv_lse, rows, g, j0);
+    else if (rows > 8) sv_weights<16>(s, sv_lse, rows, g, j0);
+    else if (rows > 4) sv_weights<8>(s, sv_lse, rows, g, j0);
+    else if (rows > 2) sv_weights<4>(s, sv_lse, rows, g, j0);
+    else if (rows > 1) sv_weights<2>(s, sv_lse, rows, g, j0);
+    else sv_weights<1>(s, sv_lse, rows, g, j0);
 }

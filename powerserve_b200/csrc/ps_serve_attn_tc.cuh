@@ -54,11 +54,6 @@ PS_D void sv_cut2(sv_f2 x, uint32_t &hi, uint32_t &lo) { // hi: the upper eleven
     lo = sv_pack(a, b);
 }
 PS_D void sv_cut(float a, float b, uint32_t &hi, uint32_t &lo) { sv_cut2(sv_two(a, b), hi, lo); }
-PS_D float sv_ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
 PS_D void sv_tm_ld16(uint32_t (&v)[16], uint32_t at) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]),
@@ -449,7 +444,7 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
             if (W && s.scores && mine) { // (nothing waits for them)
                 float4 *to = reinterpret_cast<float4 *>(s.scores) + ((int64_t)g * sv_quads(s.n_kv) + (j0 + t * SV_TILE + 32 * half) / 4) * rp + row;
 #pragma unroll
-                for (int c = 0; c < 32; c += 4, to += rp) *to = make_float4(__uint_as_float(v[c]) * f[c / 8], __uint_as_float(v[c + 1]) * f[c / 8], __uint_as_float(v[c + 2]) * f[c / 8], __uint_as_float(v[c + 3]) * f[c / 8]);
+                for (int c = 0; c < 32; c += 4, to += rp) __stcs(to, make_float4(__uint_as_float(v[c]) * f[c / 8], __uint_as_float(v[c + 1]) * f[c / 8], __uint_as_float(v[c + 2]) * f[c / 8], __uint_as_float(v[c + 3]) * f[c / 8]));
             }
         }
     } else {
