@@ -8,8 +8,8 @@
 // A tile's output leaves the tensor memory after every tile and is added up in registers, with rounding: the accumulator, which truncates, sees the
 // MMAs of one tile alone.  So groups' factors and a row's maximum may differ from tile to tile, and the soft-max of a tile knows of no other tile.
 //
-// A CTA takes up to 128 query rows (the MMAs' M side: one row, one lane of tensor memory) of one kv head over one split.  Warps 0-3 and 4-7: soft-max of a
-// tile's first and last 32 slots; 8-15: output, a row's channels in two halves; 16-23: copies and conversion; 24, 25: MMAs (26, 27 make the warpgroup whole).
+// A CTA takes up to 128 query rows (the MMAs' M side: one row, one lane of tensor memory) of one kv head over one split.  Warps 0-3 and 4-7: soft-max of
+// every other tile; 8-15: output, a row's channels in two halves; 16-23: copies and conversion; 24, 25: MMAs (26, 27 make the warpgroup whole).
 // Tiles of K and of V go through rings of three shared-memory stages each (six small ones).  A converter warp brings the rows that it will cut, two tiles ahead, as they lie
 // in memory, by asynchronous 16-byte copies, cuts them into parts in their place (eight rows become the same eight rows' parts in the K-major
 // no-swizzle layout, in the same bytes), and the MMAs read them.  Rows are 16 bytes apart from the next so that neither reading nor writing meets a bank twice.
@@ -109,10 +109,10 @@ template <typename T, int D, bool W>
 __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_constant__ SvAttn a) {
     using C = SvTc<T, D>;
     extern __shared__ __align__(128) uint8_t sv_tc_raw[];
-    __shared__ __align__(8) uint64_t ready[2][C::STAGES], unused[2][C::STAGES], s_full[2], s_free[2], p_full[2], o_full[2], o_empty[2], done;
+    __shared__ __align__(8) uint64_t ready[2][C::STAGES], unused[2][C::STAGES], s_full[4], p_full[4], sp_free[4], o_full[2], o_empty[2], done;
     __shared__ uint32_t tmem_smem;
-    __shared__ float s_top[2][SV_TC_ROWS], s_sum[2][2][SV_TC_ROWS], s_half[2][2][SV_TC_ROWS], s_qtop[2][SV_TC_ROWS];
-    __shared__ __align__(16) float s_kinv[8][8], s_vinv[8][8];
+    __shared__ float s_top[8][SV_TC_ROWS], s_sum[8][SV_TC_ROWS], s_qtop[2][SV_TC_ROWS];
+    __shared__ __align__(16) float s_kinv[16][8], s_vinv[16][8];
     __shared__ uint64_t s_live[SV_TC_TILES];
     uint8_t *sm_k = reinterpret_cast<uint8_t *>(((uintptr_t)sv_tc_raw + 127) & ~(uintptr_t)127), *sm_v = sm_k + C::STAGES * C::K_STAGE;
     constexpr int stages = C::STAGES;
@@ -126,7 +126,8 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
     if (tid == 0) {
         for (int b = 0; b < stages; b++)
             for (int v = 0; v < 2; v++) { ps_mbar_init(&ready[v][b], 4); ps_mbar_init(&unused[v][b], 1); }
-        for (int b = 0; b < 2; b++) { ps_mbar_init(&s_full[b], 1); ps_mbar_init(&s_free[b], 8); ps_mbar_init(&p_full[b], 8); ps_mbar_init(&o_full[b], 1); ps_mbar_init(&o_empty[b], 8); }
+        for (int b = 0; b < 4; b++) { ps_mbar_init(&s_full[b], 1); ps_mbar_init(&p_full[b], 4); ps_mbar_init(&sp_free[b], 1); }
+        for (int b = 0; b < 2; b++) { ps_mbar_init(&o_full[b], 1); ps_mbar_init(&o_empty[b], 8); }
         ps_mbar_init(&done, 2);
         ps_fence_barrier_init();
     }
@@ -191,13 +192,13 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
         const int n = j_end - j0 - t * SV_TILE;
         return n >= SV_TILE ? ~0ull : (1ull << n) - 1;
     };
-    // which of a tile's 32 slots from `half` on token `tok` sees
-    auto see_of = [&](int t, int half, int tok, bool mine) -> uint32_t {
-        const int j = j0 + t * SV_TILE + 32 * half;
-        uint32_t see = (uint32_t)(live_of(t) >> (32 * half));
-        if (j + 32 > past && mine) // of the step's own slots those that this token sees
-            for (int c = max(0, past - j); c < min(32, j_end - j); c++)
-                if (!sv_sees(s, tok, j + c - past)) see &= ~(1u << c);
+    // which of a tile's slots token `tok` sees
+    auto see_of = [&](int t, int tok, bool mine) -> uint64_t {
+        const int j = j0 + t * SV_TILE;
+        uint64_t see = live_of(t);
+        if (j + SV_TILE > past && mine) // of the step's own slots those that this token sees
+            for (int c = max(0, past - j); c < min(SV_TILE, j_end - j); c++)
+                if (!sv_sees(s, tok, j + c - past)) see &= ~(1ull << c);
         return see;
     };
     // queries: warps 0-3 the first half of the channels, 4-7 the second, a thread its half of a row
@@ -221,8 +222,8 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
     ps_tc_fence_before();
     __syncthreads();
     ps_tc_fence_after();
-    // columns of tensor memory: scores 2 x 64, weights 2 x (32 + 32), outputs 128 (head size 64: two), queries D / 2 + D / 2
-    const uint32_t tm = __shfl_sync(0xffffffffu, tmem_smem, 0), tm_s = tm, tm_p = tm + 2 * SV_TILE, tm_o = tm + 4 * SV_TILE, tm_q = tm_o + 128;
+    // columns of tensor memory: four tiles' scores of 64, sixteen of which become eight of the weights' hi parts and eight of lo; outputs 128 (head size 64: two); queries D / 2 + D / 2
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem_smem, 0), tm_s = tm, tm_o = tm + 4 * SV_TILE, tm_q = tm_o + 128;
     float qinv = 1.f;
     if (warp < 8) {
         const int r = (warp & 3) * 32 + lane;
@@ -245,7 +246,8 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
     __syncthreads();
     ps_tc_fence_after();
     // A barrier is waited on only by who must have passed it before it can complete again (a phase that was missed would never end): groups' and rows' factors
-    // come with the MMAs' barrier, whose issuer has waited for those who wrote them.
+    // come with the MMAs' barrier, whose issuer has waited for those who wrote them.  Scores of tile t are asked for when the outputs of tile t - 4 are there, those when tile t - 6
+    // has been taken out: so eight places for maxima and sums are enough.
     // Registers: 72 a thread at the launch, 504 over the seven warpgroups; 2 x 72 (soft-max) + 2 x 88 (output) + 2 x 72 (converters) + 40 (MMAs, copies) = 504
 
     if (warp >= 24) {
@@ -256,31 +258,33 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
             const uint32_t idesc = (1u << 4) | ((uint32_t)((pv ? D : SV_TILE) >> 3) << 17) | ((uint32_t)(SV_TC_ROWS >> 4) << 24);
             const uint64_t desc = ps_tc_smem_desc(ps_smem_u32(pv ? sm_v : sm_k), 128, 8 * (pv ? C::V_ROW : C::K_ROW));
             for (int t = 0; t < tiles; t++) {
-                const int b = t & 1, at = t % stages;
+                const int b = t & 1, sp = t & 3, at = t % stages;
                 if (!ps_tc_wait_warp(&ready[pv][at], (t / stages) & 1)) { *a.err = 12; break; }
-                if (pv) { // (head size 128: there is one output, and the tile before has to be out of it)
-                    if (!ps_tc_wait_warp(&p_full[b], (t >> 1) & 1)) { *a.err = 15; break; }
-                    if (D == 128 && t && !ps_tc_wait_warp(&o_empty[b ^ 1], ((t - 1) >> 1) & 1)) { *a.err = 13; break; }
-                } else if (t >= 2 && !ps_tc_wait_warp(&s_free[b], ((t >> 1) - 1) & 1)) { *a.err = 14; break; } // (the scores of tile t - 2 have been read)
+                if (pv) { // (head size 128: there is one output, and the tile before has to be out of it; 64: the one before that)
+                    constexpr int AGO = D == 128 ? 1 : 2;
+                    if (!ps_tc_wait_warp(&p_full[sp], (t >> 2) & 1)) { *a.err = 15; break; }
+                    if (t >= AGO && !ps_tc_wait_warp(&o_empty[(t - AGO) & 1], ((t - AGO) >> 1) & 1)) { *a.err = 13; break; }
+                } else if (t >= 4 && !ps_tc_wait_warp(&sp_free[sp], ((t >> 2) - 1) & 1)) { *a.err = 14; break; } // (the weights of tile t - 4 are used up)
                 ps_tc_fence_after();
                 const uint64_t d = desc + (uint64_t)(at * ((pv ? C::V_STAGE : C::K_STAGE) >> 4));
+                const uint32_t tile = tm_s + sp * SV_TILE;
                 if (ps_elect_one()) {
                     if (pv) {
-                        const uint32_t pa = tm_p + b * SV_TILE;
 #pragma unroll
                         for (int p = 0; p < C::PARTS + 1; p++)
 #pragma unroll
                             for (int j = 0; j < SV_TILE / 16; j++)
-                                ps_tc_mma_f16_ta(tm_o + (D == 64 ? b * D : 0), pa + (p == 0 ? SV_TILE / 2 : 0) + j * 8, d + (C::F32 && p == 1 ? C::V_LO >> 4 : 0) + j * 16, idesc, (p | j) != 0);
+                                ps_tc_mma_f16_ta(tm_o + (D == 64 ? b * D : 0), tile + j * 16 + (p == 0 ? 8 : 0), d + (C::F32 && p == 1 ? C::V_LO >> 4 : 0) + j * 16, idesc, (p | j) != 0);
+                        ps_tc_commit(&sp_free[sp]);
+                        ps_tc_commit(&o_full[b]);
                     } else {
-                        const uint32_t to = tm_s + b * SV_TILE;
 #pragma unroll
                         for (int p = 0; p < C::PARTS + 1; p++) // lo hi, hi lo, hi hi (bfloat16 caches: lo hi, hi hi)
 #pragma unroll
-                            for (int j = 0; j < D / 16; j++) ps_tc_mma_f16_ta(to, tm_q + (p == 0 ? D / 2 : 0) + j * 8, d + (C::F32 && p == 1 ? C::K_LO >> 4 : 0) + j * 16, idesc, (p | j) != 0);
+                            for (int j = 0; j < D / 16; j++) ps_tc_mma_f16_ta(tile, tm_q + (p == 0 ? D / 2 : 0) + j * 8, d + (C::F32 && p == 1 ? C::K_LO >> 4 : 0) + j * 16, idesc, (p | j) != 0);
+                        ps_tc_commit(&s_full[sp]);
                     }
                     ps_tc_commit(&unused[pv][at]);
-                    ps_tc_commit(pv ? &o_full[b] : &s_full[b]);
                 }
                 __syncwarp();
             }
@@ -356,7 +360,7 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
                         *reinterpret_cast<uint4 *>(p) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                         if (C::F32) *reinterpret_cast<uint4 *>(p + LO) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
-                    if (lane == 0) (V ? s_vinv : s_kinv)[t & 7][2 * (warp & 3) + part] = inv; // (who reads tile t - 8's is done: the ring's stages span three tiles, and what comes after MMAs two more)
+                    if (lane == 0) (V ? s_vinv : s_kinv)[t & 15][2 * (warp & 3) + part] = inv; // (who reads tile t - 16's is done: the rings span six tiles at most, and scores are four ahead of outputs)
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
@@ -370,82 +374,94 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
         else convert(std::false_type{});
         asm volatile("cp.async.wait_all;" ::: "memory"); // (what is in flight ends before the CTA does, even when a wait gave up)
     } else if (warp < 8) {
-        // ===== soft-max: thread = row, warps 0-3 take a tile's first 32 slots, 4-7 the others
-        const int r = (warp & 3) * 32 + lane, row = r0 + r, tok = row / a.R, rp = sv_rp(all_rows), half = warp >> 2;
+        // ===== soft-max: thread = row, warps 0-3 take the even tiles, 4-7 the odd ones.  The scores are read twice (there are no registers for 64), and the weights' parts take their place
+        const int r = (warp & 3) * 32 + lane, row = r0 + r, tok = row / a.R, rp = sv_rp(all_rows);
         const bool mine = r < rows, any = (warp & 3) * 32 < rows; // (any: of the warp)
         const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
         bool ok = true;
-        for (int t = 0; t < tiles; t++) {
-            const int b = t & 1;
-            const uint32_t see = see_of(t, half, tok, mine);
-            const bool whole = __all_sync(0xffffffffu, see == ~0u);
-            sv_bar_wait(&s_full[b], (t >> 1) & 1, ok, a.err, 18);
-            ps_tc_fence_after();
-            __syncwarp();
-            uint32_t v[32];
-            float mx = SV_NONE, f[4];
-            if (any && ok) {
-                uint32_t (&va)[16] = *reinterpret_cast<uint32_t (*)[16]>(v), (&vb)[16] = *reinterpret_cast<uint32_t (*)[16]>(v + 16);
-                sv_tm_ld16(va, tm_s + b * SV_TILE + 32 * half + lane_at);
-                sv_tm_ld16(vb, tm_s + b * SV_TILE + 32 * half + 16 + lane_at);
-                const float4 ki = *reinterpret_cast<const float4 *>(&s_kinv[t & 7][4 * half]);
-                // (never zero: -inf times it is -inf)
-                f[0] = fmaxf(qinv * ki.x, 0x1p-126f); f[1] = fmaxf(qinv * ki.y, 0x1p-126f); f[2] = fmaxf(qinv * ki.z, 0x1p-126f); f[3] = fmaxf(qinv * ki.w, 0x1p-126f);
-                ps_tc_ld_wait();
-                if (!whole) {
-#pragma unroll
-                    for (int c = 0; c < 32; c++)
-                        if (!(see >> c & 1)) v[c] = __float_as_uint(SV_NONE);
-                }
-                float top[4] = {SV_NONE, SV_NONE, SV_NONE, SV_NONE};
-#pragma unroll
-                for (int c = 0; c < 8; c += 2)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) top[e] = fmaxf(fmaxf(top[e], __uint_as_float(v[8 * e + c])), __uint_as_float(v[8 * e + c + 1]));
-                mx = fmaxf(fmaxf(top[0] * f[0], top[1] * f[1]), fmaxf(top[2] * f[2], top[3] * f[3]));
-            }
-            s_half[b][half][r] = mx;
-            ps_tc_fence_before();
-            __syncwarp();
-            if (lane == 0) ps_mbar_arrive(&s_free[b]); // the scores are in registers: those of tile t + 2 may come
-            if (t >= 2) sv_bar_wait(&o_empty[b], ((t >> 1) - 1) & 1, ok, a.err, 19); // (tile t - 2's weights are used up, and its maximum and sum)
-            ok = ps_bar_all(1 + (warp & 3), 64, ok); // the two warps of the same rows go on together, or give up together
+        for (int t = warp >> 2; t < tiles; t += 2) {
+            const int sp = t & 3;
+            const uint64_t see = see_of(t, tok, mine);
+            const bool whole = __all_sync(0xffffffffu, see == ~0ull);
+            sv_bar_wait(&s_full[sp], (t >> 2) & 1, ok, a.err, 18);
             if (!ok) break;
+            ps_tc_fence_after();
             if (any) {
-                mx = fmaxf(mx, s_half[b][half ^ 1][r]);
+                const uint32_t at = tm_s + sp * SV_TILE + lane_at;
+                uint32_t v0[16], v1[16];
+                float top[4] = {SV_NONE, SV_NONE, SV_NONE, SV_NONE};
+                const float *ki = s_kinv[t & 15];
+                // (a factor is never zero: -inf times it is -inf)
+                auto hide = [&](uint32_t (&v)[16], int c) {
+                    if (!whole) {
+#pragma unroll
+                        for (int e = 0; e < 16; e++)
+                            if (!(see >> (16 * c + e) & 1)) v[e] = __float_as_uint(SV_NONE);
+                    }
+                };
+                auto most = [&](uint32_t (&v)[16], int c) {
+                    hide(v, c);
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        float m = SV_NONE;
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) m = fmaxf(fmaxf(m, __uint_as_float(v[8 * h + e])), __uint_as_float(v[8 * h + e + 1]));
+                        top[2 * (c & 1) + h] = fmaxf(top[2 * (c & 1) + h], m * fmaxf(qinv * ki[2 * c + h], 0x1p-126f));
+                    }
+                };
+                sv_tm_ld16(v0, at);
+                sv_tm_ld16(v1, at + 16);
+                ps_tc_ld_wait();
+                most(v0, 0);
+                most(v1, 1);
+                sv_tm_ld16(v0, at + 32);
+                sv_tm_ld16(v1, at + 48);
+                ps_tc_ld_wait();
+                most(v0, 2);
+                most(v1, 3);
+                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                 // the weights are 2^15 p, and so is their sum
                 const float shift = mx == SV_NONE ? 15.f : 15.f - mx;
                 const sv_f2 shift2 = sv_two(shift, shift);
                 sv_f2 sum = 0ull;
-#pragma unroll
-                for (int c = 0; c < 32; c += 16) {
+                auto weigh = [&](uint32_t (&v)[16], int c) {
+                    const float f[2] = {fmaxf(qinv * ki[2 * c], 0x1p-126f), fmaxf(qinv * ki[2 * c + 1], 0x1p-126f)};
                     uint32_t hi[8], lo[8];
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        const float fe = f[(c + 2 * e) / 8];
                         float p0, p1;
-                        sv_one(sv_fma2(sv_two(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1])), sv_two(fe, fe), shift2), p0, p1);
+                        sv_one(sv_fma2(sv_two(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), sv_two(f[e / 4], f[e / 4]), shift2), p0, p1);
                         const sv_f2 p = sv_two(sv_ex2(p0), sv_ex2(p1));
                         sum = sv_add2(sum, p);
                         sv_cut2(p, hi[e], lo[e]);
                     }
-                    sv_tm_st8(tm_p + b * SV_TILE + 16 * half + c / 2 + lane_at, hi);
-                    sv_tm_st8(tm_p + b * SV_TILE + SV_TILE / 2 + 16 * half + c / 2 + lane_at, lo);
-                }
-                s_top[b][r] = mx; // (both warps write the same)
+                    sv_tm_st8(at + 16 * c, hi);
+                    sv_tm_st8(at + 16 * c + 8, lo);
+                    if (W && s.scores && mine) {
+                        float4 *to = reinterpret_cast<float4 *>(s.scores) + ((int64_t)g * sv_quads(s.n_kv) + (j0 + t * SV_TILE) / 4 + 4 * c) * rp + row;
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4, to += rp)
+                            __stcs(to, make_float4(__uint_as_float(v[e]) * f[e / 8], __uint_as_float(v[e + 1]) * f[e / 8], __uint_as_float(v[e + 2]) * f[e / 8], __uint_as_float(v[e + 3]) * f[e / 8]));
+                    }
+                };
+                weigh(v0, 2);
+                sv_tm_ld16(v0, at);
+                weigh(v1, 3);
+                sv_tm_ld16(v1, at + 16);
+                ps_tc_ld_wait();
+                hide(v0, 0);
+                weigh(v0, 0);
+                hide(v1, 1);
+                weigh(v1, 1);
+                s_top[t & 7][r] = mx;
                 float sum0, sum1;
                 sv_one(sum, sum0, sum1);
-                s_sum[b][half][r] = sum0 + sum1;
+                s_sum[t & 7][r] = sum0 + sum1;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             }
             ps_tc_fence_before();
             __syncwarp();
-            if (lane == 0) ps_mbar_arrive(&p_full[b]);
-            if (W && s.scores && mine) { // (nothing waits for them)
-                float4 *to = reinterpret_cast<float4 *>(s.scores) + ((int64_t)g * sv_quads(s.n_kv) + (j0 + t * SV_TILE + 32 * half) / 4) * rp + row;
-#pragma unroll
-                for (int c = 0; c < 32; c += 4, to += rp) __stcs(to, make_float4(__uint_as_float(v[c]) * f[c / 8], __uint_as_float(v[c + 1]) * f[c / 8], __uint_as_float(v[c + 2]) * f[c / 8], __uint_as_float(v[c + 3]) * f[c / 8]));
-            }
+            if (lane == 0) ps_mbar_arrive(&p_full[sp]);
         }
     } else {
         // ===== output: thread = row, half of the channels; the row's maximum and sum so far
@@ -465,12 +481,12 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
             ps_tc_fence_after();
             if (any) {
                 // (what has been added up changes its reference when a maximum is 2^8 above it, or the first there is: seldom)
-                const float top = s_top[b][r];
+                const float top = s_top[t & 7][r];
                 const bool up = top > m + 8.f;
                 const float mn = up ? top : m, ref = mn == SV_NONE ? 0.f : mn, fo = up ? sv_ex2(m - ref) : 1.f, fn = sv_ex2(top - ref);
-                const float4 vi = *reinterpret_cast<const float4 *>(&s_vinv[t & 7][4 * half]);
+                const float4 vi = *reinterpret_cast<const float4 *>(&s_vinv[t & 15][4 * half]);
                 const sv_f2 f[4] = {sv_two(fn * vi.x, fn * vi.x), sv_two(fn * vi.y, fn * vi.y), sv_two(fn * vi.z, fn * vi.z), sv_two(fn * vi.w, fn * vi.w)};
-                l = fmaf(l, fo, (s_sum[b][0][r] + s_sum[b][1][r]) * fn);
+                l = fmaf(l, fo, s_sum[t & 7][r] * fn);
                 m = mn;
                 if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
