@@ -403,10 +403,17 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
                     hide(v, c);
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
+                        const float f = fmaxf(qinv * ki[2 * c + h], 0x1p-126f);
+                        if (W && s.scores && mine) {
+                            float4 *to = reinterpret_cast<float4 *>(s.scores) + ((int64_t)g * sv_quads(s.n_kv) + (j0 + t * SV_TILE) / 4 + 4 * c + 2 * h) * rp + row;
+#pragma unroll
+                            for (int e = 8 * h; e < 8 * h + 8; e += 4, to += rp)
+                                __stcs(to, make_float4(__uint_as_float(v[e]) * f, __uint_as_float(v[e + 1]) * f, __uint_as_float(v[e + 2]) * f, __uint_as_float(v[e + 3]) * f));
+                        }
                         float m = SV_NONE;
 #pragma unroll
                         for (int e = 0; e < 8; e += 2) m = fmaxf(fmaxf(m, __uint_as_float(v[8 * h + e])), __uint_as_float(v[8 * h + e + 1]));
-                        top[2 * (c & 1) + h] = fmaxf(top[2 * (c & 1) + h], m * fmaxf(qinv * ki[2 * c + h], 0x1p-126f));
+                        top[2 * (c & 1) + h] = fmaxf(top[2 * (c & 1) + h], m * f);
                     }
                 };
                 sv_tm_ld16(v0, at);
@@ -437,12 +444,6 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
                     }
                     sv_tm_st8(at + 16 * c, hi);
                     sv_tm_st8(at + 16 * c + 8, lo);
-                    if (W && s.scores && mine) {
-                        float4 *to = reinterpret_cast<float4 *>(s.scores) + ((int64_t)g * sv_quads(s.n_kv) + (j0 + t * SV_TILE) / 4 + 4 * c) * rp + row;
-#pragma unroll
-                        for (int e = 0; e < 16; e += 4, to += rp)
-                            __stcs(to, make_float4(__uint_as_float(v[e]) * f[e / 8], __uint_as_float(v[e + 1]) * f[e / 8], __uint_as_float(v[e + 2]) * f[e / 8], __uint_as_float(v[e + 3]) * f[e / 8]));
-                    }
                 };
                 weigh(v0, 2);
                 sv_tm_ld16(v0, at);
