@@ -298,7 +298,8 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
         auto convert = [&](auto of_v) {
             constexpr bool V = decltype(of_v)::value;
             constexpr int ITS = D / 32, ROW = V ? C::V_ROW : C::K_ROW, LO = V ? C::V_LO : C::K_LO; // ITS: eights of a thread
-            const int sub = lane & 7, quad = lane >> 3, mode = V ? s.v_mode : s.k_mode, first = V ? 2 * C::V_GROUPS * (warp & 3) : 2 * (warp & 3);
+            constexpr int GROUPS = V ? C::V_GROUPS : 1, AT_ONCE = ITS * sizeof(typename C::Raw) <= 64 ? 2 : 1; // groups of a part; parts at a time, as registers allow
+            const int sub = lane & 7, quad = lane >> 3, mode = V ? s.v_mode : s.k_mode, first = 2 * GROUPS * (warp & 3);
             uint8_t *ring = V ? sm_v : sm_k;
             for (int t = 0; t < tiles; t++) {
                 const int st = t % stages;
@@ -306,61 +307,79 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
                 asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 2) : "memory");
                 __syncwarp();
 #pragma unroll 1
-                for (int part = 0; part < 2; part++) {
-                    uint8_t *group = ring + st * (V ? C::V_STAGE : C::K_STAGE) + (first + (V ? C::V_GROUPS * part : part)) * 8 * ROW;
+                for (int part0 = 0; part0 < 2; part0 += AT_ONCE) {
                     // eight i of the thread: K: 32 elements further along the row; V: the row's second half, then the next group of channels
-                    typename C::Raw raw[ITS];
+                    typename C::Raw raw[AT_ONCE][ITS];
+                    uint8_t *group = ring + st * (V ? C::V_STAGE : C::K_STAGE) + (first + part0 * GROUPS) * 8 * ROW;
                     if (mode) {
                         const uint8_t *from = group + sub * ROW + quad * (8 * (int)sizeof(T));
 #pragma unroll
-                        for (int i = 0; i < ITS; i++) sv_get(raw[i], from + (V ? (i >> 1) * 8 * ROW + (i & 1) * (32 * (int)sizeof(T)) : i * (32 * (int)sizeof(T))));
+                        for (int p = 0; p < AT_ONCE; p++)
+#pragma unroll
+                            for (int i = 0; i < ITS; i++) sv_get(raw[p][i], from + p * GROUPS * 8 * ROW + (V ? (i >> 1) * 8 * ROW + (i & 1) * (32 * (int)sizeof(T)) : i * (32 * (int)sizeof(T))));
                     } else { // rows that no wide copy can read: element by element
-                        const int w = 2 * (warp & 3) + part, j = j0 + t * SV_TILE;
+                        const int j = j0 + t * SV_TILE;
 #pragma unroll
-                        for (int i = 0; i < ITS; i++) {
-                            T x[8];
-                            const int slot = V ? (quad + 4 * (i & 1)) * 8 : w * 8 + sub;
-                            const T *src = V ? static_cast<const T *>(s.v) + ((int64_t)g * D + (w * C::V_GROUPS + (i >> 1)) * 8 + sub) * s.n_ctx + j + slot
-                                             : static_cast<const T *>(s.k) + (int64_t)(j + slot) * a.G * D + (int64_t)g * D + (i * 4 + quad) * 8;
+                        for (int p = 0; p < AT_ONCE; p++)
 #pragma unroll
-                            for (int e = 0; e < 8; e++) {
-                                x[e] = T(0.f);
-                                if (live >> (V ? slot + e : slot) & 1) x[e] = src[e];
+                            for (int i = 0; i < ITS; i++) {
+                                T x[8];
+                                const int w = 2 * (warp & 3) + part0 + p, slot = V ? (quad + 4 * (i & 1)) * 8 : w * 8 + sub;
+                                const T *src = V ? static_cast<const T *>(s.v) + ((int64_t)g * D + (w * C::V_GROUPS + (i >> 1)) * 8 + sub) * s.n_ctx + j + slot
+                                                 : static_cast<const T *>(s.k) + (int64_t)(j + slot) * a.G * D + (int64_t)g * D + (i * 4 + quad) * 8;
+#pragma unroll
+                                for (int e = 0; e < 8; e++) {
+                                    x[e] = T(0.f);
+                                    if (live >> (V ? slot + e : slot) & 1) x[e] = src[e];
+                                }
+                                memcpy(&raw[p][i], x, sizeof raw[p][i]);
                             }
-                            memcpy(&raw[i], x, sizeof raw[i]);
-                        }
                     }
                     if (live != ~0ull) { // what a slot that is not live holds, or was not copied, may be anything
 #pragma unroll
-                        for (int i = 0; i < ITS; i++) sv_keep(raw[i], V ? (uint32_t)(live >> (8 * (quad + 4 * (i & 1)))) : live >> (16 * (warp & 3) + 8 * part + sub) & 1 ? 0xffu : 0u);
+                        for (int p = 0; p < AT_ONCE; p++)
+#pragma unroll
+                            for (int i = 0; i < ITS; i++)
+                                sv_keep(raw[p][i], V ? (uint32_t)(live >> (8 * (quad + 4 * (i & 1)))) : live >> (16 * (warp & 3) + 8 * (part0 + p) + sub) & 1 ? 0xffu : 0u);
                     }
-                    float top = 0.f;
+                    float top[AT_ONCE];
 #pragma unroll
-                    for (int i = 0; i < ITS; i++)
+                    for (int p = 0; p < AT_ONCE; p++) {
+                        top[p] = 0.f;
 #pragma unroll
-                        for (int e = 0; e < 8; e += 2) top = fmaxf(fmaxf(top, fabsf(sv_at(raw[i], e))), fabsf(sv_at(raw[i], e + 1)));
-                    float inv;
-                    const float f1 = sv_scale(__reduce_max_sync(0xffffffffu, __float_as_uint(top)), inv); // (and all lanes have read)
-                    const sv_f2 f = sv_two(f1, f1);
-                    uint8_t *to = group + sub * 16 + quad * 128;
+                        for (int i = 0; i < ITS; i++)
 #pragma unroll
-                    for (int i = 0; i < ITS; i++) {
-                        uint32_t hi[4], lo[4];
+                            for (int e = 0; e < 8; e += 2) top[p] = fmaxf(fmaxf(top[p], fabsf(sv_at(raw[p][i], e))), fabsf(sv_at(raw[p][i], e + 1)));
+                    }
+                    float inv[AT_ONCE];
+                    sv_f2 f[AT_ONCE];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const sv_f2 x = sv_mul2(sv_two(sv_at(raw[i], 2 * e), sv_at(raw[i], 2 * e + 1)), f);
-                            if (C::F32) sv_cut2(x, hi[e], lo[e]);
-                            else { // (eight bits: hi is all of it)
-                                float x0, x1;
-                                sv_one(x, x0, x1);
-                                hi[e] = sv_pack(x0, x1);
+                    for (int p = 0; p < AT_ONCE; p++) {
+                        const float f1 = sv_scale(__reduce_max_sync(0xffffffffu, __float_as_uint(top[p])), inv[p]); // (and all lanes have read)
+                        f[p] = sv_two(f1, f1);
+                    }
+#pragma unroll
+                    for (int p = 0; p < AT_ONCE; p++) {
+                        uint8_t *to = group + p * GROUPS * 8 * ROW + sub * 16 + quad * 128;
+#pragma unroll
+                        for (int i = 0; i < ITS; i++) {
+                            uint32_t hi[4], lo[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const sv_f2 x = sv_mul2(sv_two(sv_at(raw[p][i], 2 * e), sv_at(raw[p][i], 2 * e + 1)), f[p]);
+                                if (C::F32) sv_cut2(x, hi[e], lo[e]);
+                                else { // (eight bits: hi is all of it)
+                                    float x0, x1;
+                                    sv_one(x, x0, x1);
+                                    hi[e] = sv_pack(x0, x1);
+                                }
                             }
+                            uint8_t *q = to + (V ? (i >> 1) * 8 * ROW + (i & 1) * 512 : i * 512);
+                            *reinterpret_cast<uint4 *>(q) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                            if (C::F32) *reinterpret_cast<uint4 *>(q + LO) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                         }
-                        uint8_t *p = to + (V ? (i >> 1) * 8 * ROW + (i & 1) * 512 : i * 512);
-                        *reinterpret_cast<uint4 *>(p) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        if (C::F32) *reinterpret_cast<uint4 *>(p + LO) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        if (lane == 0) (V ? s_vinv : s_kinv)[t & 15][2 * (warp & 3) + part0 + p] = inv[p]; // (who reads tile t - 16's is done: the rings span six tiles at most, and scores are four ahead of outputs)
                     }
-                    if (lane == 0) (V ? s_vinv : s_kinv)[t & 15][2 * (warp & 3) + part] = inv; // (who reads tile t - 16's is done: the rings span six tiles at most, and scores are four ahead of outputs)
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
