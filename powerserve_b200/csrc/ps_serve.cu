@@ -11,6 +11,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <type_traits>
+#include <vector>
 
 namespace {
 
@@ -54,17 +55,26 @@ int check_caches(PsServeCall *c, const char *what, const ps_cuda_cache *caches, 
     return 0;
 }
 
-// Splits of the launch: as many CTAs as the GPU takes at once, none of fewer than `least` tiles
-int split_tiles(const ps_cuda_cache *caches, int n, int per_split, int target, int least) {
-    int64_t tiles = 0;
-    for (int i = 0; i < n; i++) tiles += caches[i].n_tok > 0 ? (caches[i].n_kv + SV_TILE - 1) / SV_TILE : 0;
-    int tps = (int)std::max<int64_t>(least, tiles * per_split / std::max(target, 1));
-    for (;; tps++) { // (the last splits are short: a few more tiles for each until all fit)
+// Whether two of the arrays are the same
+bool twice(std::vector<const void *> &p) {
+    std::sort(p.begin(), p.end());
+    return std::adjacent_find(p.begin(), p.end()) != p.end();
+}
+
+// Tiles of a split: the fewest with which the launch has no more CTAs than the GPU takes at once
+int split_tiles(const ps_cuda_cache *caches, int n, int per_split, int target) {
+    int64_t lo = 1, hi = 1;
+    for (int i = 0; i < n; i++)
+        if (caches[i].n_tok > 0) hi = std::max<int64_t>(hi, (caches[i].n_kv + SV_TILE - 1) / SV_TILE); // (a split a sequence)
+    while (lo < hi) {
+        const int64_t tps = (lo + hi) / 2;
         int64_t ctas = 0;
         for (int i = 0; i < n; i++)
             if (caches[i].n_tok > 0) ctas += ((caches[i].n_kv + SV_TILE - 1) / SV_TILE + tps - 1) / tps;
-        if (ctas * per_split <= target || ctas <= n) return tps;
+        if (ctas * per_split <= target) hi = tps;
+        else lo = tps + 1;
     }
+    return (int)lo;
 }
 
 // Tiles of a split for the kernel of few rows, of which `slots` CTAs run at once: the least of an estimate in tiles' time.  A CTA costs its tiles and one more to begin and end;
@@ -99,16 +109,16 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
     if (n_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > 32) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "attn_tree: %d heads over %d kv heads", n_heads, n_kv_heads);
     const int R = n_heads / n_kv_heads, hs = head_size;
     int64_t tokens = 0;
+    std::vector<const void *> gather;
     for (int i = 0; i < n_seqs; i++) {
         const ps_cuda_cache &s = caches[i];
         if (s.n_tok < 0 || s.n_tok > s.n_kv) return fail(c, PS_CUDA_ERR_INVALID, "attn_tree: sequence %d brings %d tokens, its cache holds %d", i, s.n_tok, s.n_kv);
-        if (s.weight && s.n_tok)
-            for (int o = 0; o < i && i < 4096; o++) // (beyond that many the caller is taken at their word)
-                if (caches[o].weight == s.weight && caches[o].n_tok) return fail(c, PS_CUDA_ERR_INVALID, "attn_tree: sequences %d and %d gather their weights in the same array", o, i);
+        if (s.weight && s.n_tok) gather.push_back(s.weight);
         if (s.n_tok > PS_CUDA_TREE_TOKENS) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "attn_tree: sequence %d brings %d tokens (at most %d)", i, s.n_tok, PS_CUDA_TREE_TOKENS);
         tokens += s.n_tok;
     }
     if (tokens == 0) return 0;
+    if (twice(gather)) return fail(c, PS_CUDA_ERR_INVALID, "attn_tree: two sequences gather their weights in the same array");
     if (tokens > INT32_MAX / 1024) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "attn_tree: %lld tokens in one call", (long long)tokens);
     if (!out || !q) return fail(c, PS_CUDA_ERR_INVALID, "attn_tree: null argument");
     if (!aligned(out, 4) || !aligned(q, 4)) return fail(c, PS_CUDA_ERR_INVALID, "attn_tree: an array that is not aligned to its elements");
@@ -137,7 +147,7 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
         a.out_vec = aligned(out, 16);
         a.q_vec = aligned(q, 16);
         if (most_tok) {
-            a.tps = few ? split_few(caches + first, n, n_kv_heads, c->n_sm * (hs == 128 && cache_type == PS_TYPE_F32 ? 3 : 4)) : split_tiles(caches + first, n, n_kv_heads * row_tiles, tc ? c->n_sm : c->n_sm * 4, 1);
+            a.tps = few ? split_few(caches + first, n, n_kv_heads, c->n_sm * (hs == 128 && cache_type == PS_TYPE_F32 ? 3 : 4)) : split_tiles(caches + first, n, n_kv_heads * row_tiles, tc ? c->n_sm : c->n_sm * 4);
             if (tc) a.tps = std::min(a.tps, SV_TC_TILES);
             size_t bytes = scores;
             int units = 0;
@@ -224,6 +234,7 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
 
 int ps_serve_kv_evict(PsServeCall *c, const ps_cuda_cache *caches, int n_sets, int cache_type, int head_size, int n_kv_heads, int n_sink, int n_recent) {
     if (int rc = check_caches(c, "kv_evict", caches, n_sets, cache_type, head_size, n_kv_heads)) return rc;
+    std::vector<const void *> written, read;
     if (n_sink < 0 || n_recent < 0) return fail(c, PS_CUDA_ERR_INVALID, "kv_evict: %d first and %d latest positions", n_sink, n_recent);
     for (int i = 0; i < n_sets; i++) {
         const ps_cuda_cache &s = caches[i];
@@ -231,10 +242,18 @@ int ps_serve_kv_evict(PsServeCall *c, const ps_cuda_cache *caches, int n_sets, i
         if (s.n_kv && (!s.weight || !s.weight_to)) return fail(c, PS_CUDA_ERR_INVALID, "kv_evict: cache %d has no gathered weights", i);
         if ((s.pos != nullptr) != (s.pos_to != nullptr)) return fail(c, PS_CUDA_ERR_INVALID, "kv_evict: cache %d: pos and pos_to go together", i);
         if (!s.pos && (n_sink || n_recent)) return fail(c, PS_CUDA_ERR_INVALID, "kv_evict: cache %d has no positions to keep the first or latest of", i);
-        for (int o = 0; o < i && i < 4096 && s.n_kv; o++)
-            if (caches[o].n_kv && (caches[o].k == s.k || caches[o].v == s.v || caches[o].weight_to == s.weight_to)) return fail(c, PS_CUDA_ERR_INVALID, "kv_evict: caches %d and %d are the same", o, i);
+        if (s.n_kv) { // (what a cache writes, no other one may touch)
+            const void *own[4] = {s.k, s.v, s.weight_to, s.pos ? s.pos_to : s.k};
+            for (int e = 0; e < 4; e++)
+                if (std::find(own, own + e, own[e]) == own + e) written.push_back(own[e]);
+            if (s.weight != s.weight_to) read.push_back(s.weight);
+            if (s.pos && s.pos != s.pos_to) read.push_back(s.pos);
+        }
         if (s.hidden) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "kv_evict: cache %d has hidden slots (every kv head moves its own)", i);
     }
+    if (twice(written)) return fail(c, PS_CUDA_ERR_INVALID, "kv_evict: two caches share an array that is written");
+    for (const void *p : read) // (what is only read may be shared)
+        if (std::binary_search(written.begin(), written.end(), p)) return fail(c, PS_CUDA_ERR_INVALID, "kv_evict: two caches share an array that is written");
     for (int first = 0; first < n_sets; first += SV_SETS) {
         const int n = std::min(n_sets - first, SV_SETS);
         SvEvict a{};

@@ -68,7 +68,26 @@ int main() {
     expect("caches below zero", I, "no caches", [&](PsServeCall *c) { return ps_serve_attn_tree(c, mem, mem, &good, -1, 0, 32, 4, 2, nullptr, 1.f); });
     ps_cuda_cache two[2] = {good, good};
     expect("weights gathered twice", I, "same array", [&](PsServeCall *c) { return ps_serve_attn_tree(c, mem, mem, two, 2, 0, 32, 4, 2, nullptr, 1.f); });
-    expect("a cache cut twice", I, "the same", [&](PsServeCall *c) { return ps_serve_kv_evict(c, two, 2, 0, 32, 2, 0, 0); });
+    expect("a cache cut twice", I, "share an array", [&](PsServeCall *c) { return ps_serve_kv_evict(c, two, 2, 0, 32, 2, 0, 0); });
+    { // caches of their own, one of whose arrays another one reads or writes
+        ps_cuda_cache own[2] = {good, good};
+        own[0].n_ctx = own[0].n_kv = own[1].n_ctx = own[1].n_kv = 100;
+        for (int i = 0; i < 2; i++) {
+            char *at = reinterpret_cast<char *>(mem) + 64 * i;
+            own[i].k = at; own[i].v = at + 8; own[i].weight = reinterpret_cast<float *>(at + 16); own[i].weight_to = reinterpret_cast<float *>(at + 24);
+            own[i].pos = reinterpret_cast<int32_t *>(at + 32); own[i].pos_to = reinterpret_cast<int32_t *>(at + 40);
+        }
+        auto both = [&](PsServeCall *c) { return ps_serve_kv_evict(c, own, 2, 0, 32, 2, 1, 1); };
+        expect("caches of their own ask for memory", PS_CUDA_ERR_OOM, nullptr, both);
+        own[1].weight = own[0].weight; own[1].pos = own[0].pos;
+        expect("what is only read is shared", PS_CUDA_ERR_OOM, nullptr, both);
+        own[1].pos = own[0].pos_to;
+        expect("positions that another cache writes", I, "share an array", both);
+        own[1].pos = own[0].pos; own[1].pos_to = own[0].pos_to;
+        expect("positions written twice", I, "share an array", both);
+        own[1].pos_to = reinterpret_cast<int32_t *>(reinterpret_cast<char *>(mem) + 104); own[1].v = own[0].v;
+        expect("one V for two", I, "share an array", both);
+    }
     expect("nobody", 0, nullptr, [&](PsServeCall *c) { return ps_serve_attn_tree(c, mem, mem, nullptr, 0, 0, 32, 4, 2, nullptr, 1.f); });
 
     evict("a call that is right asks for memory", PS_CUDA_ERR_OOM, nullptr, [](ps_cuda_cache &s) { s.n_ctx = s.n_kv = 100; }, 1, 1);
