@@ -338,9 +338,11 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
                     if (live != ~0ull) { // what a slot that is not live holds, or was not copied, may be anything
 #pragma unroll
                         for (int p = 0; p < AT_ONCE; p++)
+                            if (V || (live >> (16 * (warp & 3) + 8 * (part0 + p)) & 0xffu) != 0xffu) {
 #pragma unroll
-                            for (int i = 0; i < ITS; i++)
-                                sv_keep(raw[p][i], V ? (uint32_t)(live >> (8 * (quad + 4 * (i & 1)))) : live >> (16 * (warp & 3) + 8 * (part0 + p) + sub) & 1 ? 0xffu : 0u);
+                                for (int i = 0; i < ITS; i++)
+                                    sv_keep(raw[p][i], V ? (uint32_t)(live >> (8 * (quad + 4 * (i & 1)))) : live >> (16 * (warp & 3) + 8 * (part0 + p) + sub) & 1 ? 0xffu : 0u);
+                            }
                     }
                     float top[AT_ONCE];
 #pragma unroll
@@ -401,7 +403,9 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
         for (int t = warp >> 2; t < tiles; t += 2) {
             const int sp = t & 3;
             const uint64_t see = see_of(t, tok, mine);
-            const bool whole = __all_sync(0xffffffffu, see == ~0ull);
+            uint32_t gaps = 0; // sixteen slots of which some row of the warp does not see one
+#pragma unroll
+            for (int c = 0; c < 4; c++) gaps |= __any_sync(0xffffffffu, (see >> (16 * c) & 0xffffu) != 0xffffu) ? 1u << c : 0u;
             sv_bar_wait(&s_full[sp], (t >> 2) & 1, ok, a.err, 18);
             if (!ok) break;
             ps_tc_fence_after();
@@ -412,7 +416,7 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
                 const float *ki = s_kinv[t & 15];
                 // (a factor is never zero: -inf times it is -inf)
                 auto hide = [&](uint32_t (&v)[16], int c) {
-                    if (!whole) {
+                    if (gaps >> c & 1) {
 #pragma unroll
                         for (int e = 0; e < 16; e++)
                             if (!(see >> (16 * c + e) & 1)) v[e] = __float_as_uint(SV_NONE);
