@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 && D == 128 ? 3 : 4) sv_k_
     auto scores = [&](const SvShare<T, 32> &r, int half, float (&z)[4]) {
         float inv;
         const float f = sv_group_scale(r, inv);
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
+        float d[4] = {0.f, 0.f, 0.f, 0.f}, low[4] = {0.f, 0.f, 0.f, 0.f}; // (the accumulators truncate: small products have one of their own)
 #pragma unroll
         for (int k = 0; k < 4; k++) { // 32-channel group, half of it
             uint4 hi, lo;
@@ -167,12 +167,12 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 && D == 128 ? 3 : 4) sv_k_
             sv_cut(r.at(i + 2) * f, r.at(i + 3) * f, hi.z, lo.z);
             sv_cut(r.at(18 + i) * f, r.at(19 + i) * f, hi.w, lo.w);
             const uint4 q = s_q[4 * half + k][lane];
-            sv_mma(d, hi, q.z, q.w);
-            if (F32) sv_mma(d, lo, q.x, q.y);
+            sv_mma(low, hi, q.z, q.w);
+            if (F32) sv_mma(low, lo, q.x, q.y);
             sv_mma(d, hi, q.x, q.y);
         }
 #pragma unroll
-        for (int e = 0; e < 4; e++) z[e] = half ? fmaf(d[e], inv, z[e]) : d[e] * inv;
+        for (int e = 0; e < 4; e++) z[e] = half ? fmaf(d[e] + low[e], inv, z[e]) : (d[e] + low[e]) * inv;
     };
     auto output = [&](const SvShare<T, 32> &r, int half, uint32_t ph0, uint32_t ph1, uint32_t pl0, uint32_t pl1) {
         float inv;
