@@ -148,6 +148,9 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
         a.q_vec = aligned(q, 16);
         if (most_tok) {
             a.tps = few ? split_few(caches + first, n, n_kv_heads, c->n_sm * (hs == 128 && cache_type == PS_TYPE_F32 ? 3 : 4)) : split_tiles(caches + first, n, n_kv_heads * row_tiles, tc ? c->n_sm : c->n_sm * 4);
+            // (one tile a split: more to join than it saves, but for the shortest; 12 tokens, 32 / 8 heads of 128 over 315 slots 18.5 us and 20.5 with two tiles, over 1 015 22.5 and
+            // 20.5, heads of 64 18.5 and 14.9)
+            if (tc && most_kv > 8 * SV_TILE) a.tps = std::max(a.tps, 2);
             if (tc) a.tps = std::min(a.tps, SV_TC_TILES);
             size_t bytes = scores;
             int units = 0;
