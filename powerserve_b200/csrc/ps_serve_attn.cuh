@@ -55,7 +55,7 @@ PS_D int sv_find(const SvAttn &a, int unit) {
 PS_D bool sv_sees(const SvSeq &s, int t, int back) { return back < 0 || (s.mask ? s.mask[t * s.n_tok + back] != 0 : back <= t); }
 
 // ---------------------------------------------------------------------------------------------------- any head size
-// Sixteen query rows, 32 slots at a time, everything in 32-bit arithmetic on the CUDA cores.  Thread (slot, row group) takes four scores; a warp
+// For head sizes that are not 64 or 128. Sixteen query rows, 32 slots at a time, everything in 32-bit arithmetic on the CUDA cores.  Thread (slot, row group) takes four scores; a warp
 // takes the soft-max of four rows; then a thread owns channels d, d + 128 of all sixteen rows.
 template <typename T>
 __global__ void __launch_bounds__(128) sv_k_attn(const __grid_constant__ SvAttn a) {
@@ -157,8 +157,8 @@ __global__ void __launch_bounds__(128) sv_k_attn(const __grid_constant__ SvAttn 
 inline size_t sv_attn_smem(int hs) { return 4 * ((size_t)16 * hs + 32 * (hs + 1) + (size_t)hs * 33 + 16 * 33 + 16); }
 
 // ---------------------------------------------------------------------------------------------------- joining the splits
-// A warp a row of kv head y: a lane a split takes maxima and sums at once, then eight splits' outputs are under way at a time.  (By the last of the CTAs above
-// to come it took longer: one CTA for all of a head's rows, 16 splits of 48 rows 30 us; 5 so.)
+// A warp a row of kv head y: a lane a split takes maxima and sums at once, then eight splits' outputs are under way at a time. Its start overlaps the end of the kernel before; bound by
+// latency (two dependent rounds of loads): 16 splits of 48 rows of 8 heads 5 us. (Joined by the CTA that comes last, one for all of a head's rows, 30.)
 __global__ void __launch_bounds__(256) sv_k_join(const __grid_constant__ SvAttn a) {
     ps_grid_dep_wait();
     ps_grid_dep_launch();
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(256) sv_k_join(const __grid_constant__ SvAttn 
 
 // x: 256 slots of a sequence's kv head y: their weights.  PER lanes take rows, four slots each, two such quads at a time; then the lanes exchange halves of their eight sums
 // until each has sums of its own (nine shuffles for 32 lanes instead of forty), the old weights are there by then.  Bound by memory: two sequences of 32 700 slots, 128 rows
-// of each of 8 kv heads, 268 MB
+// of each of 8 kv heads: 268 MB in 47 us = 5.7 TB/s (one old weight at a time and forty shuffles: 92 us)
 #define SV_FIN_SLOTS 256
 template <int PER> PS_D void sv_weights(const SvSeq &s, const float *lse, int rows, int g, int j0) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = lane % PER, rp = sv_rp(rows);

