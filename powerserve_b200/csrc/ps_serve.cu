@@ -152,6 +152,21 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
             // 20.5, heads of 64 18.5 and 14.9)
             if (tc && most_kv > 8 * SV_TILE) a.tps = std::max(a.tps, 2);
             if (tc) a.tps = std::min(a.tps, SV_TC_TILES);
+            // Few rows, few splits, and no more CTAs than two an SM: a sequence's splits are a cluster, which joins them itself. 32 / 8 heads of 128 over 1 000 slots, one sequence
+            // 18.5 us (20.5 with a launch to join), four 24.0 (26.6); eight, whose 512 CTAs are more than that, 42.8 (29.4)
+            auto splits_at = [&](int tps, int &active) {
+                int most = 1;
+                active = 0;
+                for (int i = 0; i < n; i++)
+                    if (caches[first + i].n_tok) active++, most = std::max(most, ((caches[first + i].n_kv + SV_TILE - 1) / SV_TILE + tps - 1) / tps);
+                return most;
+            };
+            int active, splits = splits_at(a.tps, active);
+            if (few && splits > 8 && splits <= 16) { // (one sequence of 2 000 slots, two kv heads of 64: 14.4 us for eight splits in a cluster, 16.5 for sixteen to join)
+                const int wider = ((most_kv + SV_TILE - 1) / SV_TILE + 7) / 8;
+                if ((int64_t)active * 8 * n_kv_heads <= c->n_sm * 2) a.tps = wider, splits = splits_at(wider, active);
+            }
+            a.cluster = few && splits <= 8 && (int64_t)active * splits * n_kv_heads <= c->n_sm * 2 ? splits : 1;
             size_t bytes = scores;
             int units = 0;
             bool joined = false;
@@ -163,13 +178,13 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
                 if (tree_mask) tree_mask += (size_t)s.n_tok * s.n_tok;
                 tok0 += s.n_tok;
                 const int tiles = s.n_tok ? (s.n_kv + SV_TILE - 1) / SV_TILE : 0;
-                d.splits = (tiles + a.tps - 1) / a.tps;
+                d.splits = a.cluster > 1 && s.n_tok ? a.cluster : (tiles + a.tps - 1) / a.tps;
                 d.unit0 = units;
                 const bool f32 = cache_type == PS_TYPE_F32;
                 d.k_mode = aligned(s.k, 16);
                 d.v_mode = aligned(s.v, 16) && s.n_ctx % (f32 ? 4 : 8) == 0;
                 units += d.splits;
-                joined |= d.splits > 1;
+                joined |= d.splits > 1 && a.cluster == 1;
                 if (d.weight) bytes += up(4 * (size_t)n_kv_heads * s.n_tok * R);
                 bytes += up(4 * (size_t)d.splits * n_kv_heads * s.n_tok * R * (hs + 2));
             }
@@ -191,7 +206,12 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
             if (few) {
                 const bool f32 = cache_type == PS_TYPE_F32;
                 auto kern = hs == 64 ? (f32 ? sv_k_attn_few<float, 64> : sv_k_attn_few<__nv_bfloat16, 64>) : (f32 ? sv_k_attn_few<float, 128> : sv_k_attn_few<__nv_bfloat16, 128>);
-                kern<<<grid, 128, 0, c->stream>>>(a);
+                cudaLaunchConfig_t cfg{};
+                cudaLaunchAttribute attr[1];
+                attr[0].id = cudaLaunchAttributeClusterDimension;
+                attr[0].val.clusterDim.x = a.cluster; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+                cfg.gridDim = grid; cfg.blockDim = dim3(128); cfg.stream = c->stream; cfg.attrs = attr; cfg.numAttrs = a.cluster > 1;
+                SV_CK(cudaLaunchKernelEx(&cfg, kern, a));
             } else if (tc) {
                 auto launch = [&](auto kern, int smem) -> int {
                     SV_CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
@@ -225,7 +245,7 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
                 SV_LAUNCHED("attn_tree");
                 return 0;
             };
-            if (joined || weights)
+            if (joined)
                 if (int rc = after(sv_k_join, dim3((most_tok * R + 7) / 8, n_kv_heads, n), 0)) return rc;
             if (weights)
                 if (int rc = after(sv_k_weights, dim3((most_kv + SV_FIN_SLOTS - 1) / SV_FIN_SLOTS, n_kv_heads, n), 4 * (size_t)most_tok * R)) return rc;

@@ -9,6 +9,7 @@
 #pragma once
 #include "ps_ptx.cuh"
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
 #define SV_SEQS 64      // sequences of a launch: their table is a kernel parameter
@@ -32,6 +33,7 @@ struct SvAttn {
     const float *q;
     float *out;
     int n_seqs, hs, n_heads, G, R, tps; // R: heads that share a kv head; tps: tiles of a split
+    int cluster;                        // above 1: every sequence has as many splits, and they are a cluster's CTAs
     int q_vec, out_vec;                 // aligned to 16 bytes
     float scale;                        // times log2 e
     int *err;
@@ -53,6 +55,45 @@ PS_D int sv_find(const SvAttn &a, int unit) {
 }
 // slot j, token t: back = j - (n_kv - n_tok) is the slot's number among the step's own tokens (negative: the past)
 PS_D bool sv_sees(const SvSeq &s, int t, int back) { return back < 0 || (s.mask ? s.mask[t * s.n_tok + back] != 0 : back <= t); }
+
+PS_D void sv_put_lse(const SvSeq &s, int64_t at, float top, float sum) { // (a row that sees nothing adds nothing)
+    if (s.lse) s.lse[at] = sum > 0.f ? top + log2f(sum) : INFINITY;
+}
+// The splits of a sequence are a cluster: each CTA's rows r0 .. r0 + rows of `all` lie unnormalised in its shared memory (o: ld floats a row), 2^15 times their maxima's reference as everywhere;
+// the CTAs take shares of the elements and read them from one another
+template <int D> PS_D void sv_join_cluster(const SvAttn &a, const SvSeq &s, int g, int r0, int rows, int all, float *o, int ld, float *top, float *sum) {
+    cooperative_groups::cluster_group cl = cooperative_groups::this_cluster();
+    cl.sync();
+    const int C = a.cluster;
+    for (int i = cl.block_rank() * blockDim.x + threadIdx.x; i < rows * (D / 4); i += C * blockDim.x) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4, row = r0 + r;
+        float t[8], m = SV_NONE, l = 0.f;
+        float4 x[8], v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+            t[c] = SV_NONE;
+            if (c < C) {
+                t[c] = cl.map_shared_rank(top, c)[r];
+                x[c] = *reinterpret_cast<const float4 *>(cl.map_shared_rank(o, c) + r * ld + d);
+            }
+            m = fmaxf(m, t[c]);
+        }
+        const float ref = m == SV_NONE ? 0.f : m;
+#pragma unroll
+        for (int c = 0; c < 8; c++)
+            if (c < C) {
+                const float f = sv_ex2(t[c] - ref);
+                l = fmaf(cl.map_shared_rank(sum, c)[r], f, l);
+                v.x = fmaf(x[c].x, f, v.x); v.y = fmaf(x[c].y, f, v.y); v.z = fmaf(x[c].z, f, v.z); v.w = fmaf(x[c].w, f, v.w);
+            }
+        if (d == 0) sv_put_lse(s, (int64_t)g * all + row, m, l * (1.f / 32768.f));
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        float *to = a.out + ((int64_t)(s.tok0 + row / a.R) * a.n_heads + g * a.R + row % a.R) * D + d;
+        if (a.out_vec) *reinterpret_cast<float4 *>(to) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        else { to[0] = v.x * inv; to[1] = v.y * inv; to[2] = v.z * inv; to[3] = v.w * inv; }
+    }
+    cl.sync(); // (nobody leaves while its rows are read)
+}
 
 // ---------------------------------------------------------------------------------------------------- any head size
 // For head sizes that are not 64 or 128. Sixteen query rows, 32 slots at a time, everything in 32-bit arithmetic on the CUDA cores.  Thread (slot, row group) takes four scores; a warp
@@ -136,7 +177,8 @@ __global__ void __launch_bounds__(128) sv_k_attn(const __grid_constant__ SvAttn 
     for (int r = 0; r < 4; r++) {
         const int row = r0 + warp * 4 + r;
         if (lane == 0 && row < rows) {
-            reinterpret_cast<float2 *>(ml)[((int64_t)split * a.G + g) * rows + row] = make_float2(m[r], l[r]);
+            if (s.splits == 1) sv_put_lse(s, (int64_t)g * rows + row, m[r], l[r]);
+            else reinterpret_cast<float2 *>(ml)[((int64_t)split * a.G + g) * rows + row] = make_float2(m[r], l[r]);
             sc[warp * 4 + r] = s.splits == 1 ? (l[r] > 0.f ? 1.f / l[r] : 0.f) : 1.f;
         }
     }
@@ -165,7 +207,7 @@ __global__ void __launch_bounds__(256) sv_k_join(const __grid_constant__ SvAttn 
     const int tid = threadIdx.x, lane = tid & 31, hs = a.hs, g = blockIdx.y;
     const SvSeq &s = a.seq[blockIdx.z];
     const int rows = s.n_tok * a.R, row = blockIdx.x * 8 + (tid >> 5);
-    if (row >= rows || (s.splits == 1 && !s.lse)) return;
+    if (row >= rows || s.splits == 1) return;
     const float2 *ml = reinterpret_cast<const float2 *>(s.part + (int64_t)s.splits * a.G * rows * hs);
     const int64_t at = (int64_t)g * rows + row, step = (int64_t)a.G * rows;
     float mx = SV_NONE;
@@ -181,7 +223,6 @@ __global__ void __launch_bounds__(256) sv_k_join(const __grid_constant__ SvAttn 
             f = exp2f(p.x - ref);
             l = fmaf(p.y, f, l);
         }
-        if (s.splits == 1) break;
         for (int i = 0; i < min(32, s.splits - i0); i += 8) {
             float v[8][8];
 #pragma unroll
@@ -200,8 +241,7 @@ __global__ void __launch_bounds__(256) sv_k_join(const __grid_constant__ SvAttn 
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    if (s.lse && lane == 0) s.lse[at] = l > 0.f ? mx + log2f(l) : INFINITY; // (a row that sees nothing adds nothing)
-    if (s.splits == 1) return;
+    if (lane == 0) sv_put_lse(s, at, mx, l);
     const float inv = l > 0.f ? 1.f / l : 0.f;
     float *to = a.out + ((int64_t)(s.tok0 + row / a.R) * a.n_heads + g * a.R + row % a.R) * hs;
 #pragma unroll

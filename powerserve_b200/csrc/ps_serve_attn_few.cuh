@@ -87,7 +87,9 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 && D == 128 ? 3 : 4) sv_k_
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int KS = D / 16, HALF = D / 64; // steps of the first product; items of 64 channels
     __shared__ uint4 s_q[KS][32];             // the queries' fragments: hi, hi, lo, lo
-    __shared__ float s_qinv[SV_FEW_ROWS], s_m[4][SV_FEW_ROWS], s_l[4][SV_FEW_ROWS], s_o[4][SV_FEW_ROWS][D + 4];
+    __shared__ float s_top[SV_FEW_ROWS], s_sum[SV_FEW_ROWS]; // the CTA's rows, for its cluster
+    __shared__ float s_qinv[SV_FEW_ROWS], s_m[4][SV_FEW_ROWS], s_l[4][SV_FEW_ROWS];
+    __shared__ __align__(16) float s_o[4][SV_FEW_ROWS][D + 4];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = lane & 3, n8 = lane >> 2;
     const int si = sv_find(a, blockIdx.x), split = blockIdx.x - a.seq[si].unit0, g = blockIdx.y;
     const SvSeq &s = a.seq[si];
@@ -285,8 +287,17 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 && D == 128 ? 3 : 4) sv_k_
             l = fmaf(s_l[w][r], f, l);
             v = fmaf(s_o[w][r][d], f, v);
         }
-        if (d == 0) ml[((int64_t)split * a.G + g) * rows + r] = make_float2(m, l * (1.f / 32768.f));
+        if (a.cluster > 1) { // (who writes an element of s_o[0] is the only one that reads it)
+            s_o[0][r][d] = v;
+            if (d == 0) { s_top[r] = m; s_sum[r] = l; }
+            continue;
+        }
+        if (d == 0) {
+            if (s.splits == 1) sv_put_lse(s, (int64_t)g * rows + r, m, l * (1.f / 32768.f));
+            else ml[((int64_t)split * a.G + g) * rows + r] = make_float2(m, l * (1.f / 32768.f));
+        }
         if (s.splits == 1) a.out[((int64_t)(s.tok0 + r / a.R) * a.n_heads + g * a.R + r % a.R) * D + d] = l > 0.f ? v / l : 0.f;
         else s.part[(((int64_t)split * a.G + g) * rows + r) * D + d] = v * (1.f / 32768.f);
     }
+    if (a.cluster > 1) sv_join_cluster<D>(a, s, g, 0, rows, rows, &s_o[0][0][0], D + 4, s_top, s_sum);
 }

@@ -534,7 +534,10 @@ __global__ void __launch_bounds__(SV_TC_THREADS, 1) sv_k_attn_tc(const __grid_co
             if (lane == 0) ps_mbar_arrive(&o_empty[b]);
         }
         if (r < rows) {
-            if (half == 0) reinterpret_cast<float2 *>(s.part + (int64_t)s.splits * a.G * all_rows * D)[((int64_t)split * a.G + g) * all_rows + row] = make_float2(m, l * (1.f / 32768.f));
+            if (half == 0) {
+                if (s.splits == 1) sv_put_lse(s, (int64_t)g * all_rows + row, m, l * (1.f / 32768.f));
+                else reinterpret_cast<float2 *>(s.part + (int64_t)s.splits * a.G * all_rows * D)[((int64_t)split * a.G + g) * all_rows + row] = make_float2(m, l * (1.f / 32768.f));
+            }
             const float f = s.splits == 1 ? (l > 0.f ? 1.f / l : 0.f) : 1.f / 32768.f;
             float *to = s.splits == 1 ? a.out + ((int64_t)(s.tok0 + row / a.R) * a.n_heads + g * a.R + row % a.R) * D : s.part + (((int64_t)split * a.G + g) * all_rows + row) * D;
             to += half * (D / 2);

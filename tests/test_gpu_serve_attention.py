@@ -130,6 +130,13 @@ def test_long_caches(be, D, H, G):
     check(be, c, H, weight=True)
 
 
+@pytest.mark.parametrize("D,dtype", [(64, "f32"), (64, "bf16"), (128, "f32"), (128, "bf16")])
+@pytest.mark.parametrize("lens,toks", [([1000, 130, 700], [1, 0, 2]), ([129, 64], [2, 1]), ([513, 511], [1, 1]), ([1023], [2]), ([1100], [1]), ([2100, 5], [1, 1]), ([1000] * 20, [1] * 20)])
+def test_few_rows_whose_splits_are_a_cluster_or_joined(be, D, dtype, lens, toks):
+    c = S.Caches(be, lens, toks, 2, D, dtype=dtype, hidden=True, weight=True, seed=sum(lens) + D)
+    check(be, c, 8, weight=True, seed=D)
+
+
 def test_more_sequences_than_a_table(be):
     lens = [1 + (i * 37) % 90 for i in range(150)]
     c = S.Caches(be, lens, [min(n, 1 + i % 3) if i % 11 else 0 for i, n in enumerate(lens)], 2, 64, seed=10, weight=True)
