@@ -311,8 +311,8 @@ int ps_serve_kv_evict(PsServeCall *c, const ps_cuda_cache *caches, int n_sets, i
             at += up(4 * (size_t)n_kv_heads * (1 + 2 * (size_t)a.set[i].moves));
         }
         const int keys = most_kv <= SV_KEYS ? most_kv : 0;
-        SV_CK(cudaFuncSetAttribute(sv_k_select, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * SV_KEYS));
-        sv_k_select<<<heads, SV_SEL_THREADS, 4 * (size_t)keys, c->stream>>>(a, keys);
+        SV_CK(cudaFuncSetAttribute(sv_k_select, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * sv_key_at(SV_KEYS)));
+        sv_k_select<<<heads, SV_SEL_THREADS, 4 * (size_t)sv_key_at(keys), c->stream>>>(a, keys);
         SV_LAUNCHED("kv_evict");
         if (most) {
             cudaLaunchConfig_t cfg{};

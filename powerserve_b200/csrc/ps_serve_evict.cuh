@@ -172,10 +172,13 @@ __global__ void __launch_bounds__(256) sv_k_evict_few(const __grid_constant__ Sv
     }
 }
 
+// (a thread that walks a run of slots meets other banks than its neighbours)
+PS_HD int sv_key_at(int j) { return j + (j >> 5); }
+
 // Many evictions: a CTA a head finds the border's key by three passes of a radix select and lists the moves; sv_k_move makes them. Bound by latency: eight passes over a head's keys, each with a scan
 // over the block; 32 heads of 8 190 slots 28 us alone, 96 of 5 001 21.
 __global__ void __launch_bounds__(SV_SEL_THREADS) sv_k_select(const __grid_constant__ SvEvict a, int keys) {
-    extern __shared__ uint32_t sv_keys[];   // `keys` of them: as many as the longest cache has slots, or none
+    extern __shared__ uint32_t sv_keys[];   // of `keys` slots: as many as the longest cache has, or none
     __shared__ uint32_t hist[2048], ws[32];
     __shared__ uint32_t s_bin, s_above;
     const SvSet &s = a.set[blockIdx.y];
@@ -183,10 +186,22 @@ __global__ void __launch_bounds__(SV_SEL_THREADS) sv_k_select(const __grid_const
     SvHead h(a, s, g);
     const int n = h.n, keep = h.keep;
     int32_t *list = s.list + (int64_t)g * (1 + 2 * (int64_t)s.moves);
-    h.after = sv_after(a, h, reinterpret_cast<int *>(ws));
-    uint32_t n_safe, c = 0;
+    int newest = INT32_MIN;
+#pragma unroll 4
+    for (int j = tid; j < n; j += SV_SEL_THREADS) {
+        if (keys) sv_keys[sv_key_at(j)] = sv_order(h.w[j]);
+        if (h.pos) newest = max(newest, h.pos[j]);
+    }
+    newest = sv_block_max(newest, reinterpret_cast<int *>(ws));
+    if (h.pos) h.after = (int64_t)newest - a.n_recent;
+    uint32_t n_safe, c = 0, safe_bits = 0; // (of the thread's first 32 slots)
     if (h.pos)
-        for (int j = tid; j < n; j += SV_SEL_THREADS) c += h.safe(j);
+#pragma unroll 4
+        for (int j = tid, i = 0; j < n; j += SV_SEL_THREADS, i++) {
+            const bool safe = h.safe(j);
+            c += safe;
+            if (i < 32) safe_bits |= (uint32_t)safe << i;
+        }
     sv_scan(c, ws, n_safe);
     // where the safe slots alone are more than are kept, the others are out (0) and the border lies among the safe; else the safe are above all
     const bool in_safe = n_safe >= (uint32_t)keep && keep > 0;
@@ -194,11 +209,12 @@ __global__ void __launch_bounds__(SV_SEL_THREADS) sv_k_select(const __grid_const
         const bool safe = h.safe(j);
         return safe == in_safe ? sv_order(h.w[j]) : in_safe ? 0u : SV_SAFE;
     };
-    if (keys) {
-        for (int j = tid; j < n; j += SV_SEL_THREADS) sv_keys[j] = make(j);
+    if (keys && h.pos) {
+        for (int j = tid, i = 0; j < n; j += SV_SEL_THREADS, i++)
+            if ((i < 32 ? (safe_bits >> i & 1) != 0 : h.safe(j)) != in_safe) sv_keys[sv_key_at(j)] = in_safe ? 0u : SV_SAFE;
         __syncthreads();
     }
-    auto key_of = [&](int j) { return keys ? sv_keys[j] : make(j); };
+    auto key_of = [&](int j) { return keys ? sv_keys[sv_key_at(j)] : make(j); };
     uint32_t above = 0, key = 0, mask = 0;   // slots with a larger key; the border's key as far as it is known
     for (int pass = 0; pass < 3; pass++) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
