@@ -365,30 +365,41 @@ template <bool LIST> PS_D void sv_pick(const SvSample &a, int64_t row, const SvS
     for (int w = 0; w < warp; w++) before += sh.red[w]; // (they still hold the warps' masses)
     if (goal < before || goal >= before + mine) return;
     const int from = LIST ? 0 : r.w0, to = LIST ? r.listed : r.w1;
-    for (int i = from; i < to; i += 32) {
-        float v = -INFINITY;
-        unsigned long long key = 0;
-        if (i + lane < to) {
-            const int at = LIST ? sh.lists[warp][i + lane] : i + lane;
-            v = x[at];
-            key = sv_key(v, r.i0 + at);
-        }
-        const unsigned long long m = v > -INFINITY ? mass_of(v, key) : 0;
-        unsigned long long inc = m;
+    constexpr int W = LIST ? 1 : 2; // weights under way at a time (lists are short; four cost registers: 64 rows of mixed settings 70 us, 67 with two, 64 without filters 40 and 41, with one 45)
+    for (int i = from; i < to; i += 32 * W) {
+        unsigned long long m[W], key[W], sum = 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const unsigned long long v2 = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += v2;
+        for (int e = 0; e < W; e++) {
+            const int n = i + 32 * e + lane, at = n < to ? LIST ? sh.lists[warp][n] : n : -1;
+            const float v = at >= 0 ? x[at] : -INFINITY;
+            key[e] = sv_key(v, r.i0 + at);
+            m[e] = mass_of(v, key[e]);
+            if (!(v > -INFINITY)) m[e] = 0;
+            sum += m[e];
         }
-        const unsigned ball = __ballot_sync(0xffffffffu, goal < before + inc);
-        if (ball) {
-            if (lane == __ffs(ball) - 1) {
-                a.ids[row] = (int)~(uint32_t)key;
-                if (a.probs) a.probs[row] = (float)((double)m / (double)all);
+        if (W > 1) {
+#pragma unroll
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (goal >= before + sum) { before += sum; continue; }
+        }
+#pragma unroll
+        for (int e = 0; e < W; e++) {
+            unsigned long long inc = m[e];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned long long v2 = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += v2;
             }
-            return;
+            const unsigned ball = __ballot_sync(0xffffffffu, goal < before + inc);
+            if (ball) {
+                if (lane == __ffs(ball) - 1) {
+                    a.ids[row] = (int)~(uint32_t)key[e];
+                    if (a.probs) a.probs[row] = (float)((double)m[e] / (double)all);
+                }
+                return;
+            }
+            before += __shfl_sync(0xffffffffu, inc, 31);
         }
-        before += __shfl_sync(0xffffffffu, inc, 31);
     }
 }
 

@@ -83,6 +83,13 @@ def test_few_go(be, gone, dtype):
     check(be, lens, [n - gone for n in lens], 3, 128, dtype=dtype, n_recent=1, same=True, seed=gone, weights=lambda shape, r: r.integers(0, 4, shape))
 
 
+@pytest.mark.parametrize("lens,keeps", [([40001], [9000]), ([50001], [300]), ([50001, 17, 33000], [49970, 9, 12345]), ([49152, 49153], [5000, 5000])])
+@pytest.mark.parametrize("n_recent", [100, 20000])
+def test_long_caches(be, lens, keeps, n_recent):
+    """more slots than a thread has bits for, than shared memory has keys for, and more safe ones than are kept"""
+    check(be, lens, keeps, 2, 32, dtype="bf16", n_sink=4, n_recent=n_recent, order=True, seed=len(lens) + n_recent)
+
+
 @pytest.mark.parametrize("same", [False, True])
 def test_without_positions(be, same):
     check(be, [700, 5], [350, 2], 2, 128, pos=False, same=same)
