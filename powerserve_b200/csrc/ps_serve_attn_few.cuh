@@ -239,10 +239,10 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 && D == 128 ? 3 : 4) sv_k_
         const float r0 = t0 == SV_NONE ? 0.f : t0, r1 = t1 == SV_NONE ? 0.f : t1, f0 = sv_ex2(m0 - r0), f1 = sv_ex2(m1 - r1);
         m0 = t0;
         m1 = t1;
-        // 2^15 p, and so its sum (the thread's; those of a row are joined at the end)
+        // 2^15 p, and so its sum (the thread's; those of a row are joined at the end).  The factor comes after: 15 in the exponent would cost the large weights four bits
         float p[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) p[e] = sv_ex2(z[e] + (15.f - (e & 1 ? r1 : r0)));
+        for (int e = 0; e < 4; e++) p[e] = sv_ex2(z[e] - (e & 1 ? r1 : r0)) * 32768.f;
         l0 = fmaf(l0, f0, p[0] + p[2]);
         l1 = fmaf(l1, f1, p[1] + p[3]);
         uint32_t ph0, pl0, ph1, pl1;
