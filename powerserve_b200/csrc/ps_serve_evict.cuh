@@ -175,8 +175,9 @@ __global__ void __launch_bounds__(256) sv_k_evict_few(const __grid_constant__ Sv
 // (a thread that walks a run of slots meets other banks than its neighbours)
 PS_HD int sv_key_at(int j) { return j + (j >> 5); }
 
-// Many evictions: a CTA a head finds the border's key by three passes of a radix select and lists the moves; sv_k_move makes them. Bound by latency: eight passes over a head's keys, each with a scan
-// over the block; 32 heads of 8 190 slots 28 us alone, 96 of 5 001 21.
+// Many evictions: a CTA a head finds the border's key by three passes of a radix select and lists the moves; sv_k_move makes them. Bound by latency: seven passes over a head's keys, most with a scan
+// over the block; 32 heads of 8 190 slots 20 us alone (28 with three readings of weights and positions and
+// runs of keys in one bank), 96 of 5 001 18.
 __global__ void __launch_bounds__(SV_SEL_THREADS) sv_k_select(const __grid_constant__ SvEvict a, int keys) {
     extern __shared__ uint32_t sv_keys[];   // of `keys` slots: as many as the longest cache has, or none
     __shared__ uint32_t hist[2048], ws[32];

@@ -10,8 +10,8 @@
 // the border becomes a number (logit, token) to compare with.  Rows whose lists do not fit, or whose border lies below (flat ones), go the same way over all of
 // their tokens.  No filter: the running mass over all tokens.
 // Bound by latency: a row is four to seven exchanges across its cluster, and two CTAs an SM hide little of one another's; then by the 45-bit exponentials, which top-p needs of all tokens
-// (64-bit arithmetic: borders would move with float32's). One row of 151 936: largest logit 8 us, min-p 11, top-k 40 with top-p 19, top-p alone 33; 64 rows of 128 256: 17, 27, 37, 100;
-// 256 rows of 151 936: 67 (2.3 TB/s), 104, 122, 410. Flat rows (their border is below 2^-16 of the largest) 54 / 170 / 703.
+// (64-bit arithmetic: borders would move with float32's). One row of 151 936: largest logit 8 us, min-p 11, no filter 13, top-k 40 with top-p 19, top-p alone 33; 64 rows of 128 256: 17, 27, 41, 37, 100;
+// 256 rows of 151 936: 67 (2.3 TB/s), 104, 149, 122, 408. Flat rows (their border is below 2^-16 of the largest) 54 / 170 / 703.
 #pragma once
 #include "ps_ptx.cuh"
 
