@@ -205,7 +205,11 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
             const dim3 grid(units, n_kv_heads, row_tiles);
             if (few) {
                 const bool f32 = cache_type == PS_TYPE_F32;
-                auto kern = hs == 64 ? (f32 ? sv_k_attn_few<float, 64> : sv_k_attn_few<__nv_bfloat16, 64>) : (f32 ? sv_k_attn_few<float, 128> : sv_k_attn_few<__nv_bfloat16, 128>);
+                auto pick = [&](auto cl) {
+                    constexpr bool CL = decltype(cl)::value;
+                    return hs == 64 ? (f32 ? sv_k_attn_few<float, 64, CL> : sv_k_attn_few<__nv_bfloat16, 64, CL>) : (f32 ? sv_k_attn_few<float, 128, CL> : sv_k_attn_few<__nv_bfloat16, 128, CL>);
+                };
+                auto kern = a.cluster > 1 ? pick(std::true_type{}) : pick(std::false_type{});
                 cudaLaunchConfig_t cfg{};
                 cudaLaunchAttribute attr[1];
                 attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -297,7 +301,7 @@ int ps_serve_kv_evict(PsServeCall *c, const ps_cuda_cache *caches, int n_sets, i
             bytes += up(4 * (size_t)n_kv_heads * (1 + 2 * (size_t)d.moves));
         }
         const dim3 heads(n_kv_heads, n);
-        if (most_gone <= SV_FEW) { // one by one costs a pass over the weights each: some 1 025 slots of 256 heads 16 us for one, 21 for eight; the select and its moves 25 for nine (from Python)
+        if (most_gone <= SV_FEW) { // one by one costs a pass over the weights each: some 1 025 slots of 256 heads 15 us for one, 21 for eight; the select and its moves 23 for nine (arrays apart from the old ones)
             if (es == 4) sv_k_evict_few<uint32_t><<<heads, 256, 0, c->stream>>>(a);
             else sv_k_evict_few<uint16_t><<<heads, 256, 0, c->stream>>>(a);
             SV_LAUNCHED("kv_evict");

@@ -82,7 +82,8 @@ PS_D uint32_t sv_turn(uint32_t x) { // an 8 x 8 matrix of halves, transposed
     return y;
 }
 
-template <typename T, int D>
+// CL: a sequence's splits are a cluster (that code in one kernel with the other: 64 sessions 125 -> 129 us)
+template <typename T, int D, bool CL>
 __global__ void __launch_bounds__(128, sizeof(T) == 4 && D == 128 ? 3 : 4) sv_k_attn_few(const __grid_constant__ SvAttn a) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int KS = D / 16, HALF = D / 64; // steps of the first product; items of 64 channels
@@ -287,7 +288,7 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 && D == 128 ? 3 : 4) sv_k_
             l = fmaf(s_l[w][r], f, l);
             v = fmaf(s_o[w][r][d], f, v);
         }
-        if (a.cluster > 1) { // (who writes an element of s_o[0] is the only one that reads it)
+        if (CL) { // (who writes an element of s_o[0] is the only one that reads it)
             s_o[0][r][d] = v;
             if (d == 0) { s_top[r] = m; s_sum[r] = l; }
             continue;
@@ -299,5 +300,5 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 && D == 128 ? 3 : 4) sv_k_
         if (s.splits == 1) a.out[((int64_t)(s.tok0 + r / a.R) * a.n_heads + g * a.R + r % a.R) * D + d] = l > 0.f ? v / l : 0.f;
         else s.part[(((int64_t)split * a.G + g) * rows + r) * D + d] = v * (1.f / 32768.f);
     }
-    if (a.cluster > 1) sv_join_cluster<D>(a, s, g, 0, rows, rows, &s_o[0][0][0], D + 4, s_top, s_sum);
+    if (CL) sv_join_cluster<D>(a, s, g, 0, rows, rows, &s_o[0][0][0], D + 4, s_top, s_sum);
 }
