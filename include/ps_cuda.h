@@ -241,7 +241,8 @@ const float *ps_cuda_logits_dev(ps_cuda_ctx *ctx);
 int ps_cuda_sample_topk(ps_cuda_ctx *ctx, int row, int k, float *logits_out, int32_t *tokens_out);
 
 /* ps_cuda_sample on the first `rows` rows of the last forward pass's logits (whose logits_host may have been NULL), all arrays the HOST's: a
- * server's step draws the next token of every session with its own settings, and only ids (and probabilities, if probs is not NULL) come back */
+ * server's step draws the next token of every session with its own settings, and only ids (and probabilities, if probs is not NULL) come back.
+ * ps_cuda_decode_greedy leaves its last step's row (none with tensor parallelism), a pass with lm_head = 0 none; more rows than there are are refused */
 int ps_cuda_sample_last(ps_cuda_ctx *ctx, int rows, const ps_cuda_sampler *samplers, const float *u, int32_t *ids, float *probs);
 
 /* ---------------------------------------------------------------------------------------------- tensor parallelism

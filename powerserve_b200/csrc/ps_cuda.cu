@@ -119,7 +119,7 @@ struct ps_cuda_ctx {
     float *x = nullptr, *xn = nullptr, *q = nullptr, *k = nullptr, *v = nullptr, *qr = nullptr, *att = nullptr;
     float *g = nullptr, *u = nullptr, *kq = nullptr, *logits = nullptr;
     const float *logits_last = nullptr; // where the last forward left its [bs][vocab] logits (ps_cuda_logits_dev)
-    int logits_rows = 0;                // rows of that buffer
+    int logits_rows = 0;                // rows of that buffer that the last pass wrote: 0 after one without logits, or one that failed
     unsigned long long *topk_cand = nullptr; // device top-k scratch: keys of the slices' best, then the result: ids [k], values [k]
     uint32_t *aqs = nullptr, *absp = nullptr;
     uint8_t *mk_x = nullptr; // activation records of a batch (ps_k_matmul_mk)
@@ -2860,6 +2860,7 @@ int ps_cuda_forward(ps_cuda_ctx *ctx, const int32_t *tokens, const int32_t *pos,
     if ((rc = stage_call(ctx, bs))) return rc;
     PS_CK(cudaEventRecord(ctx->ev0, ctx->stream));
     ctx->logits_last = ctx->logits;
+    ctx->logits_rows = 0;
     if (ctx->arch) {
         rc = (bs == 1 && lm_head && arch_graph_usable(ctx)) ? run_step(ctx, false, pos[0] + 1) : arch_forward(ctx, bs, lm_head, pos[0]);
     } else if (ctx->tp > 1 && bs > 1 && ctx->nccl_comm && ctx->opt_tp_batch) {
@@ -2891,8 +2892,8 @@ int ps_cuda_forward(ps_cuda_ctx *ctx, const int32_t *tokens, const int32_t *pos,
     }
     if (rc) return rc;
     PS_CK(cudaEventRecord(ctx->ev1, ctx->stream));
-    ctx->logits_rows = lm_head ? bs : 0;
     if ((rc = lm_head && logits_host ? logits_to_host(ctx, logits_host, (size_t)bs * ctx->d.vocab_size * 4) : sync_and_check(ctx))) return rc;
+    ctx->logits_rows = lm_head ? bs : 0;
     { float ms = 0.f; PS_CK(cudaEventElapsedTime(&ms, ctx->ev0, ctx->ev1)); ctx->last_ms = ms; }
     ctx->position = pos[0] + bs; // m_kv->advance(batch_size), llama_model.cpp:109
     kv_set_mask(ctx, 0, ctx->position, 0);
@@ -3057,16 +3058,17 @@ int ps_cuda_forward_sessions(ps_cuda_ctx *ctx, const int32_t *session_ids, const
     ctx->h2d += (int64_t)sizeof(float *) * 2 * d.n_layers * d.max_batch;
     PS_CK(cudaEventRecord(ctx->ev0, ctx->stream));
     SessRun sr{n_kv_max};
+    ctx->logits_last = ctx->logits;
+    ctx->logits_rows = 0;
     int rc = forward_ops(ctx, n, lm_head, 0, -1, &sr);
     if (rc) return rc;
-    ctx->logits_last = ctx->logits;
-    ctx->logits_rows = lm_head ? n : 0;
     if (lm_head && greedy_ids) {
         PS_DEP(ps_k_argmax, n, 1024, 0, ctx->logits, d.vocab_size, ctx->ids_dev, ctx->ids_dev + d.max_batch); // one CTA per column
         PS_CK(cudaMemcpyAsync(ctx->h_ids, ctx->ids_dev, (size_t)n * 4, cudaMemcpyDeviceToHost, ctx->stream));
     }
     PS_CK(cudaEventRecord(ctx->ev1, ctx->stream));
     if ((rc = lm_head && logits_host ? logits_to_host(ctx, logits_host, (size_t)n * d.vocab_size * 4) : sync_and_check(ctx))) return rc;
+    ctx->logits_rows = lm_head ? n : 0;
     if (lm_head && greedy_ids) { memcpy(greedy_ids, ctx->h_ids, (size_t)n * 4); ctx->d2h += (int64_t)n * 4; }
     { float ms = 0.f; PS_CK(cudaEventElapsedTime(&ms, ctx->ev0, ctx->ev1)); ctx->last_ms = ms; }
     for (int i = 0; i < n; i++) { // m_kv->advance(1) of every session in the batch
@@ -3106,10 +3108,11 @@ int ps_cuda_forward_tree(ps_cuda_ctx *ctx, const int32_t *tokens, const int32_t 
     if (int rc_ = stage_call(ctx, bs, true)) return rc_;
     PS_CK(cudaEventRecord(ctx->ev0, ctx->stream));
     PS_DEP(ps_k_tree_mask, dim3((unsigned)std::min<int64_t>((base + bs + 255) / 256, 64), (unsigned)bs), 256, 0, ctx->tree_bias, ctx->slot_mask_dev, ctx->tree_dev, base, bs, base + bs);
+    ctx->logits_last = ctx->logits;
+    ctx->logits_rows = 0;
     int rc = forward_ops(ctx, bs, lm_head, 0, base);
     if (rc) return rc;
     PS_CK(cudaEventRecord(ctx->ev1, ctx->stream));
-    ctx->logits_last = ctx->logits;
     if (lm_head == 2) { // greedy ids only (ProbArray + greedy_sample with top_k = 1 per row, first maximum): bs ints come back instead of bs x vocab floats
         PS_DEP(ps_k_argmax, bs, 1024, 0, ctx->logits, ctx->d.vocab_size, ctx->ids_dev, ctx->ids_dev + 2048); // one CTA per tree node
         PS_CK(cudaMemcpyAsync(ctx->h_ids, ctx->ids_dev, (size_t)bs * 4, cudaMemcpyDeviceToHost, ctx->stream));
@@ -3117,6 +3120,7 @@ int ps_cuda_forward_tree(ps_cuda_ctx *ctx, const int32_t *tokens, const int32_t 
         memcpy(logits_host, ctx->h_ids, (size_t)bs * 4);
         ctx->d2h += (int64_t)bs * 4;
     } else if ((rc = lm_head ? logits_to_host(ctx, logits_host, (size_t)bs * ctx->d.vocab_size * 4) : sync_and_check(ctx))) return rc;
+    ctx->logits_rows = lm_head ? bs : 0;
     { float ms = 0.f; PS_CK(cudaEventElapsedTime(&ms, ctx->ev0, ctx->ev1)); ctx->last_ms = ms; }
     ctx->last_batch = bs;
     kv_set_mask(ctx, base, base + bs, 0);   // advance_tokens(bs)
@@ -3135,6 +3139,8 @@ int ps_cuda_decode_greedy(ps_cuda_ctx *ctx, int32_t first_token, int n_steps, in
     ctx->h_tokens[0] = first_token;
     PS_CK(cudaMemcpyAsync(ctx->tokens_dev, ctx->h_tokens, 4, cudaMemcpyHostToDevice, ctx->stream));
     ctx->h2d += 4;
+    ctx->logits_last = ctx->logits;
+    ctx->logits_rows = 0;
     if (arch_graph_usable(ctx) || (!ctx->arch && ((ctx->opt_fused && ctx->fused_ok) || ops_graph_usable(ctx) || mv_usable(ctx)))) {
         int32_t *slot = &ctx->h_ids[4096];
         slot[0] = ctx->position;
@@ -3163,6 +3169,7 @@ int ps_cuda_decode_greedy(ps_cuda_ctx *ctx, int32_t first_token, int n_steps, in
         { float ms = 0.f; PS_CK(cudaEventElapsedTime(&ms, ctx->ev0, ctx->ev1)); ctx->last_ms = ms; }
         memcpy(ids_host, ctx->h_ids, (size_t)n_steps * 4);
         ctx->d2h += (int64_t)n_steps * 4;
+        ctx->logits_rows = ctx->tp == 1; // (the last step's; a rank of several has picked from its share alone)
         kv_set_mask(ctx, 0, ctx->position + n_steps, 0);
         ctx->position += n_steps;
         return 0;
@@ -3185,6 +3192,7 @@ int ps_cuda_decode_greedy(ps_cuda_ctx *ctx, int32_t first_token, int n_steps, in
     { float ms = 0.f; PS_CK(cudaEventElapsedTime(&ms, ctx->ev0, ctx->ev1)); ctx->last_ms = ms; }
     memcpy(ids_host, ctx->h_ids, (size_t)n_steps * 4);
     ctx->d2h += (int64_t)n_steps * 4;
+    ctx->logits_rows = 1;
     kv_set_mask(ctx, 0, ctx->position + n_steps, 0);
     ctx->position += n_steps;
     return 0;
@@ -3196,7 +3204,7 @@ int ps_cuda_sample_topk(ps_cuda_ctx *ctx, int row, int k, float *logits_out, int
     std::lock_guard<std::mutex> lock(ctx->mu);
     const int vocab = ctx->d.vocab_size;
     if (k <= 0 || k > PS_TOPK_MAX || k > vocab) return fail(ctx, PS_CUDA_ERR_INVALID, "sample_topk: k = %d outside [1,%d]", k, std::min(PS_TOPK_MAX, vocab));
-    if (!ctx->logits_last || row < 0 || row >= std::max(ctx->logits_rows, 1)) return fail(ctx, PS_CUDA_ERR_INVALID, "sample_topk: no logits row %d", row);
+    if (row < 0 || row >= ctx->logits_rows) return fail(ctx, PS_CUDA_ERR_INVALID, "sample_topk: no logits row %d, the last pass left %d", row, ctx->logits_rows);
     if (!logits_out || !tokens_out) return fail(ctx, PS_CUDA_ERR_INVALID, "sample_topk: null output");
     PS_CK(cudaSetDevice(ctx->device));
     const int n_slices = (vocab + PS_TOPK_SLICE - 1) / PS_TOPK_SLICE;
@@ -3221,7 +3229,7 @@ int ps_cuda_sample_topk(ps_cuda_ctx *ctx, int row, int k, float *logits_out, int
 
 int ps_cuda_sample_last(ps_cuda_ctx *ctx, int rows, const ps_cuda_sampler *samplers, const float *u, int32_t *ids, float *probs) {
     return serve(ctx, [&](PsServeCall *c) {
-        if (!ctx->logits_last || rows < 0 || rows > std::max(ctx->logits_rows, 1)) return fail(ctx, PS_CUDA_ERR_INVALID, "sample_last: %d rows, the last pass left %d", rows, ctx->logits_last ? std::max(ctx->logits_rows, 1) : 0);
+        if (rows < 0 || rows > ctx->logits_rows) return fail(ctx, PS_CUDA_ERR_INVALID, "sample_last: %d rows, the last pass left %d", rows, ctx->logits_rows);
         if (rows == 0) return 0;
         if (!samplers || !u || !ids) return fail(ctx, PS_CUDA_ERR_INVALID, "sample_last: null argument");
         if (rows > ctx->smp_rows) {
