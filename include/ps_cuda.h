@@ -202,7 +202,7 @@ int ps_cuda_forward(ps_cuda_ctx *ctx, const int32_t *tokens, const int32_t *pos,
  * causal), attention over the unmasked cache slots below the current position; the batch's K / V rows are appended at cache
  * slots position .. position + bs - 1 and the position advances by bs (CausalLM::Batch::save_kv + advance, causal_models.cpp:
  * 353-359) - callers roll back and `copy` the accepted tokens, as TokenTree::verify does.  bs <= min(max_batch, 32).
- * lm_head = 1: logits_host receives [bs][vocab] fp32; lm_head = 2: the greedy pick is made on the device (first maximum per row,
+ * lm_head = 1: logits_host receives [bs][vocab] fp32 (NULL: they stay on the device, for ps_cuda_sample_last or ps_cuda_sample_topk); lm_head = 2: the greedy pick is made on the device (first maximum per row,
  * llama_model.cpp:124-128 with top_k = 1) and logits_host receives bs int32 token ids instead. */
 int ps_cuda_forward_tree(ps_cuda_ctx *ctx, const int32_t *tokens, const int32_t *pos, int bs, const uint8_t *tree_mask, int lm_head,
                          float *logits_host);
@@ -233,7 +233,7 @@ int ps_cuda_host_alloc_on(int device, size_t bytes, void **host);     /* that th
 int ps_cuda_host_free(void *host);
 /* device-side logits of the last forward ([bs][vocab]) for callers that sample on the GPU */
 const float *ps_cuda_logits_dev(ps_cuda_ctx *ctx);
-/* Device-side sampling: ps_cuda_forward / ps_cuda_forward_sessions accept logits_host == NULL with
+/* Device-side sampling: ps_cuda_forward / _forward_sessions / _forward_tree accept logits_host == NULL with
  * lm_head = 1 - the logits stay on the device - and ps_cuda_sample_topk returns what ProbArray holds after
  * TopKSampler::apply (src/sampler/sampler.cpp:39-56, prob_array.hpp:43-49): the k <= 64 largest logits of row `row` of the
  * last forward pass, descending (equal logits by ascending token id), with their token ids.  2 k words cross PCIe instead of

@@ -608,14 +608,15 @@ class CudaModel:
                                               bs, int(lm_head), logits.ctypes.data if lm_head else None))
         return logits
 
-    def forward_tree(self, tokens, pos, tree_mask=None, lm_head: bool = True) -> Optional[np.ndarray]:
-        """The speculative path's forward (ps_cuda_forward_tree): arbitrary positions, in-batch tree mask [bs][bs] (None = causal)."""
+    def forward_tree(self, tokens, pos, tree_mask=None, lm_head: bool = True, want_logits: bool = True) -> Optional[np.ndarray]:
+        """The speculative path's forward (ps_cuda_forward_tree): arbitrary positions, in-batch tree mask [bs][bs] (None = causal).
+        want_logits = False: they stay on the device (draw from them with sample or sample_topk)"""
         t, p = _i32(tokens), _i32(pos)
         bs = len(t)
         m = None if tree_mask is None else np.ascontiguousarray(np.asarray(tree_mask, dtype=np.uint8).reshape(bs, bs))
-        logits = self.be.logits_pool.array(bs, self.vocab) if lm_head else None
+        logits = self.be.logits_pool.array(bs, self.vocab) if (lm_head and want_logits) else None
         self.be._ck(self.be.L.ps_cuda_forward_tree(self.be.h, t.ctypes.data_as(C.POINTER(C.c_int32)), p.ctypes.data_as(C.POINTER(C.c_int32)), bs,
-                                                   m.ctypes.data if m is not None else None, int(lm_head), logits.ctypes.data if lm_head else None))
+                                                   m.ctypes.data if m is not None else None, int(lm_head), logits.ctypes.data if logits is not None else None))
         return logits
 
     def decode_greedy(self, first_token: int, n_steps: int) -> np.ndarray:

@@ -3090,7 +3090,7 @@ int ps_cuda_forward_tree(ps_cuda_ctx *ctx, const int32_t *tokens, const int32_t 
     if (ctx->tp > 1) return fail(ctx, PS_CUDA_ERR_UNSUPPORTED, "forward_tree: tree batches are single-GPU");
     const int tb = std::min(ctx->d.max_batch, PS_TREE_MAX);
     if (bs <= 0 || bs > tb) return fail(ctx, PS_CUDA_ERR_INVALID, "forward_tree: batch %d outside [1,%d]", bs, tb);
-    if (lm_head && !logits_host) return fail(ctx, PS_CUDA_ERR_INVALID, "forward_tree: lm_head requested without an output buffer");
+    if (lm_head == 2 && !logits_host) return fail(ctx, PS_CUDA_ERR_INVALID, "forward_tree: greedy ids requested without an output buffer");
     const int base = ctx->position;
     if (base + bs > ctx->d.n_ctx) return fail(ctx, PS_CUDA_ERR_KV_FULL, "the length of kvcache is up to the preset threshold: %d", ctx->d.n_ctx);
     for (int i = 0; i < bs; i++) {
@@ -3119,7 +3119,7 @@ int ps_cuda_forward_tree(ps_cuda_ctx *ctx, const int32_t *tokens, const int32_t 
         if ((rc = sync_and_check(ctx))) return rc;
         memcpy(logits_host, ctx->h_ids, (size_t)bs * 4);
         ctx->d2h += (int64_t)bs * 4;
-    } else if ((rc = lm_head ? logits_to_host(ctx, logits_host, (size_t)bs * ctx->d.vocab_size * 4) : sync_and_check(ctx))) return rc;
+    } else if ((rc = lm_head && logits_host ? logits_to_host(ctx, logits_host, (size_t)bs * ctx->d.vocab_size * 4) : sync_and_check(ctx))) return rc;
     ctx->logits_rows = lm_head ? bs : 0;
     { float ms = 0.f; PS_CK(cudaEventElapsedTime(&ms, ctx->ev0, ctx->ev1)); ctx->last_ms = ms; }
     ctx->last_batch = bs;

@@ -98,6 +98,23 @@ def test_passes_without_logits_leave_none():
     m.close()
 
 
+def test_a_tree_s_rows_that_stay_on_the_device():
+    """a tree verified by draws: ids and probabilities come back, no logits"""
+    m = model(V, 16)
+    m.prefill(list(range(1, 40)), 16)
+    want = tree(m, 12, seed=5)
+    m.be.kv_rollback(12)
+    before = m.be.counter("d2h_bytes")
+    assert tree(m, 12, seed=5, want_logits=False) is None
+    drawn(m, want)
+    assert m.be.counter("d2h_bytes") - before == 12 * 8
+    refused(m, 13)
+    with pytest.raises(capi.PsCudaError, match="greedy ids"):
+        tree(m, 2, lm_head=2, want_logits=False)
+    drawn(m, want)          # (it was refused before anything ran)
+    m.close()
+
+
 def test_a_layer_list_model(tmp_path):
     layer = arch_synth.nufusun_layer
     cfg = arch_synth.nufusun_config(64, 500, [layer(2, 1, 16, 16, bias_max=9.0)], eps=1e-5, embed_scale=0.5)
