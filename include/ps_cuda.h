@@ -150,7 +150,7 @@ typedef struct {                /* one sequence's cache in one layer */
 /* Attention of a step's tokens - one a sequence, a chunk, or a tree of drafted ones - over the sequences' caches:
  * out[t][h] = sum_j p_j v_j with p = soft-max of scale * q[t][h] . k_j over the slots that the token sees: all that are filled and not hidden, of
  * the step's own those that tree_mask gives it (per sequence n_tok x n_tok bytes, row t = the tokens that token t sees, one sequence after another;
- * NULL: itself and the ones before).  A token that sees nothing gets zeros.  weight[g][j] += the sum of p_j over the sequence's tokens and the
+ * NULL: itself and the ones before).  A token that sees nothing gets zeros, one with a query that holds NaN or a score above float32's range NaN.  weight[g][j] += the sum of p_j over the sequence's tokens and the
  * heads of kv head g.  q and out: [tokens][n_heads * head_size] fp32, sequence after sequence; out may be q's memory only if it IS q; sequences may share K and V (a common
  * beginning), not weights.  What a filled slot that is not hidden holds must be finite.  head_size: multiples of 32 up to 256; at most 32 heads a kv head. */
 int ps_cuda_attn_tree(ps_cuda_ctx *ctx, float *out, const float *q, const ps_cuda_cache *caches, int n_seqs, int cache_type, int64_t head_size,

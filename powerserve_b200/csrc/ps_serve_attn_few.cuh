@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 && D == 128 ? 3 : 4) sv_k_
             if (s.splits == 1) sv_put_lse(s, (int64_t)g * rows + r, m, l * (1.f / 32768.f));
             else ml[((int64_t)split * a.G + g) * rows + r] = make_float2(m, l * (1.f / 32768.f));
         }
-        if (s.splits == 1) a.out[((int64_t)(s.tok0 + r / a.R) * a.n_heads + g * a.R + r % a.R) * D + d] = l > 0.f ? v / l : 0.f;
+        if (s.splits == 1) a.out[((int64_t)(s.tok0 + r / a.R) * a.n_heads + g * a.R + r % a.R) * D + d] = l == 0.f ? 0.f : v / l; // (a sum that is no number: so is the row)
         else s.part[(((int64_t)split * a.G + g) * rows + r) * D + d] = v * (1.f / 32768.f);
     }
     if (CL) sv_join_cluster<D>(a, s, g, 0, rows, rows, &s_o[0][0][0], D + 4, s_top, s_sum);
