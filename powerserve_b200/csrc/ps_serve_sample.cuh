@@ -628,11 +628,11 @@ __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_sample(const __grid_co
         bool over_any = false;
         {
             unsigned long long in = 0;
-            if (roughly) { // (no number, as with an infinite logit: the exact mass is asked for)
+            if (roughly) { // (no number, as with an infinite logit: the exact mass is asked for.  Masses are below 2^43, and sixteen times 2^59 fits 64 bits)
                 whole = sv_block<false>(sh, (unsigned long long)(rough * 16777216.f));
                 in = sv_block<false>(sh, (unsigned long long)(rough_in * 16777216.f) + 1);
                 const bool odd = __syncthreads_or(!(rough < 1e9f)) != 0;
-                if (odd) in = 1ull << 60;
+                if (odd) { in = 1ull << 59; whole = 0; }
             }
             const unsigned long long(*m)[16] = mail.post(cta, whole, in);
             unsigned long long all_in = 0;
