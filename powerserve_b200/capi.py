@@ -8,6 +8,7 @@ import atexit
 import ctypes as C
 import json
 import os
+import sys
 import threading
 import weakref
 from typing import Dict, List, Optional, Sequence
@@ -214,11 +215,29 @@ def exported_symbols() -> List[str]:
     return list(load_library()._ps_signatures.keys())
 
 
-def _dev(a) -> Optional[int]:
-    """device address of a DeviceBuffer, a tensor of another library (data_ptr), or an address"""
-    if a is None or isinstance(a, int):
+def _dev(what: str, a, device: int, need: int = 0, dtypes=None, row_stride: Optional[int] = None, sane=None) -> Optional[int]:
+    """device address of a DeviceBuffer, a torch tensor, or an address (which is taken as it is).  A buffer has to hold `need` bytes (if sane()); a tensor too, in the device's
+    memory, of one of the types named, its elements in order (a matrix with row_stride: its rows that far apart)"""
+    if a is None or isinstance(a, (int, np.integer)):
         return a
-    return a.ptr if hasattr(a, "ptr") else a.data_ptr()
+    if isinstance(a, DeviceBuffer):
+        size, p = a.nbytes, a.ptr
+    else:
+        torch = sys.modules.get("torch")
+        if torch is None or not isinstance(a, torch.Tensor):
+            raise PsCudaError(f"{what}: a DeviceBuffer, a torch tensor or an address, not a {type(a).__name__}")
+        if not a.is_cuda or a.device.index != device:
+            raise PsCudaError(f"{what}: a tensor on {a.device}, not in the memory of device {device}")
+        if dtypes and a.dtype not in [getattr(torch, t) for t in dtypes]:
+            raise PsCudaError(f"{what}: a tensor of {a.dtype}, not {' or '.join(dtypes)}")
+        size, p = a.nbytes, a.data_ptr()
+        if not a.is_contiguous():
+            if row_stride is None or a.dim() != 2 or a.stride(1) != 1 or a.stride(0) != row_stride:
+                raise PsCudaError(f"{what}: a tensor whose elements do not follow one another")
+            size = ((a.shape[0] - 1) * row_stride + a.shape[1]) * a.element_size()
+    if size < need and (sane is None or sane()):
+        raise PsCudaError(f"{what}: holds {size} bytes, the call needs {need}")
+    return p
 
 
 def _i32(a: Sequence[int]) -> np.ndarray:
@@ -367,7 +386,7 @@ class CudaBackend:
         rc = create(C.byref(h), device, C.byref(desc))
         if rc != 0:
             raise PsCudaError(f"ps_cuda_create failed ({rc}): {self.L.ps_cuda_last_error(None).decode()}")
-        self.h = h
+        self.h, self.device = h, device
         self.logits_pool = _LogitsPool(self.L, device=device)
 
     def _ck(self, rc: int):
@@ -467,7 +486,15 @@ class CudaBackend:
         """attention of a step's tokens over the caches (a CACHE array) of their sequences"""
         if caches.dtype != CACHE or not caches.flags.c_contiguous:
             raise PsCudaError("attn_tree: caches is a contiguous array of capi.CACHE records")
-        self._ck(self.L.ps_cuda_attn_tree(self.h, _dev(out), _dev(q), caches.ctypes.data, caches.size, cache_type, head_size, n_heads, n_kv_heads, _dev(tree_mask), scale))
+        tok = caches["n_tok"].astype(np.int64)
+
+        def sane():     # (where that makes no sense, the call itself says what is wrong)
+            return 0 < head_size <= 256 and head_size % 32 == 0 and 0 < n_kv_heads <= n_heads <= 32 * n_kv_heads and n_heads % n_kv_heads == 0 and bool(((tok >= 0) & (tok <= TREE_TOKENS) & (tok <= caches["n_kv"])).all())
+
+        rows = 4 * int(tok.sum()) * n_heads * head_size
+        self._ck(self.L.ps_cuda_attn_tree(
+            self.h, _dev("attn_tree: out", out, self.device, rows, ["float32"], sane=sane), _dev("attn_tree: q", q, self.device, rows, ["float32"], sane=sane), caches.ctypes.data, caches.size, cache_type,
+            head_size, n_heads, n_kv_heads, None if tree_mask is None else _dev("attn_tree: tree_mask", tree_mask, self.device, int(tok.dot(tok)), ["uint8", "bool", "int8"], sane=sane), scale))
 
     def kv_evict(self, caches: np.ndarray, n_kv_heads: int, head_size: int, n_sink: int = 0, n_recent: int = 0, cache_type: int = F32):
         """cuts every cache to its n_keep slots of the largest gathered weight, beside the first and latest positions"""
@@ -477,7 +504,11 @@ class CudaBackend:
 
     def sample(self, ids, probs, logits, vocab: int, rows: int, samplers, u, row_stride: Optional[int] = None):
         """a token of each row of logits by the row's settings (SAMPLER records on the device) and random number"""
-        self._ck(self.L.ps_cuda_sample(self.h, _dev(ids), _dev(probs), _dev(logits), vocab if row_stride is None else row_stride, vocab, rows, _dev(samplers), _dev(u)))
+        step, n = vocab if row_stride is None else row_stride, max(rows, 0)
+        last = 4 * ((n - 1) * step + vocab) if n and 0 < vocab <= min(step, 1 << 18) else 0     # (what is wrong with others the call itself says)
+        self._ck(self.L.ps_cuda_sample(self.h, _dev("sample: ids", ids, self.device, 4 * n, ["int32"]), _dev("sample: probs", probs, self.device, 4 * n, ["float32"]),
+                                       _dev("sample: logits", logits, self.device, last, ["float32"], step), step, vocab, rows,
+                                       _dev("sample: samplers", samplers, self.device, SAMPLER.itemsize * n), _dev("sample: u", u, self.device, 4 * n, ["float32"])))
 
     def read_device(self, dev_ptr: int, n_floats: int, dtype=np.float32) -> np.ndarray:
         out = np.empty(n_floats, dtype=dtype)
