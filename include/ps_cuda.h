@@ -74,7 +74,12 @@ int  ps_cuda_create(ps_cuda_ctx **out, int device, const ps_cuda_model_desc *des
 void ps_cuda_destroy(ps_cuda_ctx *ctx);
 const char *ps_cuda_last_error(const ps_cuda_ctx *ctx); /* ctx may be NULL: error of a failed create */
 int  ps_cuda_sync(ps_cuda_ctx *ctx); /* waits; PS_CUDA_ERR_CUDA if a kernel since the last report flagged a failure (results invalid) */
-void *ps_cuda_stream(ps_cuda_ctx *ctx);                 /* the cudaStream_t every call enqueues on */
+void *ps_cuda_stream(ps_cuda_ctx *ctx);                 /* the cudaStream_t every call enqueues on (it does not wait for the default stream) */
+/* For arrays that another stream of the device (a cudaStream_t; NULL: the default stream) works on: what the context is given after `enter` waits for what that stream
+ * holds then, and what that stream is given after `leave` for what the context holds then.  A stream that is being captured draws the calls between the two into its graph.
+ * In a capture of the context's own stream both do nothing for streams outside of it: the graph's launches are the caller's to put in order. */
+int ps_cuda_stream_enter(ps_cuda_ctx *ctx, void *stream);
+int ps_cuda_stream_leave(ps_cuda_ctx *ctx, void *stream);
 
 /* ---------------------------------------------------------------------------------------------- memory
  * CUDABuffer backing for graph intermediates (replaces CPUBuffer::create_buffer, src/backend/cpu_buffer.hpp:41-51)

@@ -138,6 +138,8 @@ def load_library() -> C.CDLL:
         "ps_cuda_last_error": (C.c_char_p, [vp]),
         "ps_cuda_sync": (ci, [vp]),
         "ps_cuda_stream": (vp, [vp]),
+        "ps_cuda_stream_enter": (ci, [vp, vp]),
+        "ps_cuda_stream_leave": (ci, [vp, vp]),
         "ps_cuda_malloc": (ci, [vp, sz, C.POINTER(vp)]),
         "ps_cuda_free": (ci, [vp, vp]),
         "ps_cuda_memcpy_h2d": (ci, [vp, vp, vp, sz]),
@@ -387,6 +389,7 @@ class CudaBackend:
         if rc != 0:
             raise PsCudaError(f"ps_cuda_create failed ({rc}): {self.L.ps_cuda_last_error(None).decode()}")
         self.h, self.device = h, device
+        self.stream = self.L.ps_cuda_stream(h)      # the cudaStream_t that every call enqueues on
         self.logits_pool = _LogitsPool(self.L, device=device)
 
     def _ck(self, rc: int):
@@ -481,7 +484,22 @@ class CudaBackend:
     def softmax(self, out, x, ne0, n_rows):
         self._ck(self.L.ps_cuda_softmax(self.h, out.ptr, x.ptr, ne0, n_rows))
 
-    # ---- serving operators (arrays: DeviceBuffers, tensors with data_ptr, or addresses; they belong to this context's stream while a call uses them)
+    # ---- serving operators (arrays: DeviceBuffers, torch tensors, or addresses).  In a process that uses torch on a device a call takes its place among what torch's current stream does:
+    # after what that stream holds, before what it is given next, in a capture of it as a part of the graph.  (Two to three microseconds on the
+    # host; none where torch works on the context's stream: with torch.cuda.stream(torch.cuda.ExternalStream(be.stream)).  What a tensor's memory saw on yet other streams is the caller's to order, as for torch's own operations.)
+    def _in_turn(self, call, *args):
+        torch = sys.modules.get("torch")
+        if torch is None or not torch.cuda.is_initialized():
+            return self._ck(call(self.h, *args))
+        stream = torch.cuda.current_stream(self.device).cuda_stream
+        if stream == self.stream:
+            return self._ck(call(self.h, *args))
+        self._ck(self.L.ps_cuda_stream_enter(self.h, stream))
+        try:
+            self._ck(call(self.h, *args))
+        finally:
+            self._ck(self.L.ps_cuda_stream_leave(self.h, stream))
+
     def attn_tree(self, out, q, caches: np.ndarray, n_heads: int, n_kv_heads: int, head_size: int, scale: float, tree_mask=None, cache_type: int = F32):
         """attention of a step's tokens over the caches (a CACHE array) of their sequences"""
         if caches.dtype != CACHE or not caches.flags.c_contiguous:
@@ -492,23 +510,23 @@ class CudaBackend:
             return 0 < head_size <= 256 and head_size % 32 == 0 and 0 < n_kv_heads <= n_heads <= 32 * n_kv_heads and n_heads % n_kv_heads == 0 and bool(((tok >= 0) & (tok <= TREE_TOKENS) & (tok <= caches["n_kv"])).all())
 
         rows = 4 * int(tok.sum()) * n_heads * head_size
-        self._ck(self.L.ps_cuda_attn_tree(
-            self.h, _dev("attn_tree: out", out, self.device, rows, ["float32"], sane=sane), _dev("attn_tree: q", q, self.device, rows, ["float32"], sane=sane), caches.ctypes.data, caches.size, cache_type,
-            head_size, n_heads, n_kv_heads, None if tree_mask is None else _dev("attn_tree: tree_mask", tree_mask, self.device, int(tok.dot(tok)), ["uint8", "bool", "int8"], sane=sane), scale))
+        self._in_turn(
+            self.L.ps_cuda_attn_tree, _dev("attn_tree: out", out, self.device, rows, ["float32"], sane=sane), _dev("attn_tree: q", q, self.device, rows, ["float32"], sane=sane), caches.ctypes.data, caches.size, cache_type,
+            head_size, n_heads, n_kv_heads, None if tree_mask is None else _dev("attn_tree: tree_mask", tree_mask, self.device, int(tok.dot(tok)), ["uint8", "bool", "int8"], sane=sane), scale)
 
     def kv_evict(self, caches: np.ndarray, n_kv_heads: int, head_size: int, n_sink: int = 0, n_recent: int = 0, cache_type: int = F32):
         """cuts every cache to its n_keep slots of the largest gathered weight, beside the first and latest positions"""
         if caches.dtype != CACHE or not caches.flags.c_contiguous:
             raise PsCudaError("kv_evict: caches is a contiguous array of capi.CACHE records")
-        self._ck(self.L.ps_cuda_kv_evict(self.h, caches.ctypes.data, caches.size, cache_type, head_size, n_kv_heads, n_sink, n_recent))
+        self._in_turn(self.L.ps_cuda_kv_evict, caches.ctypes.data, caches.size, cache_type, head_size, n_kv_heads, n_sink, n_recent)
 
     def sample(self, ids, probs, logits, vocab: int, rows: int, samplers, u, row_stride: Optional[int] = None):
         """a token of each row of logits by the row's settings (SAMPLER records on the device) and random number"""
         step, n = vocab if row_stride is None else row_stride, max(rows, 0)
         last = 4 * ((n - 1) * step + vocab) if n and 0 < vocab <= min(step, 1 << 18) else 0     # (what is wrong with others the call itself says)
-        self._ck(self.L.ps_cuda_sample(self.h, _dev("sample: ids", ids, self.device, 4 * n, ["int32"]), _dev("sample: probs", probs, self.device, 4 * n, ["float32"]),
-                                       _dev("sample: logits", logits, self.device, last, ["float32"], step), step, vocab, rows,
-                                       _dev("sample: samplers", samplers, self.device, SAMPLER.itemsize * n), _dev("sample: u", u, self.device, 4 * n, ["float32"])))
+        self._in_turn(self.L.ps_cuda_sample, _dev("sample: ids", ids, self.device, 4 * n, ["int32"]), _dev("sample: probs", probs, self.device, 4 * n, ["float32"]),
+                      _dev("sample: logits", logits, self.device, last, ["float32"], step), step, vocab, rows,
+                      _dev("sample: samplers", samplers, self.device, SAMPLER.itemsize * n), _dev("sample: u", u, self.device, 4 * n, ["float32"]))
 
     def read_device(self, dev_ptr: int, n_floats: int, dtype=np.float32) -> np.ndarray:
         out = np.empty(n_floats, dtype=dtype)

@@ -219,6 +219,7 @@ struct ps_cuda_ctx {
     size_t serve_ws_bytes = 0;
     uint8_t *smp_dev = nullptr, *h_smp = nullptr; // ps_cuda_sample_last: settings, random numbers, ids and probabilities of smp_rows rows, 28 bytes each
     int smp_rows = 0;
+    cudaEvent_t ev_enter = nullptr, ev_leave = nullptr; // ps_cuda_stream_enter / _leave
     std::vector<size_t> kv_k_bytes, kv_v_bytes; // per layer: bytes of the K rows / V^T rows of ONE cache set
 };
 
@@ -1626,6 +1627,23 @@ template <typename F> int serve(ps_cuda_ctx *ctx, F call) {
     return rc && c.msg[0] ? fail(ctx, rc, "%s", c.msg) : rc;
 }
 bool fits_int(int64_t v) { return v >= INT32_MIN && v <= INT32_MAX; }
+// enter: the context's stream goes on after what `s` holds now; else the other way round.  Where `s` is being captured, entering draws the context's stream into that capture and leaving joins
+// it; a capture of the context's stream that `s` is no part of stays as it is (nothing outside a capture can be waited for in it)
+int stream_order(ps_cuda_ctx *ctx, cudaStream_t s, bool enter) {
+    if (s == ctx->stream) return 0;
+    cudaStreamCaptureStatus mine = cudaStreamCaptureStatusNone, its = cudaStreamCaptureStatusNone;
+    unsigned long long my_id = 0, its_id = 0;
+    PS_CK(cudaStreamGetCaptureInfo(ctx->stream, &mine, &my_id));
+    if (cudaStreamGetCaptureInfo(s, &its, &its_id) != cudaSuccess) cudaGetLastError(); // (the default stream while another is being captured: the record below says so, if it comes to that)
+    const bool in_mine = mine != cudaStreamCaptureStatusNone, in_its = its != cudaStreamCaptureStatusNone;
+    if (in_mine && !(in_its && my_id == its_id)) return 0;
+    if (!enter && in_its && !in_mine) return 0; // (it has not been entered)
+    cudaEvent_t &ev = enter ? ctx->ev_enter : ctx->ev_leave;
+    if (!ev) PS_CK(cudaEventCreateWithFlags(&ev, cudaEventDisableTiming));
+    PS_CK(cudaEventRecord(ev, enter ? s : ctx->stream));
+    PS_CK(cudaStreamWaitEvent(enter ? ctx->stream : s, ev, 0));
+    return 0;
+}
 } // namespace
 
 extern "C" {
@@ -1909,6 +1927,8 @@ void ps_cuda_destroy(ps_cuda_ctx *ctx) {
     for (cudaEvent_t e : ctx->kt_events) cudaEventDestroy(e);
     if (ctx->ev0) cudaEventDestroy(ctx->ev0);
     if (ctx->ev1) cudaEventDestroy(ctx->ev1);
+    if (ctx->ev_enter) cudaEventDestroy(ctx->ev_enter);
+    if (ctx->ev_leave) cudaEventDestroy(ctx->ev_leave);
     if (ctx->arch) ps_arch_destroy(ctx->arch);
     if (ctx->stream) cudaStreamDestroy(ctx->stream);
     delete ctx;
@@ -2221,6 +2241,13 @@ int ps_cuda_softmax(ps_cuda_ctx *ctx, float *dst, const float *x, int64_t ne0, i
 }
 
 // ---------------------------------------------------------------------------------------------- serving operators (ps_serve.cu)
+
+int ps_cuda_stream_enter(ps_cuda_ctx *ctx, void *stream) {
+    return serve(ctx, [&](PsServeCall *) { return stream_order(ctx, static_cast<cudaStream_t>(stream), true); });
+}
+int ps_cuda_stream_leave(ps_cuda_ctx *ctx, void *stream) {
+    return serve(ctx, [&](PsServeCall *) { return stream_order(ctx, static_cast<cudaStream_t>(stream), false); });
+}
 
 int ps_cuda_attn_tree(ps_cuda_ctx *ctx, float *out, const float *q, const ps_cuda_cache *caches, int n_seqs, int cache_type, int64_t head_size, int64_t n_heads,
                       int64_t n_kv_heads, const uint8_t *tree_mask, float scale) {
