@@ -167,6 +167,8 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
                 if ((int64_t)active * 8 * n_kv_heads <= c->n_sm * 2) a.tps = wider, splits = splits_at(wider, active);
             }
             a.cluster = few && splits <= 8 && (int64_t)active * splits * n_kv_heads <= c->n_sm * 2 ? splits : 1;
+            // (one split, or a cluster's: nothing is left for another kernel)
+            auto parts = [&](const SvSeq &d) { return d.splits > 1 && a.cluster == 1 ? up(4 * (size_t)d.splits * n_kv_heads * d.n_tok * R * (hs + 2)) : 0; };
             size_t bytes = scores;
             int units = 0;
             bool joined = false;
@@ -186,7 +188,7 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
                 units += d.splits;
                 joined |= d.splits > 1 && a.cluster == 1;
                 if (d.weight) bytes += up(4 * (size_t)n_kv_heads * s.n_tok * R);
-                bytes += up(4 * (size_t)d.splits * n_kv_heads * s.n_tok * R * (hs + 2));
+                bytes += parts(d);
             }
             void *mem = nullptr;
             if (int rc = c->workspace(c->user, bytes, &mem)) return rc;
@@ -200,7 +202,7 @@ int ps_serve_attn_tree(PsServeCall *c, float *out, const float *q, const ps_cuda
                     at += up(4 * (size_t)n_kv_heads * d.n_tok * R);
                 }
                 d.part = reinterpret_cast<float *>(at);
-                at += up(4 * (size_t)d.splits * n_kv_heads * d.n_tok * R * (hs + 2));
+                at += parts(d);
             }
             const dim3 grid(units, n_kv_heads, row_tiles);
             if (few) {

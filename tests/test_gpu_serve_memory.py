@@ -1,0 +1,57 @@
+"""What the serving operators work in: calls that join nothing ask for nothing."""
+import numpy as np
+import pytest
+import torch
+
+from powerserve_b200 import capi
+from tests import _serve as S
+from tests.test_gpu_serve_paths import backend
+
+pytestmark = pytest.mark.gpu
+H, G, D, TOK = 32, 8, 64, 32        # 128 rows of a kv head: scores of n slots are 4096 n bytes
+
+
+class Steps:
+    """calls over a cache of which any beginning is filled; all keys equal, so that every output is the values' mean"""
+
+    def __init__(self, n_ctx):
+        self.be, self.n_ctx = backend(), n_ctx
+        self.k, self.v = torch.zeros(n_ctx, G * D, device="cuda"), torch.ones(G * D, n_ctx, device="cuda")
+        self.w, self.q, self.out = torch.zeros(G, n_ctx, device="cuda"), torch.ones(TOK, H * D, device="cuda"), torch.zeros(TOK, H * D, device="cuda")
+        self.mask = torch.ones(TOK, TOK, dtype=torch.uint8, device="cuda")
+        self.graphs = []
+        torch.cuda.synchronize()
+
+    def call(self, n, tok=TOK, weight=True):
+        t = np.zeros(1, capi.CACHE)
+        t["k"], t["v"], t["n_ctx"], t["n_kv"], t["n_tok"] = self.k.data_ptr(), self.v.data_ptr(), self.n_ctx, n, tok
+        t["weight"] = self.w.data_ptr() if weight else 0
+        self.be.attn_tree(self.out, self.q, t, H, G, D, 1.0, tree_mask=self.mask)
+
+    def check(self, n, calls):
+        """after `calls` calls over n slots (on the host: the device may have no room)"""
+        self.be.sync()
+        torch.cuda.synchronize()
+        assert np.abs(self.out.cpu().numpy() - 1).max() <= S.EPS * (n + 64)
+        got = self.w.cpu().numpy()[:, :n].astype(np.float64) * n / (TOK * H // G * calls)
+        assert np.abs(got - 1).max() <= S.EPS * (n + 64)
+        self.w.zero_()
+        self.out.zero_()
+
+    def close(self):
+        self.graphs.clear()
+        torch.cuda.synchronize()
+        self.be.close()
+
+
+def test_a_call_that_joins_nothing_can_be_captured_first():
+    s = Steps(4000)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, capture_error_mode="thread_local"):
+        s.call(40, tok=2, weight=False)
+    g.replay()
+    s.be.sync()
+    torch.cuda.synchronize()
+    assert np.abs(s.out[:2].cpu().numpy() - 1).max() <= S.EPS * 128
+    del g
+    s.close()
