@@ -1604,9 +1604,12 @@ int serve_workspace(void *user, size_t bytes, void **p) {
         if (st != cudaStreamCaptureStatusNone) return fail(ctx, PS_CUDA_ERR_UNSUPPORTED, "the call needs more workspace than a capture can ask for: make it once before");
         const size_t want = std::max(bytes, ctx->serve_ws_bytes + ctx->serve_ws_bytes / 2);
         void *mem = nullptr;
-        if (int rc = dev_alloc_yield(ctx, &mem, want)) return rc;
+        size_t got = want;
+        int rc = dev_alloc_yield(ctx, &mem, got);
+        if (rc == PS_CUDA_ERR_OOM && bytes < want) rc = dev_alloc_yield(ctx, &mem, got = bytes);
+        if (rc) return rc;
         ctx->serve_ws = mem;
-        ctx->serve_ws_bytes = want;
+        ctx->serve_ws_bytes = got;
     }
     *p = ctx->serve_ws;
     return 0;

@@ -1,10 +1,11 @@
-"""What the serving operators work in: calls that join nothing ask for nothing."""
+"""What the serving operators work in: it grows where the memory for half as much again is not there, and calls that join nothing ask for nothing."""
 import numpy as np
 import pytest
 import torch
 
 from powerserve_b200 import capi
 from tests import _serve as S
+from tests.test_gpu_memory_yields import MB, Filler
 from tests.test_gpu_serve_paths import backend
 
 pytestmark = pytest.mark.gpu
@@ -42,6 +43,35 @@ class Steps:
         self.graphs.clear()
         torch.cuda.synchronize()
         self.be.close()
+
+
+def test_a_graph_s_memory_stays_and_the_new_is_no_more_than_must():
+    s = Steps(24000)
+    s.call(16000)
+    s.check(16000, 1)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, capture_error_mode="thread_local"):
+        s.call(16000)
+    s.graphs.append(g)
+    fill = Filler(176 * MB)         # about 88 MB are left: enough for 79, not for half as much again as 66
+    try:
+        assert 81 * MB < fill.free < 97 * MB
+        s.call(19000)
+        s.check(19000, 1)
+        g.replay()
+        s.check(16000, 1)
+        s.call(19000)
+        g.replay()
+        s.be.sync()
+        torch.cuda.synchronize()
+        assert np.abs(s.out.cpu().numpy() - 1).max() <= S.EPS * 16064
+        with pytest.raises(capi.PsCudaError, match="cudaMalloc"):       # and no room at all is said
+            s.call(24000, tok=TOK)
+            s.call(24000, tok=TOK)
+    finally:
+        fill.close()
+    del g
+    s.close()
 
 
 def test_a_call_that_joins_nothing_can_be_captured_first():
