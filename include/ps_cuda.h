@@ -138,7 +138,7 @@ int ps_cuda_softmax(ps_cuda_ctx *ctx, float *dst, const float *x, int64_t ne0, i
  * and all other arguments are device pointers.  A context's calls run one after another; so must graphs that were captured from its
  * stream, which share its workspace.  A captured call's lengths are those of the capture; a workspace that would have to grow is
  * refused in a capture (PS_CUDA_ERR_UNSUPPORTED: make the call once before).  The workspace holds a call's partial outputs and, where weights
- * are gathered, 4 bytes for every query row and slot (1 GB of them at a time, or one sequence's).  Arrays may not overlap unless said so. */
+ * are gathered, 4 bytes for every query row and slot (1 GB of them at a time, or one sequence's); it grows by half or what must be, and what is outgrown goes back unless a capture took it.  Arrays may not overlap unless said so. */
 #define PS_CUDA_TREE_TOKENS 256 /* tokens that a sequence may bring to one ps_cuda_attn_tree call */
 typedef struct {                /* one sequence's cache in one layer */
     void    *k;                 /* rows [n_ctx][n_kv_heads * head_size] */

@@ -215,8 +215,9 @@ struct ps_cuda_ctx {
     // layer-list model (ps_cuda_create_arch): weights, workspace and kernels live in the executor (ps_arch.cu); the context keeps
     // what every model family shares - stream, staging, cache sets / sessions, positions, logits read-back, sampling
     PsArch *arch = nullptr;
-    void *serve_ws = nullptr;   // what the serving operators work in; earlier, smaller ones stay in `owned` (a captured graph may hold them)
+    void *serve_ws = nullptr;   // what the serving operators work in
     size_t serve_ws_bytes = 0;
+    bool serve_ws_held = false; // a captured graph may hold it: it stays in `owned` when it is outgrown
     uint8_t *smp_dev = nullptr, *h_smp = nullptr; // ps_cuda_sample_last: settings, random numbers, ids and probabilities of smp_rows rows, 28 bytes each
     int smp_rows = 0;
     cudaEvent_t ev_enter = nullptr, ev_leave = nullptr; // ps_cuda_stream_enter / _leave
@@ -1598,12 +1599,21 @@ namespace {
 namespace {
 int serve_workspace(void *user, size_t bytes, void **p) {
     ps_cuda_ctx *ctx = static_cast<ps_cuda_ctx *>(user);
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    if (bytes) PS_CK(cudaStreamIsCapturing(ctx->stream, &st));
+    const bool captured = st != cudaStreamCaptureStatusNone;
     if (bytes > ctx->serve_ws_bytes) {
-        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-        PS_CK(cudaStreamIsCapturing(ctx->stream, &st));
-        if (st != cudaStreamCaptureStatusNone) return fail(ctx, PS_CUDA_ERR_UNSUPPORTED, "the call needs more workspace than a capture can ask for: make it once before");
+        if (captured) return fail(ctx, PS_CUDA_ERR_UNSUPPORTED, "the call needs more workspace than a capture can ask for: make it once before");
         const size_t want = std::max(bytes, ctx->serve_ws_bytes + ctx->serve_ws_bytes / 2);
-        void *mem = nullptr;
+        void *old = ctx->serve_ws_held ? nullptr : ctx->serve_ws, *mem = nullptr;
+        ctx->serve_ws = nullptr;
+        ctx->serve_ws_bytes = 0;
+        ctx->serve_ws_held = false;
+        if (old) {
+            PS_CK(cudaStreamSynchronize(ctx->stream));
+            ctx->owned.erase(std::remove(ctx->owned.begin(), ctx->owned.end(), old), ctx->owned.end());
+            PS_CK(cudaFree(old));
+        }
         size_t got = want;
         int rc = dev_alloc_yield(ctx, &mem, got);
         if (rc == PS_CUDA_ERR_OOM && bytes < want) rc = dev_alloc_yield(ctx, &mem, got = bytes);
@@ -1611,6 +1621,7 @@ int serve_workspace(void *user, size_t bytes, void **p) {
         ctx->serve_ws = mem;
         ctx->serve_ws_bytes = got;
     }
+    ctx->serve_ws_held |= captured;
     *p = ctx->serve_ws;
     return 0;
 }

@@ -1,4 +1,5 @@
-"""What the serving operators work in: it grows where the memory for half as much again is not there, and calls that join nothing ask for nothing."""
+"""What the serving operators work in: it grows where the memory for half as much again is not there, what is outgrown goes back unless a captured graph holds it, and calls
+that join nothing ask for nothing."""
 import numpy as np
 import pytest
 import torch
@@ -43,6 +44,39 @@ class Steps:
         self.graphs.clear()
         torch.cuda.synchronize()
         self.be.close()
+
+
+def free():
+    """without what torch's allocator keeps"""
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    return torch.cuda.mem_get_info()[0]
+
+
+def test_outgrown_memory_goes_back():
+    s = Steps(24000)
+    before = None
+    for n in (4000, 6100, 9200, 13900, 20900):      # each more than half as much again: 16 to 86 MB, 212 together
+        s.call(n)
+        s.check(n, 1)
+        if before is None:
+            before = free() + 4096 * n
+    assert before - free() <= 4096 * 20900 * 1.1 + 16 * MB
+    s.close()
+
+
+def test_room_for_the_new_where_the_old_one_goes():
+    s = Steps(24000)
+    s.call(16000)
+    s.check(16000, 1)
+    fill = Filler(100 * MB)         # about 50 MB are left; 79 are needed, 66 are held
+    try:
+        assert fill.free < 70 * MB
+        s.call(19000)
+        s.check(19000, 1)
+    finally:
+        fill.close()
+    s.close()
 
 
 def test_a_graph_s_memory_stays_and_the_new_is_no_more_than_must():
