@@ -716,7 +716,11 @@ class CudaModel:
         """a token of each of the first len(u) rows of the last forward pass, on the device: (ids, probabilities).  settings: SAMPLER records or
         (temperature, top_k, top_p, min_p), one for each row or one for all; u: a random number in [0, 1) for each row"""
         u = np.ascontiguousarray(u, np.float32).reshape(-1)
-        s = np.asarray(settings) if isinstance(settings, np.ndarray) else np.array([tuple(r) for r in ([settings] if np.ndim(settings) == 1 else settings)], SAMPLER)
+        if isinstance(settings, (np.ndarray, np.void)):
+            s = np.asarray(settings)
+        else:
+            one = len(settings) > 0 and isinstance(settings[0], (int, float, np.number))
+            s = np.array([tuple(r) for r in ([settings] if one else settings)], SAMPLER)
         s = np.ascontiguousarray(np.broadcast_to(s.astype(SAMPLER, casting="no").reshape(-1), u.shape))
         ids, probs = np.empty(len(u), np.int32), np.empty(len(u), np.float32)
         self.be._ck(self.be.L.ps_cuda_sample_last(self.be.h, len(u), s.ctypes.data, u.ctypes.data, ids.ctypes.data, probs.ctypes.data))

@@ -102,6 +102,32 @@ def test_attention_refused(be, name, what, match):
     assert not be.L.calls
 
 
+def test_settings_of_the_last_pass_s_rows(be):
+    """SAMPLER records or tuples, one for each row or one for all"""
+    m = object.__new__(capi.CudaModel)
+    m.be, seen = be, []
+
+    def sample_last(h, rows, settings, u, ids, probs):
+        seen.append(np.ctypeslib.as_array((capi.C.c_uint8 * (16 * rows)).from_address(settings)).copy().view(capi.SAMPLER) if rows else None)
+        return 0
+
+    be.L.ps_cuda_sample_last = sample_last
+    rows = [(1.0, 0, 0.9, 0.0), (0.5, 40, 0.95, 0.02), (0.0, 0, 1.0, 0.0), (1.5, 7, 0.5, 0.25)]
+    table = np.array(rows, capi.SAMPLER)
+    for each in (rows, tuple(rows), table, list(table), [list(r) for r in rows], [tuple(np.float32(f) for f in r) for r in rows]):
+        m.sample(each, [0.5] * 4)
+        assert np.array_equal(seen.pop(), table)
+    for one in (rows[1], list(rows[1]), [rows[1]], table[1], table[1:2], tuple(np.float64(f) for f in rows[1])):
+        for n in (1, 4):
+            m.sample(one, [0.5] * n)
+            assert np.array_equal(seen.pop(), np.array([rows[1]] * n, capi.SAMPLER))
+    m.sample(rows[:0], [])
+    m.sample(rows[0], [])
+    for wrong in (rows[:3], table[:3], np.zeros((4, 4), np.float32)):
+        with pytest.raises((ValueError, TypeError)):
+            m.sample(wrong, [0.5] * 4)
+
+
 def test_calls_that_the_library_refuses_reach_it(be):
     """sizes follow from what is asked for; where that makes no sense, the library says so"""
     sample(be, rows=-1)
