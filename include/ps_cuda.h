@@ -157,7 +157,10 @@ typedef struct {                /* one sequence's cache in one layer */
  * the step's own those that tree_mask gives it (per sequence n_tok x n_tok bytes, row t = the tokens that token t sees, one sequence after another;
  * NULL: itself and the ones before).  A token that sees nothing gets zeros, one with a query that holds NaN or a score above float32's range NaN.  weight[g][j] += the sum of p_j over the sequence's tokens and the
  * heads of kv head g.  q and out: [tokens][n_heads * head_size] fp32, sequence after sequence; out may be q's memory only if it IS q; sequences may share K and V (a common
- * beginning), not weights.  What a filled slot that is not hidden holds must be finite.  head_size: multiples of 32 up to 256; at most 32 heads a kv head. */
+ * beginning), not weights.  What a filled slot that is not hidden holds must be finite.  head_size: multiples of 32 up to 256; at most 32 heads a kv head.
+ * Precision: sums, soft-max and weights have 32 bits.  Head sizes 64 and 128 take their products on 16-bit tensor cores, float32 numbers as two parts: 22 bits of each factor, the product of the
+ * two low parts left out, so that a product is off by at most 5 x 2^-24 of itself.  Numbers below 2^-17 of the largest beside them (a query row; 8 or 16 slots of K; 8 to 64 channels of 16 or 64
+ * slots of V) have fewer bits, to 2^-39 of that largest one.  Other head sizes: float32 throughout. */
 int ps_cuda_attn_tree(ps_cuda_ctx *ctx, float *out, const float *q, const ps_cuda_cache *caches, int n_seqs, int cache_type, int64_t head_size,
                       int64_t n_heads, int64_t n_kv_heads, const uint8_t *tree_mask, float scale);
 /* Eviction: every kv head of every cache keeps n_keep slots - those whose position is below n_sink or among the n_recent latest, then those of

@@ -5,7 +5,8 @@
 // The cache is the MMAs' 16-row side, the queries are the eight columns: S^T = K Q^T, O^T = V^T P^T.  Which element of a row a thread holds is free (a sum's order is), so
 // a thread takes neighbours: of K eight elements of a slot's row, of V four slots of a channel; row m of a score tile is slot 4 (m % 8 / 2) + m % 2 + 2 (m / 8) so that
 // those four slots are its columns in the second product.  The weights change places by movmatrix.
-// A group's sum (sixteen slots of 64 channels) is added up in 32 bits outside the MMAs, after a factor of its own.
+// A group's sum (sixteen slots of 64 channels) is added up in 32 bits outside the MMAs, after a factor of its own.  The MMAs' accumulators truncate: the scores' small products have one of their own,
+// those of the outputs come first, while their accumulator, which starts from zero for every sixteen slots, is small.
 // Bound by loads under way: 128 to 168 registers a thread hold them, and the tail of a launch by its last CTAs. Eight kv heads of 128, four heads each, float32: 8 sequences of 16 000 slots
 // 215 us = 4.9 TB/s, 64 of 2 041 234 us = 4.6, 64 of 256 to 2 041 118 us = 3.7; heads of 64: 5.2 TB/s; bfloat16 3.2 (the same instructions for half the bytes). The kernel for 128 rows
 // took 194 us where this one takes 118. Few splits are a cluster that joins them: one sequence of 1 000 slots 18.5 us, 20.5 with a launch to join.
