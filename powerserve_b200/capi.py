@@ -504,15 +504,16 @@ class CudaBackend:
         """attention of a step's tokens over the caches (a CACHE array) of their sequences"""
         if caches.dtype != CACHE or not caches.flags.c_contiguous:
             raise PsCudaError("attn_tree: caches is a contiguous array of capi.CACHE records")
-        tok = caches["n_tok"].astype(np.int64)
+        tok = caches["n_tok"].ravel().tolist()
 
         def sane():     # (where that makes no sense, the call itself says what is wrong)
-            return 0 < head_size <= 256 and head_size % 32 == 0 and 0 < n_kv_heads <= n_heads <= 32 * n_kv_heads and n_heads % n_kv_heads == 0 and bool(((tok >= 0) & (tok <= TREE_TOKENS) & (tok <= caches["n_kv"])).all())
+            n = caches["n_tok"]
+            return 0 < head_size <= 256 and head_size % 32 == 0 and 0 < n_kv_heads <= n_heads <= 32 * n_kv_heads and n_heads % n_kv_heads == 0 and bool(((n >= 0) & (n <= TREE_TOKENS) & (n <= caches["n_kv"])).all())
 
-        rows = 4 * int(tok.sum()) * n_heads * head_size
+        rows = 4 * sum(tok) * n_heads * head_size
         self._in_turn(
             self.L.ps_cuda_attn_tree, _dev("attn_tree: out", out, self.device, rows, ["float32"], sane=sane), _dev("attn_tree: q", q, self.device, rows, ["float32"], sane=sane), caches.ctypes.data, caches.size, cache_type,
-            head_size, n_heads, n_kv_heads, None if tree_mask is None else _dev("attn_tree: tree_mask", tree_mask, self.device, int(tok.dot(tok)), ["uint8", "bool", "int8"], sane=sane), scale)
+            head_size, n_heads, n_kv_heads, None if tree_mask is None else _dev("attn_tree: tree_mask", tree_mask, self.device, sum([t * t for t in tok]), ["uint8", "bool", "int8"], sane=sane), scale)
 
     def kv_evict(self, caches: np.ndarray, n_kv_heads: int, head_size: int, n_sink: int = 0, n_recent: int = 0, cache_type: int = F32):
         """cuts every cache to its n_keep slots of the largest gathered weight, beside the first and latest positions"""
