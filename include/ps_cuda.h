@@ -159,7 +159,7 @@ typedef struct {                /* one sequence's cache in one layer */
  * heads of kv head g.  q and out: [tokens][n_heads * head_size] fp32, sequence after sequence; out may be q's memory only if it IS q; sequences may share K and V (a common
  * beginning), not weights.  What a filled slot that is not hidden holds must be finite.  head_size: multiples of 32 up to 256; at most 32 heads a kv head.
  * Precision: sums, soft-max and weights have 32 bits.  Head sizes 64 and 128 take their products on 16-bit tensor cores, float32 numbers as two parts: 22 bits of each factor, the product of the
- * two low parts left out, so that a product is off by at most 5 x 2^-24 of itself.  Numbers below 2^-17 of the largest beside them (a query row; 8 or 16 slots of K; 8 to 64 channels of 16 or 64
+ * two low parts left out: a product is off by at most 24 x 2^-24 of itself (4 for each factor, 16 for what is left out), by two or three on average.  Numbers below 2^-17 of the largest beside them (a query row; 8 or 16 slots of K; 8 to 64 channels of 16 or 64
  * slots of V) have fewer bits, to 2^-39 of that largest one.  Other head sizes: float32 throughout. */
 int ps_cuda_attn_tree(ps_cuda_ctx *ctx, float *out, const float *q, const ps_cuda_cache *caches, int n_seqs, int cache_type, int64_t head_size,
                       int64_t n_heads, int64_t n_kv_heads, const uint8_t *tree_mask, float scale);

@@ -303,7 +303,9 @@ int ps_serve_kv_evict(PsServeCall *c, const ps_cuda_cache *caches, int n_sets, i
             bytes += up(4 * (size_t)n_kv_heads * (1 + 2 * (size_t)d.moves));
         }
         const dim3 heads(n_kv_heads, n);
-        if (most_gone <= SV_FEW) { // one by one costs a pass over the weights each: some 1 025 slots of 256 heads 15 us for one, 21 for eight; the select and its moves 23 for nine (arrays apart from the old ones)
+        // One by one costs a pass over the weights each. 256 heads of 1 025 slots, us one by one / by the select and its moves, arrays apart from the old ones: one 6.1 / 18.9, four 11.2 / 19.8, eight
+        // 18.5 / 20.0; of 4 097 slots 11.5 / 25, 23.6 / 26.2, and eight 39 / 27: there four would be the border
+        if (most_gone <= SV_FEW) {
             if (es == 4) sv_k_evict_few<uint32_t><<<heads, 256, 0, c->stream>>>(a);
             else sv_k_evict_few<uint16_t><<<heads, 256, 0, c->stream>>>(a);
             SV_LAUNCHED("kv_evict");
@@ -316,6 +318,7 @@ int ps_serve_kv_evict(PsServeCall *c, const ps_cuda_cache *caches, int n_sets, i
             a.set[i].list = reinterpret_cast<int32_t *>(at);
             at += up(4 * (size_t)n_kv_heads * (1 + 2 * (size_t)a.set[i].moves));
         }
+        // (with keys in shared memory / read again in every pass, us with the moves: 32 heads of 2 000 slots 16.8 / 17.8, 8 190 33 / 43, 20 000 80 / 103, 49 152 175 / 337; above there is no room: 131 072 842)
         const int keys = most_kv <= SV_KEYS ? most_kv : 0;
         SV_CK(cudaFuncSetAttribute(sv_k_select, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * sv_key_at(SV_KEYS)));
         sv_k_select<<<heads, SV_SEL_THREADS, 4 * (size_t)sv_key_at(keys), c->stream>>>(a, keys);
@@ -343,7 +346,9 @@ int ps_serve_sample(PsServeCall *c, int32_t *ids, float *probs, const float *log
     if (!aligned(ids, 4) || !aligned(probs, 4) || !aligned(logits, 4) || !aligned(samplers, 4) || !aligned(u, 4)) return fail(c, PS_CUDA_ERR_INVALID, "sample: an array that is not aligned to its elements");
     SvSample a{};
     a.logits = logits; a.samplers = samplers; a.u = u; a.ids = ids; a.probs = probs; a.row_stride = row_stride; a.vocab = (int)vocab;
-    // few rows: as many CTAs a row as a cluster can have, so that the GPU is at work; many: eight
+    // Few rows: as many CTAs a row as a cluster can have, so that the GPU is at work; many: eight.  Rows of 151 936, us for eight / sixteen CTAs: one, no filter 11.3 / 10.3, top-p 36 / 31, top-p with
+    // min-p 11.1 / 9.8, top-k with top-p 15.8 / 16.3, largest logit 5.7 / 5.6; four 18.3 / 11.1, 69 / 35, 11.2 / 10.0, 16.0 / 16.5, 5.9 / 5.7; nine 17.7 / 15.0, 42 / 43, 11.2 / 13.7, 17.2 / 20.9, 6.0 / 7.0;
+    // sixteen 20.4 / 18.4, 63 / 60, 18.2 / 19.4, 20.6 / 23.7, 7.6 / 10.8; 32: 24.4 / 30.3, 72 / 96, 16.1 / 29.7, 21.1 / 33.7, 7.8 / 16.9
     const int C = rows * 16 <= c->n_sm ? 16 : 8;
     a.chunk = (int)((vocab + C - 1) / C + 31) & ~31;
     a.vec = aligned(logits, 16) && row_stride % 4 == 0;

@@ -2,7 +2,7 @@
 //
 // Operands.  A number x is cut into two fp16 parts, the upper eleven bits of x 2^e and the others, rounded, with 2^e from the largest of its group so that the
 // group fits fp16's range from the top: what is lost is below 2^-22 of x, or 2^-39 of the group's largest.  Three MMAs (lo hi, hi lo, hi hi) replace the
-// 32-bit products; the missing lo lo is below 2^-22 of the product.  bfloat16 caches have no lo part: two MMAs.  Groups: a query row; eight slots' K rows;
+// 32-bit products; the missing lo lo is below 2^-20 of the product (2^-23 on average; the upper part is cut off, not rounded, so it has the product's sign).  bfloat16 caches have no lo part: two MMAs.  Groups: a query row; eight slots' K rows;
 // hs / 8 channels of a tile of V.  The weights p of the soft-max, at most 1, are cut after a factor 2^15.
 // The queries' parts stay in tensor memory (in shared memory they took the room of two stages).
 // A tile's output leaves the tensor memory after every tile and is added up in registers, with rounding: the accumulator, which truncates, sees the

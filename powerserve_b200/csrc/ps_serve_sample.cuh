@@ -10,8 +10,8 @@
 // the border becomes a number (logit, token) to compare with.  Rows whose lists do not fit, or whose border lies below (flat ones), go the same way over all of
 // their tokens.  No filter: the running mass over all tokens.
 // Bound by latency: a row is four to seven exchanges across its cluster, and two CTAs an SM hide little of one another's; then by the 45-bit exponentials, which top-p needs of all tokens
-// (64-bit arithmetic: borders would move with float32's). One row of 151 936: largest logit 8 us, min-p 11, no filter 13, top-k 40 with top-p 19, top-p alone 33; 64 rows of 128 256: 17, 27, 41, 37, 100;
-// 256 rows of 151 936: 67 (2.3 TB/s), 104, 149, 122, 408. Flat rows (their border is below 2^-16 of the largest) 54 / 170 / 703.
+// (64-bit arithmetic: borders would move with float32's). In a captured graph, one row of 151 936: largest logit 5.3 us, min-p 9, top-p with min-p 10, no filter 11, top-k 40 with top-p 16, top-p alone 31;
+// 64 rows of 128 256: 15, 25, 30, 40, 35, 98; 256 rows of 151 936: 67 (2.3 TB/s), 103, 128, 149, 121, 404. Flat rows (their border is below 2^-16 of the largest) 48 / 168 / 696.
 #pragma once
 #include "ps_ptx.cuh"
 
