@@ -221,7 +221,7 @@ def _dev(what: str, a, device: int, need: int = 0, dtypes=None, row_stride: Opti
     """device address of a DeviceBuffer, a torch tensor, or an address (which is taken as it is).  A buffer has to hold `need` bytes (if sane()); a tensor too, in the device's
     memory, of one of the types named, its elements in order (a matrix with row_stride: its rows that far apart)"""
     if a is None or isinstance(a, (int, np.integer)):
-        return a
+        return a if a is None else int(a)
     if isinstance(a, DeviceBuffer):
         size, p = a.nbytes, a.ptr
     else:
@@ -522,8 +522,12 @@ class CudaBackend:
         self._in_turn(self.L.ps_cuda_kv_evict, caches.ctypes.data, caches.size, cache_type, head_size, n_kv_heads, n_sink, n_recent)
 
     def sample(self, ids, probs, logits, vocab: int, rows: int, samplers, u, row_stride: Optional[int] = None):
-        """a token of each row of logits by the row's settings (SAMPLER records on the device) and random number"""
-        step, n = vocab if row_stride is None else row_stride, max(rows, 0)
+        """a token of each row of logits by the row's settings (SAMPLER records on the device) and random number.  row_stride: floats from row to row (None: as a matrix
+        of so many rows says, else vocab)"""
+        step, n = row_stride, max(rows, 0)
+        if step is None:
+            own = rows > 1 and not isinstance(logits, DeviceBuffer) and hasattr(logits, "stride") and logits.dim() == 2 and logits.shape[0] == rows
+            step = logits.stride(0) if own else vocab
         last = 4 * ((n - 1) * step + vocab) if n and 0 < vocab <= min(step, 1 << 18) else 0     # (what is wrong with others the call itself says)
         self._in_turn(self.L.ps_cuda_sample, _dev("sample: ids", ids, self.device, 4 * n, ["int32"]), _dev("sample: probs", probs, self.device, 4 * n, ["float32"]),
                       _dev("sample: logits", logits, self.device, last, ["float32"], step), step, vocab, rows,

@@ -81,12 +81,25 @@ def test_what_is_right_goes_through(be):
     assert be.L.calls[1][1][2] is None and be.L.calls[1][1][8] == 4096
 
 
+def test_rows_of_a_wider_tensor(be):
+    """with no row_stride said, a matrix of as many rows as are drawn from brings its own"""
+    strides = {"as wide": (on_device(torch.zeros(3, 10)), 10), "wider": (on_device(torch.zeros(3, 16)), 16), "a part": (on_device(torch.zeros(3, 16))[:, 2:12], 16), "flat": (on_device(torch.zeros(30)), 10),
+               "other rows": (on_device(torch.zeros(6, 5)), 10), "a buffer": (buffer(120), 10), "an address": (np.uint64(4096), 10)}
+    for name, (logits, want) in strides.items():
+        sample(be, logits=logits)
+        call = be.L.calls.pop()[1]
+        assert call[4] == want and type(call[3]) is int, name
+    one = on_device(torch.zeros(1, 16))     # (one row)
+    sample(be, rows=1, logits=one)
+    assert be.L.calls.pop()[1][4] >= 10
+
+
 @pytest.mark.parametrize("name,what,match", [
     ("logits", torch.zeros(3, 10), "not in the memory"), ("u", torch.zeros(3), "not in the memory"), ("ids", np.zeros(3, np.int32), "ndarray"), ("probs", [0.0] * 3, "list"),
     ("ids", on_device(torch.zeros(3, dtype=torch.int64)), "int64"), ("logits", on_device(torch.zeros(3, 10, dtype=torch.bfloat16)), "bfloat16"), ("u", on_device(torch.zeros(3, dtype=torch.float64)), "float64"),
     ("u", on_device(torch.zeros(3), 1), "not in the memory"), ("u", on_device(torch.zeros(2)), "holds 8 bytes"), ("samplers", on_device(torch.zeros(2, 4)), "holds 32"), ("logits", on_device(torch.zeros(2, 10)), "holds 80"),
     ("ids", buffer(8), "holds 8"), ("u", on_device(torch.zeros(6))[::2], "follow one another"), ("logits", on_device(torch.zeros(10, 3)).T, "follow one another"),
-    ("logits", on_device(torch.zeros(3, 16))[:, :10], "follow one another")])
+    ("logits", on_device(torch.zeros(3, 20))[:, ::2], "follow one another")])
 def test_samples_refused(be, name, what, match):
     with pytest.raises(capi.PsCudaError, match=match):
         sample(be, **{name: what})
