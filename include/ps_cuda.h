@@ -134,7 +134,7 @@ int ps_cuda_softmax(ps_cuda_ctx *ctx, float *dst, const float *x, int64_t ne0, i
 /* ---------------------------------------------------------------------------------------------- serving operators
  * What a step over many conversations needs beside the table above; for every context (layer-list ones too), on caches of the caller's or
  * the context's own (ps_cuda_kv_k / ps_cuda_kv_v, type PS_TYPE_F32).  They have no counterpart in the reference, so no bits to reproduce: sums run in 32 bits
- * or more, in an order that depends on the shapes alone.  `caches` is a HOST array, read before the call returns; all pointers in it
+ * or more, in an order that depends on the call's shapes alone (all of them: a sequence's last bits may change with its company).  `caches` is a HOST array, read before the call returns; all pointers in it
  * and all other arguments are device pointers.  A context's calls run one after another; so must graphs that were captured from its
  * stream, which share its workspace.  A captured call's lengths are those of the capture; a workspace that would have to grow is
  * refused in a capture (PS_CUDA_ERR_UNSUPPORTED: make the call once before).  The workspace holds a call's partial outputs and, where weights
