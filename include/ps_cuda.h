@@ -180,6 +180,76 @@ typedef struct { /* one row's settings (SamplerChain's order, src/sampler/sample
 int ps_cuda_sample(ps_cuda_ctx *ctx, int32_t *ids, float *probs, const float *logits, int64_t row_stride, int64_t vocab, int64_t rows,
                    const ps_cuda_sampler *samplers, const float *u);
 
+/* ---------------------------------------------------------------------------------------------- paged caches in 8 bits, drafted tokens
+ * More serving operators, under the same rules (HOST arrays of records, device arrays, one call after another, one workspace, captures).  A cache of pages belongs to the caller: n_pages pages
+ * of page_tokens slots (16, 32, 64 or 128) in each of n_layers layers, and a table of page numbers for every sequence: its slot j is slot j % page_tokens of page table[j / page_tokens], in all layers.
+ * Sixteen slots are a block: in a block every kv head has one scale for K and one for V, and a number is code * scale, codes -127 .. 127.
+ *   codes  [n_layers][n_pages][n_kv_heads][2: K, V][page_tokens * head_size], a page's as the tensor cores read them, blocks one after another:
+ *          K: slot t, channel d at ((t / 8) * (head_size / 16) + d / 16) * 128 + (t % 8) * 16 + d % 16;   V: at ((t / 16) * head_size + d) * 16 + t % 16
+ *   scales [n_layers][n_pages][n_kv_heads][2][page_tokens / 16] fp32
+ *   refs   [n_pages] the tables that hold a page (0: it is free); ps_cuda_paged_edit alone reads and writes it
+ * What a page holds behind its sequence's last slot may be anything.  A table's entry that is no page's number (they are checked on the device) is left out, nothing outside the cache is touched, and the next
+ * ps_cuda_sync reports it.  codes are aligned to 16 bytes, all else to its elements; head_size: multiples of 32 up to 256.  io_type: PS_TYPE_F32 or PS_TYPE_BF16, of k, v, q and out. */
+#define PS_CUDA_BLOCK_TOKENS 16
+#define PS_CUDA_EDITS 512       /* edits of one call */
+typedef struct {
+    int8_t  *codes;
+    float   *scales;
+    int32_t *refs;              /* only ps_cuda_paged_edit asks for it */
+    int32_t  n_layers, n_pages, page_tokens, n_kv_heads, head_size, reserved;
+} ps_cuda_pages;
+typedef struct {                /* one sequence */
+    const int32_t *table;       /* device: pages of its slots */
+    const uint8_t *hidden;      /* paged_attn: [n_kv], not 0 = no token sees the slot (NULL = all are seen) */
+    int32_t n_kv, n_tok;        /* slots that are filled, those of the call's tokens included; tokens of the call: the last n_tok filled slots (0: it takes no part) */
+    int32_t n_table, reserved;  /* entries of the table, at least n_kv / page_tokens, rounded up */
+} ps_cuda_paged_seq;
+/* Rows of K and V [tokens][n_kv_heads * head_size], sequence after sequence, into their slots of one layer.  A block's new scale is the largest of its old one, where slots that stay lie in it, and
+ * its new numbers' largest / 127; a code is the number / scale, rounded to the nearest, even where two are; codes that were there are rounded to code * (old scale / new scale).  All of that is float32, correctly
+ * rounded, so the codes are the same on every call.  Numbers have to be finite (no number is held as 0; the others of a block with an infinite one are 0).
+ * Sequences of a call, and pages that several tables hold, may not be written at the same block (ps_cuda_paged_edit sees to that). */
+int ps_cuda_paged_store(ps_cuda_ctx *ctx, const ps_cuda_pages *pages, int layer, const void *k, const void *v, int io_type, const ps_cuda_paged_seq *seqs, int n_seqs);
+/* The numbers that the last n_tok slots of each sequence stand for, as rows of K and V; k or v may be NULL (it is not asked for) */
+int ps_cuda_paged_load(ps_cuda_ctx *ctx, const ps_cuda_pages *pages, int layer, void *k, void *v, int io_type, const ps_cuda_paged_seq *seqs, int n_seqs);
+/* ps_cuda_attn_tree's attention over such a cache: out[t][h] = sum_j p_j v_j, p = soft-max of scale * q[t][h] . k_j over the slots that the token sees (tree_mask and hidden as there, n_tok <= 256, at most
+ * 32 heads a kv head).  A token that sees nothing gets zeros, one with a query that holds no number or an infinite one, or with a score above float32's range, NaN.  out may be q.  Tables may share pages.
+ * Precision: a query is held to 2^-23 of its row's largest number, its products with codes and their sums are exact; soft-max and sums have 32 bits, a weight is held to 2^-23 of the largest one of its row. */
+int ps_cuda_paged_attn(ps_cuda_ctx *ctx, const ps_cuda_pages *pages, int layer, void *out, const void *q, int io_type, const ps_cuda_paged_seq *seqs, int n_seqs, int64_t n_heads,
+                       const uint8_t *tree_mask, float scale);
+typedef struct {                /* one table's change */
+    int32_t       *table;       /* device */
+    const int32_t *from;        /* NULL, or the table whose first n_old tokens' pages this one shares from now on (what it held before is forgotten: release it first) */
+    int32_t n_old, n_new;       /* tokens that it holds (or shares), and that it shall have room for */
+    int32_t n_table, reserved;  /* entries of `table`, at least n_new / page_tokens, rounded up (and those of n_old) */
+} ps_cuda_page_edit;
+/* Sequences fork, grow, shrink and end.  First all edits with `from` share pages (from is read as it was before the call), then all with n_new < n_old give back the pages behind n_new, then those with
+ * n_new > n_old take pages in the order of the edits, the free pages of the lowest numbers first.  A sequence that grows is going to be written: where its last page is not full and another table holds it too, it takes a
+ * page for itself, into which the filled blocks of all layers are copied (of several that grow from one page nobody else holds, the last one keeps it).  held [n] (device, may be NULL): the tokens that each table
+ * holds now - n_new, or n_old for the first edit that finds too few free pages and those behind it that need one (or share a page with one before).
+ * A table may appear once (as `from` as often as one likes).  At most PS_CUDA_EDITS edits. */
+int ps_cuda_paged_edit(ps_cuda_ctx *ctx, const ps_cuda_pages *pages, const ps_cuda_page_edit *edits, int n, int32_t *held);
+typedef struct {                /* slots of one sequence that move together */
+    const int32_t *table;
+    const int32_t *keep;        /* device [n_keep], rising: slot first + i takes what slot first + keep[i] holds */
+    const int32_t *n_keep_dev;  /* device, or NULL: how many of them there are (at most n_keep): ps_cuda_verify's path and n_path fit */
+    int32_t first, n_kv;        /* slots before `first` stay where they are; filled slots */
+    int32_t n_keep, n_table;
+} ps_cuda_page_move;
+/* Slots that are kept - a drafted tree's accepted tokens, what an eviction leaves - move together, in all layers.  A block that one moves into takes the largest of the scales that its slots come with,
+ * their codes are rounded to code * (old scale / new scale): nothing is rounded where a block's slots come from one block.  Slots behind the last kept one keep their codes.  Two moves may not touch the same pages, from
+ * `first` on no other table may hold them.  A list that does not rise, or leaves the filled slots, ends where it does, and ps_cuda_sync reports it. */
+int ps_cuda_paged_compact(ps_cuda_ctx *ctx, const ps_cuda_pages *pages, const ps_cuda_page_move *moves, int n);
+
+/* Drafted tokens against the target's distribution p and the draft's q (each what its row of logits leaves by its ps_cuda_sampler, as ps_cuda_sample draws from it).  A sequence has n_nodes[s] nodes (HOST array; 1 .. 256):
+ * node 0 is its last token, node i > 0 the drafted token tokens[i], a child of parents[i] < i (numbers within the sequence); row i of the logits is the target's after node i, row i of draft_logits the
+ * draft's that the children of node i were drawn from (rows of childless nodes are not read).  Beginning at node 0, the children of the last accepted node are asked in order: child i with token c is accepted where u[i] < p(c) / q(c);
+ * where it is not, p becomes max(p - q, 0), normalised (p stays where nothing is left), for its siblings and the last draw.  draft_logits NULL: the drafted tokens are nobody's draws, q is 1 at c: p loses c.  What is drawn then
+ * is distributed as if the target had drawn every token.  ids[s]: the next token, drawn with u[0] from what p has become at the last accepted node (-1: its row has no number above -inf);
+ * path: the accepted nodes of each sequence, node 0 first, -1 behind them; n_path[s] their number.  A token outside the vocabulary is never accepted and changes nothing.
+ * All arrays but n_nodes on the device: parents, tokens, u, samplers, draft_samplers, path [all nodes], sequence after sequence; rows of both matrices are row_stride floats apart. */
+int ps_cuda_verify(ps_cuda_ctx *ctx, int32_t *ids, int32_t *path, int32_t *n_path, const int32_t *n_nodes, int n_seqs, const int32_t *parents, const int32_t *tokens, const float *logits, int64_t row_stride,
+                   int64_t vocab, const ps_cuda_sampler *samplers, const float *u, const float *draft_logits, const ps_cuda_sampler *draft_samplers);
+
 /* ---------------------------------------------------------------------------------------------- KV cache
  * Device implementation of the position bookkeeping of KVCacheInterface (src/core/kv_cache.hpp:97-163) that
  * Platform::get/reset_kv_position (src/backend/platform.cpp:34-50) and LlamaModel::forward (:84-86,109) use. */

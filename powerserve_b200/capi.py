@@ -101,6 +101,18 @@ CACHE = np.dtype([("k", "u8"), ("v", "u8"), ("weight", "u8"), ("weight_to", "u8"
                   ("n_ctx", "i4"), ("n_kv", "i4"), ("n_tok", "i4"), ("n_keep", "i4")])
 SAMPLER = np.dtype([("temperature", "f4"), ("top_k", "i4"), ("top_p", "f4"), ("min_p", "f4")])
 
+# ps_cuda_paged_seq, ps_cuda_page_edit and ps_cuda_page_move
+PAGED_SEQ = np.dtype([("table", "u8"), ("hidden", "u8"), ("n_kv", "i4"), ("n_tok", "i4"), ("n_table", "i4"), ("reserved", "i4")])
+PAGE_EDIT = np.dtype([("table", "u8"), ("from", "u8"), ("n_old", "i4"), ("n_new", "i4"), ("n_table", "i4"), ("reserved", "i4")])
+PAGE_MOVE = np.dtype([("table", "u8"), ("keep", "u8"), ("n_keep_dev", "u8"), ("first", "i4"), ("n_kv", "i4"), ("n_keep", "i4"), ("n_table", "i4")])
+BLOCK_TOKENS, PAGE_EDITS = 16, 512
+
+
+class Pages(C.Structure):
+    """ps_cuda_pages"""
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("refs", C.c_void_p)] + [(n, C.c_int32) for n in ("n_layers", "n_pages", "page_tokens", "n_kv_heads", "head_size", "reserved")]
+
+
 COMPUTE_BF16, COMPUTE_F32 = 0, 1
 MIXER_ATTENTION, MLP_NONE, MLP_ROUTED = 1, 0, 1
 MIXER_LATENT, MLP_DENSE = 2, 2
@@ -165,6 +177,12 @@ def load_library() -> C.CDLL:
         "ps_cuda_kv_evict": (ci, [vp, vp, ci, ci, i64, i64, ci, ci]),
         "ps_cuda_sample": (ci, [vp, vp, vp, vp, i64, i64, i64, vp, vp]),
         "ps_cuda_sample_last": (ci, [vp, ci, vp, vp, vp, vp]),
+        "ps_cuda_paged_store": (ci, [vp, vp, ci, vp, vp, ci, vp, ci]),
+        "ps_cuda_paged_load": (ci, [vp, vp, ci, vp, vp, ci, vp, ci]),
+        "ps_cuda_paged_attn": (ci, [vp, vp, ci, vp, vp, ci, vp, ci, i64, vp, C.c_float]),
+        "ps_cuda_paged_edit": (ci, [vp, vp, vp, ci, vp]),
+        "ps_cuda_paged_compact": (ci, [vp, vp, vp, ci]),
+        "ps_cuda_verify": (ci, [vp, vp, vp, vp, vp, ci, vp, vp, vp, i64, i64, vp, vp, vp, vp]),
         "ps_cuda_kv_position": (ci, [vp]),
         "ps_cuda_kv_reset": (ci, [vp]),
         "ps_cuda_kv_truncate": (ci, [vp, ci]),
@@ -375,6 +393,32 @@ class DeviceBuffer:
             self.ptr = None
 
 
+class PagedCache:
+    """A cache in 8 bits and in pages (ps_cuda_pages): its memory - DeviceBuffers, torch tensors or addresses; what is not given is made here, refs (who holds which page) with nobody's - and its shape.
+    codes: int8 [n_layers][n_pages][n_kv_heads][2][page_tokens * head_size], scales: float32 [n_layers][n_pages][n_kv_heads][2][page_tokens / 16], refs: int32 [n_pages]."""
+
+    def __init__(self, be: "CudaBackend", n_layers: int, n_pages: int, page_tokens: int, n_kv_heads: int, head_size: int, codes=None, scales=None, refs=None):
+        heads = n_layers * n_pages * n_kv_heads * 2
+        if min(n_layers, n_pages, n_kv_heads, head_size) <= 0 or page_tokens not in (16, 32, 64, 128):
+            raise PsCudaError(f"a paged cache of {n_layers} layers, {n_pages} pages of {page_tokens} tokens (16, 32, 64 or 128), {n_kv_heads} kv heads of {head_size}")
+        sizes = heads * page_tokens * head_size, heads * (page_tokens // BLOCK_TOKENS) * 4, 4 * n_pages
+        if refs is None and codes is None:
+            refs = be.upload(np.zeros(n_pages, np.int32))
+        self.codes = DeviceBuffer(be, sizes[0]) if codes is None else codes
+        self.scales = DeviceBuffer(be, sizes[1]) if scales is None else scales
+        self.refs = refs        # (kept: the addresses below are theirs)
+        self.head_size, self.n_kv_heads = head_size, n_kv_heads
+        at = [_dev(f"paged cache: {w}", a, be.device, n, [t]) for w, a, n, t in zip(("codes", "scales", "refs"), (self.codes, self.scales, refs), sizes, ("int8", "float32", "int32"))]
+        self.pages = Pages(*at, n_layers, n_pages, page_tokens, n_kv_heads, head_size, 0)
+        self.at = C.addressof(self.pages)
+
+    def free(self):
+        """gives back the DeviceBuffers"""
+        for b in (self.codes, self.scales, self.refs):
+            if isinstance(b, DeviceBuffer):
+                b.free()
+
+
 class CudaBackend:
     """Mirror of `powerserve::ggml::GGMLBackend`'s operator table (src/backend/ggml/ggml.hpp:216-244) over the C ABI.
     Method names, argument meaning and error behaviour follow the reference; tensors are DeviceBuffers."""
@@ -532,6 +576,74 @@ class CudaBackend:
         self._in_turn(self.L.ps_cuda_sample, _dev("sample: ids", ids, self.device, 4 * n, ["int32"]), _dev("sample: probs", probs, self.device, 4 * n, ["float32"]),
                       _dev("sample: logits", logits, self.device, last, ["float32"], step), step, vocab, rows,
                       _dev("sample: samplers", samplers, self.device, SAMPLER.itemsize * n), _dev("sample: u", u, self.device, 4 * n, ["float32"]))
+
+    # caches in 8 bits and in pages: `cache` is a PagedCache, `seqs` an array of PAGED_SEQ records
+    @staticmethod
+    def _records(what: str, a, kind, name: str):
+        if not isinstance(a, np.ndarray) or a.dtype != kind or not a.flags.c_contiguous:
+            raise PsCudaError(f"{what}: a contiguous array of capi.{name} records")
+        return a.ctypes.data
+
+    def _rows(self, what: str, a, need: int, io_type):
+        """address of rows and their type: a tensor's own, else io_type (None: float32)"""
+        torch = sys.modules.get("torch")
+        if torch is not None and isinstance(a, torch.Tensor):
+            t = F32 if a.dtype == torch.float32 else BF16 if a.dtype == torch.bfloat16 else None
+            if t is None or (io_type is not None and io_type != t):
+                raise PsCudaError(f"{what}: a tensor of {a.dtype}, not {'float32 or bfloat16' if io_type is None else 'of the type named'}")
+        else:
+            t = F32 if io_type is None else io_type
+        return _dev(what, a, self.device, (4 if t == F32 else 2) * need), t
+
+    def _paged_rows(self, what: str, call, cache, layer, k, v, seqs, io_type):
+        at = self._records(what, seqs, PAGED_SEQ, "PAGED_SEQ")
+        n = sum(seqs["n_tok"].ravel().tolist()) * cache.n_kv_heads * cache.head_size
+        rows = [self._rows(f"{what}: {w}", a, n, io_type) for w, a in (("k", k), ("v", v))]
+        types = {t for a, (_, t) in zip((k, v), rows) if a is not None}
+        if len(types) > 1:
+            raise PsCudaError(f"{what}: k and v of two types")
+        self._in_turn(call, cache.at, layer, rows[0][0], rows[1][0], types.pop() if types else F32, at, seqs.size)
+
+    def paged_store(self, cache, layer: int, k, v, seqs: np.ndarray, io_type: Optional[int] = None):
+        """rows of K and V into the last n_tok slots of each sequence"""
+        self._paged_rows("paged_store", self.L.ps_cuda_paged_store, cache, layer, k, v, seqs, io_type)
+
+    def paged_load(self, cache, layer: int, k, v, seqs: np.ndarray, io_type: Optional[int] = None):
+        """the numbers that the last n_tok slots of each sequence stand for, as rows (k or v: None if not asked for)"""
+        self._paged_rows("paged_load", self.L.ps_cuda_paged_load, cache, layer, k, v, seqs, io_type)
+
+    def paged_attn(self, cache, layer: int, out, q, seqs: np.ndarray, n_heads: int, scale: float, tree_mask=None, io_type: Optional[int] = None):
+        """attention of a step's tokens over the sequences' pages"""
+        at = self._records("paged_attn", seqs, PAGED_SEQ, "PAGED_SEQ")
+        tok = seqs["n_tok"].ravel().tolist()
+        n = sum(tok) * max(n_heads, 0) * cache.head_size
+        q_at, t = self._rows("paged_attn: q", q, n, io_type)
+        out_at, t_out = self._rows("paged_attn: out", out, n, io_type)
+        if t != t_out:
+            raise PsCudaError("paged_attn: q and out of two types")
+        mask = None if tree_mask is None else _dev("paged_attn: tree_mask", tree_mask, self.device, sum([t * t for t in tok]), ["uint8", "bool", "int8"])
+        self._in_turn(self.L.ps_cuda_paged_attn, cache.at, layer, out_at, q_at, t, at, seqs.size, n_heads, mask, scale)
+
+    def paged_edit(self, cache, edits: np.ndarray, held=None):
+        """sequences fork, grow, shrink and end (PAGE_EDIT records); held: int32 on the device, the tokens that each has room for then"""
+        at = self._records("paged_edit", edits, PAGE_EDIT, "PAGE_EDIT")
+        self._in_turn(self.L.ps_cuda_paged_edit, cache.at, at, edits.size, _dev("paged_edit: held", held, self.device, 4 * edits.size, ["int32"]))
+
+    def paged_compact(self, cache, moves: np.ndarray):
+        """kept slots move together, in all layers (PAGE_MOVE records)"""
+        self._in_turn(self.L.ps_cuda_paged_compact, cache.at, self._records("paged_compact", moves, PAGE_MOVE, "PAGE_MOVE"), moves.size)
+
+    def verify(self, ids, path, n_path, n_nodes, parents, tokens, logits, vocab: int, samplers, u, draft_logits=None, draft_samplers=None, row_stride: Optional[int] = None):
+        """drafted tokens are accepted or rejected, the next ones drawn (all arrays on the device but n_nodes); row_stride: floats from row to row of both matrices (None: as the target's says)"""
+        n_nodes = np.ascontiguousarray(n_nodes, np.int32).reshape(-1)
+        n, S = sum(n_nodes.tolist()), n_nodes.size
+        if row_stride is None:
+            row_stride = logits.stride(0) if not isinstance(logits, DeviceBuffer) and hasattr(logits, "stride") and logits.dim() == 2 and logits.shape[0] > 1 else vocab
+        last = 4 * ((n - 1) * row_stride + vocab) if n > 0 and 0 < vocab <= min(row_stride, 1 << 18) else 0
+        ints = [_dev(f"verify: {w}", a, self.device, 4 * k, ["int32"]) for w, a, k in (("ids", ids, S), ("path", path, n), ("n_path", n_path, S), ("parents", parents, n), ("tokens", tokens, n))]
+        rows = [_dev(f"verify: {w}", a, self.device, last, ["float32"], row_stride) for w, a in (("logits", logits), ("draft_logits", draft_logits))]
+        sets = [_dev(f"verify: {w}", a, self.device, SAMPLER.itemsize * n) for w, a in (("samplers", samplers), ("draft_samplers", draft_samplers))]
+        self._in_turn(self.L.ps_cuda_verify, *ints[:3], n_nodes.ctypes.data, S, *ints[3:], rows[0], row_stride, vocab, sets[0], _dev("verify: u", u, self.device, 4 * n, ["float32"]), rows[1], sets[1])
 
     def read_device(self, dev_ptr: int, n_floats: int, dtype=np.float32) -> np.ndarray:
         out = np.empty(n_floats, dtype=dtype)

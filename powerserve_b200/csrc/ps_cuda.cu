@@ -319,7 +319,7 @@ int sync_and_check(ps_cuda_ctx *ctx) {
         for (int k = 0; k < 4; k++) flag[k] = 0;
         if (ctx->ag_ctr) PS_CK(cudaMemsetAsync(ctx->ag_ctr, 0, (size_t)ctx->d.n_layers * ctx->nkv_l * 8, ctx->stream)); // a group that gave up leaves its counter mid-instance
         if (ctx->tc_cnt) PS_CK(cudaMemsetAsync(ctx->tc_cnt, 0, (size_t)ctx->n_sm * 4, ctx->stream)); // a GEMM that gave up leaves its counters part-way
-        return fail(ctx, PS_CUDA_ERR_CUDA, "device-side failure:%s%s%s (wait site %d; results of this call are invalid)", tc == PS_ERR_COPY ? " copy of a batch product did not arrive" : tc ? " tcgen05 pipeline time-out" : "",
+        return fail(ctx, PS_CUDA_ERR_CUDA, "device-side failure:%s%s%s (wait site %d; results of this call are invalid)", tc == PS_ERR_COPY ? " copy of a batch product did not arrive" : tc == PS_ERR_PAGE ? " a table or a list of a paged cache that names what is not there" : tc ? " tcgen05 pipeline time-out" : "",
                     tp ? " tensor-parallel peer wait gave up" : "", st ? " decode-step wait gave up" : "", st);
     }
     return 0;
@@ -2279,6 +2279,31 @@ int ps_cuda_kv_evict(ps_cuda_ctx *ctx, const ps_cuda_cache *caches, int n_sets, 
 int ps_cuda_sample(ps_cuda_ctx *ctx, int32_t *ids, float *probs, const float *logits, int64_t row_stride, int64_t vocab, int64_t rows, const ps_cuda_sampler *samplers,
                    const float *u) {
     return serve(ctx, [&](PsServeCall *c) { return ps_serve_sample(c, ids, probs, logits, row_stride, vocab, rows, samplers, u); });
+}
+int ps_cuda_paged_store(ps_cuda_ctx *ctx, const ps_cuda_pages *pages, int layer, const void *k, const void *v, int io_type, const ps_cuda_paged_seq *seqs, int n_seqs) {
+    return serve(ctx, [&](PsServeCall *c) { return ps_serve_paged_rows(c, true, pages, layer, const_cast<void *>(k), const_cast<void *>(v), io_type, seqs, n_seqs); });
+}
+int ps_cuda_paged_load(ps_cuda_ctx *ctx, const ps_cuda_pages *pages, int layer, void *k, void *v, int io_type, const ps_cuda_paged_seq *seqs, int n_seqs) {
+    return serve(ctx, [&](PsServeCall *c) { return ps_serve_paged_rows(c, false, pages, layer, k, v, io_type, seqs, n_seqs); });
+}
+int ps_cuda_paged_attn(ps_cuda_ctx *ctx, const ps_cuda_pages *pages, int layer, void *out, const void *q, int io_type, const ps_cuda_paged_seq *seqs, int n_seqs, int64_t n_heads,
+                       const uint8_t *tree_mask, float scale) {
+    return serve(ctx, [&](PsServeCall *c) {
+        if (!fits_int(n_heads)) return fail(ctx, PS_CUDA_ERR_INVALID, "paged_attn: head geometry");
+        return ps_serve_paged_attn(c, pages, layer, out, q, io_type, seqs, n_seqs, (int)n_heads, tree_mask, scale);
+    });
+}
+int ps_cuda_paged_edit(ps_cuda_ctx *ctx, const ps_cuda_pages *pages, const ps_cuda_page_edit *edits, int n, int32_t *held) {
+    return serve(ctx, [&](PsServeCall *c) { return ps_serve_paged_edit(c, pages, edits, n, held); });
+}
+int ps_cuda_paged_compact(ps_cuda_ctx *ctx, const ps_cuda_pages *pages, const ps_cuda_page_move *moves, int n) {
+    return serve(ctx, [&](PsServeCall *c) { return ps_serve_paged_compact(c, pages, moves, n); });
+}
+int ps_cuda_verify(ps_cuda_ctx *ctx, int32_t *ids, int32_t *path, int32_t *n_path, const int32_t *n_nodes, int n_seqs, const int32_t *parents, const int32_t *tokens, const float *logits, int64_t row_stride,
+                   int64_t vocab, const ps_cuda_sampler *samplers, const float *u, const float *draft_logits, const ps_cuda_sampler *draft_samplers) {
+    return serve(ctx, [&](PsServeCall *c) {
+        return ps_serve_verify(c, ids, path, n_path, n_nodes, n_seqs, parents, tokens, logits, row_stride, vocab, samplers, u, draft_logits, draft_samplers);
+    });
 }
 
 // ---------------------------------------------------------------------------------------------- KV cache

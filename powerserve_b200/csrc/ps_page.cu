@@ -1,0 +1,249 @@
+// ps_page.cu - host side of the caches in 8 bits and in pages (ps_serve.h): what the calls accept, and their launches.
+#include "ps_page_attn.cuh"
+#include "ps_page_edit.cuh"
+#include "ps_page_rows.cuh"
+
+#include <algorithm>
+#include <cstdarg>
+#include <cstdio>
+#include <vector>
+
+namespace {
+
+int fail(PsServeCall *c, int code, const char *fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(c->msg, sizeof c->msg, fmt, ap);
+    va_end(ap);
+    return code;
+}
+
+#define PG_CK(call)                                                                                                    \
+    do {                                                                                                               \
+        const cudaError_t e_ = (call);                                                                                 \
+        if (e_ != cudaSuccess) return fail(c, PS_CUDA_ERR_CUDA, "%s failed: %s", #call, cudaGetErrorString(e_));       \
+    } while (0)
+#define PG_LAUNCHED(what)                                                                                              \
+    do {                                                                                                               \
+        const cudaError_t e_ = cudaGetLastError();                                                                     \
+        if (e_ != cudaSuccess) return fail(c, PS_CUDA_ERR_CUDA, "%s: launch failed: %s", what, cudaGetErrorString(e_)); \
+        c->launches++;                                                                                                 \
+    } while (0)
+
+bool aligned(const void *p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+size_t up(size_t v) { return (v + 255) & ~(size_t)255; }
+
+int check_pages(PsServeCall *c, const char *what, const ps_cuda_pages *p, bool data) {
+    if (!p) return fail(c, PS_CUDA_ERR_INVALID, "%s: no cache", what);
+    if (p->page_tokens != 16 && p->page_tokens != 32 && p->page_tokens != 64 && p->page_tokens != 128)
+        return fail(c, PS_CUDA_ERR_UNSUPPORTED, "%s: pages of %d tokens (16, 32, 64 and 128 are there)", what, p->page_tokens);
+    if (p->head_size <= 0 || p->head_size % 32 || p->head_size > 256) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "%s: head size %d (multiples of 32 up to 256)", what, p->head_size);
+    if (p->n_kv_heads <= 0 || p->n_kv_heads > 1024) return fail(c, PS_CUDA_ERR_INVALID, "%s: %d kv heads", what, p->n_kv_heads);
+    if (p->n_layers <= 0 || p->n_layers > 4096 || p->n_pages <= 0 || p->n_pages > 1 << 26) return fail(c, PS_CUDA_ERR_INVALID, "%s: %d layers of %d pages", what, p->n_layers, p->n_pages);
+    if (data) {
+        if (!p->codes || !p->scales) return fail(c, PS_CUDA_ERR_INVALID, "%s: a cache without codes or scales", what);
+        if (!aligned(p->codes, 16) || !aligned(p->scales, 4)) return fail(c, PS_CUDA_ERR_INVALID, "%s: codes that are not aligned to 16 bytes, or scales to 4", what);
+    }
+    return 0;
+}
+int64_t layer_codes(const ps_cuda_pages *p) { return (int64_t)p->n_pages * p->n_kv_heads * 2 * p->page_tokens * p->head_size; }
+int64_t layer_scales(const ps_cuda_pages *p) { return (int64_t)p->n_pages * p->n_kv_heads * 2 * (p->page_tokens / PG_BLOCK); }
+PgPool pool_of(PsServeCall *c, const ps_cuda_pages *p, int layer) {
+    PgPool q{};
+    q.codes = p->codes ? p->codes + layer * layer_codes(p) : nullptr;
+    q.scales = p->scales ? p->scales + layer * layer_scales(p) : nullptr;
+    q.n_pages = p->n_pages; q.P = p->page_tokens; q.G = p->n_kv_heads; q.hs = p->head_size; q.err = c->err_dev;
+    for (q.shift = 0; 1 << q.shift < q.P;) q.shift++;
+    return q;
+}
+int64_t pages_of(int64_t n, int P) { return (n + P - 1) / P; }
+
+int check_seqs(PsServeCall *c, const char *what, const ps_cuda_pages *p, int layer, const ps_cuda_paged_seq *seqs, int n, int io_type, int64_t &tokens) {
+    if (int rc = check_pages(c, what, p, true)) return rc;
+    if (layer < 0 || layer >= p->n_layers) return fail(c, PS_CUDA_ERR_INVALID, "%s: layer %d of %d", what, layer, p->n_layers);
+    if (io_type != PS_TYPE_F32 && io_type != PS_TYPE_BF16) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "%s: type %d (float32 and bfloat16 are there)", what, io_type);
+    if (n < 0 || (n > 0 && !seqs)) return fail(c, PS_CUDA_ERR_INVALID, "%s: no sequences", what);
+    tokens = 0;
+    for (int i = 0; i < n; i++) {
+        const ps_cuda_paged_seq &s = seqs[i];
+        if (s.n_kv < 0 || s.n_kv > 1 << 30) return fail(c, PS_CUDA_ERR_INVALID, "%s: sequence %d holds %d slots (at most 2^30)", what, i, s.n_kv);
+        if (s.n_tok < 0 || s.n_tok > s.n_kv) return fail(c, PS_CUDA_ERR_INVALID, "%s: sequence %d has %d tokens of its %d slots", what, i, s.n_tok, s.n_kv);
+        if (!s.n_tok) continue;
+        if (!s.table || !aligned(s.table, 4)) return fail(c, PS_CUDA_ERR_INVALID, "%s: sequence %d has no table, or one that is not aligned to its elements", what, i);
+        if (s.n_table < pages_of(s.n_kv, p->page_tokens)) return fail(c, PS_CUDA_ERR_INVALID, "%s: sequence %d holds %d slots, its table has %d pages", what, i, s.n_kv, s.n_table);
+        tokens += s.n_tok;
+    }
+    if (tokens > INT32_MAX / 1024) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "%s: %lld tokens in one call", what, (long long)tokens);
+    return 0;
+}
+
+// f(a std::integral_constant of head size / 32)
+template <typename F> auto by_items(int hs, F f) {
+    switch (hs / 32) {
+    case 1: return f(std::integral_constant<int, 1>{});
+    case 2: return f(std::integral_constant<int, 2>{});
+    case 3: return f(std::integral_constant<int, 3>{});
+    case 4: return f(std::integral_constant<int, 4>{});
+    case 5: return f(std::integral_constant<int, 5>{});
+    case 6: return f(std::integral_constant<int, 6>{});
+    case 7: return f(std::integral_constant<int, 7>{});
+    default: return f(std::integral_constant<int, 8>{});
+    }
+}
+
+} // namespace
+
+int ps_serve_paged_rows(PsServeCall *c, bool store, const ps_cuda_pages *pages, int layer, void *k, void *v, int io_type, const ps_cuda_paged_seq *seqs, int n_seqs) {
+    const char *what = store ? "paged_store" : "paged_load";
+    int64_t tokens;
+    if (int rc = check_seqs(c, what, pages, layer, seqs, n_seqs, io_type, tokens)) return rc;
+    if (!tokens) return 0;
+    const int es = io_type == PS_TYPE_F32 ? 4 : 2;
+    if (store ? !k || !v : !k && !v) return fail(c, PS_CUDA_ERR_INVALID, "%s: null argument", what);
+    if (!aligned(k, es) || !aligned(v, es)) return fail(c, PS_CUDA_ERR_INVALID, "%s: an array that is not aligned to its elements", what);
+    PgRows a{};
+    a.pool = pool_of(c, pages, layer);
+    a.k = k; a.v = v; a.k_vec = aligned(k, 16); a.v_vec = aligned(v, 16);
+    for (int i = 0, tok0 = 0; i < n_seqs;) {
+        int64_t blocks = 0;
+        a.n_seqs = 0;
+        for (; i < n_seqs && a.n_seqs < PG_SEQS; i++) {
+            const ps_cuda_paged_seq &s = seqs[i];
+            if (!s.n_tok) continue;
+            a.seq[a.n_seqs++] = PgRowSeq{s.table, s.n_kv, s.n_tok, tok0, (int)blocks};
+            blocks += (s.n_kv - 1) / PG_BLOCK - (s.n_kv - s.n_tok) / PG_BLOCK + 1;
+            tok0 += s.n_tok;
+        }
+        if (!a.n_seqs) break;
+        a.blocks = (int)blocks; // (tokens fit an int's thousandth part)
+        const unsigned grid = (unsigned)((blocks * 2 * pages->n_kv_heads + PG_ROW_WARPS - 1) / PG_ROW_WARPS);
+        if (store)
+            by_items(pages->head_size, [&](auto items) {
+                constexpr int I = decltype(items)::value;
+                if (es == 4) pg_k_store<float, I><<<grid, 32 * PG_ROW_WARPS, 0, c->stream>>>(a);
+                else pg_k_store<__nv_bfloat16, I><<<grid, 32 * PG_ROW_WARPS, 0, c->stream>>>(a);
+            });
+        else if (es == 4) pg_k_load<float><<<grid, 32 * PG_ROW_WARPS, 0, c->stream>>>(a);
+        else pg_k_load<__nv_bfloat16><<<grid, 32 * PG_ROW_WARPS, 0, c->stream>>>(a);
+        PG_LAUNCHED(what);
+    }
+    return 0;
+}
+
+int ps_serve_paged_attn(PsServeCall *c, const ps_cuda_pages *pages, int layer, void *out, const void *q, int io_type, const ps_cuda_paged_seq *seqs, int n_seqs, int n_heads, const uint8_t *tree_mask,
+                        float scale) {
+    int64_t tokens;
+    if (int rc = check_seqs(c, "paged_attn", pages, layer, seqs, n_seqs, io_type, tokens)) return rc;
+    const int G = pages->n_kv_heads;
+    if (n_heads <= 0 || n_heads % G || n_heads / G > 32) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "paged_attn: %d heads over %d kv heads", n_heads, G);
+    for (int i = 0; i < n_seqs; i++)
+        if (seqs[i].n_tok > PS_CUDA_TREE_TOKENS) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "paged_attn: sequence %d brings %d tokens (at most %d)", i, seqs[i].n_tok, PS_CUDA_TREE_TOKENS);
+    if (!tokens) return 0;
+    const int es = io_type == PS_TYPE_F32 ? 4 : 2;
+    if (!out || !q) return fail(c, PS_CUDA_ERR_INVALID, "paged_attn: null argument");
+    if (!aligned(out, es) || !aligned(q, es)) return fail(c, PS_CUDA_ERR_INVALID, "paged_attn: an array that is not aligned to its elements");
+    PgAttn a{};
+    a.pool = pool_of(c, pages, layer);
+    a.q = q; a.out = out; a.n_heads = n_heads; a.R = n_heads / G; a.scale = scale * 1.4426950408889634f;
+    for (int i = 0, tok0 = 0; i < n_seqs;) {
+        int most = 0;
+        a.n_seqs = 0;
+        for (; i < n_seqs && a.n_seqs < PG_SEQS; i++) {
+            const ps_cuda_paged_seq &s = seqs[i];
+            if (!s.n_tok) continue;
+            a.seq[a.n_seqs++] = PgAttnSeq{s.table, s.hidden, tree_mask, s.n_kv, s.n_tok, tok0, 0};
+            tok0 += s.n_tok;
+            if (tree_mask) tree_mask += (size_t)s.n_tok * s.n_tok;
+            most = std::max(most, s.n_tok);
+        }
+        if (!a.n_seqs) break;
+        const dim3 grid(a.n_seqs, G, (most * a.R + 15) / 16);
+        const size_t smem = pg_attn_smem(pages->head_size);
+        auto kern = es == 4 ? pg_k_attn<float> : pg_k_attn<__nv_bfloat16>;
+        PG_CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        kern<<<grid, 128, smem, c->stream>>>(a);
+        PG_LAUNCHED("paged_attn");
+    }
+    return 0;
+}
+
+int ps_serve_paged_edit(PsServeCall *c, const ps_cuda_pages *pages, const ps_cuda_page_edit *edits, int n, int32_t *held) {
+    if (int rc = check_pages(c, "paged_edit", pages, true)) return rc;
+    if (!pages->refs || !aligned(pages->refs, 4)) return fail(c, PS_CUDA_ERR_INVALID, "paged_edit: a cache without refs, or with ones that are not aligned to their elements");
+    if (n < 0 || (n > 0 && !edits)) return fail(c, PS_CUDA_ERR_INVALID, "paged_edit: no edits");
+    if (n > PS_CUDA_EDITS) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "paged_edit: %d edits (at most %d)", n, PS_CUDA_EDITS);
+    if (!aligned(held, 4)) return fail(c, PS_CUDA_ERR_INVALID, "paged_edit: an array that is not aligned to its elements");
+    if (n == 0) return 0;
+    PgEdits a{};
+    const int P = pages->page_tokens;
+    int64_t most = 0;
+    int copies = 0;
+    std::vector<const void *> tables;
+    for (int i = 0; i < n; i++) {
+        const ps_cuda_page_edit &e = edits[i];
+        if (e.n_old < 0 || e.n_new < 0 || e.n_old > 1 << 30 || e.n_new > 1 << 30) return fail(c, PS_CUDA_ERR_INVALID, "paged_edit: edit %d: from %d to %d tokens", i, e.n_old, e.n_new);
+        if (e.from && e.n_new < e.n_old) return fail(c, PS_CUDA_ERR_INVALID, "paged_edit: edit %d shares %d tokens and shall hold %d", i, e.n_old, e.n_new);
+        const int64_t need = pages_of(std::max(e.n_old, e.n_new), P);
+        if (need > e.n_table) return fail(c, PS_CUDA_ERR_INVALID, "paged_edit: edit %d: %d tokens, its table has %d pages", i, std::max(e.n_old, e.n_new), e.n_table);
+        if ((need && !e.table) || !aligned(e.table, 4) || !aligned(e.from, 4)) return fail(c, PS_CUDA_ERR_INVALID, "paged_edit: edit %d has no table, or one that is not aligned to its elements", i);
+        if (e.table) tables.push_back(e.table);
+        a.op[i] = PgEditOp{e.table, e.from, e.n_old, e.n_new};
+        if (e.n_new > e.n_old) {
+            const bool part = e.n_old % P != 0;
+            most += pages_of(e.n_new, P) - pages_of(e.n_old, P) + part;
+            copies = part ? i + 1 : copies;
+        }
+    }
+    std::sort(tables.begin(), tables.end());
+    if (std::adjacent_find(tables.begin(), tables.end()) != tables.end()) return fail(c, PS_CUDA_ERR_INVALID, "paged_edit: two edits of one table");
+    if (most > INT32_MAX / 8) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "paged_edit: %lld pages in one call", (long long)most);
+    void *mem = nullptr;
+    const size_t list = up(sizeof(int4) * (size_t)n);
+    if (most)
+        if (int rc = c->workspace(c->user, list + up(4 * (size_t)most), &mem)) return rc;
+    a.copies = copies ? static_cast<int4 *>(mem) : nullptr;
+    a.free = reinterpret_cast<int32_t *>(static_cast<char *>(mem) + list);
+    a.refs = pages->refs; a.held = held; a.n = n; a.n_pages = pages->n_pages; a.err = c->err_dev;
+    const PgPool pool = pool_of(c, pages, 0);
+    a.shift = pool.shift;
+    pg_k_edit<<<1, PG_EDIT_THREADS, 0, c->stream>>>(a);
+    PG_LAUNCHED("paged_edit");
+    if (copies) {
+        PgCopies b{pool, a.copies, layer_codes(pages), layer_scales(pages)};
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.gridDim = dim3(copies, pages->n_layers, 1); cfg.blockDim = dim3(256); cfg.stream = c->stream; cfg.attrs = attr; cfg.numAttrs = 1;
+        PG_CK(cudaLaunchKernelEx(&cfg, pg_k_copy, b));
+        PG_LAUNCHED("paged_edit");
+    }
+    return 0;
+}
+
+int ps_serve_paged_compact(PsServeCall *c, const ps_cuda_pages *pages, const ps_cuda_page_move *moves, int n) {
+    if (int rc = check_pages(c, "paged_compact", pages, true)) return rc;
+    if (n < 0 || (n > 0 && !moves)) return fail(c, PS_CUDA_ERR_INVALID, "paged_compact: no moves");
+    PgMoves a{};
+    a.pool = pool_of(c, pages, 0);
+    a.layer_codes = layer_codes(pages); a.layer_scales = layer_scales(pages);
+    for (int i = 0; i < n; i++) {
+        const ps_cuda_page_move &m = moves[i];
+        if (m.first < 0 || m.n_kv < m.first || m.n_kv > 1 << 30) return fail(c, PS_CUDA_ERR_INVALID, "paged_compact: move %d: from slot %d of %d", i, m.first, m.n_kv);
+        if (m.n_keep < 0 || m.n_keep > m.n_kv - m.first) return fail(c, PS_CUDA_ERR_INVALID, "paged_compact: move %d keeps %d of %d slots", i, m.n_keep, m.n_kv - m.first);
+        if (!m.n_keep) continue;
+        if (!m.table || !m.keep || !aligned(m.table, 4) || !aligned(m.keep, 4) || !aligned(m.n_keep_dev, 4))
+            return fail(c, PS_CUDA_ERR_INVALID, "paged_compact: move %d has no table or list, or one that is not aligned to its elements", i);
+        if (m.n_table < pages_of(m.n_kv, pages->page_tokens)) return fail(c, PS_CUDA_ERR_INVALID, "paged_compact: move %d: %d slots, its table has %d pages", i, m.n_kv, m.n_table);
+    }
+    const int heads = 2 * pages->n_kv_heads * pages->n_layers;
+    for (int i = 0; i < n;) {
+        int k = 0;
+        for (; i < n && k < PG_SEQS; i++)
+            if (moves[i].n_keep) a.op[k++] = PgMoveOp{moves[i].table, moves[i].keep, moves[i].n_keep_dev, moves[i].first, moves[i].n_kv, moves[i].n_keep};
+        if (!k) break;
+        by_items(pages->head_size, [&](auto items) { pg_k_compact<decltype(items)::value><<<dim3(heads, k), 256, 0, c->stream>>>(a); });
+        PG_LAUNCHED("paged_compact");
+    }
+    return 0;
+}

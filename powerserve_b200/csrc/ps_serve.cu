@@ -6,6 +6,7 @@
 #include "ps_serve_attn_few.cuh"
 #include "ps_serve_evict.cuh"
 #include "ps_serve_sample.cuh"
+#include "ps_serve_verify.cuh"
 
 #include <algorithm>
 #include <cstdarg>
@@ -366,6 +367,67 @@ int ps_serve_sample(PsServeCall *c, int32_t *ids, float *probs, const float *log
         SV_LAUNCHED("sample");
         a.logits += (int64_t)n * row_stride; a.samplers += n; a.u += n; a.ids += n;
         if (a.probs) a.probs += n;
+    }
+    return 0;
+}
+
+int ps_serve_verify(PsServeCall *c, int32_t *ids, int32_t *path, int32_t *n_path, const int32_t *n_nodes, int n_seqs, const int32_t *parents, const int32_t *tokens, const float *logits, int64_t row_stride, int64_t vocab,
+                    const ps_cuda_sampler *samplers, const float *u, const float *draft_logits, const ps_cuda_sampler *draft_samplers) {
+    if (n_seqs < 0 || (n_seqs > 0 && !n_nodes)) return fail(c, PS_CUDA_ERR_INVALID, "verify: no sequences");
+    if (vocab <= 0 || vocab > 1 << 18 || row_stride < vocab) return fail(c, PS_CUDA_ERR_INVALID, "verify: rows of %lld tokens (1 to 262144), %lld apart", (long long)vocab, (long long)row_stride);
+    int64_t rows = 0;
+    for (int i = 0; i < n_seqs; i++) {
+        if (n_nodes[i] < 1) return fail(c, PS_CUDA_ERR_INVALID, "verify: sequence %d has %d nodes", i, n_nodes[i]);
+        if (n_nodes[i] > PS_CUDA_TREE_TOKENS) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "verify: sequence %d has %d nodes (at most %d)", i, n_nodes[i], PS_CUDA_TREE_TOKENS);
+        rows += n_nodes[i];
+    }
+    if (rows == 0) return 0;
+    if (rows > 1 << 20) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "verify: %lld nodes in one call", (long long)rows);
+    if (!ids || !path || !n_path || !parents || !tokens || !logits || !samplers || !u) return fail(c, PS_CUDA_ERR_INVALID, "verify: null argument");
+    if ((draft_logits != nullptr) != (draft_samplers != nullptr)) return fail(c, PS_CUDA_ERR_INVALID, "verify: the draft's rows and their settings go together");
+    for (const void *p : {(const void *)ids, (const void *)path, (const void *)n_path, (const void *)parents, (const void *)tokens, (const void *)logits, (const void *)samplers, (const void *)u, (const void *)draft_logits, (const void *)draft_samplers})
+        if (!aligned(p, 4)) return fail(c, PS_CUDA_ERR_INVALID, "verify: an array that is not aligned to its elements");
+    for (int s0 = 0; s0 < n_seqs;) {
+        SvVerify v{};
+        int n = 0;
+        v.first[0] = 0;
+        for (; s0 + n < n_seqs && n < SV_VERIFY_SEQS; n++) v.first[n + 1] = v.first[n] + n_nodes[s0 + n];
+        const int nodes = v.first[n];
+        void *mem = nullptr;
+        if (int rc = c->workspace(c->user, 2 * sizeof(SvRowStats) * (size_t)nodes, &mem)) return rc;
+        SvRowStats *stats[2] = {static_cast<SvRowStats *>(mem), static_cast<SvRowStats *>(mem) + nodes};
+        v.target = stats[0]; v.draft = stats[1];
+        v.ids = ids; v.path = path; v.n_path = n_path; v.parents = parents; v.tokens = tokens; v.logits = logits; v.draft_logits = draft_logits; v.samplers = samplers; v.draft_samplers = draft_samplers;
+        v.u = u; v.row_stride = row_stride; v.vocab = (int)vocab;
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute at[2];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.blockDim = dim3(SV_SMP_THREADS); cfg.stream = c->stream; cfg.attrs = at; cfg.numAttrs = 1;
+        for (int d = 0; d < (draft_logits ? 2 : 1); d++) {
+            SvStats a{};
+            a.s.logits = d ? draft_logits : logits; a.s.samplers = d ? draft_samplers : samplers; a.s.row_stride = row_stride; a.s.vocab = (int)vocab; a.s.stats = stats[d];
+            a.parents = d ? parents : nullptr; a.n_seqs = n;
+            std::copy(v.first, v.first + n + 1, a.first);
+            const int C = nodes * 16 <= c->n_sm ? 16 : 8; // (as in ps_serve_sample)
+            a.s.chunk = (int)((vocab + C - 1) / C + 31) & ~31;
+            a.s.vec = aligned(a.s.logits, 16) && row_stride % 4 == 0;
+            const size_t smem = sizeof(SvSmpShared) + 4 * (size_t)a.s.chunk;
+            at[0].val.clusterDim.x = C;
+            cfg.gridDim = dim3(nodes * C); cfg.dynamicSmemBytes = smem;
+            SV_CK(cudaFuncSetAttribute(sv_k_stats, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            SV_CK(cudaFuncSetAttribute(sv_k_stats, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+            SV_CK(cudaLaunchKernelEx(&cfg, sv_k_stats, a));
+            SV_LAUNCHED("verify");
+        }
+        at[0].val.clusterDim.x = SV_VERIFY_CTAS;
+        cfg.gridDim = dim3(n * SV_VERIFY_CTAS); cfg.dynamicSmemBytes = 0;
+        v.chunk = (int)((vocab + SV_VERIFY_CTAS - 1) / SV_VERIFY_CTAS + 31) & ~31;
+        SV_CK(cudaLaunchKernelEx(&cfg, sv_k_verify, v));
+        SV_LAUNCHED("verify");
+        ids += n; n_path += n; path += nodes; parents += nodes; tokens += nodes; u += nodes; samplers += nodes; logits += (int64_t)nodes * row_stride;
+        if (draft_logits) { draft_logits += (int64_t)nodes * row_stride; draft_samplers += nodes; }
+        s0 += n;
     }
     return 0;
 }

@@ -24,6 +24,12 @@
 #define SV_SMP_SPAN 16.0    // log2 of the least weight that is listed, negative
 #define SV_ONE (1ull << 44)
 
+// What the settings leave of a row: its tokens of which the number sv_key is at least kappa and the weight at least min_p, and their mass (0: one token alone, `only`; -1: none)
+struct SvRowStats {
+    unsigned long long kappa, all;
+    float top;
+    int only;
+};
 struct SvSample {
     const float *logits;
     const ps_cuda_sampler *samplers;
@@ -33,6 +39,7 @@ struct SvSample {
     int64_t row_stride;
     int vocab, chunk;       // tokens; tokens of a CTA
     int vec;                // rows begin at 16-byte boundaries
+    SvRowStats *stats;      // sv_sample<true>: what is left of a row is asked for, no token
 };
 struct alignas(16) SvSmpShared { // (the logits lie behind it, read and written sixteen bytes at a time)
     union {
@@ -61,7 +68,7 @@ struct SvScale {
 };
 // 2^t as a whole number of 2^-44: 2^t = 2^n 2^(j / 32) 2^r, |r| <= 1/64, the last by the exponential's series to the fifth power (the sixth is below 2^-48).
 // Without branches, so that several are under way at once: one alone takes 300 cycles
-PS_D unsigned long long sv_weight(const SvSmpShared &sh, double t) {
+PS_D unsigned long long sv_weight(const double *pow2, double t) {
     const double magic = 211106232532992.0;        // 1.5 2^47: its last bit is 1/32
     const double z = t + magic;
     const int j = __double2loint(z);
@@ -70,12 +77,13 @@ PS_D unsigned long long sv_weight(const SvSmpShared &sh, double t) {
     p = fma(p, r, 5.5504108664821580e-2);
     p = fma(p, r, 2.4022650695910072e-1);
     p = fma(p, r, 6.9314718055994531e-1);
-    const double b = sh.pow2[j & 31];
+    const double b = pow2[j & 31];
     const double w = fma(p * r, b, b);
     const double big = __hiloint2double(__double2hiint(w) + (((j >> 5) + 44) << 20), __double2loint(w));
     const unsigned long long n = (unsigned long long)__double_as_longlong(big + 4503599627370496.0) & 0xfffffffffffffull; // (2^52: the sum's mantissa is the whole number)
     return (uint32_t)__double2hiint(t) < 0xc0470000u ? n : 0; // above -46
 }
+PS_D unsigned long long sv_weight(const SvSmpShared &sh, double t) { return sv_weight(sh.pow2, t); }
 template <bool MAX> PS_D unsigned long long sv_block(SvSmpShared &sh, unsigned long long v) { // sum or maximum over the block
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     auto join = [](unsigned long long x, unsigned long long y) { return MAX ? (x > y ? x : y) : x + y; };
@@ -337,7 +345,7 @@ template <bool LIST> PS_D bool sv_borders(const SvSmpRow &r, SvSmpShared &sh, Sv
 }
 
 // the token: the warps' kept masses, and in the warp where u times all of them falls its tokens in order
-template <bool LIST> PS_D void sv_pick(const SvSample &a, int64_t row, const SvSmpRow &r, SvSmpShared &sh, SvMail &mail, const float *x, unsigned long long kappa, bool filters) {
+template <bool LIST, bool STATS> PS_D void sv_pick(const SvSample &a, int64_t row, const SvSmpRow &r, SvSmpShared &sh, SvMail &mail, const float *x, unsigned long long kappa, bool filters) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     auto mass_of = [&](float v, unsigned long long key) -> unsigned long long {
         if (key < kappa) return 0;
@@ -357,6 +365,10 @@ template <bool LIST> PS_D void sv_pick(const SvSample &a, int64_t row, const SvS
             if (o < mail.rank) before += m[0][o];
             all += m[0][o];
         }
+    }
+    if (STATS) {
+        if (mail.rank == 0 && threadIdx.x == 0) a.stats[row] = SvRowStats{kappa, all, r.log2w.top, 0};
+        return;
     }
     const float u = a.u[row];
     unsigned long long goal = u > 0.f ? (unsigned long long)((double)fminf(u, 1.f) * (double)all) : 0;
@@ -426,7 +438,7 @@ PS_D unsigned long long sv_before(SvSmpShared &sh, unsigned long long v, unsigne
 }
 
 // Few tokens are listed: one CTA has them all in sh.list, in the vocabulary's order, and goes on alone
-PS_D void sv_few(const SvSample &a, int64_t row, const SvSmpRow &r, SvSmpShared &sh, int n, unsigned long long held) {
+template <bool STATS> PS_D void sv_few(const SvSample &a, int64_t row, const SvSmpRow &r, SvSmpShared &sh, int n, unsigned long long held) {
     const int tid = threadIdx.x;
     unsigned long long kappa = 0, all, mine[2], key[2];
     if (r.use_k || r.use_p) {
@@ -470,6 +482,10 @@ PS_D void sv_few(const SvSample &a, int64_t row, const SvSmpRow &r, SvSmpShared 
         sum += mine[e];
     }
     unsigned long long before = sv_before(sh, sum, all);
+    if (STATS) {
+        if (tid == 0) a.stats[row] = SvRowStats{kappa, all, r.log2w.top, 0};
+        return;
+    }
     const float u = a.u[row];
     unsigned long long goal = u > 0.f ? (unsigned long long)((double)fminf(u, 1.f) * (double)all) : 0;
     goal = min(goal, all - 1);
@@ -483,7 +499,8 @@ PS_D void sv_few(const SvSample &a, int64_t row, const SvSmpRow &r, SvSmpShared 
     }
 }
 
-__global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_sample(const __grid_constant__ SvSample a) {
+// STATS: for the verification of drafted tokens, what the settings leave of the row
+template <bool STATS> PS_D void sv_sample(const SvSample &a) {
     extern __shared__ __align__(16) uint8_t sv_smp_raw[];
     SvSmpShared &sh = *reinterpret_cast<SvSmpShared *>(sv_smp_raw);
     float *x = reinterpret_cast<float *>(sv_smp_raw + sizeof(SvSmpShared));
@@ -558,8 +575,11 @@ __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_sample(const __grid_co
         uint32_t most_not = 0;
         for (int o = 0; o < C; o++) most_not = max(most_not, (uint32_t)m[0][o]);
         if (mail.rank == 0 && tid == 0) {
-            a.ids[row] = best ? (int)~most_not : -1;
-            if (a.probs) a.probs[row] = best ? 1.f : 0.f;
+            if (STATS) a.stats[row] = SvRowStats{0, 0, r.log2w.top, best ? (int)~most_not : -1};
+            else {
+                a.ids[row] = best ? (int)~most_not : -1;
+                if (a.probs) a.probs[row] = best ? 1.f : 0.f;
+            }
         }
         return; // (after the last barrier a CTA looks at its own memory alone)
     }
@@ -662,12 +682,13 @@ __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_sample(const __grid_co
                 to->list[at + i] = sv_key(x[l], r.i0 + l);
             }
             mail.cl.sync();
-            if (mail.rank == 0) sv_few(a, row, r, sh, (int)total, whole);
+            if (mail.rank == 0) sv_few<STATS>(a, row, r, sh, (int)total, whole);
             return; // (nobody's memory is asked for any more)
         }
         listed = !over_any && (r.use_k || r.use_p ? sv_borders<true>(r, sh, mail, x, whole, kappa) : least);
         if (!listed && (r.use_k || r.use_p)) sv_borders<false>(r, sh, mail, x, whole, kappa);
     }
-    if (listed) sv_pick<true>(a, row, r, sh, mail, x, kappa, filters);
-    else sv_pick<false>(a, row, r, sh, mail, x, kappa, filters);
+    if (listed) sv_pick<true, STATS>(a, row, r, sh, mail, x, kappa, filters);
+    else sv_pick<false, STATS>(a, row, r, sh, mail, x, kappa, filters);
 }
+__global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_sample(const __grid_constant__ SvSample a) { sv_sample<false>(a); }
