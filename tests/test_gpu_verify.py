@@ -1,0 +1,196 @@
+"""Verification of drafted tokens against the definition in 64 bits: paths and next tokens are equal; chains and trees, with the draft's rows and without, every kind of settings, rows that are odd; and the
+distribution that comes out is the target's."""
+import numpy as np
+import pytest
+
+from powerserve_b200 import capi
+from tests import _paged as P
+from tests import _serve as S
+from tests.test_gpu_serve_attention import be  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+KINDS = [(0.8, 40, 0.95, 0.0), (1.0, 0, 0.9, 0.0), (1.3, 0, 1.0, 0.05), (0.0, 0, 1.0, 0.0), (1.0, 0, 1.0, 0.0), (0.6, 500, 0.8, 0.1), (1.5, 2000, 0.99, 0.001), (1.0, 1, 1.0, 0.0)]
+
+
+def make(V, sizes, fan, seed, near=0.6, draft=True, kinds=KINDS):
+    """(parents, tokens, u, logits, settings, draft logits, draft settings), all sequences after one another"""
+    r = np.random.default_rng(seed)
+    n = sum(sizes)
+    logits = (r.standard_normal((n, V)) * 2.5).astype(np.float32)
+    for row in logits:
+        row[r.integers(0, V, 12)] += r.random(12).astype(np.float32) * 10
+    guess = (logits + r.standard_normal((n, V)) * near).astype(np.float32)
+    parents, tokens, t0 = np.zeros(n, np.int32), np.zeros(n, np.int32), 0
+    sets = np.zeros(n, capi.SAMPLER)
+    for s, m in enumerate(sizes):
+        sets[t0:t0 + m] = tuple(kinds[s % len(kinds)])
+        parents[t0] = -1
+        for i in range(1, m):
+            p = int(r.integers(max(0, i - fan), i))
+            d = P.distribution(guess[t0 + p], *sets[t0 + p].tolist())
+            parents[t0 + i] = p
+            tokens[t0 + i] = r.choice(V, p=d) if r.random() < 0.9 else int(r.integers(0, V))
+        t0 += m
+    return parents, tokens, r.random(n).astype(np.float32), logits, sets, guess if draft else None, sets if draft else None
+
+
+def run(be, V, sizes, parents, tokens, u, logits, sets, guess=None, guess_sets=None, pad=0):  # noqa: F811
+    n, S_ = sum(sizes), len(sizes)
+    wide = lambda x: np.concatenate([x, np.full((n, pad), 1e30, np.float32)], 1) if pad else x      # noqa: E731
+    up = [be.upload(a) for a in (parents, tokens, wide(logits), sets, u)]
+    g = [None, None] if guess is None else [be.upload(wide(guess)), be.upload(guess_sets)]
+    ids, path, n_path = be.upload(np.full(S_ + 1, -9, np.int32)), be.upload(np.full(n + 1, -9, np.int32)), be.upload(np.full(S_ + 1, -9, np.int32))
+    be.verify(ids, path, n_path, sizes, up[0], up[1], up[2], V, up[3], up[4], draft_logits=g[0], draft_samplers=g[1], row_stride=V + pad)
+    got = ids.numpy(np.int32), path.numpy(np.int32), n_path.numpy(np.int32)
+    for b in up + [x for x in g if x] + [ids, path, n_path]:
+        b.free()
+    assert got[0][-1] == got[1][-1] == got[2][-1] == -9
+    return got[0][:-1], got[1][:-1], got[2][:-1]
+
+
+def check(be, V, sizes, parents, tokens, u, logits, sets, guess=None, guess_sets=None, pad=0):  # noqa: F811
+    ids, path, n_path = run(be, V, sizes, parents, tokens, u, logits, sets, guess, guess_sets, pad)
+    t0 = 0
+    for s, m in enumerate(sizes):
+        e = slice(t0, t0 + m)
+        want, token = P.verify(parents[e], tokens[e], u[e], logits[e], sets[e].tolist(), None if guess is None else guess[e], None if guess is None else guess_sets[e].tolist())
+        assert path[e].tolist() == want + [-1] * (m - len(want)) and n_path[s] == len(want), s
+        assert ids[s] == token, (s, ids[s], token)
+        t0 += m
+    return n_path
+
+
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("V", [5, 100, 2049, 32000])
+@pytest.mark.parametrize("fan", [1, 3])
+def test_trees_of_all_sizes(be, draft, V, fan):  # noqa: F811
+    for seed in range(3):
+        check(be, V, [1, 2, 5, 12, 8, 3, 1, 20], *make(V, [1, 2, 5, 12, 8, 3, 1, 20], fan, 100 * V + seed, draft=draft))
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_large_vocabulary(be, draft):  # noqa: F811
+    a = make(151936, [5, 12], 2, 7, draft=draft)
+    check(be, 151936, [5, 12], *a)
+    check(be, 151936, [5, 12], *a, pad=3)
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_many_sequences(be, draft):  # noqa: F811
+    sizes = [1 + i % 3 for i in range(1100)]
+    n = check(be, 300, sizes, *make(300, sizes, 2, 8, draft=draft))
+    assert len(set(n.tolist())) == 3
+
+
+def test_widest_tree(be):  # noqa: F811
+    for fan in (1, 200):
+        check(be, 500, [256, 256], *make(500, [256, 256], fan, fan, near=0.1))
+        check(be, 500, [256, 256], *make(500, [256, 256], fan, fan, near=0.1, draft=False))
+
+
+def test_a_draft_of_the_same_mind_is_always_right(be):  # noqa: F811
+    parents, tokens, u, logits, sets, _, _ = make(4000, [9] * 8, 1, 9, near=0.0)
+    for s in range(8):          # (drawn tokens only)
+        for i in range(1, 9):
+            d = P.distribution(logits[9 * s + i - 1], *sets[9 * s].tolist())
+            tokens[9 * s + i] = np.random.default_rng(s * 10 + i).choice(4000, p=d)
+    u[:] = np.float32(1) - np.float32(2.0 ** -24)
+    n = check(be, 4000, [9] * 8, parents, tokens, u, logits, sets, logits, sets)
+    assert (n == 9).all()
+
+
+def test_the_same_sibling_twice_and_tokens_outside(be):  # noqa: F811
+    """a token that was rejected has nothing left; one outside the vocabulary changes nothing"""
+    for draft in (False, True):
+        parents, tokens, u, logits, sets, g, gs = make(64, [8] * 40, 8, 10, draft=draft, kinds=[(1.0, 0, 1.0, 0.0)])
+        parents.reshape(40, 8)[:, 1:] = 0
+        tokens.reshape(40, 8)[:, 2] = tokens.reshape(40, 8)[:, 1]
+        tokens.reshape(40, 8)[:, 3], tokens.reshape(40, 8)[:, 5], tokens.reshape(40, 8)[:, 6] = -1, 64, 2 ** 31 - 1
+        u.reshape(40, 8)[:, 1:] = 0.9
+        check(be, 64, [8] * 40, parents, tokens, u, logits, sets, g, gs)
+
+
+def test_odd_rows(be):  # noqa: F811
+    """no numbers, nothing but -inf, one infinite logit, all equal, one token that has all"""
+    for draft in (False, True):
+        parents, tokens, u, logits, sets, g, gs = make(200, [4] * 12, 2, 11, draft=draft, kinds=KINDS[:2] + KINDS[4:5])
+        L = logits.reshape(12, 4, 200)
+        L[0, :, ::3] = np.nan
+        L[1] = -np.inf
+        L[2, 1] = np.nan
+        L[3, :, 17] = np.inf
+        L[4] = 1.5
+        L[5, :, :] = -1e30
+        L[5, :, 40] = 50.0
+        tokens.reshape(12, 4)[5, 1:] = 40
+        tokens.reshape(12, 4)[3, 1:] = 17
+        if draft:
+            g.reshape(12, 4, 200)[6] = -np.inf
+            g.reshape(12, 4, 200)[7, 0] = np.nan
+            g.reshape(12, 4, 200)[8, :, 3] = np.inf
+        check(be, 200, [4] * 12, parents, tokens, u, logits, sets, g, gs)
+
+
+@pytest.mark.parametrize("u0", [0.0, 1.0 - 2.0 ** -24, 1.0, 2.0, -1.0, np.nan])
+def test_random_numbers_at_the_ends(be, u0):  # noqa: F811
+    for draft in (False, True):
+        parents, tokens, u, logits, sets, g, gs = make(3000, [3] * 8, 2, 12, draft=draft)
+        u.reshape(8, 3)[:, 0] = u0
+        args = parents, tokens, u, logits, sets, g, gs
+        ids, path, n_path = run(be, 3000, [3] * 8, *args)
+        for s in range(8):
+            e, clamped = slice(3 * s, 3 * s + 3), u.copy()
+            clamped[3 * s] = min(max(u0, 0.0), 1.0) if u0 == u0 else 0.0
+            want, token = P.verify(parents[e], tokens[e], clamped[e], logits[e], sets[e].tolist(), None if g is None else g[e], None if g is None else gs[e].tolist())
+            assert path[e].tolist()[:len(want)] == want and ids[s] == token
+
+
+def test_tests_at_the_ends(be):  # noqa: F811
+    """u = 0 accepts what the target may draw at all, u = 1 only what the draft does not hold for likelier"""
+    for draft in (False, True):
+        for u1 in (0.0, 1.0):
+            parents, tokens, u, logits, sets, g, gs = make(500, [4] * 16, 2, 13, draft=draft)
+            u.reshape(16, 4)[:, 1:] = u1
+            check(be, 500, [4] * 16, parents, tokens, u, logits, sets, g, gs)
+
+
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("fan", [1, 3])
+def test_what_comes_out_is_the_targets_distribution(be, draft, fan):  # noqa: F811
+    """the first token after the root over 60 000 trials of one tree, drafted tokens drawn anew: counts within six standard deviations of what the target's own draws would give.
+    (Without the draft's rows the drafted tokens are fixed, and the law holds for those too.)"""
+    V, N, m = 8, 60000, 3
+    r = np.random.default_rng(14)
+    logits, guess = [(r.standard_normal((m, V)) * 1.2).astype(np.float32) for _ in range(2)]
+    sets = np.zeros(N * m, capi.SAMPLER)
+    sets[:] = (1.0, 0, 1.0, 0.0)
+    parents = np.tile(np.array([-1, 0, 0 if fan > 1 else 1], np.int32), N)
+    q = P.distribution(guess[0], 1.0, 0, 1.0, 0.0)
+    q1 = P.distribution(guess[1], 1.0, 0, 1.0, 0.0)
+    tokens = np.zeros((N, m), np.int32)
+    tokens[:, 1] = r.choice(V, N, p=q) if draft else 2
+    tokens[:, 2] = (r.choice(V, N, p=q if fan > 1 else q1)) if draft else 5
+    u = r.random((N, m)).astype(np.float32)
+    every = lambda x: np.ascontiguousarray(np.broadcast_to(x, (N, m, V))).reshape(-1, V)    # noqa: E731
+    got = np.zeros(V)
+    ids, path, n_path = run(be, V, [m] * N, parents, tokens.reshape(-1), u.reshape(-1), every(logits), sets, every(guess) if draft else None, sets if draft else None)
+    first = np.where(n_path > 1, tokens[np.arange(N), path.reshape(N, m)[:, 1].clip(0)], ids)
+    got = np.bincount(first, minlength=V)
+    p = P.distribution(logits[0], 1.0, 0, 1.0, 0.0)
+    assert (np.abs(got - N * p) <= 6 * np.sqrt(N * p * (1 - p))).all(), (got / N, p)
+
+
+def test_sampling_is_what_it_was(be):  # noqa: F811
+    """a sequence of one node is a row of ps_cuda_sample"""
+    r = np.random.default_rng(15)
+    V, n = 32000, 40
+    logits = (r.standard_normal((n, V)) * 3).astype(np.float32)
+    sets = S.settings([KINDS[i % len(KINDS)] for i in range(n)])
+    u = r.random(n).astype(np.float32)
+    ids, path, n_path = run(be, V, [1] * n, np.full(n, -1, np.int32), np.zeros(n, np.int32), u, logits, sets)
+    up = [be.upload(a) for a in (logits, sets, u)]
+    want = be.upload(np.zeros(n, np.int32))
+    be.sample(want, None, up[0], V, n, up[1], up[2])
+    assert np.array_equal(want.numpy(np.int32), ids) and (n_path == 1).all() and (path == 0).all()
+    for b in up + [want]:
+        b.free()
