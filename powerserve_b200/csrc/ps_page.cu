@@ -142,27 +142,86 @@ int ps_serve_paged_attn(PsServeCall *c, const ps_cuda_pages *pages, int layer, v
     const int es = io_type == PS_TYPE_F32 ? 4 : 2;
     if (!out || !q) return fail(c, PS_CUDA_ERR_INVALID, "paged_attn: null argument");
     if (!aligned(out, es) || !aligned(q, es)) return fail(c, PS_CUDA_ERR_INVALID, "paged_attn: an array that is not aligned to its elements");
+    const int hs = pages->head_size, R = n_heads / G;
     PgAttn a{};
     a.pool = pool_of(c, pages, layer);
-    a.q = q; a.out = out; a.n_heads = n_heads; a.R = n_heads / G; a.scale = scale * 1.4426950408889634f;
+    a.q = q; a.out = out; a.n_heads = n_heads; a.R = R; a.scale = scale * 1.4426950408889634f; a.bf16 = es == 2; a.q_vec = aligned(q, 4 * es);
     for (int i = 0, tok0 = 0; i < n_seqs;) {
-        int most = 0;
-        a.n_seqs = 0;
-        for (; i < n_seqs && a.n_seqs < PG_SEQS; i++) {
+        PgAttnSeq all[PG_SEQS];
+        int most = 0, n = 0;
+        int64_t tiles = 0;
+        for (; i < n_seqs && n < PG_SEQS; i++) {
             const ps_cuda_paged_seq &s = seqs[i];
             if (!s.n_tok) continue;
-            a.seq[a.n_seqs++] = PgAttnSeq{s.table, s.hidden, tree_mask, s.n_kv, s.n_tok, tok0, 0};
+            const int t = (s.n_kv + PG_TILE - 1) / PG_TILE;
+            if (n && tiles + (int64_t)t * G > INT32_MAX / 2) break;
+            tiles += (int64_t)t * G;
+            all[n++] = PgAttnSeq{s.table, s.hidden, tree_mask, s.n_kv, s.n_tok, tok0, t};
             tok0 += s.n_tok;
             if (tree_mask) tree_mask += (size_t)s.n_tok * s.n_tok;
-            most = std::max(most, s.n_tok);
+            most = std::max(most, s.n_tok * R);
         }
-        if (!a.n_seqs) break;
-        const dim3 grid(a.n_seqs, G, (most * a.R + 15) / 16);
-        const size_t smem = pg_attn_smem(pages->head_size);
-        auto kern = es == 4 ? pg_k_attn<float> : pg_k_attn<__nv_bfloat16>;
-        PG_CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        kern<<<grid, 128, smem, c->stream>>>(a);
-        PG_LAUNCHED("paged_attn");
+        if (!n) break;
+        if (tiles > INT32_MAX / 2) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "paged_attn: %lld tiles of one sequence", (long long)tiles);
+        auto launch = [&](auto cfg) -> int {
+            using C = decltype(cfg);
+            constexpr int RT = C::RT;
+            auto kern = pg_k_attn<C::RT, C::MT, C::SG>;
+            // those with more row tiles first: a run of row tiles is that of the first so many
+            auto row_tiles = [&](const PgAttnSeq &s) { return (s.n_tok * R + RT - 1) / RT; };
+            std::stable_sort(all, all + n, [&](const PgAttnSeq &x, const PgAttnSeq &y) { return row_tiles(x) > row_tiles(y); });
+            a.n_seqs = n;
+            a.tile0[0] = 0;
+            for (int k = 0; k < n; k++) { a.seq[k] = all[k]; a.tile0[k + 1] = a.tile0[k] + all[k].tiles * G; }
+            a.n_lanes = row_tiles(all[0]);
+            int64_t total = 0;
+            for (int z = 0, k = n; z < a.n_lanes; z++) {
+                while (row_tiles(all[k - 1]) <= z) k--;
+                a.lane_tiles[z] = a.tile0[k];
+                total += a.lane_tiles[z];
+            }
+            const int slots = c->n_sm * C::CTAS;
+            a.n_ctas = 0;
+            for (int z = 0; z < a.n_lanes; z++) {
+                a.lane_cta0[z] = a.n_ctas;
+                a.n_ctas += (int)std::max<int64_t>(1, std::min<int64_t>(a.lane_tiles[z], (int64_t)slots * a.lane_tiles[z] / total));
+            }
+            a.lane_cta0[a.n_lanes] = a.n_ctas;
+            // stages: what the CTAs' shares of shared memory hold
+            const int stage = PG_TILE * hs, room = (C::CTAS == 2 ? 112 : 220) * 1024 - 128 - C::tail(hs) - (C::SG == 1 ? 4096 : 9216);
+            a.stages = std::max(2, std::min(PG_STAGES, room / (2 * stage)));
+            const size_t smem = 128 + (size_t)a.stages * 2 * stage + C::tail(hs);
+            void *mem = nullptr;
+            if (int rc = c->workspace(c->user, up(4 * (size_t)a.n_ctas * 2 * RT * (hs + 2)), &mem)) return rc;
+            a.part = static_cast<float *>(mem);
+            PG_CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            kern<<<a.n_ctas, C::THREADS, smem, c->stream>>>(a);
+            PG_LAUNCHED("paged_attn");
+            // whether runs begin where rows' tiles do
+            bool split = false;
+            for (int z = 0; z < a.n_lanes && !split; z++) {
+                const int m = a.lane_cta0[z + 1] - a.lane_cta0[z];
+                for (int k = 1, s = 0; k < m && !split; k++) {
+                    const int x = (int)pg_run(a.lane_tiles[z], m, k);
+                    while (a.tile0[s + 1] <= x) s++;
+                    split = (x - a.tile0[s]) % all[s].tiles != 0;
+                }
+            }
+            if (split) {
+                cudaLaunchConfig_t cfg2{};
+                cudaLaunchAttribute attr[1];
+                attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+                attr[0].val.programmaticStreamSerializationAllowed = 1;
+                cfg2.gridDim = dim3((most + 7) / 8, G, n); cfg2.blockDim = dim3(256); cfg2.stream = c->stream; cfg2.attrs = attr; cfg2.numAttrs = 1;
+                PG_CK(cudaLaunchKernelEx(&cfg2, pg_k_join, a, RT));
+                PG_LAUNCHED("paged_attn");
+            }
+            return 0;
+        };
+        int rc;
+        if (hs <= 128) rc = most <= 5 ? launch(PgCfg<5, 1, 1>{}) : most <= 10 ? launch(PgCfg<10, 1, 1>{}) : most <= 16 ? launch(PgCfg<16, 1, 1>{}) : launch(PgCfg<32, 1, 2>{});
+        else rc = most <= 5 ? launch(PgCfg<5, 2, 1>{}) : launch(PgCfg<16, 2, 1>{});
+        if (rc) return rc;
     }
     return 0;
 }

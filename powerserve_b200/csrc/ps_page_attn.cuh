@@ -1,116 +1,686 @@
-// ps_page_attn.cuh - attention of a step's tokens over caches in 8 bits and in pages.
+// ps_page_attn.cuh - attention of a step's tokens over caches in 8 bits and in pages, on the fifth-generation tensor cores' whole numbers.
 //
 //   z[t][h][j] = scale q[t][h] . k[j][g(h)],   p = soft-max over the slots j that token t sees,   out[t][h] = sum_j p[t][h][j] v[g(h)][j]
+//
+// The codes are the operand as they lie in the pages: nothing is converted.  What meets them is cut into digits of eight bits, lowest first.  A query row is a whole number of 24 bits times a
+// factor of its own, three signed digits; a weight times its slot's V scale over the tile's largest is one of 23 bits, three digits without a sign.  The products and their sums are exact (32 bits: 2^7 2^7 256
+// channels, 2^8 2^7 128 slots), and the digits' sums are put together in float32.  Digits are columns of the product, so three of them cost no more instructions than a wider N does.
+//
+// The cache is the MMAs' M side: scores^T[128 slots][rows x digits] = K Q^T, then out^T[channels][rows x digits] = V^T P^T, a lane of tensor memory a slot, then a channel.  A thread of the soft-max has a slot,
+// so its scales are its own, the row's largest score is a reduction over the warp (redux) and over four warps (an atomic of shared memory); a weight's digits are three bytes stored.  A thread of the
+// output has a channel: it adds a tile's sums to what it holds, so the accumulator sees one tile alone and tiles may have factors and references of their own.
+//
+// A CTA takes a run of tiles (128 slots of one kv head and up to RT of its query rows), from one sequence and head into the next: all CTAs have the same number of tiles, whatever the sequences' lengths.  A run that does
+// not have all tiles of its rows leaves the sums in the workspace, and pg_k_join joins them.  Rows above RT are other CTAs', which take the same tiles at the same time (L2).
+// Roles: soft-max (SG groups of four warps, on alternate tiles), output (four), and a warp each for copies (a page's K or V of a head is one run of bytes), MMAs, scales and live slots, and queries.
 #pragma once
 #include "ps_page.cuh"
+
+#define PG_TILE 128
+#define PG_STAGES 8         // at most, of K's ring and of V's
+#define PG_LANES 512        // runs of row tiles at most: 256 tokens of 32 heads, 16 rows a tile
+#define PG_META 8
+#define PG_LOW (-3.4028234663852886e38f) // below every score
+#define PG_ONE 8388600.f    // a weight of 1 in whole numbers: 2^23 less what an exponential may be above 1
+#define PG_Q_ONE 8355711.f  // 127 (2^16 + 2^8 + 1)
 
 struct PgAttnSeq {
     const int32_t *table;
     const uint8_t *hidden, *mask;
-    int n_kv, n_tok, tok0, unit0;
+    int n_kv, n_tok, tok0, tiles;
 };
 struct PgAttn {
     PgAttnSeq seq[PG_SEQS];
+    int tile0[PG_SEQS + 1];     // tiles of all heads before a sequence; those with more rows come first, so a run of row tiles takes the sequences up to some one
+    int lane_cta0[PG_LANES + 1], lane_tiles[PG_LANES];
     PgPool pool;
     const void *q;
     void *out;
-    int n_seqs, n_heads, R;
-    float scale; // times log2 e
+    float *part;                // [CTA][2][RT][hs], then [CTA][2][RT] pairs of reference and sum
+    int n_seqs, n_lanes, n_ctas, n_heads, R, stages, bf16, q_vec;
+    float scale;                // times log2 e
 };
 PS_D bool pg_sees(const PgAttnSeq &s, int t, int back) { return back < 0 || (s.mask ? s.mask[t * s.n_tok + back] != 0 : back <= t); }
+PS_HD int64_t pg_run(int64_t tiles, int n, int k) { return tiles * k / n; } // where run k of n begins
 
-// right and simple: sixteen query rows, 32 slots at a time, everything in 32 bits on the CUDA cores
-template <typename T>
-__global__ void __launch_bounds__(128) pg_k_attn(const __grid_constant__ PgAttn a) {
-    extern __shared__ float pg_sm[];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hs = a.pool.hs, g = blockIdx.y;
-    const PgAttnSeq &s = a.seq[blockIdx.x];
-    const int rows = s.n_tok * a.R, r0 = blockIdx.z * 16, B = a.pool.P / PG_BLOCK;
-    if (r0 >= rows) return;
-    const int kp = hs + 1;
-    float *sq = pg_sm, *sk = sq + 16 * hs, *sv = sk + 32 * kp, *sp = sv + hs * 33, *sc = sp + 16 * 33;
-    const T *q = static_cast<const T *>(a.q);
-    T *out = static_cast<T *>(a.out);
-    for (int i = tid; i < 16 * hs; i += 128) {
-        const int r = r0 + i / hs, t = r / a.R, h = g * a.R + r % a.R;
-        sq[i] = r < rows ? pg_num(q[((int64_t)(s.tok0 + t) * a.n_heads + h) * hs + i % hs]) * a.scale : 0.f;
-    }
-    float acc[2][16], m[4], l[4];
+template <int RT_, int MT_, int SG_> struct PgCfg {
+    static constexpr int RT = RT_, MT = MT_, SG = SG_;         // query rows; products of 128 channels; soft-max groups
+    static constexpr int N = (3 * RT + 15) / 16 * 16;          // columns of a product
+    static constexpr int QW = RT > 16 ? 4 : RT > 10 ? 2 : 1;   // warps that cut queries
+    static constexpr int W_OUT = 4 * SG, W_COPY = W_OUT + 4, W_MMA = W_COPY + 1, W_META = W_MMA + 1, W_Q = W_META + 1, THREADS = 32 * (W_Q + QW);
+    static constexpr int COLS = 2 * N * (1 + MT), TM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+    static constexpr int P_ROW = 8 * 144, P_BYTES = N / 8 * P_ROW; // weights: sixteen slots' core matrices 144 bytes apart, so that a warp's bytes meet other banks
+    static constexpr int CTAS = MT == 1 && TM <= 256 ? 2 : 1;
+    static int tail(int hs) { return 2 * P_BYTES + 2 * N * hs; } // shared memory behind the rings
+    static_assert(COLS <= 512, "tensor memory");
+};
+
+PS_D void pg_mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+PS_D void pg_tm_ld8(int (&v)[8], uint32_t at) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(at)
+                 : "memory");
+}
+PS_D float pg_ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+PS_D float pg_redux_max(float x) { // (no number counts as nothing)
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
+}
+PS_D int pg_order(float x) { // whole numbers in the order of the floats; its own inverse
+    const int b = __float_as_int(x);
+    return b ^ (b >> 31 & 0x7fffffff);
+}
+PS_D float pg_unorder(int b) { return __int_as_float(b ^ (b >> 31 & 0x7fffffff)); }
+// three digits' sums: the lower two are whole numbers of 31 bits together
+PS_D float pg_digits(int d0, int d1, int d2) { return fmaf((float)d2, 65536.f, (float)(d1 * 256 + d0)); }
+// the sums of RT rows, f(row, sum): eight rows at a time
+template <int RT, typename F> PS_D void pg_sums(uint32_t at, F f) {
+    if constexpr (RT % 8 == 0) {
 #pragma unroll
-    for (int r = 0; r < 16; r++) acc[0][r] = acc[1][r] = 0.f;
+        for (int c = 0; c < RT; c += 8) {
+            int a[8], b[8], d[8];
+            pg_tm_ld8(a, at + c);
+            pg_tm_ld8(b, at + RT + c);
+            pg_tm_ld8(d, at + 2 * RT + c);
+            ps_tc_ld_wait();
 #pragma unroll
-    for (int r = 0; r < 4; r++) { m[r] = -INFINITY; l[r] = 0.f; }
-    const int past = s.n_kv - s.n_tok;
-    for (int j0 = 0; j0 < s.n_kv; j0 += 32) {
-        __syncthreads();
-        for (int i = tid; i < 2 * 32 * hs; i += 128) {
-            const int kv = i / (32 * hs), e = i % (32 * hs), j = j0 + (kv ? e & 31 : e / hs), d = kv ? e >> 5 : e % hs;
-            float x = 0.f;
-            if (j < s.n_kv && !(s.hidden && s.hidden[j])) {
-                const int page = s.table[j >> a.pool.shift], o = j & (a.pool.P - 1);
-                if (a.pool.has(page)) {
-                    const int64_t at = a.pool.at(page, g, kv);
-                    x = (float)a.pool.codes[at * a.pool.page_codes() + (kv ? ((int64_t)(o / 16) * hs + d) * 16 + o % 16 : ((int64_t)(o / 8) * (hs / 16) + d / 16) * 128 + (o % 8) * 16 + d % 16)] *
-                        a.pool.scales[at * B + o / PG_BLOCK];
-                }
-            }
-            if (kv) sv[d * 33 + (j - j0)] = x;
-            else sk[(j - j0) * kp + d] = x;
+            for (int r = 0; r < 8; r++) f(c + r, pg_digits(a[r], b[r], d[r]));
         }
-        __syncthreads();
-        const int j = j0 + lane;
-        const bool in = j < s.n_kv && !(s.hidden && s.hidden[j]) && a.pool.has(s.table[j >> a.pool.shift]);
-        float z[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int d = 0; d < hs; d++) {
-            const float kv = sk[lane * kp + d];
+    } else {
+        constexpr int N = (3 * RT + 7) / 8;
+        int v[N][8];
 #pragma unroll
-            for (int r = 0; r < 4; r++) z[r] = fmaf(sq[(warp * 4 + r) * hs + d], kv, z[r]);
-        }
+        for (int c = 0; c < N; c++) pg_tm_ld8(v[c], at + 8 * c);
+        ps_tc_ld_wait();
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int row = r0 + warp * 4 + r;
-            if (!in || row >= rows || !pg_sees(s, row / a.R, j - past)) z[r] = -INFINITY;
-            float mx = z[r];
-#pragma unroll
-            for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            const float mn = fmaxf(m[r], mx), ref = mn == -INFINITY ? 0.f : mn, f = exp2f(m[r] - ref), p = exp2f(z[r] - ref);
-            float sum = p;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            l[r] = l[r] * f + sum;
-            m[r] = mn;
-            sp[(warp * 4 + r) * 33 + lane] = p;
-            if (lane == 0) sc[warp * 4 + r] = f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-            const int d = tid + 128 * c;
-            if (d >= hs) break;
-#pragma unroll
-            for (int r = 0; r < 16; r++) acc[c][r] *= sc[r];
-            for (int jj = 0; jj < 32; jj++) {
-                const float v = sv[d * 33 + jj];
-#pragma unroll
-                for (int r = 0; r < 16; r++) acc[c][r] = fmaf(sp[r * 33 + jj], v, acc[c][r]);
-            }
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < 4; r++)
-        if (lane == 0) sc[warp * 4 + r] = l[r] == 0.f ? 0.f : 1.f / l[r];
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < 2; c++) {
-        const int d = tid + 128 * c;
-        if (d >= hs) break;
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-            const int row = r0 + r;
-            if (row >= rows) break;
-            out[((int64_t)(s.tok0 + row / a.R) * a.n_heads + g * a.R + row % a.R) * hs + d] = pg_to<T>(acc[c][r] * sc[r]);
-        }
+        for (int r = 0; r < RT; r++) f(r, pg_digits(v[r / 8][r % 8], v[(RT + r) / 8][(RT + r) % 8], v[(2 * RT + r) / 8][(2 * RT + r) % 8]));
     }
 }
-inline size_t pg_attn_smem(int hs) { return 4 * ((size_t)16 * hs + 32 * (hs + 1) + (size_t)hs * 33 + 16 * 33 + 16); }
+
+// A CTA's way through its tiles: runs of one sequence and head
+struct PgSeg { int s, g, t0, t1; };
+struct PgWalk {
+    const PgAttn &a;
+    int s, u, left; // u: tile within the sequence's heads
+    PS_D PgWalk(const PgAttn &a_, int lane) : a(a_) {
+        const int k = blockIdx.x - a.lane_cta0[lane], n = a.lane_cta0[lane + 1] - a.lane_cta0[lane];
+        const int x = (int)pg_run(a.lane_tiles[lane], n, k);
+        left = (int)pg_run(a.lane_tiles[lane], n, k + 1) - x;
+        int lo = 0, hi = a.n_seqs - 1; // the last sequence that begins at or before x
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (a.tile0[mid] <= x) lo = mid;
+            else hi = mid - 1;
+        }
+        s = lo;
+        u = x - a.tile0[s];
+    }
+    PS_D bool next(PgSeg &o) {
+        if (left <= 0) return false;
+        const int tiles = a.seq[s].tiles;
+        o.s = s; o.g = u / tiles; o.t0 = u - o.g * tiles;
+        o.t1 = min(tiles, o.t0 + left);
+        left -= o.t1 - o.t0;
+        u += o.t1 - o.t0;
+        if (u == tiles * a.pool.G) { u = 0; s++; }
+        return true;
+    }
+};
+
+struct alignas(16) PgMeta { // of a tile: by blocks of sixteen slots
+    float ks[8], vq[8];     // K's scale; V's over the tile's largest, times PG_ONE
+    uint32_t live[4];       // slots that are filled, not hidden, and of a page
+    float vmax;             // V's largest scale over PG_ONE
+};
+struct PgRing { // of a number known at launch: index and the parity of the round
+    int n, i = 0;
+    uint32_t round = 0;
+    PS_D PgRing(int n_) : n(n_) {}
+    PS_D void step() {
+        if (++i == n) { i = 0; round ^= 1; }
+    }
+};
+
+template <int RT, int MT, int SG>
+__global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>::CTAS) pg_k_attn(const __grid_constant__ PgAttn a) {
+    using C = PgCfg<RT, MT, SG>;
+    constexpr int N = C::N;
+    extern __shared__ __align__(128) uint8_t pg_raw[];
+    __shared__ __align__(8) uint64_t k_full[PG_STAGES], v_full[PG_STAGES], k_free[PG_STAGES], v_free[PG_STAGES], s_full[2], s_free[2], p_full[2], o_full[2], o_free[2], q_full[2], fin[2], fin_free[2],
+        meta_full[PG_META], meta_free[PG_META], done;
+    __shared__ PgMeta s_meta[PG_META];
+    __shared__ int s_ref[SG][4][RT];                                    // largest score / row factor so far, in order of whole numbers
+    __shared__ __align__(16) float s_row[SG * 4 + 4][2][(RT + 3) / 4 * 4]; // a warp's numbers of the rows
+    __shared__ float s_qs[2][RT], s_m[4][RT], s_vm[4], s_l[2][SG * 4][RT], s_mend[2][SG][RT];
+    __shared__ uint32_t s_tmem;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, D = a.pool.hs, stage = PG_TILE * D;
+    // shared memory: K's ring, V's ring, weights, queries (a product of 128 channels of fewer reads behind its stage, never behind the queries)
+    uint8_t *sm_k = reinterpret_cast<uint8_t *>(((uintptr_t)pg_raw + 127) & ~(uintptr_t)127), *sm_v = sm_k + a.stages * stage, *sm_p = sm_v + a.stages * stage, *sm_q = sm_p + 2 * C::P_BYTES;
+    int rt = 0; // row tile
+    while (rt + 1 < a.n_lanes && (int)blockIdx.x >= a.lane_cta0[rt + 1]) rt++;
+    const int r0 = rt * RT;
+
+    if (tid == 0) {
+        for (int b = 0; b < PG_STAGES; b++) { ps_mbar_init(&k_full[b], 1); ps_mbar_init(&v_full[b], 1); ps_mbar_init(&k_free[b], 1); ps_mbar_init(&v_free[b], 1); }
+        for (int b = 0; b < 2; b++) {
+            ps_mbar_init(&s_full[b], 1); ps_mbar_init(&s_free[b], 4); ps_mbar_init(&p_full[b], 4); ps_mbar_init(&o_full[b], 1); ps_mbar_init(&o_free[b], 4);
+            ps_mbar_init(&q_full[b], C::QW); ps_mbar_init(&fin[b], 4 * SG); ps_mbar_init(&fin_free[b], 4);
+        }
+        for (int b = 0; b < PG_META; b++) { ps_mbar_init(&meta_full[b], 1); ps_mbar_init(&meta_free[b], 4); }
+        ps_mbar_init(&done, 1);
+        ps_fence_barrier_init();
+    }
+    if (warp == C::W_MMA) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ps_smem_u32(&s_tmem)), "n"(C::TM) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    ps_tc_fence_before();
+    __syncthreads();
+    ps_tc_fence_after();
+    const uint32_t tm = __shfl_sync(0xffffffffu, s_tmem, 0), tm_o = tm + 2 * N;
+    PgWalk walk(a, rt);
+    PgSeg sg;
+    bool ok = true;
+    // i counts the CTA's tiles, n its runs.  Whoever gives up a wait leaves his loops; the others' waits give up after him
+    auto wait = [&](uint64_t *bar, uint32_t parity, int site) {
+        if (ok && !ps_tc_wait_warp(bar, parity)) { *a.pool.err = site; ok = false; }
+        return ok;
+    };
+
+    if (warp == C::W_COPY) {
+        // ===== copies: a lane a page
+        PgRing ring(a.stages);
+        const int pages = PG_TILE >> a.pool.shift, bytes = a.pool.P * D;
+        int i = 0;
+        while (ok && walk.next(sg)) {
+            const PgAttnSeq &s = a.seq[sg.s];
+            const int last = (s.n_kv + a.pool.P - 1) >> a.pool.shift;
+            auto page_of = [&](int t) {
+                const int p = t * pages + lane;
+                return lane < pages && p < last && t < sg.t1 ? s.table[p] : -2;
+            };
+            int ahead = page_of(sg.t0);
+            for (int t = sg.t0; t < sg.t1; t++, i++) {
+                const int page = ahead;
+                ahead = page_of(t + 1);
+                const bool have = page != -2 && a.pool.has(page);
+                const uint32_t tx = __popc(__ballot_sync(0xffffffffu, have)) * (uint32_t)bytes;
+                const int8_t *src = have ? a.pool.codes + a.pool.at(page, sg.g, 0) * bytes : nullptr;
+                for (int v = 0; v < 2; v++) {
+                    uint64_t *full = (v ? v_full : k_full) + ring.i;
+                    if (i >= a.stages && !wait((v ? v_free : k_free) + ring.i, ring.round ^ 1, 11)) break;
+                    if (lane == 0) ps_mbar_expect_tx(full, tx);
+                    __syncwarp();
+                    if (have) ps_bulk_g2s((v ? sm_v : sm_k) + ring.i * stage + lane * bytes, src + (v ? bytes : 0), bytes, full);
+                }
+                if (!ok) break;
+                ring.step();
+            }
+        }
+        if (!ok) // (copies in flight end before the CTA does)
+            for (int b = 0; b < a.stages && b < i; b++) {
+                const uint32_t round = (uint32_t)((i - 1 - b) / a.stages) & 1;
+                ps_tc_wait_warp(&k_full[b], round, PS_COPY_CYCLES);
+                ps_tc_wait_warp(&v_full[b], round, PS_COPY_CYCLES);
+            }
+    } else if (warp == C::W_MMA) {
+        // ===== MMAs.  Scores of the next tile are asked for before the outputs of this one
+        const uint32_t id = (2u << 4) | (1u << 7) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(PG_TILE >> 4) << 24), id_s = id | (1u << 10); // whole numbers; K, V, queries signed, weights not
+        const uint64_t d_k = ps_tc_smem_desc(ps_smem_u32(sm_k), 128, 8 * D), d_v = ps_tc_smem_desc(ps_smem_u32(sm_v), 16 * D, 128), d_q = ps_tc_smem_desc(ps_smem_u32(sm_q), 128, 8 * D),
+                       d_p = ps_tc_smem_desc(ps_smem_u32(sm_p), 144, C::P_ROW);
+        PgRing rk(a.stages), rv(a.stages);
+        int n = 0, total = walk.left;
+        int s_left = 0; // tiles of the run whose scores are being asked for
+        auto scores = [&](int i) {
+            if (s_left == 0) {
+                walk.next(sg);
+                s_left = sg.t1 - sg.t0;
+                if (!wait(&q_full[n & 1], (n >> 1) & 1, 12)) return;
+                n++;
+            }
+            s_left--;
+            if (!wait(&k_full[rk.i], rk.round, 13) || (i >= 2 && !wait(&s_free[i & 1], ((i >> 1) - 1) & 1, 14))) return;
+            ps_tc_fence_after();
+            if (ps_elect_one()) {
+                const uint64_t x = d_k + (uint64_t)(rk.i * (stage >> 4)), y = d_q + (uint64_t)(((n - 1) & 1) * (N * D >> 4));
+                for (int c = 0; c < D / 32; c++) pg_mma_i8(tm + (i & 1) * N, x + 16 * c, y + 16 * c, id_s, c != 0);
+                ps_tc_commit(&k_free[rk.i]);
+                ps_tc_commit(&s_full[i & 1]);
+            }
+            __syncwarp();
+            rk.step();
+        };
+        if (total > 0) scores(0);
+        for (int i = 0; ok && i < total; i++) {
+            if (i + 1 < total) scores(i + 1);
+            if (!wait(&v_full[rv.i], rv.round, 15) || !wait(&p_full[i & 1], (i >> 1) & 1, 16) || (i >= 2 && !wait(&o_free[i & 1], ((i >> 1) - 1) & 1, 17))) break;
+            ps_tc_fence_after();
+            if (ps_elect_one()) {
+                const uint64_t x = d_v + (uint64_t)(rv.i * (stage >> 4)), y = d_p + (uint64_t)((i & 1) * (C::P_BYTES >> 4));
+#pragma unroll
+                for (int m = 0; m < MT; m++)
+#pragma unroll
+                    for (int c = 0; c < PG_TILE / 32; c++) pg_mma_i8(tm_o + (i & 1) * MT * N + m * N, x + 128 * m + 2 * D * c, y + 18 * c, id, c != 0);
+                ps_tc_commit(&v_free[rv.i]);
+                ps_tc_commit(&o_full[i & 1]);
+            }
+            __syncwarp();
+            rv.step();
+        }
+        if (ps_elect_one()) ps_tc_commit(&done); // MMAs in flight end before the tensor memory is given back
+        __syncwarp();
+        if (!ps_tc_wait_warp(&done, 0)) *a.pool.err = 18;
+    } else if (warp == C::W_META) {
+        // ===== scales and live slots, two tiles at a time: lanes 0-15 the first's blocks, K then V, 16-31 the second's
+        const int half = lane >> 4, b = lane & 7, kv = lane >> 3 & 1, B = a.pool.P / PG_BLOCK;
+        int i = 0;
+        while (ok && walk.next(sg)) {
+            const PgAttnSeq &s = a.seq[sg.s];
+            auto page_of = [&](int t) {
+                const int j = t * PG_TILE + b * PG_BLOCK;
+                return t < sg.t1 && j < s.n_kv ? s.table[j >> a.pool.shift] : -2;
+            };
+            int ahead = page_of(sg.t0 + half);
+            for (int t = sg.t0; ok && t < sg.t1; t += 2) {
+                const int page = ahead, j0 = (t + half) * PG_TILE;
+                ahead = page_of(t + 2 + half);
+                const bool have = page != -2 && (unsigned)page < (unsigned)a.pool.n_pages; // (the copies' warp reports)
+                float x = have ? a.pool.scales[a.pool.at(page, sg.g, kv) * B + ((j0 + b * PG_BLOCK) & (a.pool.P - 1)) / PG_BLOCK] : 0.f;
+                const unsigned has = __ballot_sync(0xffffffffu, have);
+                unsigned live[2][4];
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        const int j = (t + h) * PG_TILE + 32 * w + lane;
+                        live[h][w] = __ballot_sync(0xffffffffu, j < s.n_kv && (has >> (16 * h + 2 * w + (lane >> 4)) & 1) && !(s.hidden && s.hidden[min(j, s.n_kv - 1)]));
+                    }
+                const unsigned word = half ? (b < 2 ? live[1][0] : b < 4 ? live[1][1] : b < 6 ? live[1][2] : live[1][3]) : (b < 2 ? live[0][0] : b < 4 ? live[0][1] : b < 6 ? live[0][2] : live[0][3]);
+                if (!(word >> (b & 1 ? 16 : 0) & 0xffffu)) x = 0.f; // (a block without live slots may have any scale)
+                float top = kv ? x : 0.f;
+#pragma unroll
+                for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if (t + h >= sg.t1) break;
+                    PgMeta &m = s_meta[i % PG_META];
+                    if (i >= PG_META && !wait(&meta_free[i % PG_META], ((i / PG_META) - 1) & 1, 19)) break;
+                    if (half == h) {
+                        if (kv) m.vq[b] = top > 0.f ? x / top * PG_ONE : 0.f;
+                        else m.ks[b] = x;
+                        if ((lane & 15) < 4) m.live[lane & 3] = (lane & 3) == 0 ? live[h][0] : (lane & 3) == 1 ? live[h][1] : (lane & 3) == 2 ? live[h][2] : live[h][3];
+                        if ((lane & 15) == 8) m.vmax = top * (1.f / PG_ONE);
+                    }
+                    __syncwarp();
+                    if (lane == 0) ps_mbar_arrive(&meta_full[i % PG_META]);
+                    i++;
+                }
+            }
+        }
+    } else if (warp >= C::W_Q) {
+        // ===== queries into digits, a warp a row
+        int n = 0;
+        for (; ok && walk.next(sg); n++) {
+            const PgAttnSeq &s = a.seq[sg.s];
+            const int rows = s.n_tok * a.R;
+            if (n >= 2 && !wait(&fin[n & 1], ((n >> 1) - 1) & 1, 20)) break; // (all that read the queries of the run before last are through)
+            uint8_t *to = sm_q + (n & 1) * (N * D);
+            for (int r = warp - C::W_Q; r < RT; r += C::QW) {
+                const int row = r0 + r;
+                const int64_t at = row < rows ? ((int64_t)(s.tok0 + row / a.R) * a.n_heads + sg.g * a.R + row % a.R) * D : -1;
+                float x[2][4], top = 0.f;
+                bool none = false;
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const int d = c * 128 + lane * 4;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[c][e] = 0.f;
+                    if (d < D && at >= 0) {
+                        if (a.bf16) {
+                            const __nv_bfloat16 *p = static_cast<const __nv_bfloat16 *>(a.q) + at + d;
+                            if (a.q_vec) {
+                                const uint2 w = __ldg(reinterpret_cast<const uint2 *>(p));
+                                x[c][0] = __uint_as_float(w.x << 16); x[c][1] = __uint_as_float(w.x & 0xffff0000u); x[c][2] = __uint_as_float(w.y << 16); x[c][3] = __uint_as_float(w.y & 0xffff0000u);
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 4; e++) x[c][e] = __bfloat162float(p[e]);
+                            }
+                        } else {
+                            const float *p = static_cast<const float *>(a.q) + at + d;
+                            if (a.q_vec) {
+                                const float4 w = __ldg(reinterpret_cast<const float4 *>(p));
+                                x[c][0] = w.x; x[c][1] = w.y; x[c][2] = w.z; x[c][3] = w.w;
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 4; e++) x[c][e] = p[e];
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        top = fmaxf(top, fabsf(x[c][e]));
+                        none |= x[c][e] != x[c][e];
+                    }
+                }
+                top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+                none = __any_sync(0xffffffffu, none) || top == INFINITY;
+                // (numbers so small that the factor would leave float32's range are multiplied by 2^64 before, and all of them are as good as zeros in the end)
+                const float pre = top < 0x1p-100f ? 0x1p64f : 1.f, f = top > 0.f && !none ? PG_Q_ONE / (top * pre) : 0.f, sign = a.scale < 0.f ? -f : f;
+                if (lane == 0) s_qs[n & 1][r] = none ? NAN : top * fabsf(a.scale) * (1.f / PG_Q_ONE);
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const int d = c * 128 + lane * 4;
+                    if (d >= D) break;
+                    uint32_t w[3] = {0, 0, 0};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        int v = __float2int_rn(fminf(fmaxf((none ? 0.f : x[c][e]) * pre * sign, -PG_Q_ONE), PG_Q_ONE));
+#pragma unroll
+                        for (int k = 0; k < 3; k++) {
+                            const int digit = (int8_t)v;
+                            w[k] |= (uint32_t)(digit & 255) << (8 * e);
+                            v = (v - digit) >> 8;
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 3; k++) {
+                        const int col = k * RT + r;
+                        *reinterpret_cast<uint32_t *>(to + (col >> 3) * 8 * D + (d >> 4) * 128 + (col & 7) * 16 + (d & 15)) = w[k];
+                    }
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) ps_mbar_arrive(&q_full[n & 1]);
+        }
+    } else if (warp < C::W_OUT) {
+        // ===== soft-max: thread = slot.  A warp that gave up a wait goes on to the group's next barrier, which tells the others: nobody is left alone at one
+        const int group = warp >> 2, w = warp & 3, slot = w * 32 + lane;
+        const uint32_t lane_at = (uint32_t)(w * 32) << 16;
+        float *mine = s_row[warp][0], *factor = s_row[warp][1];
+        int i = 0, n = 0, turn = 0;
+        const int bar = SG == 1 ? 1 : 1 + group;
+        for (; walk.next(sg); n++) {
+            const PgAttnSeq &s = a.seq[sg.s];
+            const int rows = min(s.n_tok * a.R - r0, RT), past = s.n_kv - s.n_tok;
+            float l[RT], run = PG_LOW, qs = 0.f; // run, qs: row `lane`'s
+#pragma unroll
+            for (int r = 0; r < RT; r++) l[r] = 0.f;
+            ok = ps_bar_all(bar, 128, ok); // (a run begins: nobody of the group reads the last one's numbers any more)
+            if (!ok) break;
+            if (slot < RT)
+#pragma unroll
+                for (int b = 0; b < 4; b++) s_ref[group][b][slot] = pg_order(PG_LOW);
+            ps_bar_sync(bar, 128);
+            bool first = true;
+            for (int t = sg.t0; t < sg.t1; t++, i++) {
+                if (SG > 1 && (i & 1) != group) continue;
+                wait(&meta_full[i % PG_META], (i / PG_META) & 1, 21);
+                const PgMeta &m = s_meta[i % PG_META];
+                const float ks = m.ks[slot >> 4], vq = m.vq[slot >> 4], vmax = m.vmax;
+                const bool live = m.live[w] >> lane & 1;
+                __syncwarp();
+                if (lane == 0) ps_mbar_arrive(&meta_free[i % PG_META]);
+                // rows that see the slot
+                uint32_t see = live ? ~0u : 0u;
+                const int back = t * PG_TILE + slot - past;
+                if (live && back >= 0) {
+                    int tok = r0 / a.R, rest = r0 % a.R;
+                    see = 0;
+                    for (int r = 0; r < rows; tok++, rest = 0) {
+                        const int many = min(a.R - rest, rows - r);
+                        if (pg_sees(s, tok, back)) see |= (many == 32 ? ~0u : (1u << many) - 1) << r;
+                        r += many;
+                    }
+                }
+                const bool gaps = __any_sync(0xffffffffu, see != ~0u);
+                wait(&s_full[i & 1], (i >> 1) & 1, 22);
+                ps_tc_fence_after();
+                if (first) { // (they come with the first scores)
+                    qs = lane < RT ? s_qs[n & 1][lane] : 0.f;
+                    if (lane < RT) factor[lane] = qs;
+                    first = false;
+                }
+                float y[RT];
+                pg_sums<RT>(tm + (i & 1) * N + lane_at, [&](int r, float x) { y[r] = x * ks; });
+                ps_tc_fence_before();
+                __syncwarp();
+                if (lane == 0) ps_mbar_arrive(&s_free[i & 1]);
+                if (gaps) {
+#pragma unroll
+                    for (int r = 0; r < RT; r++)
+                        if (!(see >> r & 1)) y[r] = -INFINITY;
+                }
+                float top = PG_LOW; // row `lane`'s
+#pragma unroll
+                for (int r = 0; r < RT; r++) {
+                    const float x = pg_redux_max(y[r]);
+                    if (lane == r) top = fmaxf(top, x);
+                }
+                int *ref = s_ref[group][turn & 3];
+                if (lane < RT) atomicMax(&ref[lane], pg_order(fmaxf(run, top)));
+                ok = ps_bar_all(bar, 128, ok);
+                if (!ok) break;
+                const float was = run;
+                float now = PG_LOW, z = 0.f; // z: the reference, as the scores are: rounded up, so that no weight is above 1
+                if (lane < RT) {
+                    now = pg_unorder(ref[lane]);
+                    z = now == PG_LOW ? 0.f : __fmul_ru(now, qs);
+                    if (fabsf(z) == INFINITY) z = NAN;
+                }
+                turn++;
+                run = now;
+                if (i >= 2 && !wait(&o_full[i & 1], ((i >> 1) - 1) & 1, 23)) continue; // (the weights of tile i - 2 are used up, its outputs are taken)
+                if (w == 0 && lane < RT) {
+                    s_m[i & 3][lane] = now == PG_LOW ? PG_LOW : z;
+                    if (lane == 0) s_vm[i & 3] = vmax;
+                }
+                if (__any_sync(0xffffffffu, lane < RT && now > was)) { // sums so far follow their references
+                    if (lane < RT) mine[lane] = pg_ex2((was == PG_LOW ? PG_LOW : __fmul_ru(was, qs)) - z);
+                    __syncwarp();
+#pragma unroll
+                    for (int r = 0; r < RT; r++) l[r] *= mine[r];
+                    __syncwarp();
+                }
+                if (lane < RT) mine[lane] = -z;
+                __syncwarp();
+                uint8_t *to = sm_p + (i & 1) * C::P_BYTES + (slot >> 4) * 144 + (slot & 15);
+#pragma unroll
+                for (int r = 0; r < RT; r++) {
+                    float p = pg_ex2(fmaf(y[r], factor[r], mine[r]));
+                    if (gaps && !(see >> r & 1)) p = 0.f;
+                    l[r] += p;
+                    const uint32_t d = __float_as_uint(fmaf(p, vq, 8388608.f)); // 2^23 + the weight: its lower three bytes are the digits
+#pragma unroll
+                    for (int k = 0; k < 3; k++) {
+                        const int col = k * RT + r;
+                        to[(col >> 3) * C::P_ROW + (col & 7) * 16] = (uint8_t)(d >> (8 * k));
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) ps_mbar_arrive(&p_full[i & 1]);
+            }
+            // the run's sums
+            if (!ok || (n >= 2 && !wait(&fin_free[n & 1], ((n >> 1) - 1) & 1, 24))) continue;
+#pragma unroll
+            for (int r = 0; r < RT; r++) {
+                float x = l[r];
+#pragma unroll
+                for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+                if (lane == r) s_l[n & 1][warp][r] = x;
+            }
+            if (w == 0 && lane < RT) s_mend[n & 1][group][lane] = run == PG_LOW ? PG_LOW : __fmul_ru(run, qs);
+            __syncwarp();
+            if (lane == 0) ps_mbar_arrive(&fin[n & 1]);
+        }
+    } else {
+        // ===== output: thread = channel (of each product)
+        const int w = warp - C::W_OUT, ch = w * 32 + lane;
+        const uint32_t lane_at = (uint32_t)(w * 32) << 16;
+        float *mine = s_row[SG * 4 + w][0];
+        int i = 0, n = 0;
+        for (; ok && walk.next(sg); n++) {
+            const PgAttnSeq &s = a.seq[sg.s];
+            const int rows = min(s.n_tok * a.R - r0, RT);
+            float acc[MT][RT], M = PG_LOW;
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int r = 0; r < RT; r++) acc[m][r] = 0.f;
+            for (int t = sg.t0; t < sg.t1; t++, i++) {
+                if (!wait(&o_full[i & 1], (i >> 1) & 1, 25)) break;
+                ps_tc_fence_after();
+                float fo = 1.f, fn = 0.f;
+                if (lane < RT) {
+                    const float m = s_m[i & 3][lane], top = fmaxf(M, m);
+                    fo = pg_ex2(M - top);
+                    fn = pg_ex2(m - top) * s_vm[i & 3];
+                    M = top;
+                }
+                if (__any_sync(0xffffffffu, fo != 1.f)) {
+                    __syncwarp();
+                    if (lane < RT) mine[lane] = fo;
+                    __syncwarp();
+#pragma unroll
+                    for (int r = 0; r < RT; r++) {
+                        const float f = mine[r];
+#pragma unroll
+                        for (int m = 0; m < MT; m++) acc[m][r] *= f;
+                    }
+                }
+                __syncwarp();
+                if (lane < RT) mine[lane] = fn;
+                __syncwarp();
+#pragma unroll
+                for (int m = 0; m < MT; m++) pg_sums<RT>(tm_o + (i & 1) * MT * N + m * N + lane_at, [&](int r, float x) { acc[m][r] = fmaf(x, mine[r], acc[m][r]); });
+                ps_tc_fence_before();
+                __syncwarp();
+                if (lane == 0) ps_mbar_arrive(&o_free[i & 1]);
+            }
+            if (!ok || !wait(&fin[n & 1], (n >> 1) & 1, 26)) break;
+            float L = 0.f;
+            if (lane < RT) {
+#pragma unroll
+                for (int g = 0; g < SG; g++) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) sum += s_l[n & 1][g * 4 + k][lane];
+                    L = fmaf(sum, pg_ex2(s_mend[n & 1][g][lane] - M), L);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) ps_mbar_arrive(&fin_free[n & 1]);
+            const bool whole = sg.t0 == 0 && sg.t1 == s.tiles;
+            if (lane < RT) mine[lane] = whole ? (L == 0.f ? 0.f : 1.f / L) : 1.f;
+            __syncwarp();
+            const int64_t slot = (int64_t)blockIdx.x * 2 + (n > 0);
+            if (!whole && w == 0 && lane < RT) reinterpret_cast<float2 *>(a.part + (int64_t)a.n_ctas * 2 * RT * D)[slot * RT + lane] = make_float2(M, L);
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                const int d = m * 128 + ch;
+                if (d >= D) break;
+                if (whole) {
+                    int64_t at = ((int64_t)(s.tok0 + r0 / a.R) * a.n_heads + sg.g * a.R + r0 % a.R) * D + d;
+                    int rest = r0 % a.R;
+#pragma unroll
+                    for (int r = 0; r < RT; r++) {
+                        if (r >= rows) break;
+                        const float x = acc[m][r] * mine[r];
+                        if (a.bf16) static_cast<__nv_bfloat16 *>(a.out)[at] = __float2bfloat16_rn(x);
+                        else static_cast<float *>(a.out)[at] = x;
+                        at += D;
+                        if (++rest == a.R) { rest = 0; at += (int64_t)(a.n_heads - a.R) * D; }
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < RT; r++)
+                        if (r < rows) a.part[(slot * RT + r) * D + d] = acc[m][r];
+                }
+            }
+            __syncwarp();
+        }
+    }
+    ps_tc_fence_before();
+    __syncthreads();
+    ps_tc_fence_after();
+    if (warp == C::W_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(C::TM) : "memory");
+}
+
+// ---------------------------------------------------------------------------------------------------- joining the runs
+// A warp a row of kv head y of sequence z: the runs that share its tiles are found from where runs begin; its start overlaps the end of the kernel before
+__global__ void __launch_bounds__(256) pg_k_join(const __grid_constant__ PgAttn a, int RT) {
+    ps_grid_dep_wait();
+    const int lane = threadIdx.x & 31, D = a.pool.hs, g = blockIdx.y, si = blockIdx.z;
+    const PgAttnSeq &s = a.seq[si];
+    const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= s.n_tok * a.R) return;
+    const int rt = row / RT, n = a.lane_cta0[rt + 1] - a.lane_cta0[rt], T = a.lane_tiles[rt];
+    const int u0 = a.tile0[si] + g * s.tiles, u1 = u0 + s.tiles;
+    auto of = [&](int x) { // the run that has tile x
+        int k = (int)((int64_t)x * n / T);
+        while (k + 1 < n && pg_run(T, n, k + 1) <= x) k++;
+        while (k > 0 && pg_run(T, n, k) > x) k--;
+        return k;
+    };
+    const int k0 = of(u0), k1 = of(u1 - 1);
+    if (k0 == k1) return;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.part + (int64_t)a.n_ctas * 2 * RT * D);
+    auto place = [&](int k) { // a run that begins before the row's tiles has come to them later
+        return ((int64_t)(a.lane_cta0[rt] + k) * 2 + (pg_run(T, n, k) < u0)) * RT + row % RT;
+    };
+    float top = PG_LOW, l = 0.f, acc[8] = {};
+    for (int k = k0 + lane; k <= k1; k += 32) top = fmaxf(top, ml[place(k)].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int i0 = k0; i0 <= k1; i0 += 32) {
+        float f = 0.f;
+        int64_t at = 0;
+        if (i0 + lane <= k1) {
+            at = place(i0 + lane);
+            const float2 p = ml[at];
+            f = pg_ex2(p.x - top);
+            l = fmaf(p.y, f, l);
+        }
+        for (int i = 0; i < min(32, k1 + 1 - i0); i += 4) {
+            float v[4][8];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int64_t from = __shfl_sync(0xffffffffu, at, i + e);
+#pragma unroll
+                for (int c = 0; c < 8; c++)
+                    if (c * 32 < D && i0 + i + e <= k1) v[e][c] = a.part[from * D + c * 32 + lane];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float fe = __shfl_sync(0xffffffffu, f, i + e);
+#pragma unroll
+                for (int c = 0; c < 8; c++)
+                    if (c * 32 < D && i0 + i + e <= k1) acc[c] = fmaf(v[e][c], fe, acc[c]);
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int64_t to = ((int64_t)(s.tok0 + row / a.R) * a.n_heads + g * a.R + row % a.R) * D;
+#pragma unroll
+    for (int c = 0; c < 8; c++)
+        if (c * 32 < D) {
+            const float x = acc[c] * inv;
+            if (a.bf16) static_cast<__nv_bfloat16 *>(a.out)[to + c * 32 + lane] = __float2bfloat16_rn(x);
+            else static_cast<float *>(a.out)[to + c * 32 + lane] = x;
+        }
+}
