@@ -12,7 +12,7 @@
 //
 // A CTA takes a run of tiles (128 slots of one kv head and up to RT of its query rows), from one sequence and head into the next: all CTAs have the same number of tiles, whatever the sequences' lengths.  A run that does
 // not have all tiles of its rows leaves the sums in the workspace, and pg_k_join joins them.  Rows above RT are other CTAs', which take the same tiles at the same time (L2).
-// Roles: soft-max (SG groups of four warps, on alternate tiles), output (four), and a warp each for copies (a page's K or V of a head is one run of bytes), MMAs, scales and live slots, and queries.
+// Roles: soft-max (SG groups of four warps, on alternate tiles), output (four), and a warp each for copies (a page's K or V of a head is one run of bytes), the MMAs of either product, scales and live slots, and queries.
 #pragma once
 #include "ps_page.cuh"
 
@@ -47,7 +47,7 @@ template <int RT_, int MT_, int SG_> struct PgCfg {
     static constexpr int RT = RT_, MT = MT_, SG = SG_;         // query rows; products of 128 channels; soft-max groups
     static constexpr int N = (3 * RT + 15) / 16 * 16;          // columns of a product
     static constexpr int QW = RT > 16 ? 4 : RT > 10 ? 2 : 1;   // warps that cut queries
-    static constexpr int W_OUT = 4 * SG, W_COPY = W_OUT + 4, W_MMA = W_COPY + 1, W_META = W_MMA + 1, W_Q = W_META + 1, THREADS = 32 * (W_Q + QW);
+    static constexpr int W_OUT = 4 * SG, W_COPY = W_OUT + 4, W_MMA = W_COPY + 1, W_META = W_MMA + 2, W_Q = W_META + 1, THREADS = 32 * (W_Q + QW);
     static constexpr int COLS = 2 * N * (1 + MT), TM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
     static constexpr int P_ROW = 8 * 144, P_BYTES = N / 8 * P_ROW; // weights: sixteen slots' core matrices 144 bytes apart, so that a warp's bytes meet other banks
     static constexpr int CTAS = MT == 1 && TM <= 256 ? 2 : 1;
@@ -62,9 +62,10 @@ PS_D void pg_mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t 
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-PS_D void pg_tm_ld8(int (&v)[8], uint32_t at) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+PS_D void pg_tm_ld16(int (&v)[16], uint32_t at) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]),
+                   "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
                  : "r"(at)
                  : "memory");
 }
@@ -85,27 +86,38 @@ PS_D int pg_order(float x) { // whole numbers in the order of the floats; its ow
 PS_D float pg_unorder(int b) { return __int_as_float(b ^ (b >> 31 & 0x7fffffff)); }
 // three digits' sums: the lower two are whole numbers of 31 bits together
 PS_D float pg_digits(int d0, int d1, int d2) { return fmaf((float)d2, 65536.f, (float)(d1 * 256 + d0)); }
-// the sums of RT rows, f(row, sum): eight rows at a time
-template <int RT, typename F> PS_D void pg_sums(uint32_t at, F f) {
-    if constexpr (RT % 8 == 0) {
+// a number of each row, from shared memory
+template <int RT, typename F> PS_D void pg_rows(const float *x, F f) {
 #pragma unroll
-        for (int c = 0; c < RT; c += 8) {
-            int a[8], b[8], d[8];
-            pg_tm_ld8(a, at + c);
-            pg_tm_ld8(b, at + RT + c);
-            pg_tm_ld8(d, at + 2 * RT + c);
+    for (int c = 0; c < RT; c += 4) {
+        const float4 v = *reinterpret_cast<const float4 *>(x + c);
+        f(c, v.x);
+        if (c + 1 < RT) f(c + 1, v.y);
+        if (c + 2 < RT) f(c + 2, v.z);
+        if (c + 3 < RT) f(c + 3, v.w);
+    }
+}
+// the sums of RT rows, f(row, sum): sixteen rows at a time
+template <int RT, typename F> PS_D void pg_sums(uint32_t at, F f) {
+    if constexpr (RT % 16 == 0) {
+#pragma unroll
+        for (int c = 0; c < RT; c += 16) {
+            int a[16], b[16], d[16];
+            pg_tm_ld16(a, at + c);
+            pg_tm_ld16(b, at + RT + c);
+            pg_tm_ld16(d, at + 2 * RT + c);
             ps_tc_ld_wait();
 #pragma unroll
-            for (int r = 0; r < 8; r++) f(c + r, pg_digits(a[r], b[r], d[r]));
+            for (int r = 0; r < 16; r++) f(c + r, pg_digits(a[r], b[r], d[r]));
         }
     } else {
-        constexpr int N = (3 * RT + 7) / 8;
-        int v[N][8];
+        constexpr int N = (3 * RT + 15) / 16;
+        int v[N][16];
 #pragma unroll
-        for (int c = 0; c < N; c++) pg_tm_ld8(v[c], at + 8 * c);
+        for (int c = 0; c < N; c++) pg_tm_ld16(v[c], at + 16 * c);
         ps_tc_ld_wait();
 #pragma unroll
-        for (int r = 0; r < RT; r++) f(r, pg_digits(v[r / 8][r % 8], v[(RT + r) / 8][(RT + r) % 8], v[(2 * RT + r) / 8][(2 * RT + r) % 8]));
+        for (int r = 0; r < RT; r++) f(r, pg_digits(v[r / 16][r % 16], v[(RT + r) / 16][(RT + r) % 16], v[(2 * RT + r) / 16][(2 * RT + r) % 16]));
     }
 }
 
@@ -179,7 +191,7 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
             ps_mbar_init(&q_full[b], C::QW); ps_mbar_init(&fin[b], 4 * SG); ps_mbar_init(&fin_free[b], 4);
         }
         for (int b = 0; b < PG_META; b++) { ps_mbar_init(&meta_full[b], 1); ps_mbar_init(&meta_free[b], 4); }
-        ps_mbar_init(&done, 1);
+        ps_mbar_init(&done, 2);
         ps_fence_barrier_init();
     }
     if (warp == C::W_MMA) {
@@ -235,49 +247,43 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
                 ps_tc_wait_warp(&k_full[b], round, PS_COPY_CYCLES);
                 ps_tc_wait_warp(&v_full[b], round, PS_COPY_CYCLES);
             }
-    } else if (warp == C::W_MMA) {
-        // ===== MMAs.  Scores of the next tile are asked for before the outputs of this one
+    } else if (warp == C::W_MMA || warp == C::W_MMA + 1) {
+        // ===== MMAs: scores by one warp, outputs by another, so that neither's waits hold up the other's
         const uint32_t id = (2u << 4) | (1u << 7) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(PG_TILE >> 4) << 24), id_s = id | (1u << 10); // whole numbers; K, V, queries signed, weights not
         const uint64_t d_k = ps_tc_smem_desc(ps_smem_u32(sm_k), 128, 8 * D), d_v = ps_tc_smem_desc(ps_smem_u32(sm_v), 16 * D, 128), d_q = ps_tc_smem_desc(ps_smem_u32(sm_q), 128, 8 * D),
                        d_p = ps_tc_smem_desc(ps_smem_u32(sm_p), 144, C::P_ROW);
-        PgRing rk(a.stages), rv(a.stages);
-        int n = 0, total = walk.left;
-        int s_left = 0; // tiles of the run whose scores are being asked for
-        auto scores = [&](int i) {
-            if (s_left == 0) {
-                walk.next(sg);
-                s_left = sg.t1 - sg.t0;
-                if (!wait(&q_full[n & 1], (n >> 1) & 1, 12)) return;
-                n++;
-            }
-            s_left--;
-            if (!wait(&k_full[rk.i], rk.round, 13) || (i >= 2 && !wait(&s_free[i & 1], ((i >> 1) - 1) & 1, 14))) return;
-            ps_tc_fence_after();
-            if (ps_elect_one()) {
-                const uint64_t x = d_k + (uint64_t)(rk.i * (stage >> 4)), y = d_q + (uint64_t)(((n - 1) & 1) * (N * D >> 4));
-                for (int c = 0; c < D / 32; c++) pg_mma_i8(tm + (i & 1) * N, x + 16 * c, y + 16 * c, id_s, c != 0);
-                ps_tc_commit(&k_free[rk.i]);
-                ps_tc_commit(&s_full[i & 1]);
-            }
-            __syncwarp();
-            rk.step();
-        };
-        if (total > 0) scores(0);
-        for (int i = 0; ok && i < total; i++) {
-            if (i + 1 < total) scores(i + 1);
-            if (!wait(&v_full[rv.i], rv.round, 15) || !wait(&p_full[i & 1], (i >> 1) & 1, 16) || (i >= 2 && !wait(&o_free[i & 1], ((i >> 1) - 1) & 1, 17))) break;
-            ps_tc_fence_after();
-            if (ps_elect_one()) {
-                const uint64_t x = d_v + (uint64_t)(rv.i * (stage >> 4)), y = d_p + (uint64_t)((i & 1) * (C::P_BYTES >> 4));
+        const bool pv = warp == C::W_MMA + 1;
+        PgRing ring(a.stages);
+        int i = 0, n = 0;
+        for (; ok && walk.next(sg); n++) {
+            if (!pv && !wait(&q_full[n & 1], (n >> 1) & 1, 12)) break;
+            const uint64_t y0 = pv ? d_p : d_q + (uint64_t)((n & 1) * (N * D >> 4));
+            for (int t = sg.t0; t < sg.t1; t++, i++) {
+                const int b = i & 1;
+                const uint32_t before = ((i >> 1) - 1) & 1; // (of tile i - 2)
+                if (pv) {
+                    if (!wait(&v_full[ring.i], ring.round, 15) || !wait(&p_full[b], (i >> 1) & 1, 16) || (i >= 2 && !wait(&o_free[b], before, 17))) break;
+                } else if (!wait(&k_full[ring.i], ring.round, 13) || (i >= 2 && !wait(&s_free[b], before, 14))) break;
+                ps_tc_fence_after();
+                if (ps_elect_one()) {
+                    if (pv) {
+                        const uint64_t x = d_v + (uint64_t)(ring.i * (stage >> 4)), y = y0 + (uint64_t)(b * (C::P_BYTES >> 4));
 #pragma unroll
-                for (int m = 0; m < MT; m++)
+                        for (int m = 0; m < MT; m++)
 #pragma unroll
-                    for (int c = 0; c < PG_TILE / 32; c++) pg_mma_i8(tm_o + (i & 1) * MT * N + m * N, x + 128 * m + 2 * D * c, y + 18 * c, id, c != 0);
-                ps_tc_commit(&v_free[rv.i]);
-                ps_tc_commit(&o_full[i & 1]);
+                            for (int c = 0; c < PG_TILE / 32; c++) pg_mma_i8(tm_o + b * MT * N + m * N, x + 128 * m + 2 * D * c, y + 18 * c, id, c != 0);
+                        ps_tc_commit(&v_free[ring.i]);
+                        ps_tc_commit(&o_full[b]);
+                    } else {
+                        const uint64_t x = d_k + (uint64_t)(ring.i * (stage >> 4));
+                        for (int c = 0; c < D / 32; c++) pg_mma_i8(tm + b * N, x + 16 * c, y0 + 16 * c, id_s, c != 0);
+                        ps_tc_commit(&k_free[ring.i]);
+                        ps_tc_commit(&s_full[b]);
+                    }
+                }
+                __syncwarp();
+                ring.step();
             }
-            __syncwarp();
-            rv.step();
         }
         if (ps_elect_one()) ps_tc_commit(&done); // MMAs in flight end before the tensor memory is given back
         __syncwarp();
@@ -450,7 +456,7 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
                 ps_tc_fence_after();
                 if (first) { // (they come with the first scores)
                     qs = lane < RT ? s_qs[n & 1][lane] : 0.f;
-                    if (lane < RT) factor[lane] = qs;
+                    if (lane < RT) factor[lane] = fmaxf(qs, 0x1p-126f); // (above zero, and a number: -inf times it is -inf)
                     first = false;
                 }
                 float y[RT];
@@ -477,8 +483,8 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
                 float now = PG_LOW, z = 0.f; // z: the reference, as the scores are: rounded up, so that no weight is above 1
                 if (lane < RT) {
                     now = pg_unorder(ref[lane]);
-                    z = now == PG_LOW ? 0.f : __fmul_ru(now, qs);
-                    if (fabsf(z) == INFINITY) z = NAN;
+                    z = now == PG_LOW ? 0.f : __fmul_ru(now, fmaxf(qs, 0x1p-126f));
+                    if (fabsf(z) == INFINITY || (now != PG_LOW && qs != qs)) z = NAN;
                 }
                 turn++;
                 run = now;
@@ -488,26 +494,39 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
                     if (lane == 0) s_vm[i & 3] = vmax;
                 }
                 if (__any_sync(0xffffffffu, lane < RT && now > was)) { // sums so far follow their references
-                    if (lane < RT) mine[lane] = pg_ex2((was == PG_LOW ? PG_LOW : __fmul_ru(was, qs)) - z);
+                    if (lane < RT) mine[lane] = pg_ex2((was == PG_LOW ? PG_LOW : __fmul_ru(was, fmaxf(qs, 0x1p-126f))) - z);
                     __syncwarp();
-#pragma unroll
-                    for (int r = 0; r < RT; r++) l[r] *= mine[r];
+                    pg_rows<RT>(mine, [&](int r, float f) { l[r] *= f; });
                     __syncwarp();
                 }
                 if (lane < RT) mine[lane] = -z;
                 __syncwarp();
-                uint8_t *to = sm_p + (i & 1) * C::P_BYTES + (slot >> 4) * 144 + (slot & 15);
+                const uint32_t to = ps_smem_u32(sm_p) + (i & 1) * C::P_BYTES + (slot >> 4) * 144 + (slot & 15);
 #pragma unroll
-                for (int r = 0; r < RT; r++) {
-                    float p = pg_ex2(fmaf(y[r], factor[r], mine[r]));
-                    if (gaps && !(see >> r & 1)) p = 0.f;
-                    l[r] += p;
-                    const uint32_t d = __float_as_uint(fmaf(p, vq, 8388608.f)); // 2^23 + the weight: its lower three bytes are the digits
+                for (int c = 0; c < RT; c += 8) { // (the numbers of eight rows come before the bytes go: the compiler keeps loads behind stores)
+                    constexpr int W = RT < 8 ? RT : 8;
+                    float f[8], zs[8];
 #pragma unroll
-                    for (int k = 0; k < 3; k++) {
-                        const int col = k * RT + r;
-                        to[(col >> 3) * C::P_ROW + (col & 7) * 16] = (uint8_t)(d >> (8 * k));
+                    for (int e = 0; e < W && c + e < RT; e += 4) {
+                        *reinterpret_cast<float4 *>(f + e) = *reinterpret_cast<const float4 *>(factor + c + e);
+                        *reinterpret_cast<float4 *>(zs + e) = *reinterpret_cast<const float4 *>(mine + c + e);
                     }
+                    uint32_t d[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (c + e < RT) {
+                            const float p = pg_ex2(fmaf(y[c + e], f[e], zs[e])); // (a slot that is not seen: -inf)
+                            l[c + e] += p;
+                            d[e] = __float_as_uint(fmaf(p, vq, 8388608.f)); // 2^23 + the weight: its lower three bytes are the digits
+                        }
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (c + e < RT)
+#pragma unroll
+                            for (int k = 0; k < 3; k++) {
+                                const int col = k * RT + c + e;
+                                asm volatile("st.shared.u8 [%0], %1;" ::"r"(to + (col >> 3) * C::P_ROW + (col & 7) * 16), "r"(d[e] >> (8 * k)));
+                            }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
@@ -522,7 +541,7 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
                 for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
                 if (lane == r) s_l[n & 1][warp][r] = x;
             }
-            if (w == 0 && lane < RT) s_mend[n & 1][group][lane] = run == PG_LOW ? PG_LOW : __fmul_ru(run, qs);
+            if (w == 0 && lane < RT) s_mend[n & 1][group][lane] = run == PG_LOW ? PG_LOW : __fmul_ru(run, fmaxf(qs, 0x1p-126f));
             __syncwarp();
             if (lane == 0) ps_mbar_arrive(&fin[n & 1]);
         }
@@ -554,18 +573,18 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
                     __syncwarp();
                     if (lane < RT) mine[lane] = fo;
                     __syncwarp();
-#pragma unroll
-                    for (int r = 0; r < RT; r++) {
-                        const float f = mine[r];
+                    pg_rows<RT>(mine, [&](int r, float f) {
 #pragma unroll
                         for (int m = 0; m < MT; m++) acc[m][r] *= f;
-                    }
+                    });
                 }
                 __syncwarp();
                 if (lane < RT) mine[lane] = fn;
                 __syncwarp();
+                float f[(RT + 3) / 4 * 4];
+                pg_rows<RT>(mine, [&](int r, float v) { f[r] = v; });
 #pragma unroll
-                for (int m = 0; m < MT; m++) pg_sums<RT>(tm_o + (i & 1) * MT * N + m * N + lane_at, [&](int r, float x) { acc[m][r] = fmaf(x, mine[r], acc[m][r]); });
+                for (int m = 0; m < MT; m++) pg_sums<RT>(tm_o + (i & 1) * MT * N + m * N + lane_at, [&](int r, float x) { acc[m][r] = fmaf(x, f[r], acc[m][r]); });
                 ps_tc_fence_before();
                 __syncwarp();
                 if (lane == 0) ps_mbar_arrive(&o_free[i & 1]);
