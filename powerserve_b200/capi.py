@@ -535,7 +535,8 @@ class CudaBackend:
         torch = sys.modules.get("torch")
         if torch is None or not torch.cuda.is_initialized():
             return self._ck(call(self.h, *args))
-        stream = torch.cuda.current_stream(self.device).cuda_stream
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # (without making a Stream object, which takes longer than the rest of this)
+        stream = raw(self.device) if raw is not None else torch.cuda.current_stream(self.device).cuda_stream
         if stream == self.stream:
             return self._ck(call(self.h, *args))
         self._ck(self.L.ps_cuda_stream_enter(self.h, stream))
@@ -597,31 +598,30 @@ class CudaBackend:
 
     def _paged_rows(self, what: str, call, cache, layer, k, v, seqs, io_type):
         at = self._records(what, seqs, PAGED_SEQ, "PAGED_SEQ")
-        n = sum(seqs["n_tok"].ravel().tolist()) * cache.n_kv_heads * cache.head_size
-        rows = [self._rows(f"{what}: {w}", a, n, io_type) for w, a in (("k", k), ("v", v))]
-        types = {t for a, (_, t) in zip((k, v), rows) if a is not None}
-        if len(types) > 1:
+        n = int(seqs["n_tok"].sum()) * cache.n_kv_heads * cache.head_size
+        (k_at, t), (v_at, t_v) = self._rows(what, k, n, io_type), self._rows(what, v, n, io_type)
+        if t != t_v and k is not None and v is not None:
             raise PsCudaError(f"{what}: k and v of two types")
-        self._in_turn(call, cache.at, layer, rows[0][0], rows[1][0], types.pop() if types else F32, at, seqs.size)
+        self._in_turn(call, cache.at, layer, k_at, v_at, t_v if k is None else t, at, seqs.size)
 
     def paged_store(self, cache, layer: int, k, v, seqs: np.ndarray, io_type: Optional[int] = None):
         """rows of K and V into the last n_tok slots of each sequence"""
-        self._paged_rows("paged_store", self.L.ps_cuda_paged_store, cache, layer, k, v, seqs, io_type)
+        self._paged_rows("paged_store: rows", self.L.ps_cuda_paged_store, cache, layer, k, v, seqs, io_type)
 
     def paged_load(self, cache, layer: int, k, v, seqs: np.ndarray, io_type: Optional[int] = None):
         """the numbers that the last n_tok slots of each sequence stand for, as rows (k or v: None if not asked for)"""
-        self._paged_rows("paged_load", self.L.ps_cuda_paged_load, cache, layer, k, v, seqs, io_type)
+        self._paged_rows("paged_load: rows", self.L.ps_cuda_paged_load, cache, layer, k, v, seqs, io_type)
 
     def paged_attn(self, cache, layer: int, out, q, seqs: np.ndarray, n_heads: int, scale: float, tree_mask=None, io_type: Optional[int] = None):
         """attention of a step's tokens over the sequences' pages"""
         at = self._records("paged_attn", seqs, PAGED_SEQ, "PAGED_SEQ")
-        tok = seqs["n_tok"].ravel().tolist()
-        n = sum(tok) * max(n_heads, 0) * cache.head_size
+        tok = seqs["n_tok"]
+        n = int(tok.sum()) * max(n_heads, 0) * cache.head_size
         q_at, t = self._rows("paged_attn: q", q, n, io_type)
         out_at, t_out = self._rows("paged_attn: out", out, n, io_type)
         if t != t_out:
             raise PsCudaError("paged_attn: q and out of two types")
-        mask = None if tree_mask is None else _dev("paged_attn: tree_mask", tree_mask, self.device, sum([t * t for t in tok]), ["uint8", "bool", "int8"])
+        mask = None if tree_mask is None else _dev("paged_attn: tree_mask", tree_mask, self.device, int((tok.astype(np.int64) ** 2).sum()), ["uint8", "bool", "int8"])
         self._in_turn(self.L.ps_cuda_paged_attn, cache.at, layer, out_at, q_at, t, at, seqs.size, n_heads, mask, scale)
 
     def paged_edit(self, cache, edits: np.ndarray, held=None):

@@ -73,7 +73,7 @@ int check_seqs(PsServeCall *c, const char *what, const ps_cuda_pages *p, int lay
         if (s.n_table < pages_of(s.n_kv, p->page_tokens)) return fail(c, PS_CUDA_ERR_INVALID, "%s: sequence %d holds %d slots, its table has %d pages", what, i, s.n_kv, s.n_table);
         tokens += s.n_tok;
     }
-    if (tokens > INT32_MAX / 1024) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "%s: %lld tokens in one call", what, (long long)tokens);
+    if (tokens > INT32_MAX / 2048) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "%s: %lld tokens in one call", what, (long long)tokens);
     return 0;
 }
 
@@ -115,14 +115,13 @@ int ps_serve_paged_rows(PsServeCall *c, bool store, const ps_cuda_pages *pages, 
             tok0 += s.n_tok;
         }
         if (!a.n_seqs) break;
-        a.blocks = (int)blocks; // (tokens fit an int's thousandth part)
-        const unsigned grid = (unsigned)((blocks * 2 * pages->n_kv_heads + PG_ROW_WARPS - 1) / PG_ROW_WARPS);
-        if (store)
-            by_items(pages->head_size, [&](auto items) {
-                constexpr int I = decltype(items)::value;
-                if (es == 4) pg_k_store<float, I><<<grid, 32 * PG_ROW_WARPS, 0, c->stream>>>(a);
-                else pg_k_store<__nv_bfloat16, I><<<grid, 32 * PG_ROW_WARPS, 0, c->stream>>>(a);
-            });
+        a.blocks = (int)blocks; // (tokens fit an int's 2 048th part, so all that follows fits 32 bits)
+        const int64_t tasks = blocks * 2 * pages->n_kv_heads;
+        const unsigned grid = (unsigned)((tasks + PG_ROW_WARPS - 1) / PG_ROW_WARPS);
+        if (store) {
+            if (es == 4) pg_k_store<float><<<(unsigned)tasks, pages->head_size, 0, c->stream>>>(a);
+            else pg_k_store<__nv_bfloat16><<<(unsigned)tasks, pages->head_size, 0, c->stream>>>(a);
+        }
         else if (es == 4) pg_k_load<float><<<grid, 32 * PG_ROW_WARPS, 0, c->stream>>>(a);
         else pg_k_load<__nv_bfloat16><<<grid, 32 * PG_ROW_WARPS, 0, c->stream>>>(a);
         PG_LAUNCHED(what);
@@ -181,10 +180,16 @@ int ps_serve_paged_attn(PsServeCall *c, const ps_cuda_pages *pages, int layer, v
                 total += a.lane_tiles[z];
             }
             const int slots = c->n_sm * C::CTAS;
+            // Nothing to join where no sequence has many more tiles than a fair share: the kernel that joins takes as long as four tiles
+            int64_t units = 0;
+            int longest = 0;
+            for (int k = 0; k < n; k++) { units += (int64_t)G * row_tiles(all[k]); longest = std::max(longest, all[k].tiles); }
+            a.whole = units <= slots && longest <= total / slots + 4;
             a.n_ctas = 0;
-            for (int z = 0; z < a.n_lanes; z++) {
+            for (int z = 0, k = n; z < a.n_lanes; z++) {
                 a.lane_cta0[z] = a.n_ctas;
-                a.n_ctas += (int)std::max<int64_t>(1, std::min<int64_t>(a.lane_tiles[z], (int64_t)slots * a.lane_tiles[z] / total));
+                while (row_tiles(all[k - 1]) <= z) k--;
+                a.n_ctas += a.whole ? k * G : (int)std::max<int64_t>(1, std::min<int64_t>(a.lane_tiles[z], (int64_t)slots * a.lane_tiles[z] / total));
             }
             a.lane_cta0[a.n_lanes] = a.n_ctas;
             // stages: what the CTAs' shares of shared memory hold
@@ -199,10 +204,10 @@ int ps_serve_paged_attn(PsServeCall *c, const ps_cuda_pages *pages, int layer, v
             PG_LAUNCHED("paged_attn");
             // whether runs begin where rows' tiles do
             bool split = false;
-            for (int z = 0; z < a.n_lanes && !split; z++) {
+            for (int z = 0; z < a.n_lanes && !split && !a.whole; z++) {
                 const int m = a.lane_cta0[z + 1] - a.lane_cta0[z];
                 for (int k = 1, s = 0; k < m && !split; k++) {
-                    const int x = (int)pg_run(a.lane_tiles[z], m, k);
+                    const int x = pg_run(a.lane_tiles[z], m, k);
                     while (a.tile0[s + 1] <= x) s++;
                     split = (x - a.tile0[s]) % all[s].tiles != 0;
                 }
@@ -297,11 +302,22 @@ int ps_serve_paged_compact(PsServeCall *c, const ps_cuda_pages *pages, const ps_
     }
     const int heads = 2 * pages->n_kv_heads * pages->n_layers;
     for (int i = 0; i < n;) {
-        int k = 0;
-        for (; i < n && k < PG_SEQS; i++)
-            if (moves[i].n_keep) a.op[k++] = PgMoveOp{moves[i].table, moves[i].keep, moves[i].n_keep_dev, moves[i].first, moves[i].n_kv, moves[i].n_keep};
+        int k = 0, most = 0;
+        for (; i < n && k < PG_SEQS; i++) {
+            const ps_cuda_page_move &m = moves[i];
+            if (!m.n_keep) continue;
+            a.op[k++] = PgMoveOp{m.table, m.keep, m.n_keep_dev, m.first, m.n_kv, m.n_keep};
+            most = std::max(most, (m.first + m.n_keep - 1) / PG_BLOCK - m.first / PG_BLOCK + 1);
+        }
         if (!k) break;
-        by_items(pages->head_size, [&](auto items) { pg_k_compact<decltype(items)::value><<<dim3(heads, k), 256, 0, c->stream>>>(a); });
+        // few blocks: a warp a head, one block after the other; many: a CTA a head, a block a warp
+        const bool few = most <= PG_MOVE_FEW;
+        a.heads = heads;
+        by_items(pages->head_size, [&](auto items) {
+            constexpr int I = decltype(items)::value;
+            if (few) pg_k_compact<I, false><<<dim3((heads + PG_MOVE_WARPS(false) - 1) / PG_MOVE_WARPS(false), k), 32 * PG_MOVE_WARPS(false), 0, c->stream>>>(a);
+            else pg_k_compact<I, true><<<dim3(heads, k), 32 * PG_MOVE_WARPS(true), 0, c->stream>>>(a);
+        });
         PG_LAUNCHED("paged_compact");
     }
     return 0;

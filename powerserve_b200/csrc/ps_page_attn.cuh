@@ -38,10 +38,11 @@ struct PgAttn {
     void *out;
     float *part;                // [CTA][2][RT][hs], then [CTA][2][RT] pairs of reference and sum
     int n_seqs, n_lanes, n_ctas, n_heads, R, stages, bf16, q_vec;
+    int whole;                  // a CTA takes the tiles of one sequence and head, all of them: nothing is left to join
     float scale;                // times log2 e
 };
 PS_D bool pg_sees(const PgAttnSeq &s, int t, int back) { return back < 0 || (s.mask ? s.mask[t * s.n_tok + back] != 0 : back <= t); }
-PS_HD int64_t pg_run(int64_t tiles, int n, int k) { return tiles * k / n; } // where run k of n begins
+PS_HD int pg_run(int tiles, int n, int k) { const int r = tiles % n; return tiles / n * k + (k < r ? k : r); } // where run k of n begins: the first ones have a tile more
 
 template <int RT_, int MT_, int SG_> struct PgCfg {
     static constexpr int RT = RT_, MT = MT_, SG = SG_;         // query rows; products of 128 channels; soft-max groups
@@ -128,8 +129,14 @@ struct PgWalk {
     int s, u, left; // u: tile within the sequence's heads
     PS_D PgWalk(const PgAttn &a_, int lane) : a(a_) {
         const int k = blockIdx.x - a.lane_cta0[lane], n = a.lane_cta0[lane + 1] - a.lane_cta0[lane];
-        const int x = (int)pg_run(a.lane_tiles[lane], n, k);
-        left = (int)pg_run(a.lane_tiles[lane], n, k + 1) - x;
+        if (a.whole) {
+            s = k / a.pool.G;
+            left = a.seq[s].tiles;
+            u = (k - s * a.pool.G) * left;
+            return;
+        }
+        const int x = pg_run(a.lane_tiles[lane], n, k);
+        left = pg_run(a.lane_tiles[lane], n, k + 1) - x;
         int lo = 0, hi = a.n_seqs - 1; // the last sequence that begins at or before x
         while (lo < hi) {
             const int mid = (lo + hi + 1) / 2;
@@ -184,6 +191,7 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
     while (rt + 1 < a.n_lanes && (int)blockIdx.x >= a.lane_cta0[rt + 1]) rt++;
     const int r0 = rt * RT;
 
+    ps_grid_dep_launch(); // (the kernel that joins may take its place: it waits for the end of this one)
     if (tid == 0) {
         for (int b = 0; b < PG_STAGES; b++) { ps_mbar_init(&k_full[b], 1); ps_mbar_init(&v_full[b], 1); ps_mbar_init(&k_free[b], 1); ps_mbar_init(&v_free[b], 1); }
         for (int b = 0; b < 2; b++) {
@@ -648,17 +656,14 @@ __global__ void __launch_bounds__(256) pg_k_join(const __grid_constant__ PgAttn 
     if (row >= s.n_tok * a.R) return;
     const int rt = row / RT, n = a.lane_cta0[rt + 1] - a.lane_cta0[rt], T = a.lane_tiles[rt];
     const int u0 = a.tile0[si] + g * s.tiles, u1 = u0 + s.tiles;
-    auto of = [&](int x) { // the run that has tile x
-        int k = (int)((int64_t)x * n / T);
-        while (k + 1 < n && pg_run(T, n, k + 1) <= x) k++;
-        while (k > 0 && pg_run(T, n, k) > x) k--;
-        return k;
-    };
+    const int q = T / n, more = T % n;
+    auto of = [&](int x) { return x < more * (q + 1) ? x / (q + 1) : more + (x - more * (q + 1)) / q; }; // the run that has tile x
+    auto begins = [&](int k) { return q * k + min(k, more); };
     const int k0 = of(u0), k1 = of(u1 - 1);
     if (k0 == k1) return;
     const float2 *ml = reinterpret_cast<const float2 *>(a.part + (int64_t)a.n_ctas * 2 * RT * D);
     auto place = [&](int k) { // a run that begins before the row's tiles has come to them later
-        return ((int64_t)(a.lane_cta0[rt] + k) * 2 + (pg_run(T, n, k) < u0)) * RT + row % RT;
+        return ((int64_t)(a.lane_cta0[rt] + k) * 2 + (begins(k) < u0)) * RT + row % RT;
     };
     float top = PG_LOW, l = 0.f, acc[8] = {};
     for (int k = k0 + lane; k <= k1; k += 32) top = fmaxf(top, ml[place(k)].x);

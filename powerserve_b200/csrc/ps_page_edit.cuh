@@ -178,74 +178,79 @@ struct PgMoves {
     PgMoveOp op[PG_SEQS];
     PgPool pool;
     int64_t layer_codes, layer_scales;
+    int heads;              // K and V of all layers' heads
 };
+#define PG_MOVE_WARPS(wide) ((wide) ? 32 : 16) // of a CTA
+#define PG_MOVE_FEW 4       // blocks
 
-// x: a layer's head's K or V, y: move.  A warp takes a block; the CTA's eight blocks are read before one of them is written, and what a later block reads lies behind it, as the list rises: so they may
-// move in place.  ITEMS: head size / 32
-template <int ITEMS>
-__global__ void __launch_bounds__(256) pg_k_compact(const __grid_constant__ PgMoves a) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hs = 32 * ITEMS, B = a.pool.P / PG_BLOCK;
+// A block of sixteen slots is a warp's: lane: a slot's source, then a channel (V) or a slot's sixteen channels (K).  WIDE: x a layer's head's K or V, the CTA's blocks are all read before one of them is written; else
+// a warp a head, which reads a block and writes it before the next.  What a later block reads lies behind what is written, as the list rises: so slots may move in place.  ITEMS: head size / 32.
+// Bound by latency: a chain of five loads (count, list, table, scale, codes) for a block, or a round of blocks; the next round's list, table and scales are asked for before this one is written
+template <int ITEMS, bool WIDE>
+__global__ void __launch_bounds__(32 * PG_MOVE_WARPS(WIDE)) pg_k_compact(const __grid_constant__ PgMoves a) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hs = 32 * ITEMS, B = a.pool.P / PG_BLOCK, step = WIDE ? PG_MOVE_WARPS(true) : 1;
     const PgMoveOp &op = a.op[blockIdx.y];
-    const int heads = 2 * a.pool.G, layer = blockIdx.x / heads, h = blockIdx.x % heads, kv = h & 1;
+    const int head = WIDE ? blockIdx.x : blockIdx.x * PG_MOVE_WARPS(false) + warp, heads = 2 * a.pool.G, layer = head / heads, h = head % heads, kv = h & 1;
+    if (!WIDE && head >= a.heads) return;
     int8_t *codes = a.pool.codes + (int64_t)layer * a.layer_codes + (int64_t)h * a.pool.page_codes();
     float *scales = a.pool.scales + (int64_t)layer * a.layer_scales + (int64_t)h * B;
     const int64_t page_codes = (int64_t)heads * a.pool.page_codes(), page_scales = (int64_t)heads * B;
     const int n_keep = op.n_dev ? min(*op.n_dev, op.n_keep) : op.n_keep;
     if (n_keep <= 0) return;
     const int b0 = op.first / PG_BLOCK, b1 = (op.first + n_keep - 1) / PG_BLOCK;
-    bool bad = false;
-    for (int b = b0; b <= b1; b += 8) {
-        const int j = (b + warp) * PG_BLOCK + (lane & 15), i = j - op.first; // lane: a slot of the block
-        const bool mine = b + warp <= b1 && lane < 16;
-        // where the slot comes from: before `first`, itself
-        int src = -1;
-        if (mine && i < n_keep && !bad) {
-            const int k = i < 0 ? 0 : op.keep[i], ahead = i <= 0 ? -1 : op.keep[i - 1];
-            if (i < 0) src = j;
-            else if (k >= i && k > ahead && k < op.n_kv - op.first) src = op.first + k;
+    struct Slot { int src, page, to; float was; bool bad; };
+    auto look = [&](int b) { // where the slots of a block come from: before `first`, from themselves
+        Slot o{-1, -1, -1, 0.f, false};
+        const int j = b * PG_BLOCK + (lane & 15), i = j - op.first;
+        if (b > b1 || lane >= 16 || i >= n_keep) return o;
+        if (i < 0) o.src = j;
+        else {
+            const int k = op.keep[i], ahead = i ? op.keep[i - 1] : -1;
+            if (k >= i && k > ahead && k < op.n_kv - op.first) o.src = op.first + k;
         }
-        bad = __syncthreads_or(bad || (mine && i < n_keep && src < 0)) != 0; // (the list ends here: these eight blocks stay as they are)
-        if (bad) {
-            if (threadIdx.x == 0) *a.pool.err = PS_ERR_PAGE;
+        if (o.src >= 0) {
+            o.page = op.table[o.src >> a.pool.shift];
+            o.to = op.table[j >> a.pool.shift];
+            if (!a.pool.has(o.page) || !a.pool.has(o.to)) o.src = -1;
+        }
+        if (o.src < 0) { o.bad = true; return o; }
+        o.was = scales[o.page * page_scales + (o.src & (a.pool.P - 1)) / PG_BLOCK];
+        return o;
+    };
+    Slot now_at = look(b0 + (WIDE ? warp : 0));
+    for (int b = b0; b <= b1; b += step) {
+        const int mine = b + (WIDE ? warp : 0);
+        const Slot at = now_at;
+        // (the list ends where it goes wrong: this block, or these 32, and all behind them stay as they are)
+        if (WIDE ? __syncthreads_or(at.bad) : __any_sync(0xffffffffu, at.bad)) {
+            if ((WIDE ? threadIdx.x : lane) == 0) *a.pool.err = PS_ERR_PAGE;
             break;
         }
-        int page = -1, to = -1;
-        if (src >= 0) {
-            page = op.table[src >> a.pool.shift];
-            to = op.table[j >> a.pool.shift];
-            if (!a.pool.has(page) || !a.pool.has(to)) page = to = -1;
-        }
-        const bool lost = __syncthreads_or(src >= 0 && page < 0) != 0;
-        if (lost) break;
-        const float was = page >= 0 ? scales[page * page_scales + (src & (a.pool.P - 1)) / PG_BLOCK] : 0.f;
-        const float now = pg_warp_max(was), f = pg_follow(was, now);
-        const unsigned live = __ballot_sync(0xffffffffu, page >= 0), moves = __ballot_sync(0xffffffffu, page >= 0 && (src != j || was != now));
-        to = __shfl_sync(0xffffffffu, to, live ? __ffs(live) - 1 : 0); // (a block's slots are one page's)
+        const int j = mine * PG_BLOCK + (lane & 15);
+        const float now = pg_warp_max(at.was), f = pg_follow(at.was, now);
+        const unsigned live = __ballot_sync(0xffffffffu, at.src >= 0), moves = __ballot_sync(0xffffffffu, at.src >= 0 && (at.src != j || at.was != now));
+        const int to = __shfl_sync(0xffffffffu, at.to, 0); // (a block's slots are one page's; the first one is there if any is)
         uint4 out[ITEMS];
-        const int off = src & (a.pool.P - 1); // slot of the page
-        int8_t *dst = codes + to * page_codes + (int64_t)((b + warp) * PG_BLOCK & (a.pool.P - 1)) * hs;
+        const int off = at.src & (a.pool.P - 1); // slot of the page
+        int8_t *dst = codes + to * page_codes + (int64_t)(mine * PG_BLOCK & (a.pool.P - 1)) * hs;
         if (moves) {
             if (kv) {       // a channel's sixteen slots, byte by byte
 #pragma unroll
-                for (int e = 0; e < ITEMS; e++) {
-                    const int ch = e * 32 + lane;
-                    out[e] = reinterpret_cast<const uint4 *>(dst)[ch]; // (slots behind the last one stay)
-                }
-                const int64_t base = page * page_codes + (int64_t)(off & ~15) * hs;
+                for (int e = 0; e < ITEMS; e++) out[e] = reinterpret_cast<const uint4 *>(dst)[e * 32 + lane]; // (slots behind the last one stay)
+                const int64_t base = at.page * page_codes + (int64_t)(off & ~15) * hs + (off & 15);
 #pragma unroll
                 for (int s = 0; s < 16; s++) {
                     if (!(live >> s & 1)) continue;
-                    const int8_t *from = codes + __shfl_sync(0xffffffffu, base, s) + __shfl_sync(0xffffffffu, off & 15, s);
+                    const uint8_t *from = reinterpret_cast<const uint8_t *>(codes) + __shfl_sync(0xffffffffu, base, s);
                     const float fs = __shfl_sync(0xffffffffu, f, s);
 #pragma unroll
                     for (int e = 0; e < ITEMS; e++) {
-                        const uint32_t c = (uint32_t)pg_recode(from[(e * 32 + lane) * 16], fs) & 255u;
                         uint32_t &w = s < 8 ? (s < 4 ? out[e].x : out[e].y) : (s < 12 ? out[e].z : out[e].w);
-                        w = (w & ~(255u << (8 * (s & 3)))) | c << (8 * (s & 3));
+                        w = __byte_perm(w, pg_recode(from[(e * 32 + lane) * 16], 0, fs), (s & 3) == 0 ? 0x3214 : (s & 3) == 1 ? 0x3240 : (s & 3) == 2 ? 0x3410 : 0x4210);
                     }
                 }
             } else {        // a slot's sixteen channels
-                const int64_t base = page * page_codes + (int64_t)(off / 8) * 8 * hs + (off % 8) * 16;
+                const int64_t base = at.page * page_codes + (int64_t)(off / 8) * 8 * hs + (off % 8) * 16;
 #pragma unroll
                 for (int e = 0; e < ITEMS; e++) {
                     const int it = e * 32 + lane, s = it / (hs / 2) * 8 + it % 8, c = it % (hs / 2) / 8;
@@ -253,26 +258,21 @@ __global__ void __launch_bounds__(256) pg_k_compact(const __grid_constant__ PgMo
                     const float fs = __shfl_sync(0xffffffffu, f, s);
                     if (!(live >> s & 1)) continue;
                     const uint4 v = *reinterpret_cast<const uint4 *>(codes + from + c * 128);
-                    uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        uint32_t r = 0;
-#pragma unroll
-                        for (int k = 0; k < 4; k++) r |= ((uint32_t)pg_recode((int8_t)(w[q] >> (8 * k)), fs) & 255u) << (8 * k);
-                        w[q] = r;
-                    }
-                    out[e] = make_uint4(w[0], w[1], w[2], w[3]);
+                    out[e] = make_uint4(pg_recode4(v.x, fs), pg_recode4(v.y, fs), pg_recode4(v.z, fs), pg_recode4(v.w, fs));
                 }
             }
         }
-        __syncthreads();
+        now_at = look(mine + step);
+        if (WIDE) __syncthreads();
+        else __syncwarp();
         if (moves) {
 #pragma unroll
             for (int e = 0; e < ITEMS; e++) {
                 const int it = e * 32 + lane;
                 if (kv || (live >> (it / (hs / 2) * 8 + it % 8) & 1)) reinterpret_cast<uint4 *>(dst)[it] = out[e];
             }
-            if (lane == 0) scales[to * page_scales + ((b + warp) * PG_BLOCK & (a.pool.P - 1)) / PG_BLOCK] = now;
+            if (lane == 0) scales[to * page_scales + (mine * PG_BLOCK & (a.pool.P - 1)) / PG_BLOCK] = now;
         }
+        if (!WIDE) __syncwarp();
     }
 }

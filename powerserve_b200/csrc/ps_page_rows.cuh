@@ -2,8 +2,9 @@
 //
 //   scale' = max(scale, where earlier slots lie in the block; max |x| / 127),   code = rint(x / scale'),   earlier codes rint(code * (scale / scale'))
 //
-// A warp takes a block of sixteen slots of one head's K or V: it holds the block's numbers, so that they are read once, finds their largest by shuffles, and writes sixteen bytes a lane, lane after
-// lane.  K: a lane's item is a slot's sixteen channels; V: a channel's sixteen slots.  Bound by memory for prompts, by latency (a chain of table, scale, numbers) for single tokens.
+// store: a CTA takes a block of sixteen slots of one head's K or V, a thread sixteen of its numbers, which are read once: a slot's sixteen channels (K), a channel's sixteen slots (V), so that sixteen bytes a lane go to
+// memory lane after lane.  Bound by memory for prompts, by latency (a chain of table, numbers, the CTA's largest) for single tokens.  (A warp a block, 64 numbers a lane: 10 000 tokens 55 us for few warps an SM.)
+// load: a warp a block.
 #pragma once
 #include "ps_page.cuh"
 
@@ -26,13 +27,12 @@ struct PgRowTask { // a warp's block
     int block;              // of the page
     bool there;
 };
-PS_D PgRowTask pg_row_task(const PgRows &a) {
+PS_D PgRowTask pg_row_task(const PgRows &a, uint32_t task) {
     const int heads = 2 * a.pool.G;
-    const int64_t task = (int64_t)blockIdx.x * PG_ROW_WARPS + (threadIdx.x >> 5);
     PgRowTask t;
-    t.there = task < (int64_t)a.blocks * heads;
+    const int u = (int)(task / (uint32_t)heads), h = (int)(task % (uint32_t)heads);
+    t.there = u < a.blocks;
     if (!t.there) return t;
-    const int u = (int)(task / heads), h = (int)(task % heads);
     t.kv = h & 1; t.g = h >> 1;
     int lo = 0, hi = a.n_seqs - 1; // the last sequence that begins at or before block u
     while (lo < hi) {
@@ -65,78 +65,66 @@ template <typename T> PS_D void pg_get16(float (&x)[16], const T *p, bool vec) {
         for (int i = 0; i < 16; i++) x[i] = pg_num(p[i]);
     }
 }
-PS_D uint4 pg_pack(const int (&c)[16]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) w[i] = (uint32_t)(c[4 * i] & 255) | (uint32_t)(c[4 * i + 1] & 255) << 8 | (uint32_t)(c[4 * i + 2] & 255) << 16 | (uint32_t)c[4 * i + 3] << 24;
-    return make_uint4(w[0], w[1], w[2], w[3]);
+PS_D uint32_t pg_bytes_from(int n) { return n <= 0 ? ~0u : n >= 4 ? 0u : ~0u << (8 * n); } // a word's bytes n, n + 1, ...
+// bytes below lo from `below`, below hi from x, the others from `above`
+PS_D uint4 pg_three(const uint4 &below, const uint4 &x, const uint4 &above, int lo, int hi) {
+    auto one = [&](uint32_t a, uint32_t b, uint32_t c, int at) {
+        const uint32_t from_lo = pg_bytes_from(lo - at), from_hi = pg_bytes_from(hi - at);
+        return (a & ~from_lo) | (b & from_lo & ~from_hi) | (c & from_hi);
+    };
+    return make_uint4(one(below.x, x.x, above.x, 0), one(below.y, x.y, above.y, 4), one(below.z, x.z, above.z, 8), one(below.w, x.w, above.w, 12));
 }
 
-// ITEMS: head size / 32
-template <typename T, int ITEMS>
-__global__ void __launch_bounds__(32 * PG_ROW_WARPS) pg_k_store(const __grid_constant__ PgRows a) {
-    const int lane = threadIdx.x & 31, hs = 32 * ITEMS, ld = a.pool.G * hs;
-    const PgRowTask t = pg_row_task(a);
-    if (!t.there) return;
+// as many threads as a head has channels
+template <typename T>
+__global__ void __launch_bounds__(256, 4) pg_k_store(const __grid_constant__ PgRows a) {
+    __shared__ float s_top[8];
+    const int i = threadIdx.x, hs = blockDim.x, ld = a.pool.G * hs;
+    const PgRowTask t = pg_row_task(a, blockIdx.x);
+    if (!t.there) return; // (the whole CTA)
     const T *x = static_cast<const T *>(t.kv ? a.v : a.k) + (int64_t)t.g * hs;
-    uint4 *codes = reinterpret_cast<uint4 *>(a.pool.codes + t.at * a.pool.page_codes() + (int64_t)t.block * PG_BLOCK * hs);
+    uint4 *codes = reinterpret_cast<uint4 *>(a.pool.codes + t.at * a.pool.page_codes() + (int64_t)t.block * PG_BLOCK * hs) + i;
     float *scale = a.pool.scales + t.at * (a.pool.P / PG_BLOCK) + t.block;
+    const int second = i >= hs / 2, slot = second * 8 + (i & 7), c = (i - second * (hs / 2)) >> 3; // K's
+    const bool part = t.lo > 0 || t.hi < 16;
     const float was = t.lo ? *scale : 0.f;
-    float n[ITEMS][16], top = 0.f;
+    uint4 old = make_uint4(0, 0, 0, 0);
+    if (part) old = *codes;
+    float n[16], top = 0.f;
+    if (t.kv) {
+        const T *x0 = x + t.row * ld + i;
 #pragma unroll
-    for (int e = 0; e < ITEMS; e++) {
-        const int i = e * 32 + lane;
-        if (t.kv) {         // channel i of every slot
+        for (int s = 0; s < 16; s++) n[s] = s >= t.lo && s < t.hi ? pg_num(x0[s * ld]) : 0.f;
+    } else if (slot >= t.lo && slot < t.hi) pg_get16(n, x + (t.row + slot) * ld + c * 16, a.k_vec);
+    else {
 #pragma unroll
-            for (int s = 0; s < 16; s++) n[e][s] = s >= t.lo && s < t.hi ? pg_num(x[(t.row + s) * ld + i]) : 0.f;
-        } else {            // slot, sixteen channels
-            const int slot = i / (hs / 2) * 8 + i % 8, c = i % (hs / 2) / 8;
-            if (slot >= t.lo && slot < t.hi) pg_get16(n[e], x + (t.row + slot) * ld + c * 16, a.k_vec);
-            else {
-#pragma unroll
-                for (int s = 0; s < 16; s++) n[e][s] = 0.f;
-            }
-        }
-#pragma unroll
-        for (int s = 0; s < 16; s++) top = fmaxf(top, fabsf(n[e][s])); // (fmaxf passes over what is no number)
+        for (int s = 0; s < 16; s++) n[s] = 0.f;
     }
-    const float now = fmaxf(was, __fdiv_rn(pg_warp_max(top), 127.f)), f = pg_follow(was, now);
-    const bool move = t.lo > 0 && now != was; // codes that stay get another scale
 #pragma unroll
-    for (int e = 0; e < ITEMS; e++) {
-        const int i = e * 32 + lane;
-        int c[16];
-#pragma unroll
-        for (int s = 0; s < 16; s++) c[s] = pg_code(n[e][s], now);
-        if (t.kv) {
-            if (t.lo > 0 || t.hi < 16) {
-                const uint4 old = codes[i];
-#pragma unroll
-                for (int s = 0; s < 16; s++) {
-                    const int o = pg_byte(old, s);
-                    if (s < t.lo) c[s] = move ? pg_recode(o, f) : o;
-                    else if (s >= t.hi) c[s] = o;
-                }
-            }
-            codes[i] = pg_pack(c);
-        } else {
-            const int slot = i / (hs / 2) * 8 + i % 8;
-            if (slot >= t.lo && slot < t.hi) codes[i] = pg_pack(c);
-            else if (slot < t.lo && move) {
-                const uint4 old = codes[i];
-#pragma unroll
-                for (int s = 0; s < 16; s++) c[s] = pg_recode(pg_byte(old, s), f);
-                codes[i] = pg_pack(c);
-            }
+    for (int s = 0; s < 16; s++) top = fmaxf(top, fabsf(n[s])); // (fmaxf passes over what is no number)
+    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+    if ((i & 31) == 0) s_top[i >> 5] = top;
+    __syncthreads();
+    for (int w = 0; w < hs / 32; w++) top = fmaxf(top, s_top[w]);
+    const float now = fmaxf(was, __fdiv_rn(top, 127.f));
+    const uint4 codes_now = PgDivide(now)(n);
+    if (!part) *codes = codes_now;
+    else {
+        uint4 r = old;
+        if (t.lo > 0 && now != was) { // codes that stay get another scale
+            const float f = pg_follow(was, now);
+            r = make_uint4(pg_recode4(old.x, f), pg_recode4(old.y, f), pg_recode4(old.z, f), pg_recode4(old.w, f));
         }
+        if (t.kv) *codes = pg_three(r, codes_now, old, t.lo, t.hi);
+        else if (slot < t.hi) *codes = slot < t.lo ? r : codes_now;
     }
-    if (lane == 0) *scale = now;
+    if (i == 0) *scale = now;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(32 * PG_ROW_WARPS) pg_k_load(const __grid_constant__ PgRows a) {
     const int lane = threadIdx.x & 31, hs = a.pool.hs, ld = a.pool.G * hs;
-    const PgRowTask t = pg_row_task(a);
+    const PgRowTask t = pg_row_task(a, blockIdx.x * PG_ROW_WARPS + (threadIdx.x >> 5));
     T *x = static_cast<T *>(t.there ? (t.kv ? a.v : a.k) : nullptr);
     if (!x) return;
     x += (int64_t)t.g * hs;
@@ -147,9 +135,9 @@ __global__ void __launch_bounds__(32 * PG_ROW_WARPS) pg_k_load(const __grid_cons
         if (t.kv) {
 #pragma unroll
             for (int s = 0; s < 16; s++)
-                if (s >= t.lo && s < t.hi) x[(t.row + s) * ld + i] = pg_to<T>((float)pg_byte(c, s) * scale);
+                if (s >= t.lo && s < t.hi) (x + t.row * ld + i)[s * ld] = pg_to<T>((float)pg_byte(c, s) * scale);
         } else {
-            const int slot = i / (hs / 2) * 8 + i % 8, ch = i % (hs / 2) / 8;
+            const int second = i >= hs / 2, slot = second * 8 + (i & 7), ch = (i - second * (hs / 2)) >> 3;
             if (slot < t.lo || slot >= t.hi) continue;
             T *to = x + (t.row + slot) * ld + ch * 16;
             alignas(16) T n[16];

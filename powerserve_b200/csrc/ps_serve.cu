@@ -420,9 +420,11 @@ int ps_serve_verify(PsServeCall *c, int32_t *ids, int32_t *path, int32_t *n_path
             SV_CK(cudaLaunchKernelEx(&cfg, sv_k_stats, a));
             SV_LAUNCHED("verify");
         }
-        at[0].val.clusterDim.x = SV_VERIFY_CTAS;
-        cfg.gridDim = dim3(n * SV_VERIFY_CTAS); cfg.dynamicSmemBytes = 0;
-        v.chunk = (int)((vocab + SV_VERIFY_CTAS - 1) / SV_VERIFY_CTAS + 31) & ~31;
+        const int C = n * 16 <= c->n_sm * 2 ? 16 : 8;
+        at[0].val.clusterDim.x = C;
+        cfg.gridDim = dim3(n * C); cfg.dynamicSmemBytes = 0;
+        v.chunk = (int)((vocab + C - 1) / C + 31) & ~31;
+        SV_CK(cudaFuncSetAttribute(sv_k_verify, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         SV_CK(cudaLaunchKernelEx(&cfg, sv_k_verify, v));
         SV_LAUNCHED("verify");
         ids += n; n_path += n; path += nodes; parents += nodes; tokens += nodes; u += nodes; samplers += nodes; logits += (int64_t)nodes * row_stride;

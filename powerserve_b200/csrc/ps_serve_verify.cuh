@@ -10,7 +10,6 @@
 #include "ps_serve_sample.cuh"
 
 #define SV_VERIFY_SEQS 1024 // sequences of a launch: their first nodes are a kernel parameter
-#define SV_VERIFY_CTAS 8
 #define SV_P_ONE 0x1p58     // a residual's unit: sums stay below 2^59
 
 struct SvStats {
@@ -63,57 +62,93 @@ struct SvDist {
         else only = -1;
         inv = 1.0 / (double)all;
     }
-    PS_D unsigned long long of(const double *pow2, float v, int i) const {
-        if (i == only) return SV_ONE;
-        if (!(v > -INFINITY) || sv_key(v, i) < kappa) return 0;
+    PS_D unsigned long long of(const double *pow2, float v, int i) const { // (without branches, so that several are under way at once)
+        const bool in = v > -INFINITY && sv_key(v, i) >= kappa;
         const unsigned long long w = sv_weight(pow2, log2w(v));
-        return w >= min_w ? w : 0;
+        return i == only ? SV_ONE : in && w >= min_w ? w : 0;
     }
     PS_D unsigned long long operator()(const double *pow2, int i) const { return of(pow2, x[i], i); }
 };
 
-__global__ void __cluster_dims__(SV_VERIFY_CTAS) __launch_bounds__(SV_SMP_THREADS, 2) sv_k_verify(const __grid_constant__ SvVerify a) {
+__global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_verify(const __grid_constant__ SvVerify a) {
     namespace cg = cooperative_groups;
-    constexpr int C = SV_VERIFY_CTAS, WARPS = SV_SMP_THREADS / 32;
-    __shared__ double pow2[32];
-    __shared__ unsigned long long mail[2][C], warp_sum[WARPS];
+    constexpr int WARPS = SV_SMP_THREADS / 32;
+    __shared__ double pow2[32], s_pc[PS_CUDA_TREE_TOKENS], s_qc[PS_CUDA_TREE_TOKENS];
+    __shared__ unsigned long long mail[2][16], warp_sum[WARPS], s_w[PS_CUDA_TREE_TOKENS], s_all[PS_CUDA_TREE_TOKENS];
     __shared__ int s_parent[PS_CUDA_TREE_TOKENS], s_token[PS_CUDA_TREE_TOKENS], s_path[PS_CUDA_TREE_TOKENS], s_gone[PS_CUDA_TREE_TOKENS];
     __shared__ float s_u[PS_CUDA_TREE_TOKENS];
     cg::cluster_group cl = cg::this_cluster();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = cl.block_rank();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = cl.block_rank(), C = cl.num_blocks();
     const int seq = blockIdx.x / C, base = a.first[seq], n = a.first[seq + 1] - base;
     int turn = 0;
     if (tid < 32) pow2[tid] = exp2(tid / 32.0);
-    for (int i = tid; i < n; i += SV_SMP_THREADS) {
-        s_parent[i] = a.parents[base + i];
-        s_token[i] = a.tokens[base + i];
+    __syncthreads();
+    auto target = [&](SvDist &d, int i) { d.load(a.logits + (int64_t)(base + i) * a.row_stride, a.target[base + i], a.samplers[base + i]); };
+    auto draft = [&](SvDist &d, int i) { d.load(a.draft_logits + (int64_t)(base + i) * a.row_stride, a.draft[base + i], a.draft_samplers[base + i]); };
+    // what the tests ask for: a thread a node, all at once
+    if (tid < n) {
+        const int i = tid, up = a.parents[base + i], c = a.tokens[base + i];
+        const unsigned long long all = a.target[base + i].all;
+        s_parent[i] = up;
         s_u[i] = a.u[base + i];
+        s_all[i] = all ? all : SV_ONE;
+        const bool in = i > 0 && up >= 0 && up < i && c >= 0 && c < a.vocab;
+        s_token[i] = in ? c : -1;
+        if (in) {
+            SvDist d;
+            target(d, up);
+            const unsigned long long w = d(pow2, c);
+            s_w[i] = w;
+            s_pc[i] = (double)w * d.inv;
+            if (a.draft_logits) {
+                draft(d, up);
+                s_qc[i] = (double)d(pow2, c) * d.inv;
+            }
+        }
     }
     __syncthreads();
     SvDist p, q;
     int cur = 0, n_path = 1, n_gone = 0;
     double t = 0.0, T = 1.0;
-    unsigned long long left; // without a draft: mass of what p still has
-    bool have_q = false;
-    p.load(a.logits + (int64_t)base * a.row_stride, a.target[base], a.samplers[base]);
-    left = p.all;
+    unsigned long long left = s_all[0]; // without a draft: mass of what p still has
+    bool have = false;                  // p and q are row cur's
     const int i0 = min(rank * a.chunk, a.vocab), i1 = min(i0 + a.chunk, a.vocab);
     const int run = ((i1 - i0 + WARPS - 1) / WARPS + 31) & ~31, w0 = min(i0 + warp * run, i1), w1 = min(w0 + run, i1); // the warp's tokens
-    // what token i still has, in whole numbers
-    auto mass = [&](int i) -> unsigned long long {
-        unsigned long long w = p(pow2, i);
-        if (t > 0.0) {
-            const double r = (double)w * p.inv - t * ((double)q(pow2, i) * q.inv);
-            return r > 0.0 ? (unsigned long long)(r * SV_P_ONE) : 0;
-        }
+    // what tokens i + 32 e still have, in whole numbers: E weights of a row are under way at a time
+    auto masses = [&](int i, auto &m) {
+        constexpr int E = sizeof(m) / sizeof(m[0]);
+        float x[E], y[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) x[e] = i + 32 * e < w1 ? p.x[i + 32 * e] : -INFINITY;
+        if (t > 0.0)
+#pragma unroll
+            for (int e = 0; e < E; e++) y[e] = i + 32 * e < w1 ? q.x[i + 32 * e] : -INFINITY;
+#pragma unroll
+        for (int e = 0; e < E; e++) m[e] = i + 32 * e < w1 ? p.of(pow2, x[e], i + 32 * e) : 0;
+        if (t > 0.0)
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const double r = i + 32 * e < w1 ? (double)m[e] * p.inv - t * ((double)q.of(pow2, y[e], i + 32 * e) * q.inv) : 0.0;
+                m[e] = r > 0.0 ? (unsigned long long)(r * SV_P_ONE) : 0;
+            }
         for (int g = 0; g < n_gone; g++)
-            if (s_gone[g] == i) w = 0;
-        return w;
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (s_gone[g] == i + 32 * e) m[e] = 0;
     };
     auto warp_mass = [&]() {
+        if (!have) {
+            target(p, cur);
+            if (t > 0.0) draft(q, cur);
+            have = true;
+        }
         unsigned long long sum = 0;
-#pragma unroll 4
-        for (int i = w0 + lane; i < w1; i += 32) sum += mass(i);
+        for (int i = w0 + lane; i < w1; i += 128) {
+            unsigned long long m[4];
+            masses(i, m);
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum += m[e];
+        }
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         return sum;
@@ -133,17 +168,12 @@ __global__ void __cluster_dims__(SV_VERIFY_CTAS) __launch_bounds__(SV_SMP_THREAD
         return mail[turn];
     };
     for (int i = 1; i < n; i++) {
-        if (s_parent[i] != cur) continue;
         const int c = s_token[i];
-        if (c < 0 || c >= a.vocab) continue;
-        const unsigned long long w = p(pow2, c);
+        if (s_parent[i] != cur || c < 0) continue;
         bool yes;
-        if (a.draft_logits) {
-            if (!have_q) q.load(a.draft_logits + (int64_t)(base + cur) * a.row_stride, a.draft[base + cur], a.draft_samplers[base + cur]);
-            have_q = true;
-            const double pc = (double)w * p.inv, qc = (double)q(pow2, c) * q.inv;
-            yes = (double)s_u[i] * T * qc < pc - t * qc;
-        } else {
+        if (a.draft_logits) yes = (double)s_u[i] * T * s_qc[i] < s_pc[i] - t * s_qc[i];
+        else {
+            const unsigned long long w = s_w[i];
             bool gone = false;
             for (int g = 0; g < n_gone; g++) gone |= s_gone[g] == c;
             yes = !gone && (double)s_u[i] * (double)left < (double)w;
@@ -159,11 +189,11 @@ __global__ void __cluster_dims__(SV_VERIFY_CTAS) __launch_bounds__(SV_SMP_THREAD
             if (tid == 0) s_path[n_path] = i;
             n_path++;
             cur = i;
-            p.load(a.logits + (int64_t)(base + cur) * a.row_stride, a.target[base + cur], a.samplers[base + cur]);
-            left = p.all;
-            t = 0.0; T = 1.0; n_gone = 0; have_q = false;
+            left = s_all[i];
+            t = 0.0; T = 1.0; n_gone = 0; have = false;
         } else if (a.draft_logits) {
             const double t_was = t;
+            if (t == 0.0) have = false; // (q is asked for, too)
             t += T;
             const unsigned long long *m = meet(warp_mass());
             unsigned long long sum = 0;
@@ -195,19 +225,23 @@ __global__ void __cluster_dims__(SV_VERIFY_CTAS) __launch_bounds__(SV_SMP_THREAD
     if (goal < before || goal >= before + block) return;
     for (int w = 0; w < warp; w++) before += warp_sum[w];
     if (goal < before || goal >= before + mine) return;
-    for (int i = w0; i < w1; i += 32) {
-        const unsigned long long w = i + lane < w1 ? mass(i + lane) : 0;
-        unsigned long long inc = w;
+    for (int i = w0; i < w1; i += 64) {
+        unsigned long long w[2];
+        masses(i + lane, w);
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const unsigned long long v = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += v;
+        for (int e = 0; e < 2; e++) {
+            unsigned long long inc = w[e];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned long long v = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += v;
+            }
+            const unsigned ball = __ballot_sync(0xffffffffu, goal < before + inc);
+            if (ball) {
+                if (lane == __ffs(ball) - 1) a.ids[seq] = i + 32 * e + lane;
+                return;
+            }
+            before += __shfl_sync(0xffffffffu, inc, 31);
         }
-        const unsigned ball = __ballot_sync(0xffffffffu, goal < before + inc);
-        if (ball) {
-            if (lane == __ffs(ball) - 1) a.ids[seq] = i + lane;
-            return;
-        }
-        before += __shfl_sync(0xffffffffu, inc, 31);
     }
 }
