@@ -85,8 +85,6 @@ PS_D int pg_order(float x) { // whole numbers in the order of the floats; its ow
     return b ^ (b >> 31 & 0x7fffffff);
 }
 PS_D float pg_unorder(int b) { return __int_as_float(b ^ (b >> 31 & 0x7fffffff)); }
-// three digits' sums: the lower two are whole numbers of 31 bits together
-PS_D float pg_digits(int d0, int d1, int d2) { return fmaf((float)d2, 65536.f, (float)(d1 * 256 + d0)); }
 // a number of each row, from shared memory
 template <int RT, typename F> PS_D void pg_rows(const float *x, F f) {
 #pragma unroll
@@ -98,7 +96,18 @@ template <int RT, typename F> PS_D void pg_rows(const float *x, F f) {
         if (c + 3 < RT) f(c + 3, v.w);
     }
 }
-// the sums of RT rows, f(row, sum): sixteen rows at a time
+// two floats an instruction
+using pg_f2 = unsigned long long;
+PS_D pg_f2 pg_two(float a, float b) { pg_f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+PS_D void pg_one(pg_f2 x, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+PS_D pg_f2 pg_mul2(pg_f2 a, pg_f2 b) { pg_f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+PS_D pg_f2 pg_add2(pg_f2 a, pg_f2 b) { pg_f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+PS_D pg_f2 pg_fma2(pg_f2 a, pg_f2 b, pg_f2 c) { pg_f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+// three digits' sums, of two neighbouring columns a, b: the lower two are whole numbers of 31 bits together
+PS_D pg_f2 pg_digits2(int a0, int b0, int a1, int b1, int a2, int b2) {
+    return pg_fma2(pg_two((float)a2, (float)b2), pg_two(65536.f, 65536.f), pg_two((float)(a1 * 256 + a0), (float)(b1 * 256 + b0)));
+}
+// the digits' sums of RT rows put together, f(pair of rows, sums): sixteen rows at a time
 template <int RT, typename F> PS_D void pg_sums(uint32_t at, F f) {
     if constexpr (RT % 16 == 0) {
 #pragma unroll
@@ -109,7 +118,7 @@ template <int RT, typename F> PS_D void pg_sums(uint32_t at, F f) {
             pg_tm_ld16(d, at + 2 * RT + c);
             ps_tc_ld_wait();
 #pragma unroll
-            for (int r = 0; r < 16; r++) f(c + r, pg_digits(a[r], b[r], d[r]));
+            for (int r = 0; r < 16; r += 2) f((c + r) / 2, pg_digits2(a[r], a[r + 1], b[r], b[r + 1], d[r], d[r + 1]));
         }
     } else {
         constexpr int N = (3 * RT + 15) / 16;
@@ -118,8 +127,49 @@ template <int RT, typename F> PS_D void pg_sums(uint32_t at, F f) {
         for (int c = 0; c < N; c++) pg_tm_ld16(v[c], at + 16 * c);
         ps_tc_ld_wait();
 #pragma unroll
-        for (int r = 0; r < RT; r++) f(r, pg_digits(v[r / 16][r % 16], v[(RT + r) / 16][(RT + r) % 16], v[(2 * RT + r) / 16][(2 * RT + r) % 16]));
+        for (int r = 0; r < RT; r += 2) {
+            auto d = [&](int k, int row) { return row < RT ? v[(k * RT + row) / 16][(k * RT + row) % 16] : 0; };
+            f(r / 2, pg_digits2(d(0, r), d(0, r + 1), d(1, r), d(1, r + 1), d(2, r), d(2, r + 1)));
+        }
     }
+}
+// Fragments: lane l has, of every eight columns, the columns 2 (l % 4) and the next, of the sixteen rows l / 4 and l / 4 + 8 in this order
+template <int CG> PS_D void pg_tm_frag(int (&v)[4 * CG], uint32_t at) {
+    if constexpr (CG == 1)
+        asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
+    else if constexpr (CG == 2)
+        asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                     : "r"(at)
+                     : "memory");
+    else
+        asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+                       "=r"(v[14]), "=r"(v[15])
+                     : "r"(at)
+                     : "memory");
+}
+// bytes in such fragments to rows of sixteen bytes, one for every column: a matrix of eight columns from every eight lanes' addresses
+template <int CG> PS_D void pg_put_frag(uint32_t at, const uint32_t (&w)[CG]) {
+    if constexpr (CG == 1) asm volatile("stmatrix.sync.aligned.m16n8.x1.trans.shared.b8 [%0], {%1};" ::"r"(at), "r"(w[0]));
+    else if constexpr (CG == 2) asm volatile("stmatrix.sync.aligned.m16n8.x2.trans.shared.b8 [%0], {%1, %2};" ::"r"(at), "r"(w[0]), "r"(w[1]));
+    else asm volatile("stmatrix.sync.aligned.m16n8.x4.trans.shared.b8 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]));
+}
+// v[i] of lanes with the same l % 4 put together: lane l ends with that of i = (l / 4) / (8 / NR)
+template <int NR, typename F> PS_D float pg_across(float (&v)[NR], F f) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 16, half = NR / 2; o >= 4; o /= 2, half /= 2) {
+        if (half) {
+#pragma unroll
+            for (int i = 0; i < NR / 2; i++)
+                if (i < half) {
+                    const float keep = lane & o ? v[i + half] : v[i], give = lane & o ? v[i] : v[i + half];
+                    v[i] = f(keep, __shfl_xor_sync(0xffffffffu, give, o));
+                }
+        } else v[0] = f(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
+    }
+    return v[0];
 }
 
 // A CTA's way through its tiles: runs of one sequence and head
@@ -420,121 +470,211 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
             if (lane == 0) ps_mbar_arrive(&q_full[n & 1]);
         }
     } else if (warp < C::W_OUT) {
-        // ===== soft-max: thread = slot.  A warp that gave up a wait goes on to the group's next barrier, which tells the others: nobody is left alone at one
-        const int group = warp >> 2, w = warp & 3, slot = w * 32 + lane;
-        const uint32_t lane_at = (uint32_t)(w * 32) << 16;
+        // ===== soft-max.  A warp that gave up a wait goes on to the group's next barrier, which tells the others: nobody is left alone at one.
+        // RT a multiple of eight: a lane has four slots, lane / 4 and every eighth of its warp's behind it, and of every eight rows two, 2 (lane % 4) and the next; five rows: a slot and all rows.  The numbers of a
+        // row (its reference, its factor) are those of the lanes whose `own` it is
+        constexpr bool FRAG = RT % 8 == 0;
+        constexpr int CG = FRAG ? RT / 8 : 1, NR = 2 * CG, NS = FRAG ? 4 : 1, NL = FRAG ? NR : RT; // eights of rows; rows, slots, sums of a lane
+        const int group = warp >> 2, w = warp & 3, bar = SG == 1 ? 1 : 1 + group, quad = 2 * (lane & 3);
+        const int idx = (lane >> 2) / (FRAG ? 8 / NR : 1), own = FRAG ? idx / 2 * 8 + quad + (idx & 1) : min(lane, RT - 1);
+        const bool owner = FRAG ? (lane >> 2) % (FRAG ? 8 / NR : 1) == 0 : lane < RT;
+        auto slot_of = [&](int e) { return w * 32 + (FRAG ? e * 8 + (lane >> 2) : lane); };
         float *mine = s_row[warp][0], *factor = s_row[warp][1];
         int i = 0, n = 0, turn = 0;
-        const int bar = SG == 1 ? 1 : 1 + group;
         for (; walk.next(sg); n++) {
             const PgAttnSeq &s = a.seq[sg.s];
             const int rows = min(s.n_tok * a.R - r0, RT), past = s.n_kv - s.n_tok;
-            float l[RT], run = PG_LOW, qs = 0.f; // run, qs: row `lane`'s
+            float run = PG_LOW, qs = 0.f; // row own's largest score over its factor, and the factor
+            float l[NL];
+            pg_f2 qs2[CG];
 #pragma unroll
-            for (int r = 0; r < RT; r++) l[r] = 0.f;
+            for (int r = 0; r < NL; r++) l[r] = 0.f;
             ok = ps_bar_all(bar, 128, ok); // (a run begins: nobody of the group reads the last one's numbers any more)
             if (!ok) break;
-            if (slot < RT)
+            if (w * 32 + lane < RT)
 #pragma unroll
-                for (int b = 0; b < 4; b++) s_ref[group][b][slot] = pg_order(PG_LOW);
+                for (int b = 0; b < 4; b++) s_ref[group][b][w * 32 + lane] = pg_order(PG_LOW);
             ps_bar_sync(bar, 128);
             bool first = true;
             for (int t = sg.t0; t < sg.t1; t++, i++) {
                 if (SG > 1 && (i & 1) != group) continue;
                 wait(&meta_full[i % PG_META], (i / PG_META) & 1, 21);
                 const PgMeta &m = s_meta[i % PG_META];
-                const float ks = m.ks[slot >> 4], vq = m.vq[slot >> 4], vmax = m.vmax;
-                const bool live = m.live[w] >> lane & 1;
+                const float ks0 = m.ks[FRAG ? 2 * w : 2 * w + (lane >> 4)], vq0 = m.vq[FRAG ? 2 * w : 2 * w + (lane >> 4)], ks1 = FRAG ? m.ks[2 * w + 1] : 0.f, vq1 = FRAG ? m.vq[2 * w + 1] : 0.f, vmax = m.vmax;
+                const uint32_t live = m.live[w];
                 __syncwarp();
                 if (lane == 0) ps_mbar_arrive(&meta_free[i % PG_META]);
-                // rows that see the slot
-                uint32_t see = live ? ~0u : 0u;
-                const int back = t * PG_TILE + slot - past;
-                if (live && back >= 0) {
-                    int tok = r0 / a.R, rest = r0 % a.R;
-                    see = 0;
-                    for (int r = 0; r < rows; tok++, rest = 0) {
-                        const int many = min(a.R - rest, rows - r);
-                        if (pg_sees(s, tok, back)) see |= (many == 32 ? ~0u : (1u << many) - 1) << r;
-                        r += many;
+                // rows that see the lane's slots
+                const bool gaps = live != ~0u || t * PG_TILE + w * 32 + 32 > past;
+                uint32_t see[NS];
+                if (gaps) {
+#pragma unroll
+                    for (int e = 0; e < NS; e++) {
+                        const int back = t * PG_TILE + slot_of(e) - past;
+                        see[e] = live >> (slot_of(e) & 31) & 1 ? ~0u : 0u;
+                        if (see[e] && back >= 0) {
+                            int tok = r0 / a.R, rest = r0 % a.R;
+                            see[e] = 0;
+                            for (int r = 0; r < rows; tok++, rest = 0) {
+                                const int many = min(a.R - rest, rows - r);
+                                if (pg_sees(s, tok, back)) see[e] |= (many == 32 ? ~0u : (1u << many) - 1) << r;
+                                r += many;
+                            }
+                        }
                     }
                 }
-                const bool gaps = __any_sync(0xffffffffu, see != ~0u);
                 wait(&s_full[i & 1], (i >> 1) & 1, 22);
                 ps_tc_fence_after();
                 if (first) { // (they come with the first scores)
-                    qs = lane < RT ? s_qs[n & 1][lane] : 0.f;
-                    if (lane < RT) factor[lane] = fmaxf(qs, 0x1p-126f); // (above zero, and a number: -inf times it is -inf)
+                    qs = s_qs[n & 1][own];
+                    factor[own] = fmaxf(qs, 0x1p-126f); // (above zero, and a number: -inf times it is -inf)
+                    __syncwarp();
+                    if constexpr (FRAG) {
+#pragma unroll
+                        for (int c = 0; c < CG; c++) qs2[c] = *reinterpret_cast<const pg_f2 *>(factor + 8 * c + quad);
+                    }
                     first = false;
                 }
-                float y[RT];
-                pg_sums<RT>(tm + (i & 1) * N + lane_at, [&](int r, float x) { y[r] = x * ks; });
+                // scores over the rows' factors
+                const uint32_t at = tm + (i & 1) * N + ((uint32_t)(w * 32) << 16);
+                pg_f2 y2[FRAG ? 2 : 1][2][CG];
+                float y[FRAG ? 1 : RT], top;
+                if constexpr (FRAG) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        int d[3][4 * CG];
+#pragma unroll
+                        for (int k = 0; k < 3; k++) pg_tm_frag<CG>(d[k], at + k * RT + ((uint32_t)(16 * h) << 16));
+                        ps_tc_ld_wait();
+                        const pg_f2 ks = h ? pg_two(ks1, ks1) : pg_two(ks0, ks0);
+#pragma unroll
+                        for (int c = 0; c < CG; c++)
+#pragma unroll
+                            for (int b = 0; b < 2; b++) {
+                                const int f = 4 * c + 2 * b;
+                                y2[h][b][c] = pg_mul2(pg_digits2(d[0][f], d[0][f + 1], d[1][f], d[1][f + 1], d[2][f], d[2][f + 1]), ks);
+                            }
+                    }
+                } else
+                    pg_sums<RT>(at, [&](int r, pg_f2 x) {
+                        float x0, x1;
+                        pg_one(x, x0, x1);
+                        y[2 * r] = x0 * ks0;
+                        if (2 * r + 1 < RT) y[2 * r + 1] = x1 * ks0;
+                    });
                 ps_tc_fence_before();
                 __syncwarp();
                 if (lane == 0) ps_mbar_arrive(&s_free[i & 1]);
-                if (gaps) {
+                if constexpr (FRAG) {
+                    float most[NR];
+                    if (gaps) {
 #pragma unroll
-                    for (int r = 0; r < RT; r++)
-                        if (!(see >> r & 1)) y[r] = -INFINITY;
-                }
-                float top = PG_LOW; // row `lane`'s
+                        for (int c = 0; c < CG; c++)
 #pragma unroll
-                for (int r = 0; r < RT; r++) {
-                    const float x = pg_redux_max(y[r]);
-                    if (lane == r) top = fmaxf(top, x);
+                            for (int e = 0; e < 4; e++) {
+                                float x0, x1;
+                                pg_one(y2[e >> 1][e & 1][c], x0, x1);
+                                const uint32_t bits = see[e] >> (8 * c + quad);
+                                y2[e >> 1][e & 1][c] = pg_two(bits & 1 ? x0 : -INFINITY, bits & 2 ? x1 : -INFINITY);
+                            }
+                    }
+#pragma unroll
+                    for (int c = 0; c < CG; c++) {
+                        float x0[4], x1[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) pg_one(y2[e >> 1][e & 1][c], x0[e], x1[e]);
+                        most[2 * c] = fmaxf(fmaxf(x0[0], x0[1]), fmaxf(x0[2], x0[3]));
+                        most[2 * c + 1] = fmaxf(fmaxf(x1[0], x1[1]), fmaxf(x1[2], x1[3]));
+                    }
+                    top = fmaxf(PG_LOW, pg_across<NR>(most, [](float x0, float x1) { return fmaxf(x0, x1); }));
+                } else {
+                    if (gaps) {
+#pragma unroll
+                        for (int r = 0; r < RT; r++)
+                            if (!(see[0] >> r & 1)) y[r] = -INFINITY;
+                    }
+                    top = PG_LOW;
+#pragma unroll
+                    for (int r = 0; r < RT; r++) {
+                        const float x = pg_redux_max(y[r]);
+                        if (lane == r) top = fmaxf(top, x);
+                    }
                 }
                 int *ref = s_ref[group][turn & 3];
-                if (lane < RT) atomicMax(&ref[lane], pg_order(fmaxf(run, top)));
+                if (owner) atomicMax(&ref[own], pg_order(fmaxf(run, top)));
                 ok = ps_bar_all(bar, 128, ok);
                 if (!ok) break;
                 const float was = run;
-                float now = PG_LOW, z = 0.f; // z: the reference, as the scores are: rounded up, so that no weight is above 1
-                if (lane < RT) {
-                    now = pg_unorder(ref[lane]);
-                    z = now == PG_LOW ? 0.f : __fmul_ru(now, fmaxf(qs, 0x1p-126f));
-                    if (fabsf(z) == INFINITY || (now != PG_LOW && qs != qs)) z = NAN;
-                }
+                run = pg_unorder(ref[own]);
+                float z = run == PG_LOW ? 0.f : __fmul_ru(run, fmaxf(qs, 0x1p-126f)); // the reference, as the scores are: rounded up, so that no weight is above 1
+                if (fabsf(z) == INFINITY || (run != PG_LOW && qs != qs)) z = NAN;
                 turn++;
-                run = now;
                 if (i >= 2 && !wait(&o_full[i & 1], ((i >> 1) - 1) & 1, 23)) continue; // (the weights of tile i - 2 are used up, its outputs are taken)
-                if (w == 0 && lane < RT) {
-                    s_m[i & 3][lane] = now == PG_LOW ? PG_LOW : z;
-                    if (lane == 0) s_vm[i & 3] = vmax;
+                if (w == 0 && owner) {
+                    s_m[i & 3][own] = run == PG_LOW ? PG_LOW : z;
+                    if (own == 0) s_vm[i & 3] = vmax;
                 }
-                if (__any_sync(0xffffffffu, lane < RT && now > was)) { // sums so far follow their references
-                    if (lane < RT) mine[lane] = pg_ex2((was == PG_LOW ? PG_LOW : __fmul_ru(was, fmaxf(qs, 0x1p-126f))) - z);
+                if (__any_sync(0xffffffffu, run > was)) { // sums so far follow their references
+                    if (owner) mine[own] = pg_ex2((was == PG_LOW ? PG_LOW : __fmul_ru(was, fmaxf(qs, 0x1p-126f))) - z);
                     __syncwarp();
-                    pg_rows<RT>(mine, [&](int r, float f) { l[r] *= f; });
+                    if constexpr (FRAG) {
+#pragma unroll
+                        for (int r = 0; r < NR; r++) l[r] *= mine[r / 2 * 8 + quad + (r & 1)];
+                    } else pg_rows<RT>(mine, [&](int r, float f) { l[r] *= f; });
                     __syncwarp();
                 }
-                if (lane < RT) mine[lane] = -z;
+                if (owner) mine[own] = -z;
                 __syncwarp();
-                const uint32_t to = ps_smem_u32(sm_p) + (i & 1) * C::P_BYTES + (slot >> 4) * 144 + (slot & 15);
+                // weights 2^23 + p, whose lower three bytes are the digits
+                const uint32_t to = ps_smem_u32(sm_p) + (i & 1) * C::P_BYTES;
+                if constexpr (FRAG) {
+                    pg_f2 z2[CG];
 #pragma unroll
-                for (int c = 0; c < RT; c += 8) { // (the numbers of eight rows come before the bytes go: the compiler keeps loads behind stores)
-                    constexpr int W = RT < 8 ? RT : 8;
-                    float f[8], zs[8];
+                    for (int c = 0; c < CG; c++) z2[c] = *reinterpret_cast<const pg_f2 *>(mine + 8 * c + quad);
+                    const pg_f2 one = pg_two(8388608.f, 8388608.f);
 #pragma unroll
-                    for (int e = 0; e < W && c + e < RT; e += 4) {
-                        *reinterpret_cast<float4 *>(f + e) = *reinterpret_cast<const float4 *>(factor + c + e);
-                        *reinterpret_cast<float4 *>(zs + e) = *reinterpret_cast<const float4 *>(mine + c + e);
-                    }
-                    uint32_t d[8];
+                    for (int h = 0; h < 2; h++) {
+                        const pg_f2 vq = h ? pg_two(vq1, vq1) : pg_two(vq0, vq0);
+                        uint32_t digit[3][CG];
 #pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        if (c + e < RT) {
-                            const float p = pg_ex2(fmaf(y[c + e], f[e], zs[e])); // (a slot that is not seen: -inf)
-                            l[c + e] += p;
-                            d[e] = __float_as_uint(fmaf(p, vq, 8388608.f)); // 2^23 + the weight: its lower three bytes are the digits
+                        for (int c = 0; c < CG; c++) {
+                            uint32_t d[4];
+#pragma unroll
+                            for (int b = 0; b < 2; b++) {
+                                float x0, x1;
+                                pg_one(pg_fma2(y2[h][b][c], qs2[c], z2[c]), x0, x1);
+                                x0 = pg_ex2(x0); x1 = pg_ex2(x1); // (a slot that is not seen: -inf)
+                                l[2 * c] += x0; l[2 * c + 1] += x1;
+                                pg_one(pg_fma2(pg_two(x0, x1), vq, one), x0, x1);
+                                d[2 * b] = __float_as_uint(x0); d[2 * b + 1] = __float_as_uint(x1);
+                            }
+                            const uint32_t lo = __byte_perm(d[0], d[1], 0x5140), hi = __byte_perm(d[2], d[3], 0x5140);
+                            digit[0][c] = __byte_perm(lo, hi, 0x5410);
+                            digit[1][c] = __byte_perm(lo, hi, 0x7632);
+                            digit[2][c] = __byte_perm(__byte_perm(d[0], d[1], 0x0062), __byte_perm(d[2], d[3], 0x0062), 0x5410);
                         }
 #pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        if (c + e < RT)
+                        for (int k = 0; k < 3; k++) pg_put_frag<CG>(to + (k * CG + (lane >> 3) % CG) * C::P_ROW + (2 * w + h) * 144 + (lane & 7) * 16, digit[k]);
+                    }
+                } else {
+                    float f[8], zs[8]; // (they come before the bytes go: the compiler keeps loads behind stores)
 #pragma unroll
-                            for (int k = 0; k < 3; k++) {
-                                const int col = k * RT + c + e;
-                                asm volatile("st.shared.u8 [%0], %1;" ::"r"(to + (col >> 3) * C::P_ROW + (col & 7) * 16), "r"(d[e] >> (8 * k)));
-                            }
+                    for (int e = 0; e < RT; e += 4) {
+                        *reinterpret_cast<float4 *>(f + e) = *reinterpret_cast<const float4 *>(factor + e);
+                        *reinterpret_cast<float4 *>(zs + e) = *reinterpret_cast<const float4 *>(mine + e);
+                    }
+                    const uint32_t byte = to + (2 * w + (lane >> 4)) * 144 + (lane & 15);
+#pragma unroll
+                    for (int r = 0; r < RT; r++) {
+                        const float p = pg_ex2(fmaf(y[r], f[r], zs[r]));
+                        l[r] += p;
+                        const uint32_t d = __float_as_uint(fmaf(p, vq0, 8388608.f));
+#pragma unroll
+                        for (int k = 0; k < 3; k++) {
+                            const int col = k * RT + r;
+                            asm volatile("st.shared.u8 [%0], %1;" ::"r"(byte + (col >> 3) * C::P_ROW + (col & 7) * 16), "r"(d >> (8 * k)));
+                        }
+                    }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
@@ -542,14 +682,19 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
             }
             // the run's sums
             if (!ok || (n >= 2 && !wait(&fin_free[n & 1], ((n >> 1) - 1) & 1, 24))) continue;
+            if constexpr (FRAG) {
+                const float x = pg_across<NR>(l, [](float x0, float x1) { return x0 + x1; });
+                if (owner) s_l[n & 1][warp][own] = x;
+            } else {
 #pragma unroll
-            for (int r = 0; r < RT; r++) {
-                float x = l[r];
+                for (int r = 0; r < RT; r++) {
+                    float x = l[r];
 #pragma unroll
-                for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-                if (lane == r) s_l[n & 1][warp][r] = x;
+                    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+                    if (lane == r) s_l[n & 1][warp][r] = x;
+                }
             }
-            if (w == 0 && lane < RT) s_mend[n & 1][group][lane] = run == PG_LOW ? PG_LOW : __fmul_ru(run, fmaxf(qs, 0x1p-126f));
+            if (w == 0 && owner) s_mend[n & 1][group][own] = run == PG_LOW ? PG_LOW : __fmul_ru(run, fmaxf(qs, 0x1p-126f));
             __syncwarp();
             if (lane == 0) ps_mbar_arrive(&fin[n & 1]);
         }
@@ -562,11 +707,13 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
         for (; ok && walk.next(sg); n++) {
             const PgAttnSeq &s = a.seq[sg.s];
             const int rows = min(s.n_tok * a.R - r0, RT);
-            float acc[MT][RT], M = PG_LOW;
+            constexpr int H = RT / 2 + RT % 2; // pairs of rows
+            pg_f2 acc[MT][H];
+            float M = PG_LOW;
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
-                for (int r = 0; r < RT; r++) acc[m][r] = 0.f;
+                for (int r = 0; r < H; r++) acc[m][r] = 0ull;
             for (int t = sg.t0; t < sg.t1; t++, i++) {
                 if (!wait(&o_full[i & 1], (i >> 1) & 1, 25)) break;
                 ps_tc_fence_after();
@@ -581,18 +728,18 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
                     __syncwarp();
                     if (lane < RT) mine[lane] = fo;
                     __syncwarp();
-                    pg_rows<RT>(mine, [&](int r, float f) {
 #pragma unroll
-                        for (int m = 0; m < MT; m++) acc[m][r] *= f;
-                    });
+                    for (int r = 0; r < H; r++) {
+                        const pg_f2 f = *reinterpret_cast<const pg_f2 *>(mine + 2 * r);
+#pragma unroll
+                        for (int m = 0; m < MT; m++) acc[m][r] = pg_mul2(acc[m][r], f);
+                    }
                 }
                 __syncwarp();
                 if (lane < RT) mine[lane] = fn;
                 __syncwarp();
-                float f[(RT + 3) / 4 * 4];
-                pg_rows<RT>(mine, [&](int r, float v) { f[r] = v; });
 #pragma unroll
-                for (int m = 0; m < MT; m++) pg_sums<RT>(tm_o + (i & 1) * MT * N + m * N + lane_at, [&](int r, float x) { acc[m][r] = fmaf(x, f[r], acc[m][r]); });
+                for (int m = 0; m < MT; m++) pg_sums<RT>(tm_o + (i & 1) * MT * N + m * N + lane_at, [&](int r, pg_f2 x) { acc[m][r] = pg_fma2(x, *reinterpret_cast<const pg_f2 *>(mine + 2 * r), acc[m][r]); });
                 ps_tc_fence_before();
                 __syncwarp();
                 if (lane == 0) ps_mbar_arrive(&o_free[i & 1]);
@@ -625,7 +772,9 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
 #pragma unroll
                     for (int r = 0; r < RT; r++) {
                         if (r >= rows) break;
-                        const float x = acc[m][r] * mine[r];
+                        float x0, x1;
+                        pg_one(acc[m][r / 2], x0, x1);
+                        const float x = (r & 1 ? x1 : x0) * mine[r];
                         if (a.bf16) static_cast<__nv_bfloat16 *>(a.out)[at] = __float2bfloat16_rn(x);
                         else static_cast<float *>(a.out)[at] = x;
                         at += D;
@@ -634,7 +783,11 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
                 } else {
 #pragma unroll
                     for (int r = 0; r < RT; r++)
-                        if (r < rows) a.part[(slot * RT + r) * D + d] = acc[m][r];
+                        if (r < rows) {
+                            float x0, x1;
+                            pg_one(acc[m][r / 2], x0, x1);
+                            a.part[(slot * RT + r) * D + d] = r & 1 ? x1 : x0;
+                        }
                 }
             }
             __syncwarp();
