@@ -394,7 +394,7 @@ int ps_serve_verify(PsServeCall *c, int32_t *ids, int32_t *path, int32_t *n_path
         for (; s0 + n < n_seqs && n < SV_VERIFY_SEQS; n++) v.first[n + 1] = v.first[n] + n_nodes[s0 + n];
         const int nodes = v.first[n];
         void *mem = nullptr;
-        if (int rc = c->workspace(c->user, 2 * sizeof(SvRowStats) * (size_t)nodes, &mem)) return rc;
+        if (int rc = c->workspace(c->user, 2 * (sizeof(SvRowStats) + 1) * (size_t)nodes, &mem)) return rc;
         SvRowStats *stats[2] = {static_cast<SvRowStats *>(mem), static_cast<SvRowStats *>(mem) + nodes};
         v.target = stats[0]; v.draft = stats[1];
         v.ids = ids; v.path = path; v.n_path = n_path; v.parents = parents; v.tokens = tokens; v.logits = logits; v.draft_logits = draft_logits; v.samplers = samplers; v.draft_samplers = draft_samplers;
@@ -404,26 +404,36 @@ int ps_serve_verify(PsServeCall *c, int32_t *ids, int32_t *path, int32_t *n_path
         at[0].id = cudaLaunchAttributeClusterDimension;
         at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
         cfg.blockDim = dim3(SV_SMP_THREADS); cfg.stream = c->stream; cfg.attrs = at; cfg.numAttrs = 1;
-        for (int d = 0; d < (draft_logits ? 2 : 1); d++) {
-            SvStats a{};
-            a.s.logits = d ? draft_logits : logits; a.s.samplers = d ? draft_samplers : samplers; a.s.row_stride = row_stride; a.s.vocab = (int)vocab; a.s.stats = stats[d];
-            a.parents = d ? parents : nullptr; a.n_seqs = n;
-            std::copy(v.first, v.first + n + 1, a.first);
-            const int C = nodes * 16 <= c->n_sm ? 16 : 8; // (as in ps_serve_sample)
-            a.s.chunk = (int)((vocab + C - 1) / C + 31) & ~31;
-            a.s.vec = aligned(a.s.logits, 16) && row_stride % 4 == 0;
-            const size_t smem = sizeof(SvSmpShared) + 4 * (size_t)a.s.chunk;
+        auto chunk_of = [&](int C) { return (int)((vocab + C - 1) / C + 31) & ~31; };
+        const int all = nodes * (draft_logits ? 2 : 1);
+        SvStats a{};
+        a.logits[0] = logits; a.logits[1] = draft_logits; a.samplers[0] = samplers; a.samplers[1] = draft_samplers; a.stats[0] = stats[0]; a.stats[1] = stats[1]; a.parents = parents; a.row_stride = row_stride;
+        a.vocab = (int)vocab; a.n_seqs = n;
+        for (int d = 0; d < 2; d++) a.vec[d] = aligned(a.logits[d], 16) && row_stride % 4 == 0;
+        std::copy(v.first, v.first + n + 1, a.first);
+        if (all > 2 * c->n_sm / 8) { // (more rows than clusters run at once)
+            a.todo = reinterpret_cast<uint8_t *>(stats[1] + nodes);
+            sv_k_rows<<<all, SV_SMP_THREADS, 0, c->stream>>>(a);
+            SV_LAUNCHED("verify");
+        }
+        {
+            const int C = all * 16 <= c->n_sm ? 16 : 8; // (as in ps_serve_sample)
+            a.chunk = chunk_of(C);
+            const size_t smem = sizeof(SvSmpShared) + 4 * (size_t)a.chunk;
             at[0].val.clusterDim.x = C;
-            cfg.gridDim = dim3(nodes * C); cfg.dynamicSmemBytes = smem;
+            at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            at[1].val.programmaticStreamSerializationAllowed = 1;
+            cfg.numAttrs = a.todo ? 2 : 1;
+            cfg.gridDim = dim3(all * C); cfg.dynamicSmemBytes = smem;
             SV_CK(cudaFuncSetAttribute(sv_k_stats, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
             SV_CK(cudaFuncSetAttribute(sv_k_stats, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
             SV_CK(cudaLaunchKernelEx(&cfg, sv_k_stats, a));
             SV_LAUNCHED("verify");
         }
         const int C = n * 16 <= c->n_sm * 2 ? 16 : 8;
+        v.chunk = chunk_of(C);
         at[0].val.clusterDim.x = C;
-        cfg.gridDim = dim3(n * C); cfg.dynamicSmemBytes = 0;
-        v.chunk = (int)((vocab + C - 1) / C + 31) & ~31;
+        cfg.gridDim = dim3(n * C); cfg.dynamicSmemBytes = 0; cfg.numAttrs = 1;
         SV_CK(cudaFuncSetAttribute(sv_k_verify, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         SV_CK(cudaLaunchKernelEx(&cfg, sv_k_verify, v));
         SV_LAUNCHED("verify");

@@ -25,7 +25,7 @@
 #define SV_ONE (1ull << 44)
 
 // What the settings leave of a row: its tokens of which the number sv_key is at least kappa and the weight at least min_p, and their mass (0: one token alone, `only`; -1: none)
-struct SvRowStats {
+struct alignas(16) SvRowStats {
     unsigned long long kappa, all;
     float top;
     int only;
@@ -153,9 +153,26 @@ template <bool LIST, typename F> PS_D void sv_each(const SvSmpRow &r, const SvSm
         if (LIST || v > -INFINITY) f(v, sv_key(v, r.i0 + at));
     }
 }
-// the mass of all tokens of the warp
-PS_D unsigned long long sv_all(const SvSmpRow &r, const SvSmpShared &sh, const float *x) {
+// The mass of all tokens of the warp.  ROUGH: by float32 exponentials, off by less than 2^-21 of itself, for those that compare it with a test's random number: a bit of 2^-44 decides a draw among 100 000 tokens, but
+// not whether p(c) / q(c) is above u
+template <bool ROUGH> PS_D unsigned long long sv_all(const SvSmpRow &r, const SvSmpShared &sh, const float *x) {
     unsigned long long sum = 0;
+    if (ROUGH) {
+        const float rs = r.log2w.top == INFINITY ? 1.f : (float)r.log2w.s; // (beside an infinite logit all others weigh nothing)
+        float part[4] = {};
+        double all = 0.0;
+        for (int i = r.w0 + (threadIdx.x & 31), k = 0; i < r.w1; i += 128, k++) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float v = i + 32 * e < r.w1 ? x[i + 32 * e] : -INFINITY;
+                float w;
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(v == r.log2w.top ? 0.f : (v - r.log2w.top) * rs));
+                part[e] += v > -INFINITY ? w : 0.f;
+            }
+        }
+        all = ((double)part[0] + (double)part[1]) + ((double)part[2] + (double)part[3]);
+        return (unsigned long long)(all * (double)SV_ONE);
+    }
     for (int i = r.w0 + (threadIdx.x & 31); i < r.w1; i += 128) {
         unsigned long long w[4];
 #pragma unroll
@@ -353,7 +370,7 @@ template <bool LIST, bool STATS> PS_D void sv_pick(const SvSample &a, int64_t ro
         return w >= r.min_w ? w : 0;
     };
     unsigned long long mine = 0;
-    if (!LIST && !filters) mine = sv_all(r, sh, x);
+    if (!LIST && !filters) mine = sv_all<STATS>(r, sh, x);
     else sv_each<LIST>(r, sh, x, [&](float v, unsigned long long key) { mine += mass_of(v, key); });
 #pragma unroll
     for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
@@ -499,15 +516,29 @@ template <bool STATS> PS_D void sv_few(const SvSample &a, int64_t row, const SvS
     }
 }
 
+// what a row's settings ask for, once its largest logit is known (r.log2w.top); floor: the least one; reach: a number that top_k logits reach, or 0
+PS_D void sv_settings(SvSmpRow &r, float floor, uint32_t reach) {
+    r.log2w.s = 1.4426950408889634 / (double)r.p.temperature;
+    r.log2w.off = -(double)r.log2w.top * r.log2w.s;
+    if (r.log2w.top == INFINITY) { r.log2w.s = 0.0; r.log2w.off = -INFINITY; } // (all others weigh nothing)
+    r.use_k = r.p.top_k > 0 && r.p.top_k < r.vocab;
+    r.use_p = r.p.top_p < 1.f;
+    r.min_w = r.p.min_p > 0.f ? (unsigned long long)ceil((double)fminf(r.p.min_p, 1.f) * (double)SV_ONE) : 0;
+    // what lies `span` below the top in log2 w (and what a weight's rounding to 2^-44 takes for it), rounded outwards
+    auto down = [&](double span) { return r.log2w.s > 0.0 ? __double2float_rd((double)r.log2w.top - (span + 1e-8) / r.log2w.s) : -INFINITY; };
+    r.low = fmaxf(down(46.0), floor);
+    // (what weighs less than min_p goes in the end: it need not be listed, unless top-p asks for the mass of the top_k)
+    r.cut = fmaxf(down(r.min_w >= SV_ONE >> (int)SV_SMP_SPAN && !(r.use_k && r.use_p) ? -log2((double)fminf(r.p.min_p, 1.f)) : SV_SMP_SPAN), floor);
+    if (r.use_k && reach) r.cut = fmaxf(r.min_w >= SV_ONE >> (int)SV_SMP_SPAN && !r.use_p ? r.cut : floor, sv_unrank(reach));
+}
 // STATS: for the verification of drafted tokens, what the settings leave of the row
-template <bool STATS> PS_D void sv_sample(const SvSample &a) {
+template <bool STATS> PS_D void sv_sample(const SvSample &a, int64_t row) {
     extern __shared__ __align__(16) uint8_t sv_smp_raw[];
     SvSmpShared &sh = *reinterpret_cast<SvSmpShared *>(sv_smp_raw);
     float *x = reinterpret_cast<float *>(sv_smp_raw + sizeof(SvSmpShared));
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     SvMail mail(sh);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, C = mail.size;
-    const int64_t row = blockIdx.x / C;
     const float *from = a.logits + row * a.row_stride;
     SvSmpRow r;
     r.vocab = a.vocab;
@@ -583,19 +614,7 @@ template <bool STATS> PS_D void sv_sample(const SvSample &a) {
         }
         return; // (after the last barrier a CTA looks at its own memory alone)
     }
-    r.log2w.s = 1.4426950408889634 / (double)r.p.temperature;
-    r.log2w.off = -(double)r.log2w.top * r.log2w.s;
-    if (r.log2w.top == INFINITY) { r.log2w.s = 0.0; r.log2w.off = -INFINITY; } // (all others weigh nothing)
-    r.use_k = r.p.top_k > 0 && r.p.top_k < a.vocab;
-    r.use_p = r.p.top_p < 1.f;
-    r.min_w = r.p.min_p > 0.f ? (unsigned long long)ceil((double)fminf(r.p.min_p, 1.f) * (double)SV_ONE) : 0;
-    // what lies `span` below the top in log2 w (and what a weight's rounding to 2^-44 takes for it), rounded outwards
-    auto down = [&](double span) { return r.log2w.s > 0.0 ? __double2float_rd((double)r.log2w.top - (span + 1e-8) / r.log2w.s) : -INFINITY; };
-    const float floor = sv_unrank(worst);
-    r.low = fmaxf(down(46.0), floor);
-    // (what weighs less than min_p goes in the end: it need not be listed, unless top-p asks for the mass of the top_k)
-    r.cut = fmaxf(down(r.min_w >= SV_ONE >> (int)SV_SMP_SPAN && !(r.use_k && r.use_p) ? -log2((double)fminf(r.p.min_p, 1.f)) : SV_SMP_SPAN), floor);
-    if (r.use_k && reach) r.cut = fmaxf(r.min_w >= SV_ONE >> (int)SV_SMP_SPAN && !r.use_p ? r.cut : floor, sv_unrank(reach));
+    sv_settings(r, sv_unrank(worst), reach);
     const int run = ((r.n + SV_SMP_THREADS / 32 - 1) / (SV_SMP_THREADS / 32) + 31) & ~31;
     r.w0 = min(warp * run, r.n);
     r.w1 = min(r.w0 + run, r.n);
@@ -612,7 +631,7 @@ template <bool STATS> PS_D void sv_sample(const SvSample &a) {
         const bool exactly = r.use_p && !r.use_k && !least;
         const float rs = (float)r.log2w.s;
         float rough = 0.f, rough_in = 0.f;
-        if (exactly) whole = sv_block<false>(sh, sv_all(r, sh, x));
+        if (exactly) whole = sv_block<false>(sh, sv_all<STATS>(r, sh, x));
         for (int i = r.w0; i < r.w1; i += 128) {
             float v[4];
 #pragma unroll
@@ -667,7 +686,7 @@ template <bool STATS> PS_D void sv_sample(const SvSample &a) {
             if (roughly) {
                 if (1.002 * (double)all_in < (double)fmaxf(r.p.top_p, 0.f) * (double)whole) r.use_p = false;
                 else {
-                    const unsigned long long mine = sv_block<false>(sh, sv_all(r, sh, x));
+                    const unsigned long long mine = sv_block<false>(sh, sv_all<STATS>(r, sh, x));
                     const unsigned long long(*n)[16] = mail.post(mine);
                     whole = 0;
                     for (int o = 0; o < C; o++) whole += n[0][o];
@@ -691,4 +710,4 @@ template <bool STATS> PS_D void sv_sample(const SvSample &a) {
     if (listed) sv_pick<true, STATS>(a, row, r, sh, mail, x, kappa, filters);
     else sv_pick<false, STATS>(a, row, r, sh, mail, x, kappa, filters);
 }
-__global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_sample(const __grid_constant__ SvSample a) { sv_sample<false>(a); }
+__global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_sample(const __grid_constant__ SvSample a) { sv_sample<false>(a, blockIdx.x / cooperative_groups::this_cluster().num_blocks()); }

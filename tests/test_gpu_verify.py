@@ -131,6 +131,34 @@ def test_odd_rows(be):  # noqa: F811
         check(be, 200, [4] * 12, parents, tokens, u, logits, sets, g, gs)
 
 
+@pytest.mark.parametrize("kind", range(len(KINDS)))
+@pytest.mark.parametrize("V", [40, 3001])
+def test_odd_rows_under_every_kind_of_settings(be, kind, V):  # noqa: F811
+    """few rows, which clusters look at, and many, which a CTA each looks at first"""
+    for sizes in ([3, 2], [4] * 24):
+        for draft in (False, True):
+            parents, tokens, u, logits, sets, g, gs = make(V, sizes, 2, 20 + kind, draft=draft, kinds=[KINDS[kind]])
+            r = np.random.default_rng(kind)
+            for x in (logits,) if g is None else (logits, g):
+                x[r.integers(0, len(x), len(x) // 4), :] = 0.25                                  # all equal
+                x[r.integers(0, len(x), len(x) // 4), int(r.integers(0, V))] = np.inf
+                x[r.integers(0, len(x), len(x) // 8), :] = -np.inf
+                x[r.integers(0, len(x), len(x) // 4), ::2] = np.nan
+                x[r.integers(0, len(x), len(x) // 8), int(r.integers(0, V))] = 80.0
+            check(be, V, sizes, parents, tokens, u, logits, sets, g, gs)
+
+
+def test_rows_that_a_cta_cannot_decide(be):  # noqa: F811
+    """many rows, flat ones: thousands of likely tokens; top_k above what is kept of them; a top-p whose border lies among the unlikely ones"""
+    V, sizes = 20000, [3] * 30
+    for draft in (False, True):
+        parents, tokens, u, logits, sets, g, gs = make(V, sizes, 1, 31, draft=draft, kinds=[(1.0, 0, 0.9, 0.0), (1.0, 3000, 1.0, 0.0), (2.0, 600, 0.7, 0.0), (1.0, 0, 0.99999, 0.0), (0.05, 0, 0.999, 0.0), (1.0, 0, 0.95, 0.5)])
+        for x in (logits,) if g is None else (logits, g):
+            x[::2] *= 0.1
+            x[1::7, 5] = 40.0
+        check(be, V, sizes, parents, tokens, u, logits, sets, g, gs)
+
+
 @pytest.mark.parametrize("u0", [0.0, 1.0 - 2.0 ** -24, 1.0, 2.0, -1.0, np.nan])
 def test_random_numbers_at_the_ends(be, u0):  # noqa: F811
     for draft in (False, True):
