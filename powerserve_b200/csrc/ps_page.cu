@@ -147,7 +147,7 @@ int ps_serve_paged_attn(PsServeCall *c, const ps_cuda_pages *pages, int layer, v
     a.q = q; a.out = out; a.n_heads = n_heads; a.R = R; a.scale = scale * 1.4426950408889634f; a.bf16 = es == 2; a.q_vec = aligned(q, 4 * es);
     for (int i = 0, tok0 = 0; i < n_seqs;) {
         PgAttnSeq all[PG_SEQS];
-        int most = 0, n = 0;
+        int most = 0, n = 0; // most: query rows of a kv head
         int64_t tiles = 0;
         for (; i < n_seqs && n < PG_SEQS; i++) {
             const ps_cuda_paged_seq &s = seqs[i];
@@ -179,7 +179,15 @@ int ps_serve_paged_attn(PsServeCall *c, const ps_cuda_pages *pages, int layer, v
                 a.lane_tiles[z] = a.tile0[k];
                 total += a.lane_tiles[z];
             }
-            const int slots = c->n_sm * C::CTAS;
+            // CTAs of an SM, and the stages that their shares of its shared memory hold: two at least
+            static const int fixed = [&] { cudaFuncAttributes f{}; return cudaFuncGetAttributes(&f, kern) == cudaSuccess ? (int)f.sharedSizeBytes : 1 << 20; }();
+            const int stage = PG_TILE * hs;
+            int per_sm = C::CTAS, room;
+            while ((room = 233472 / per_sm - 1024 - fixed - 128 - C::tail(hs)) < 4 * stage && per_sm > 1) per_sm--;
+            room = std::min(room, 232448 - fixed - 128 - C::tail(hs)); // (what one CTA can have)
+            a.stages = std::min(PG_STAGES, room / (2 * stage));
+            if (a.stages < 2) return fail(c, PS_CUDA_ERR_CUDA, "paged_attn: no room for two stages in %d bytes of shared memory", room);
+            const int slots = c->n_sm * per_sm;
             // Nothing to join where no sequence has many more tiles than a fair share: the kernel that joins takes as long as four tiles
             int64_t units = 0;
             int longest = 0;
@@ -192,9 +200,6 @@ int ps_serve_paged_attn(PsServeCall *c, const ps_cuda_pages *pages, int layer, v
                 a.n_ctas += a.whole ? k * G : (int)std::max<int64_t>(1, std::min<int64_t>(a.lane_tiles[z], (int64_t)slots * a.lane_tiles[z] / total));
             }
             a.lane_cta0[a.n_lanes] = a.n_ctas;
-            // stages: what the CTAs' shares of shared memory hold
-            const int stage = PG_TILE * hs, room = (C::CTAS == 2 ? 112 : 220) * 1024 - 128 - C::tail(hs) - (C::SG == 1 ? 4096 : 9216);
-            a.stages = std::max(2, std::min(PG_STAGES, room / (2 * stage)));
             const size_t smem = 128 + (size_t)a.stages * 2 * stage + C::tail(hs);
             void *mem = nullptr;
             if (int rc = c->workspace(c->user, up(4 * (size_t)a.n_ctas * 2 * RT * (hs + 2)), &mem)) return rc;
@@ -217,8 +222,8 @@ int ps_serve_paged_attn(PsServeCall *c, const ps_cuda_pages *pages, int layer, v
                 cudaLaunchAttribute attr[1];
                 attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
                 attr[0].val.programmaticStreamSerializationAllowed = 1;
-                cfg2.gridDim = dim3((most + 7) / 8, G, n); cfg2.blockDim = dim3(256); cfg2.stream = c->stream; cfg2.attrs = attr; cfg2.numAttrs = 1;
-                PG_CK(cudaLaunchKernelEx(&cfg2, pg_k_join, a, RT));
+                cfg2.gridDim = dim3(a.n_ctas, (RT + 7) / 8); cfg2.blockDim = dim3(256); cfg2.stream = c->stream; cfg2.attrs = attr; cfg2.numAttrs = 1;
+                PG_CK(cudaLaunchKernelEx(&cfg2, pg_k_join<RT>, a));
                 PG_LAUNCHED("paged_attn");
             }
             return 0;

@@ -51,7 +51,7 @@ template <int RT_, int MT_, int SG_> struct PgCfg {
     static constexpr int W_OUT = 4 * SG, W_COPY = W_OUT + 4, W_MMA = W_COPY + 1, W_META = W_MMA + 2, W_Q = W_META + 1, THREADS = 32 * (W_Q + QW);
     static constexpr int COLS = 2 * N * (1 + MT), TM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
     static constexpr int P_ROW = 8 * 144, P_BYTES = N / 8 * P_ROW; // weights: sixteen slots' core matrices 144 bytes apart, so that a warp's bytes meet other banks
-    static constexpr int CTAS = MT == 1 && TM <= 256 ? 2 : 1;
+    static constexpr int CTAS = MT == 2 || TM > 256 ? 1 : RT > 8 ? 2 : 3; // of an SM, where shared memory allows
     static int tail(int hs) { return 2 * P_BYTES + 2 * N * hs; } // shared memory behind the rings
     static_assert(COLS <= 512, "tensor memory");
 };
@@ -242,24 +242,30 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
     const int r0 = rt * RT;
 
     ps_grid_dep_launch(); // (the kernel that joins may take its place: it waits for the end of this one)
-    if (tid == 0) {
-        for (int b = 0; b < PG_STAGES; b++) { ps_mbar_init(&k_full[b], 1); ps_mbar_init(&v_full[b], 1); ps_mbar_init(&k_free[b], 1); ps_mbar_init(&v_free[b], 1); }
-        for (int b = 0; b < 2; b++) {
-            ps_mbar_init(&s_full[b], 1); ps_mbar_init(&s_free[b], 4); ps_mbar_init(&p_full[b], 4); ps_mbar_init(&o_full[b], 1); ps_mbar_init(&o_free[b], 4);
-            ps_mbar_init(&q_full[b], C::QW); ps_mbar_init(&fin[b], 4 * SG); ps_mbar_init(&fin_free[b], 4);
+    // The copies' warp makes the barriers and goes on; the others meet when they and the tensor memory are there
+    if (warp == C::W_COPY) {
+        if (lane == 0) {
+            for (int b = 0; b < PG_STAGES; b++) { ps_mbar_init(&k_full[b], 1); ps_mbar_init(&v_full[b], 1); ps_mbar_init(&k_free[b], 1); ps_mbar_init(&v_free[b], 1); }
+            for (int b = 0; b < 2; b++) {
+                ps_mbar_init(&s_full[b], 1); ps_mbar_init(&s_free[b], 4); ps_mbar_init(&p_full[b], 4); ps_mbar_init(&o_full[b], 1); ps_mbar_init(&o_free[b], 4);
+                ps_mbar_init(&q_full[b], C::QW); ps_mbar_init(&fin[b], 4 * SG); ps_mbar_init(&fin_free[b], 4);
+            }
+            for (int b = 0; b < PG_META; b++) { ps_mbar_init(&meta_full[b], 1); ps_mbar_init(&meta_free[b], 4); }
+            ps_mbar_init(&done, 2);
+            ps_fence_barrier_init();
         }
-        for (int b = 0; b < PG_META; b++) { ps_mbar_init(&meta_full[b], 1); ps_mbar_init(&meta_free[b], 4); }
-        ps_mbar_init(&done, 2);
-        ps_fence_barrier_init();
+        __syncwarp();
+        asm volatile("barrier.cta.arrive 15, %0;" ::"n"(C::THREADS) : "memory");
+    } else {
+        if (warp == C::W_MMA) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ps_smem_u32(&s_tmem)), "n"(C::TM) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+        ps_tc_fence_before();
+        asm volatile("barrier.cta.sync 15, %0;" ::"n"(C::THREADS) : "memory");
+        ps_tc_fence_after();
     }
-    if (warp == C::W_MMA) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ps_smem_u32(&s_tmem)), "n"(C::TM) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    ps_tc_fence_before();
-    __syncthreads();
-    ps_tc_fence_after();
-    const uint32_t tm = __shfl_sync(0xffffffffu, s_tmem, 0), tm_o = tm + 2 * N;
+    const uint32_t tm = warp == C::W_COPY ? 0u : __shfl_sync(0xffffffffu, s_tmem, 0), tm_o = tm + 2 * N;
     PgWalk walk(a, rt);
     PgSeg sg;
     bool ok = true;
@@ -800,64 +806,74 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
 }
 
 // ---------------------------------------------------------------------------------------------------- joining the runs
-// A warp a row of kv head y of sequence z: the runs that share its tiles are found from where runs begin; its start overlaps the end of the kernel before
-__global__ void __launch_bounds__(256) pg_k_join(const __grid_constant__ PgAttn a, int RT) {
-    ps_grid_dep_wait();
-    const int lane = threadIdx.x & 31, D = a.pool.hs, g = blockIdx.y, si = blockIdx.z;
-    const PgAttnSeq &s = a.seq[si];
-    const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (row >= s.n_tok * a.R) return;
-    const int rt = row / RT, n = a.lane_cta0[rt + 1] - a.lane_cta0[rt], T = a.lane_tiles[rt];
-    const int u0 = a.tile0[si] + g * s.tiles, u1 = u0 + s.tiles;
-    const int q = T / n, more = T % n;
+// x: the beginning of a run, y: eight of its rows.  Where it lies inside the tiles of some sequence and head, and no run before it begins there, the block joins all runs that have some of them, a warp a row.  (A warp for every row of
+// the call, joined or not: 64 sequences 10 us of a kernel whose 512 blocks came in waves.)  Its start overlaps the end of the kernel before
+template <int RT> __global__ void __launch_bounds__(256) pg_k_join(const __grid_constant__ PgAttn a) {
+    int rt = 0;
+    while (rt + 1 < a.n_lanes && (int)blockIdx.x >= a.lane_cta0[rt + 1]) rt++;
+    const int k = blockIdx.x - a.lane_cta0[rt], n = a.lane_cta0[rt + 1] - a.lane_cta0[rt], T = a.lane_tiles[rt], q = T / n, more = T % n;
     auto of = [&](int x) { return x < more * (q + 1) ? x / (q + 1) : more + (x - more * (q + 1)) / q; }; // the run that has tile x
-    auto begins = [&](int k) { return q * k + min(k, more); };
-    const int k0 = of(u0), k1 = of(u1 - 1);
-    if (k0 == k1) return;
-    const float2 *ml = reinterpret_cast<const float2 *>(a.part + (int64_t)a.n_ctas * 2 * RT * D);
-    auto place = [&](int k) { // a run that begins before the row's tiles has come to them later
-        return ((int64_t)(a.lane_cta0[rt] + k) * 2 + (begins(k) < u0)) * RT + row % RT;
-    };
-    float top = PG_LOW, l = 0.f, acc[8] = {};
-    for (int k = k0 + lane; k <= k1; k += 32) top = fmaxf(top, ml[place(k)].x);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    for (int i0 = k0; i0 <= k1; i0 += 32) {
-        float f = 0.f;
-        int64_t at = 0;
-        if (i0 + lane <= k1) {
-            at = place(i0 + lane);
-            const float2 p = ml[at];
-            f = pg_ex2(p.x - top);
-            l = fmaf(p.y, f, l);
-        }
-        for (int i = 0; i < min(32, k1 + 1 - i0); i += 4) {
-            float v[4][8];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int64_t from = __shfl_sync(0xffffffffu, at, i + e);
-#pragma unroll
-                for (int c = 0; c < 8; c++)
-                    if (c * 32 < D && i0 + i + e <= k1) v[e][c] = a.part[from * D + c * 32 + lane];
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float fe = __shfl_sync(0xffffffffu, f, i + e);
-#pragma unroll
-                for (int c = 0; c < 8; c++)
-                    if (c * 32 < D && i0 + i + e <= k1) acc[c] = fmaf(v[e][c], fe, acc[c]);
-            }
-        }
+    auto begins = [&](int r) { return q * r + min(r, more); };
+    const int x = begins(k);
+    int lo = 0, hi = a.n_seqs - 1; // the last sequence that begins at or before x
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (a.tile0[mid] <= x) lo = mid;
+        else hi = mid - 1;
     }
+    const PgAttnSeq &s = a.seq[lo];
+    const int g = (x - a.tile0[lo]) / s.tiles, u0 = a.tile0[lo] + g * s.tiles, k0 = k - 1, k1 = of(u0 + s.tiles - 1);
+    if (k == 0 || x == u0 || begins(k - 1) > u0) return;
+    ps_grid_dep_wait();
+    const int lane = threadIdx.x & 31, D = a.pool.hs, rows = min(s.n_tok * a.R - rt * RT, RT);
+    const float2 *ml = reinterpret_cast<const float2 *>(a.part + (int64_t)a.n_ctas * 2 * RT * D);
+    const int r = blockIdx.y * 8 + (threadIdx.x >> 5);
+    if (r < rows) {
+        auto place = [&](int run) { // a run that begins before these tiles has come to them later
+            return ((int64_t)(a.lane_cta0[rt] + run) * 2 + (begins(run) < u0)) * RT + r;
+        };
+        float top = PG_LOW, l = 0.f, acc[8] = {};
+        for (int i = k0 + lane; i <= k1; i += 32) top = fmaxf(top, ml[place(i)].x);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int64_t to = ((int64_t)(s.tok0 + row / a.R) * a.n_heads + g * a.R + row % a.R) * D;
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int i0 = k0; i0 <= k1; i0 += 32) {
+            float f = 0.f;
+            int64_t at = 0;
+            if (i0 + lane <= k1) {
+                at = place(i0 + lane);
+                const float2 p = ml[at];
+                f = pg_ex2(p.x - top);
+                l = fmaf(p.y, f, l);
+            }
+            for (int i = 0; i < min(32, k1 + 1 - i0); i += 4) {
+                float v[4][8];
 #pragma unroll
-    for (int c = 0; c < 8; c++)
-        if (c * 32 < D) {
-            const float x = acc[c] * inv;
-            if (a.bf16) static_cast<__nv_bfloat16 *>(a.out)[to + c * 32 + lane] = __float2bfloat16_rn(x);
-            else static_cast<float *>(a.out)[to + c * 32 + lane] = x;
+                for (int e = 0; e < 4; e++) {
+                    const int64_t from = __shfl_sync(0xffffffffu, at, i + e);
+#pragma unroll
+                    for (int c = 0; c < 8; c++)
+                        if (c * 32 < D && i0 + i + e <= k1) v[e][c] = a.part[from * D + c * 32 + lane];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float fe = __shfl_sync(0xffffffffu, f, i + e);
+#pragma unroll
+                    for (int c = 0; c < 8; c++)
+                        if (c * 32 < D && i0 + i + e <= k1) acc[c] = fmaf(v[e][c], fe, acc[c]);
+                }
+            }
         }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int row = rt * RT + r;
+        const int64_t to = ((int64_t)(s.tok0 + row / a.R) * a.n_heads + g * a.R + row % a.R) * D;
+#pragma unroll
+        for (int c = 0; c < 8; c++)
+            if (c * 32 < D) {
+                const float y = acc[c] * inv;
+                if (a.bf16) static_cast<__nv_bfloat16 *>(a.out)[to + c * 32 + lane] = __float2bfloat16_rn(y);
+                else static_cast<float *>(a.out)[to + c * 32 + lane] = y;
+            }
+    }
 }
