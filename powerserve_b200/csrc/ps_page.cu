@@ -165,7 +165,7 @@ int ps_serve_paged_attn(PsServeCall *c, const ps_cuda_pages *pages, int layer, v
         auto launch = [&](auto cfg) -> int {
             using C = decltype(cfg);
             constexpr int RT = C::RT;
-            auto kern = pg_k_attn<C::RT, C::MT, C::SG>;
+            auto kern = pg_k_attn<C::RT, C::MT, C::SG, C::OG>;
             // those with more row tiles first: a run of row tiles is that of the first so many
             auto row_tiles = [&](const PgAttnSeq &s) { return (s.n_tok * R + RT - 1) / RT; };
             std::stable_sort(all, all + n, [&](const PgAttnSeq &x, const PgAttnSeq &y) { return row_tiles(x) > row_tiles(y); });
@@ -229,8 +229,8 @@ int ps_serve_paged_attn(PsServeCall *c, const ps_cuda_pages *pages, int layer, v
             return 0;
         };
         int rc;
-        if (hs <= 128) rc = most <= 5 ? launch(PgCfg<5, 1, 1>{}) : most <= 8 ? launch(PgCfg<8, 1, 1>{}) : most <= 16 ? launch(PgCfg<16, 1, 1>{}) : launch(PgCfg<32, 1, 2>{});
-        else rc = most <= 5 ? launch(PgCfg<5, 2, 1>{}) : launch(PgCfg<16, 2, 1>{});
+        if (hs <= 128) rc = most <= 5 ? launch(PgCfg<5, 1, 1, 1>{}) : most <= 8 ? launch(PgCfg<8, 1, 1, 1>{}) : most <= 16 ? launch(PgCfg<16, 1, 1, 1>{}) : launch(PgCfg<32, 1, 2, 2>{});
+        else rc = most <= 5 ? launch(PgCfg<5, 2, 1, 1>{}) : launch(PgCfg<16, 2, 1, 1>{});
         if (rc) return rc;
     }
     return 0;

@@ -44,15 +44,16 @@ struct PgAttn {
 PS_D bool pg_sees(const PgAttnSeq &s, int t, int back) { return back < 0 || (s.mask ? s.mask[t * s.n_tok + back] != 0 : back <= t); }
 PS_HD int pg_run(int tiles, int n, int k) { const int r = tiles % n; return tiles / n * k + (k < r ? k : r); } // where run k of n begins: the first ones have a tile more
 
-template <int RT_, int MT_, int SG_> struct PgCfg {
-    static constexpr int RT = RT_, MT = MT_, SG = SG_;         // query rows; products of 128 channels; soft-max groups
+template <int RT_, int MT_, int SG_, int OG_> struct PgCfg {
+    static constexpr int RT = RT_, MT = MT_, SG = SG_, OG = OG_; // query rows; products of 128 channels; soft-max groups, of alternate tiles; output groups, of shares of the rows
     static constexpr int N = (3 * RT + 15) / 16 * 16;          // columns of a product
     static constexpr int QW = RT > 16 ? 4 : RT > 10 ? 2 : 1;   // warps that cut queries
-    static constexpr int W_OUT = 4 * SG, W_COPY = W_OUT + 4, W_MMA = W_COPY + 1, W_META = W_MMA + 2, W_Q = W_META + 1, THREADS = 32 * (W_Q + QW);
-    static constexpr int COLS = 2 * N * (1 + MT), TM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+    static constexpr int SB = SG == 3 ? 3 : 2;                 // tiles of scores, and of weights, at a time
+    static constexpr int W_OUT = 4 * SG, W_COPY = W_OUT + 4 * OG, W_MMA = W_COPY + 1, W_META = W_MMA + 2, W_Q = W_META + 1, THREADS = 32 * (W_Q + QW);
+    static constexpr int COLS = N * (SB + 2 * MT), TM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
     static constexpr int P_ROW = 8 * 144, P_BYTES = N / 8 * P_ROW; // weights: sixteen slots' core matrices 144 bytes apart, so that a warp's bytes meet other banks
     static constexpr int CTAS = MT == 2 || TM > 256 ? 1 : RT > 8 ? 2 : 3; // of an SM, where shared memory allows
-    static int tail(int hs) { return 2 * P_BYTES + 2 * N * hs; } // shared memory behind the rings
+    static int tail(int hs) { return SB * P_BYTES + 2 * N * hs; } // shared memory behind the rings
     static_assert(COLS <= 512, "tensor memory");
 };
 
@@ -107,20 +108,21 @@ PS_D pg_f2 pg_fma2(pg_f2 a, pg_f2 b, pg_f2 c) { pg_f2 r; asm("fma.rn.f32x2 %0, %
 PS_D pg_f2 pg_digits2(int a0, int b0, int a1, int b1, int a2, int b2) {
     return pg_fma2(pg_two((float)a2, (float)b2), pg_two(65536.f, 65536.f), pg_two((float)(a1 * 256 + a0), (float)(b1 * 256 + b0)));
 }
-// the digits' sums of RT rows put together, f(pair of rows, sums): sixteen rows at a time
-template <int RT, typename F> PS_D void pg_sums(uint32_t at, F f) {
+// the digits' sums of RT rows put together, f(pair of rows, sums): sixteen rows at a time; a digit's columns begin STRIDE after the one before
+template <int RT, int STRIDE, typename F> PS_D void pg_sums(uint32_t at, F f) {
     if constexpr (RT % 16 == 0) {
 #pragma unroll
         for (int c = 0; c < RT; c += 16) {
             int a[16], b[16], d[16];
             pg_tm_ld16(a, at + c);
-            pg_tm_ld16(b, at + RT + c);
-            pg_tm_ld16(d, at + 2 * RT + c);
+            pg_tm_ld16(b, at + STRIDE + c);
+            pg_tm_ld16(d, at + 2 * STRIDE + c);
             ps_tc_ld_wait();
 #pragma unroll
             for (int r = 0; r < 16; r += 2) f((c + r) / 2, pg_digits2(a[r], a[r + 1], b[r], b[r + 1], d[r], d[r + 1]));
         }
     } else {
+        static_assert(RT == STRIDE, "");
         constexpr int N = (3 * RT + 15) / 16;
         int v[N][16];
 #pragma unroll
@@ -222,21 +224,21 @@ struct PgRing { // of a number known at launch: index and the parity of the roun
     }
 };
 
-template <int RT, int MT, int SG>
-__global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>::CTAS) pg_k_attn(const __grid_constant__ PgAttn a) {
-    using C = PgCfg<RT, MT, SG>;
-    constexpr int N = C::N;
+template <int RT, int MT, int SG, int OG>
+__global__ void __launch_bounds__(PgCfg<RT, MT, SG, OG>::THREADS, PgCfg<RT, MT, SG, OG>::CTAS) pg_k_attn(const __grid_constant__ PgAttn a) {
+    using C = PgCfg<RT, MT, SG, OG>;
+    constexpr int N = C::N, SB = C::SB;
     extern __shared__ __align__(128) uint8_t pg_raw[];
-    __shared__ __align__(8) uint64_t k_full[PG_STAGES], v_full[PG_STAGES], k_free[PG_STAGES], v_free[PG_STAGES], s_full[2], s_free[2], p_full[2], o_full[2], o_free[2], q_full[2], fin[2], fin_free[2],
+    __shared__ __align__(8) uint64_t k_full[PG_STAGES], v_full[PG_STAGES], k_free[PG_STAGES], v_free[PG_STAGES], s_full[SB], s_free[SB], p_full[SB], p_free[SB], o_full[2], o_free[2], q_full[2], fin[2], fin_free[2],
         meta_full[PG_META], meta_free[PG_META], done;
     __shared__ PgMeta s_meta[PG_META];
     __shared__ int s_ref[SG][4][RT];                                    // largest score / row factor so far, in order of whole numbers
-    __shared__ __align__(16) float s_row[SG * 4 + 4][2][(RT + 3) / 4 * 4]; // a warp's numbers of the rows
-    __shared__ float s_qs[2][RT], s_m[4][RT], s_vm[4], s_l[2][SG * 4][RT], s_mend[2][SG][RT];
+    __shared__ __align__(16) float s_row[SG * 4 + OG * 4][2][(RT + 3) / 4 * 4]; // a warp's numbers of the rows
+    __shared__ float s_qs[2][RT], s_m[8][RT], s_vm[8], s_l[2][SG * 4][RT], s_mend[2][SG][RT];
     __shared__ uint32_t s_tmem;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, D = a.pool.hs, stage = PG_TILE * D;
     // shared memory: K's ring, V's ring, weights, queries (a product of 128 channels of fewer reads behind its stage, never behind the queries)
-    uint8_t *sm_k = reinterpret_cast<uint8_t *>(((uintptr_t)pg_raw + 127) & ~(uintptr_t)127), *sm_v = sm_k + a.stages * stage, *sm_p = sm_v + a.stages * stage, *sm_q = sm_p + 2 * C::P_BYTES;
+    uint8_t *sm_k = reinterpret_cast<uint8_t *>(((uintptr_t)pg_raw + 127) & ~(uintptr_t)127), *sm_v = sm_k + a.stages * stage, *sm_p = sm_v + a.stages * stage, *sm_q = sm_p + SB * C::P_BYTES;
     int rt = 0; // row tile
     while (rt + 1 < a.n_lanes && (int)blockIdx.x >= a.lane_cta0[rt + 1]) rt++;
     const int r0 = rt * RT;
@@ -246,9 +248,10 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
     if (warp == C::W_COPY) {
         if (lane == 0) {
             for (int b = 0; b < PG_STAGES; b++) { ps_mbar_init(&k_full[b], 1); ps_mbar_init(&v_full[b], 1); ps_mbar_init(&k_free[b], 1); ps_mbar_init(&v_free[b], 1); }
+            for (int b = 0; b < SB; b++) { ps_mbar_init(&s_full[b], 1); ps_mbar_init(&s_free[b], 4); ps_mbar_init(&p_full[b], 4); ps_mbar_init(&p_free[b], 1); }
             for (int b = 0; b < 2; b++) {
-                ps_mbar_init(&s_full[b], 1); ps_mbar_init(&s_free[b], 4); ps_mbar_init(&p_full[b], 4); ps_mbar_init(&o_full[b], 1); ps_mbar_init(&o_free[b], 4);
-                ps_mbar_init(&q_full[b], C::QW); ps_mbar_init(&fin[b], 4 * SG); ps_mbar_init(&fin_free[b], 4);
+                ps_mbar_init(&o_full[b], 1); ps_mbar_init(&o_free[b], 4 * OG);
+                ps_mbar_init(&q_full[b], C::QW); ps_mbar_init(&fin[b], 4 * SG); ps_mbar_init(&fin_free[b], 4 * OG);
             }
             for (int b = 0; b < PG_META; b++) { ps_mbar_init(&meta_full[b], 1); ps_mbar_init(&meta_free[b], 4); }
             ps_mbar_init(&done, 2);
@@ -265,7 +268,10 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
         asm volatile("barrier.cta.sync 15, %0;" ::"n"(C::THREADS) : "memory");
         ps_tc_fence_after();
     }
-    const uint32_t tm = warp == C::W_COPY ? 0u : __shfl_sync(0xffffffffu, s_tmem, 0), tm_o = tm + 2 * N;
+    const uint32_t tm = warp == C::W_COPY ? 0u : __shfl_sync(0xffffffffu, s_tmem, 0), tm_o = tm + SB * N;
+    // 32 rows: 80 registers a thread at the launch, 480 over the six warpgroups; 2 x 112 (soft-max) + 2 x 80 (output) + 2 x 48 (the others) = 480
+    auto less = [] { if constexpr (RT == 32) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;"); };
+    auto more = [] { if constexpr (RT == 32) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;"); };
     PgWalk walk(a, rt);
     PgSeg sg;
     bool ok = true;
@@ -276,6 +282,7 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
     };
 
     if (warp == C::W_COPY) {
+        less();
         // ===== copies: a lane a page
         PgRing ring(a.stages);
         const int pages = PG_TILE >> a.pool.shift, bytes = a.pool.P * D;
@@ -312,6 +319,7 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
                 ps_tc_wait_warp(&v_full[b], round, PS_COPY_CYCLES);
             }
     } else if (warp == C::W_MMA || warp == C::W_MMA + 1) {
+        less();
         // ===== MMAs: scores by one warp, outputs by another, so that neither's waits hold up the other's
         const uint32_t id = (2u << 4) | (1u << 7) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(PG_TILE >> 4) << 24), id_s = id | (1u << 10); // whole numbers; K, V, queries signed, weights not
         const uint64_t d_k = ps_tc_smem_desc(ps_smem_u32(sm_k), 128, 8 * D), d_v = ps_tc_smem_desc(ps_smem_u32(sm_v), 16 * D, 128), d_q = ps_tc_smem_desc(ps_smem_u32(sm_q), 128, 8 * D),
@@ -323,11 +331,10 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
             if (!pv && !wait(&q_full[n & 1], (n >> 1) & 1, 12)) break;
             const uint64_t y0 = pv ? d_p : d_q + (uint64_t)((n & 1) * (N * D >> 4));
             for (int t = sg.t0; t < sg.t1; t++, i++) {
-                const int b = i & 1;
-                const uint32_t before = ((i >> 1) - 1) & 1; // (of tile i - 2)
-                if (pv) {
-                    if (!wait(&v_full[ring.i], ring.round, 15) || !wait(&p_full[b], (i >> 1) & 1, 16) || (i >= 2 && !wait(&o_free[b], before, 17))) break;
-                } else if (!wait(&k_full[ring.i], ring.round, 13) || (i >= 2 && !wait(&s_free[b], before, 14))) break;
+                const int b = i % SB, o = i & 1;
+                if (pv) { // (outputs of tile i - 2 are taken)
+                    if (!wait(&v_full[ring.i], ring.round, 15) || !wait(&p_full[b], (i / SB) & 1, 16) || (i >= 2 && !wait(&o_free[o], ((i >> 1) - 1) & 1, 17))) break;
+                } else if (!wait(&k_full[ring.i], ring.round, 13) || (i >= SB && !wait(&s_free[b], (i / SB - 1) & 1, 14))) break;
                 ps_tc_fence_after();
                 if (ps_elect_one()) {
                     if (pv) {
@@ -335,9 +342,10 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
 #pragma unroll
                         for (int m = 0; m < MT; m++)
 #pragma unroll
-                            for (int c = 0; c < PG_TILE / 32; c++) pg_mma_i8(tm_o + b * MT * N + m * N, x + 128 * m + 2 * D * c, y + 18 * c, id, c != 0);
+                            for (int c = 0; c < PG_TILE / 32; c++) pg_mma_i8(tm_o + o * MT * N + m * N, x + 128 * m + 2 * D * c, y + 18 * c, id, c != 0);
                         ps_tc_commit(&v_free[ring.i]);
-                        ps_tc_commit(&o_full[b]);
+                        ps_tc_commit(&p_free[b]);
+                        ps_tc_commit(&o_full[o]);
                     } else {
                         const uint64_t x = d_k + (uint64_t)(ring.i * (stage >> 4));
                         for (int c = 0; c < D / 32; c++) pg_mma_i8(tm + b * N, x + 16 * c, y0 + 16 * c, id_s, c != 0);
@@ -353,33 +361,47 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
         __syncwarp();
         if (!ps_tc_wait_warp(&done, 0)) *a.pool.err = 18;
     } else if (warp == C::W_META) {
-        // ===== scales and live slots, two tiles at a time: lanes 0-15 the first's blocks, K then V, 16-31 the second's
+        less();
+        // ===== scales and live slots, two tiles at a time: lanes 0-15 the first's blocks, K then V, 16-31 the second's.  What two tiles need is asked for while the two before are written, their pages one step
+        // earlier (asked for in turn, with a branch for every hidden byte: 1 450 cycles a tile, 3 100 with hidden slots, more than all other roles)
         const int half = lane >> 4, b = lane & 7, kv = lane >> 3 & 1, B = a.pool.P / PG_BLOCK;
         int i = 0;
         while (ok && walk.next(sg)) {
             const PgAttnSeq &s = a.seq[sg.s];
             auto page_of = [&](int t) {
-                const int j = t * PG_TILE + b * PG_BLOCK;
-                return t < sg.t1 && j < s.n_kv ? s.table[j >> a.pool.shift] : -2;
+                const int j = (t + half) * PG_TILE + b * PG_BLOCK;
+                return t + half < sg.t1 && j < s.n_kv ? s.table[j >> a.pool.shift] : -2;
             };
-            int ahead = page_of(sg.t0 + half);
+            auto is_page = [&](int page) { return (unsigned)page < (unsigned)a.pool.n_pages; }; // (the copies' warp reports)
+            auto scale_of = [&](int t, int page) {
+                return is_page(page) ? a.pool.scales[a.pool.at(page, sg.g, kv) * B + (((t + half) * PG_TILE + b * PG_BLOCK) & (a.pool.P - 1)) / PG_BLOCK] : 0.f;
+            };
+            auto hidden_of = [&](int t, int (&h)[8]) {
+#pragma unroll
+                for (int w = 0; w < 8; w++) h[w] = s.hidden ? s.hidden[min(t * PG_TILE + 32 * w + lane, s.n_kv - 1)] : 0;
+            };
+            int page = page_of(sg.t0), ahead = page_of(sg.t0 + 2), hidden[8];
+            float x = scale_of(sg.t0, page);
+            hidden_of(sg.t0, hidden);
             for (int t = sg.t0; ok && t < sg.t1; t += 2) {
-                const int page = ahead, j0 = (t + half) * PG_TILE;
-                ahead = page_of(t + 2 + half);
-                const bool have = page != -2 && (unsigned)page < (unsigned)a.pool.n_pages; // (the copies' warp reports)
-                float x = have ? a.pool.scales[a.pool.at(page, sg.g, kv) * B + ((j0 + b * PG_BLOCK) & (a.pool.P - 1)) / PG_BLOCK] : 0.f;
+                const bool have = is_page(page);
+                const float mine = x;
                 const unsigned has = __ballot_sync(0xffffffffu, have);
                 unsigned live[2][4];
 #pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        const int j = (t + h) * PG_TILE + 32 * w + lane;
-                        live[h][w] = __ballot_sync(0xffffffffu, j < s.n_kv && (has >> (16 * h + 2 * w + (lane >> 4)) & 1) && !(s.hidden && s.hidden[min(j, s.n_kv - 1)]));
-                    }
+                for (int w = 0; w < 8; w++) {
+                    const int j = t * PG_TILE + 32 * w + lane;
+                    live[w >> 2][w & 3] = __ballot_sync(0xffffffffu, (j < s.n_kv) & (has >> (16 * (w >> 2) + 2 * (w & 3) + (lane >> 4)) & 1) & (hidden[w] == 0));
+                }
+                page = ahead;
+                if (t + 2 < sg.t1) {
+                    x = scale_of(t + 2, page);
+                    hidden_of(t + 2, hidden);
+                    ahead = page_of(t + 4);
+                }
                 const unsigned word = half ? (b < 2 ? live[1][0] : b < 4 ? live[1][1] : b < 6 ? live[1][2] : live[1][3]) : (b < 2 ? live[0][0] : b < 4 ? live[0][1] : b < 6 ? live[0][2] : live[0][3]);
-                if (!(word >> (b & 1 ? 16 : 0) & 0xffffu)) x = 0.f; // (a block without live slots may have any scale)
-                float top = kv ? x : 0.f;
+                const float scale = word >> (b & 1 ? 16 : 0) & 0xffffu ? mine : 0.f; // (a block without live slots may have any scale)
+                float top = kv ? scale : 0.f;
 #pragma unroll
                 for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 #pragma unroll
@@ -388,8 +410,8 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
                     PgMeta &m = s_meta[i % PG_META];
                     if (i >= PG_META && !wait(&meta_free[i % PG_META], ((i / PG_META) - 1) & 1, 19)) break;
                     if (half == h) {
-                        if (kv) m.vq[b] = top > 0.f ? x / top * PG_ONE : 0.f;
-                        else m.ks[b] = x;
+                        if (kv) m.vq[b] = top > 0.f ? scale / top * PG_ONE : 0.f;
+                        else m.ks[b] = scale;
                         if ((lane & 15) < 4) m.live[lane & 3] = (lane & 3) == 0 ? live[h][0] : (lane & 3) == 1 ? live[h][1] : (lane & 3) == 2 ? live[h][2] : live[h][3];
                         if ((lane & 15) == 8) m.vmax = top * (1.f / PG_ONE);
                     }
@@ -400,6 +422,7 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
             }
         }
     } else if (warp >= C::W_Q) {
+        less();
         // ===== queries into digits, a warp a row
         int n = 0;
         for (; ok && walk.next(sg); n++) {
@@ -476,6 +499,7 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
             if (lane == 0) ps_mbar_arrive(&q_full[n & 1]);
         }
     } else if (warp < C::W_OUT) {
+        more();
         // ===== soft-max.  A warp that gave up a wait goes on to the group's next barrier, which tells the others: nobody is left alone at one.
         // RT a multiple of eight: a lane has four slots, lane / 4 and every eighth of its warp's behind it, and of every eight rows two, 2 (lane % 4) and the next; five rows: a slot and all rows.  The numbers of a
         // row (its reference, its factor) are those of the lanes whose `own` it is
@@ -503,7 +527,7 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
             ps_bar_sync(bar, 128);
             bool first = true;
             for (int t = sg.t0; t < sg.t1; t++, i++) {
-                if (SG > 1 && (i & 1) != group) continue;
+                if (SG > 1 && i % SG != group) continue;
                 wait(&meta_full[i % PG_META], (i / PG_META) & 1, 21);
                 const PgMeta &m = s_meta[i % PG_META];
                 const float ks0 = m.ks[FRAG ? 2 * w : 2 * w + (lane >> 4)], vq0 = m.vq[FRAG ? 2 * w : 2 * w + (lane >> 4)], ks1 = FRAG ? m.ks[2 * w + 1] : 0.f, vq1 = FRAG ? m.vq[2 * w + 1] : 0.f, vmax = m.vmax;
@@ -529,7 +553,7 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
                         }
                     }
                 }
-                wait(&s_full[i & 1], (i >> 1) & 1, 22);
+                wait(&s_full[i % SB], (i / SB) & 1, 22);
                 ps_tc_fence_after();
                 if (first) { // (they come with the first scores)
                     qs = s_qs[n & 1][own];
@@ -542,7 +566,7 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
                     first = false;
                 }
                 // scores over the rows' factors
-                const uint32_t at = tm + (i & 1) * N + ((uint32_t)(w * 32) << 16);
+                const uint32_t at = tm + i % SB * N + ((uint32_t)(w * 32) << 16);
                 pg_f2 y2[FRAG ? 2 : 1][2][CG];
                 float y[FRAG ? 1 : RT], top;
                 if constexpr (FRAG) {
@@ -562,7 +586,7 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
                             }
                     }
                 } else
-                    pg_sums<RT>(at, [&](int r, pg_f2 x) {
+                    pg_sums<RT, RT>(at, [&](int r, pg_f2 x) {
                         float x0, x1;
                         pg_one(x, x0, x1);
                         y[2 * r] = x0 * ks0;
@@ -570,7 +594,7 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
                     });
                 ps_tc_fence_before();
                 __syncwarp();
-                if (lane == 0) ps_mbar_arrive(&s_free[i & 1]);
+                if (lane == 0) ps_mbar_arrive(&s_free[i % SB]);
                 if constexpr (FRAG) {
                     float most[NR];
                     if (gaps) {
@@ -615,10 +639,10 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
                 float z = run == PG_LOW ? 0.f : __fmul_ru(run, fmaxf(qs, 0x1p-126f)); // the reference, as the scores are: rounded up, so that no weight is above 1
                 if (fabsf(z) == INFINITY || (run != PG_LOW && qs != qs)) z = NAN;
                 turn++;
-                if (i >= 2 && !wait(&o_full[i & 1], ((i >> 1) - 1) & 1, 23)) continue; // (the weights of tile i - 2 are used up, its outputs are taken)
+                if (i >= SB && !wait(&p_free[i % SB], (i / SB - 1) & 1, 23)) continue; // (the weights of tile i - SB are used up, so outputs before it are taken, and of eight places for references this one is free)
                 if (w == 0 && owner) {
-                    s_m[i & 3][own] = run == PG_LOW ? PG_LOW : z;
-                    if (own == 0) s_vm[i & 3] = vmax;
+                    s_m[i & 7][own] = run == PG_LOW ? PG_LOW : z;
+                    if (own == 0) s_vm[i & 7] = vmax;
                 }
                 if (__any_sync(0xffffffffu, run > was)) { // sums so far follow their references
                     if (owner) mine[own] = pg_ex2((was == PG_LOW ? PG_LOW : __fmul_ru(was, fmaxf(qs, 0x1p-126f))) - z);
@@ -632,7 +656,7 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
                 if (owner) mine[own] = -z;
                 __syncwarp();
                 // weights 2^23 + p, whose lower three bytes are the digits
-                const uint32_t to = ps_smem_u32(sm_p) + (i & 1) * C::P_BYTES;
+                const uint32_t to = ps_smem_u32(sm_p) + i % SB * C::P_BYTES;
                 if constexpr (FRAG) {
                     pg_f2 z2[CG];
 #pragma unroll
@@ -684,7 +708,7 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) ps_mbar_arrive(&p_full[i & 1]);
+                if (lane == 0) ps_mbar_arrive(&p_full[i % SB]);
             }
             // the run's sums
             if (!ok || (n >= 2 && !wait(&fin_free[n & 1], ((n >> 1) - 1) & 1, 24))) continue;
@@ -705,15 +729,16 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
             if (lane == 0) ps_mbar_arrive(&fin[n & 1]);
         }
     } else {
-        // ===== output: thread = channel (of each product)
-        const int w = warp - C::W_OUT, ch = w * 32 + lane;
+        // ===== output: thread = channel (of each product), a group its share of the rows
+        constexpr int RO = RT / OG;
+        const int share = (warp - C::W_OUT) >> 2, w = warp & 3, ch = w * 32 + lane, own = share * RO + min(lane, RO - 1), from = r0 + share * RO;
         const uint32_t lane_at = (uint32_t)(w * 32) << 16;
-        float *mine = s_row[SG * 4 + w][0];
+        float *mine = s_row[warp][0];
         int i = 0, n = 0;
         for (; ok && walk.next(sg); n++) {
             const PgAttnSeq &s = a.seq[sg.s];
-            const int rows = min(s.n_tok * a.R - r0, RT);
-            constexpr int H = RT / 2 + RT % 2; // pairs of rows
+            const int rows = min(s.n_tok * a.R - from, RO);
+            constexpr int H = RO / 2 + RO % 2; // pairs of rows
             pg_f2 acc[MT][H];
             float M = PG_LOW;
 #pragma unroll
@@ -724,15 +749,15 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
                 if (!wait(&o_full[i & 1], (i >> 1) & 1, 25)) break;
                 ps_tc_fence_after();
                 float fo = 1.f, fn = 0.f;
-                if (lane < RT) {
-                    const float m = s_m[i & 3][lane], top = fmaxf(M, m);
+                if (lane < RO) {
+                    const float m = s_m[i & 7][own], top = fmaxf(M, m);
                     fo = pg_ex2(M - top);
-                    fn = pg_ex2(m - top) * s_vm[i & 3];
+                    fn = pg_ex2(m - top) * s_vm[i & 7];
                     M = top;
                 }
                 if (__any_sync(0xffffffffu, fo != 1.f)) {
                     __syncwarp();
-                    if (lane < RT) mine[lane] = fo;
+                    if (lane < RO) mine[lane] = fo;
                     __syncwarp();
 #pragma unroll
                     for (int r = 0; r < H; r++) {
@@ -742,41 +767,41 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
                     }
                 }
                 __syncwarp();
-                if (lane < RT) mine[lane] = fn;
+                if (lane < RO) mine[lane] = fn;
                 __syncwarp();
 #pragma unroll
-                for (int m = 0; m < MT; m++) pg_sums<RT>(tm_o + (i & 1) * MT * N + m * N + lane_at, [&](int r, pg_f2 x) { acc[m][r] = pg_fma2(x, *reinterpret_cast<const pg_f2 *>(mine + 2 * r), acc[m][r]); });
+                for (int m = 0; m < MT; m++) pg_sums<RO, RT>(tm_o + (i & 1) * MT * N + m * N + share * RO + lane_at, [&](int r, pg_f2 x) { acc[m][r] = pg_fma2(x, *reinterpret_cast<const pg_f2 *>(mine + 2 * r), acc[m][r]); });
                 ps_tc_fence_before();
                 __syncwarp();
                 if (lane == 0) ps_mbar_arrive(&o_free[i & 1]);
             }
             if (!ok || !wait(&fin[n & 1], (n >> 1) & 1, 26)) break;
             float L = 0.f;
-            if (lane < RT) {
+            if (lane < RO) {
 #pragma unroll
                 for (int g = 0; g < SG; g++) {
                     float sum = 0.f;
 #pragma unroll
-                    for (int k = 0; k < 4; k++) sum += s_l[n & 1][g * 4 + k][lane];
-                    L = fmaf(sum, pg_ex2(s_mend[n & 1][g][lane] - M), L);
+                    for (int k = 0; k < 4; k++) sum += s_l[n & 1][g * 4 + k][own];
+                    L = fmaf(sum, pg_ex2(s_mend[n & 1][g][own] - M), L);
                 }
             }
             __syncwarp();
             if (lane == 0) ps_mbar_arrive(&fin_free[n & 1]);
             const bool whole = sg.t0 == 0 && sg.t1 == s.tiles;
-            if (lane < RT) mine[lane] = whole ? (L == 0.f ? 0.f : 1.f / L) : 1.f;
+            if (lane < RO) mine[lane] = whole ? (L == 0.f ? 0.f : 1.f / L) : 1.f;
             __syncwarp();
             const int64_t slot = (int64_t)blockIdx.x * 2 + (n > 0);
-            if (!whole && w == 0 && lane < RT) reinterpret_cast<float2 *>(a.part + (int64_t)a.n_ctas * 2 * RT * D)[slot * RT + lane] = make_float2(M, L);
+            if (!whole && w == 0 && lane < RO) reinterpret_cast<float2 *>(a.part + (int64_t)a.n_ctas * 2 * RT * D)[slot * RT + own] = make_float2(M, L);
 #pragma unroll
             for (int m = 0; m < MT; m++) {
                 const int d = m * 128 + ch;
                 if (d >= D) break;
                 if (whole) {
-                    int64_t at = ((int64_t)(s.tok0 + r0 / a.R) * a.n_heads + sg.g * a.R + r0 % a.R) * D + d;
-                    int rest = r0 % a.R;
+                    int64_t at = ((int64_t)(s.tok0 + from / a.R) * a.n_heads + sg.g * a.R + from % a.R) * D + d;
+                    int rest = from % a.R;
 #pragma unroll
-                    for (int r = 0; r < RT; r++) {
+                    for (int r = 0; r < RO; r++) {
                         if (r >= rows) break;
                         float x0, x1;
                         pg_one(acc[m][r / 2], x0, x1);
@@ -788,11 +813,11 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG>::THREADS, PgCfg<RT, MT, SG>:
                     }
                 } else {
 #pragma unroll
-                    for (int r = 0; r < RT; r++)
+                    for (int r = 0; r < RO; r++)
                         if (r < rows) {
                             float x0, x1;
                             pg_one(acc[m][r / 2], x0, x1);
-                            a.part[(slot * RT + r) * D + d] = r & 1 ? x1 : x0;
+                            a.part[(slot * RT + share * RO + r) * D + d] = r & 1 ? x1 : x0;
                         }
                 }
             }
