@@ -229,7 +229,7 @@ int ps_serve_paged_attn(PsServeCall *c, const ps_cuda_pages *pages, int layer, v
             return 0;
         };
         int rc;
-        if (hs <= 128) rc = most <= 5 ? launch(PgCfg<5, 1, 1, 1>{}) : most <= 8 ? launch(PgCfg<8, 1, 1, 1>{}) : most <= 16 ? launch(PgCfg<16, 1, 1, 1>{}) : launch(PgCfg<32, 1, 2, 2>{});
+        if (hs <= 128) rc = most <= 5 ? launch(PgCfg<5, 1, 1, 1>{}) : most <= 8 ? launch(PgCfg<8, 1, 1, 1>{}) : most <= 16 ? launch(PgCfg<16, 1, 1, 1>{}) : launch(PgCfg<32, 1, 3, 2>{});
         else rc = most <= 5 ? launch(PgCfg<5, 2, 1, 1>{}) : launch(PgCfg<16, 2, 1, 1>{});
         if (rc) return rc;
     }

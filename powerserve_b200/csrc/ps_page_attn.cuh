@@ -269,9 +269,9 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG, OG>::THREADS, PgCfg<RT, MT, 
         ps_tc_fence_after();
     }
     const uint32_t tm = warp == C::W_COPY ? 0u : __shfl_sync(0xffffffffu, s_tmem, 0), tm_o = tm + SB * N;
-    // 32 rows: 80 registers a thread at the launch, 480 over the six warpgroups; 2 x 112 (soft-max) + 2 x 80 (output) + 2 x 48 (the others) = 480
+    // 32 rows: 72 registers a thread at the launch, 504 over the seven warpgroups; 3 x 88 (soft-max) + 2 x 72 (output) + 2 x 48 (the others) = 504
     auto less = [] { if constexpr (RT == 32) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;"); };
-    auto more = [] { if constexpr (RT == 32) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;"); };
+    auto more = [] { if constexpr (RT == 32) asm volatile("setmaxnreg.inc.sync.aligned.u32 88;"); };
     PgWalk walk(a, rt);
     PgSeg sg;
     bool ok = true;
@@ -283,21 +283,32 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG, OG>::THREADS, PgCfg<RT, MT, 
 
     if (warp == C::W_COPY) {
         less();
-        // ===== copies: a lane a page
+        // ===== copies: a lane a page.  The pages' numbers come 32 at a time, before they are needed (a tile's asked for one tile ahead: 1 500 cycles a tile, whatever the other roles did)
         PgRing ring(a.stages);
-        const int pages = PG_TILE >> a.pool.shift, bytes = a.pool.P * D;
+        const int pages = PG_TILE >> a.pool.shift, bytes = a.pool.P * D, block = 32 / pages; // block: tiles whose pages the lanes hold
+        auto numbers = [&](const PgSeg &g, int t) {
+            const PgAttnSeq &s = a.seq[g.s];
+            const int p = t * pages + lane;
+            return t + lane / pages < g.t1 && p < (s.n_kv + a.pool.P - 1) >> a.pool.shift ? s.table[p] : -2;
+        };
         int i = 0;
-        while (ok && walk.next(sg)) {
-            const PgAttnSeq &s = a.seq[sg.s];
-            const int last = (s.n_kv + a.pool.P - 1) >> a.pool.shift;
-            auto page_of = [&](int t) {
-                const int p = t * pages + lane;
-                return lane < pages && p < last && t < sg.t1 ? s.table[p] : -2;
-            };
-            int ahead = page_of(sg.t0);
-            for (int t = sg.t0; t < sg.t1; t++, i++) {
-                const int page = ahead;
-                ahead = page_of(t + 1);
+        PgSeg next;
+        bool more = walk.next(next);
+        int first = more ? numbers(next, next.t0) : -2;
+        while (ok && more) {
+            sg = next;
+            int now = first, ahead = sg.t0 + block < sg.t1 ? numbers(sg, sg.t0 + block) : -2;
+            more = walk.next(next);
+            if (more) first = numbers(next, next.t0);
+            int at = 0; // tile of the block
+            for (int t = sg.t0; t < sg.t1; t++, i++, at++) {
+                if (at == block) {
+                    at = 0;
+                    now = ahead;
+                    if (t + block < sg.t1) ahead = numbers(sg, t + block);
+                }
+                int page = __shfl_sync(0xffffffffu, now, (at * pages + lane) & 31);
+                if (lane >= pages) page = -2;
                 const bool have = page != -2 && a.pool.has(page);
                 const uint32_t tx = __popc(__ballot_sync(0xffffffffu, have)) * (uint32_t)bytes;
                 const int8_t *src = have ? a.pool.codes + a.pool.at(page, sg.g, 0) * bytes : nullptr;
