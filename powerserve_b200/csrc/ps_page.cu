@@ -201,13 +201,7 @@ int ps_serve_paged_attn(PsServeCall *c, const ps_cuda_pages *pages, int layer, v
             }
             a.lane_cta0[a.n_lanes] = a.n_ctas;
             const size_t smem = 128 + (size_t)a.stages * 2 * stage + C::tail(hs);
-            void *mem = nullptr;
-            if (int rc = c->workspace(c->user, up(4 * (size_t)a.n_ctas * 2 * RT * (hs + 2)), &mem)) return rc;
-            a.part = static_cast<float *>(mem);
-            PG_CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-            kern<<<a.n_ctas, C::THREADS, smem, c->stream>>>(a);
-            PG_LAUNCHED("paged_attn");
-            // whether runs begin where rows' tiles do
+            // whether runs begin where rows' tiles do: nothing is left to join, and no memory asked for
             bool split = false;
             for (int z = 0; z < a.n_lanes && !split && !a.whole; z++) {
                 const int m = a.lane_cta0[z + 1] - a.lane_cta0[z];
@@ -217,6 +211,14 @@ int ps_serve_paged_attn(PsServeCall *c, const ps_cuda_pages *pages, int layer, v
                     split = (x - a.tile0[s]) % all[s].tiles != 0;
                 }
             }
+            if (split) {
+                void *mem = nullptr;
+                if (int rc = c->workspace(c->user, up(4 * (size_t)a.n_ctas * 2 * RT * (hs + 2)), &mem)) return rc;
+                a.part = static_cast<float *>(mem);
+            }
+            PG_CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            kern<<<a.n_ctas, C::THREADS, smem, c->stream>>>(a);
+            PG_LAUNCHED("paged_attn");
             if (split) {
                 cudaLaunchConfig_t cfg2{};
                 cudaLaunchAttribute attr[1];
