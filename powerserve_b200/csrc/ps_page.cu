@@ -256,6 +256,7 @@ int ps_serve_paged_edit(PsServeCall *c, const ps_cuda_pages *pages, const ps_cud
         if (e.from && e.n_new < e.n_old) return fail(c, PS_CUDA_ERR_INVALID, "paged_edit: edit %d shares %d tokens and shall hold %d", i, e.n_old, e.n_new);
         const int64_t need = pages_of(std::max(e.n_old, e.n_new), P);
         if (need > e.n_table) return fail(c, PS_CUDA_ERR_INVALID, "paged_edit: edit %d: %d tokens, its table has %d pages", i, std::max(e.n_old, e.n_new), e.n_table);
+        if (e.from && e.from == e.table) return fail(c, PS_CUDA_ERR_INVALID, "paged_edit: edit %d: a table that begins as itself", i);
         if ((need && !e.table) || !aligned(e.table, 4) || !aligned(e.from, 4)) return fail(c, PS_CUDA_ERR_INVALID, "paged_edit: edit %d has no table, or one that is not aligned to its elements", i);
         if (e.table) tables.push_back(e.table);
         a.op[i] = PgEditOp{e.table, e.from, e.n_old, e.n_new};

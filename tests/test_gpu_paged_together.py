@@ -149,7 +149,7 @@ def test_between_a_caller_s_operations(stream):  # noqa: F811
     be.close()
 
 
-@pytest.mark.parametrize("toks", [[20, 7, 1], [1, 1, 1]])
+@pytest.mark.parametrize("toks", [[20, 7, 1], [1, 1, 1], [20, 20, 12]])
 def test_captured_and_replayed(toks):
     """two graphs of one context, which share its workspace, replayed in turn with other inputs, and eager calls between them"""
     be = backend()

@@ -114,6 +114,7 @@ int main() {
     edit("odd table", I, "no table", [](ps_cuda_page_edit &e) { e.table = odd<int32_t>(); });
     edit("odd beginning", I, "no table", [](ps_cuda_page_edit &e) { e.from = odd<int32_t>(2); });
     edit("shares and shrinks", I, "shares", [](ps_cuda_page_edit &e) { e.from = reinterpret_cast<int32_t *>(mem + 64); e.n_new = 10; });
+    edit("begins as itself", I, "as itself", [](ps_cuda_page_edit &e) { e.from = e.table; });
     edit("odd answer", I, "aligned", [](ps_cuda_page_edit &) {}, odd<int32_t>());
     {
         ps_cuda_page_edit two[2] = {grow, grow};
