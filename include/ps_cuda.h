@@ -183,12 +183,12 @@ int ps_cuda_sample(ps_cuda_ctx *ctx, int32_t *ids, float *probs, const float *lo
 /* ---------------------------------------------------------------------------------------------- paged caches in 8 bits, drafted tokens
  * More serving operators, under the same rules (HOST arrays of records, device arrays, one call after another, one workspace, captures).  A cache of pages belongs to the caller: n_pages pages
  * of page_tokens slots (16, 32, 64 or 128) in each of n_layers layers, and a table of page numbers for every sequence: its slot j is slot j % page_tokens of page table[j / page_tokens], in all layers.
- * Sixteen slots are a block: in a block every kv head has one scale for K and one for V, and a number is code * scale, codes -127 .. 127.
+ * Sixteen slots are a block: in a block every kv head has one scale for K and one for V, and a number is code * scale, codes -127 .. 127 (what else a byte may hold is taken as it is).
  *   codes  [n_layers][n_pages][n_kv_heads][2: K, V][page_tokens * head_size], a page's as the tensor cores read them, blocks one after another:
  *          K: slot t, channel d at ((t / 8) * (head_size / 16) + d / 16) * 128 + (t % 8) * 16 + d % 16;   V: at ((t / 16) * head_size + d) * 16 + t % 16
  *   scales [n_layers][n_pages][n_kv_heads][2][page_tokens / 16] fp32
  *   refs   [n_pages] the tables that hold a page (0: it is free); ps_cuda_paged_edit alone reads and writes it
- * What a page holds behind its sequence's last slot may be anything.  A table's entry that is no page's number (they are checked on the device) is left out, nothing outside the cache is touched, and the next
+ * Scales are not negative. What a page holds behind its sequence's last slot may be anything.  A table's entry that is no page's number (they are checked on the device) is left out, nothing outside the cache is touched, and the next
  * ps_cuda_sync reports it.  codes are aligned to 16 bytes, all else to its elements; head_size: multiples of 32 up to 256.  io_type: PS_TYPE_F32 or PS_TYPE_BF16, of k, v, q and out. */
 #define PS_CUDA_BLOCK_TOKENS 16
 #define PS_CUDA_EDITS 512       /* edits of one call */
@@ -213,7 +213,8 @@ int ps_cuda_paged_store(ps_cuda_ctx *ctx, const ps_cuda_pages *pages, int layer,
 int ps_cuda_paged_load(ps_cuda_ctx *ctx, const ps_cuda_pages *pages, int layer, void *k, void *v, int io_type, const ps_cuda_paged_seq *seqs, int n_seqs);
 /* ps_cuda_attn_tree's attention over such a cache: out[t][h] = sum_j p_j v_j, p = soft-max of scale * q[t][h] . k_j over the slots that the token sees (tree_mask and hidden as there, n_tok <= 256, at most
  * 32 heads a kv head).  A token that sees nothing gets zeros, one with a query that holds no number or an infinite one, or with a score above float32's range, NaN.  out may be q.  Tables may share pages.
- * Precision: a query is held to 2^-23 of its row's largest number, its products with codes and their sums are exact; soft-max and sums have 32 bits, a weight is held to 2^-23 of the largest one of its row. */
+ * Precision: a query is held to 2^-23 of its row's largest number, its products with codes and their sums are exact; soft-max and sums have 32 bits, a weight (times its block's V scale) is held to
+ * 2^-22 of the largest one of its row (times the largest V scale of 128 slots). */
 int ps_cuda_paged_attn(ps_cuda_ctx *ctx, const ps_cuda_pages *pages, int layer, void *out, const void *q, int io_type, const ps_cuda_paged_seq *seqs, int n_seqs, int64_t n_heads,
                        const uint8_t *tree_mask, float scale);
 typedef struct {                /* one table's change */
@@ -222,11 +223,11 @@ typedef struct {                /* one table's change */
     int32_t n_old, n_new;       /* tokens that it holds (or shares), and that it shall have room for */
     int32_t n_table, reserved;  /* entries of `table`, at least n_new / page_tokens, rounded up (and those of n_old) */
 } ps_cuda_page_edit;
-/* Sequences fork, grow, shrink and end.  First all edits with `from` share pages (from is read as it was before the call), then all with n_new < n_old give back the pages behind n_new, then those with
+/* Sequences fork, grow, shrink and end.  (In a capture a call's lengths are those of the capture, the pages that are found free those of the replay.)  First all edits with `from` share pages (from is read as it was before the call), then all with n_new < n_old give back the pages behind n_new, then those with
  * n_new > n_old take pages in the order of the edits, the free pages of the lowest numbers first.  A sequence that grows is going to be written: where its last page is not full and another table holds it too, it takes a
  * page for itself, into which the filled blocks of all layers are copied (of several that grow from one page nobody else holds, the last one keeps it).  held [n] (device, may be NULL): the tokens that each table
  * holds now - n_new, or n_old for the first edit that finds too few free pages and those behind it that need one (or share a page with one before).
- * A table may appear once (as `from` as often as one likes).  At most PS_CUDA_EDITS edits. */
+ * A table may appear once (as `from` as often as one likes, not as its own).  A page given back that nobody holds stays free, and ps_cuda_sync reports it.  At most PS_CUDA_EDITS edits. */
 int ps_cuda_paged_edit(ps_cuda_ctx *ctx, const ps_cuda_pages *pages, const ps_cuda_page_edit *edits, int n, int32_t *held);
 typedef struct {                /* slots of one sequence that move together */
     const int32_t *table;
