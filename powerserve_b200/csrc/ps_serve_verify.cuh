@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_verify(const __grid_co
     constexpr int WARPS = SV_SMP_THREADS / 32;
     __shared__ double pow2[32], s_pc[PS_CUDA_TREE_TOKENS], s_qc[PS_CUDA_TREE_TOKENS];
     __shared__ unsigned long long mail[2][16], warp_sum[WARPS], s_w[PS_CUDA_TREE_TOKENS], s_all[PS_CUDA_TREE_TOKENS];
-    __shared__ int s_parent[PS_CUDA_TREE_TOKENS], s_token[PS_CUDA_TREE_TOKENS], s_path[PS_CUDA_TREE_TOKENS], s_gone[PS_CUDA_TREE_TOKENS];
+    __shared__ int s_parent[PS_CUDA_TREE_TOKENS], s_token[PS_CUDA_TREE_TOKENS], s_path[PS_CUDA_TREE_TOKENS], s_gone[PS_CUDA_TREE_TOKENS], s_last[PS_CUDA_TREE_TOKENS]; // s_last: a node's last child
     __shared__ float s_u[PS_CUDA_TREE_TOKENS];
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = cl.block_rank(), C = cl.num_blocks();
@@ -229,8 +229,10 @@ __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_verify(const __grid_co
         s_parent[i] = up;
         s_u[i] = a.u[base + i];
         s_token[i] = i > 0 && up >= 0 && up < i && c >= 0 && c < a.vocab ? c : -1; // (-1: never accepted)
+        s_last[i] = -1;
     }
     __syncthreads();
+    if (tid < n && s_token[tid] >= 0) atomicMax(&s_last[s_parent[tid]], tid);
     // what the tests ask for: a thread a node, all at once
     if (tid < n) {
         const int i = tid;
@@ -252,7 +254,7 @@ __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_verify(const __grid_co
     __syncthreads();
     SvDist p, q;
     int cur = 0, n_path = 1, n_gone = 0;
-    double t = 0.0, T = 1.0;
+    double t = 0.0, T = 1.0, before = 0.0; // before: t before the last rejection
     unsigned long long left = s_all[0]; // without a draft: mass of what p still has
     bool have = false;                  // p and q are row cur's
     const int i0 = min(rank * a.chunk, a.vocab), i1 = min(i0 + a.chunk, a.vocab);
@@ -341,24 +343,31 @@ __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_verify(const __grid_co
             left = s_all[i];
             t = 0.0; T = 1.0; n_gone = 0; have = false;
         } else if (a.draft_logits) {
-            const double t_was = t;
+            before = t;
             if (t == 0.0) have = false; // (q is asked for, too)
             t += T;
-            const unsigned long long *m = meet(warp_mass());
-            unsigned long long sum = 0;
-            for (int o = 0; o < C; o++) sum += m[o];
-            if (sum) T = (double)sum * (1.0 / SV_P_ONE);
-            else t = t_was;
+            if (s_last[cur] > i) { // (a sibling asks for T)
+                const unsigned long long *m = meet(warp_mass());
+                unsigned long long sum = 0;
+                for (int o = 0; o < C; o++) sum += m[o];
+                if (sum) T = (double)sum * (1.0 / SV_P_ONE);
+                else t = before;
+            }
         }
     }
     // the next token
-    const unsigned long long mine = warp_mass();
-    const unsigned long long *m = meet(mine);
-    unsigned long long before = 0, block = 0, all = 0;
-    for (int o = 0; o < C; o++) {
-        if (o < rank) before += m[o];
-        if (o == rank) block = m[o];
-        all += m[o];
+    unsigned long long mine, start, block, all;
+    for (int again = 0;; again++) {
+        mine = warp_mass();
+        const unsigned long long *m = meet(mine);
+        start = block = all = 0;
+        for (int o = 0; o < C; o++) {
+            if (o < rank) start += m[o];
+            if (o == rank) block = m[o];
+            all += m[o];
+        }
+        if (all || t == 0.0 || again) break;
+        t = before; // (nothing is left of p: it stays what it was)
     }
     if (rank == 0) {
         for (int i = tid; i < n; i += SV_SMP_THREADS) a.path[base + i] = i == 0 ? 0 : i < n_path ? s_path[i] : -1;
@@ -371,9 +380,9 @@ __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_verify(const __grid_co
     const float u = s_u[0];
     unsigned long long goal = u > 0.f ? (unsigned long long)((double)fminf(u, 1.f) * (double)all) : 0;
     goal = min(goal, all - 1);
-    if (goal < before || goal >= before + block) return;
-    for (int w = 0; w < warp; w++) before += warp_sum[w];
-    if (goal < before || goal >= before + mine) return;
+    if (goal < start || goal >= start + block) return;
+    for (int w = 0; w < warp; w++) start += warp_sum[w];
+    if (goal < start || goal >= start + mine) return;
     for (int i = w0; i < w1; i += 64) {
         unsigned long long w[2];
         masses(i + lane, w);
@@ -385,12 +394,12 @@ __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_verify(const __grid_co
                 const unsigned long long v = __shfl_up_sync(0xffffffffu, inc, o);
                 if (lane >= o) inc += v;
             }
-            const unsigned ball = __ballot_sync(0xffffffffu, goal < before + inc);
+            const unsigned ball = __ballot_sync(0xffffffffu, goal < start + inc);
             if (ball) {
                 if (lane == __ffs(ball) - 1) a.ids[seq] = i + 32 * e + lane;
                 return;
             }
-            before += __shfl_sync(0xffffffffu, inc, 31);
+            start += __shfl_sync(0xffffffffu, inc, 31);
         }
     }
 }
