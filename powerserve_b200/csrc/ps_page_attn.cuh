@@ -12,7 +12,9 @@
 //
 // A CTA takes a run of tiles (128 slots of one kv head and up to RT of its query rows), from one sequence and head into the next: all CTAs have the same number of tiles, whatever the sequences' lengths.  A run that does
 // not have all tiles of its rows leaves the sums in the workspace, and pg_k_join joins them.  Rows above RT are other CTAs', which take the same tiles at the same time (L2).
-// Roles: soft-max (SG groups of four warps, on alternate tiles), output (four), and a warp each for copies (a page's K or V of a head is one run of bytes), the MMAs of either product, scales and live slots, and queries.
+// Roles: soft-max (SG groups of four warps, tiles in turn), output (OG groups of four, likewise), and a warp each for copies (a page's K or V of a head is one run of bytes), the MMAs of either product, scales and live
+// slots, and queries.  One row a head: 64 sequences of up to 2 040 slots, 8 heads of 128, 33 us + 6 of pg_k_join: 5.5 TB/s while tiles stream, the rest is the CTAs' start and end.  32 rows: 2 x 32 tokens over 32 700 slots
+// 108 + 6: bound by the soft-max's instructions and waits (1 600 cycles for 128 slots x 32 rows), matrix pipe 23 %; three soft-max and two output groups 114, two and one 125, either one alone no better.
 #pragma once
 #include "ps_page.cuh"
 
