@@ -409,14 +409,14 @@ class PagedCache:
         self.refs = refs        # (kept: the addresses below are theirs)
         self.head_size, self.n_kv_heads = head_size, n_kv_heads
         at = [_dev(f"paged cache: {w}", a, be.device, n, [t]) for w, a, n, t in zip(("codes", "scales", "refs"), (self.codes, self.scales, refs), sizes, ("int8", "float32", "int32"))]
-        self.pages = Pages(*at, n_layers, n_pages, page_tokens, n_kv_heads, head_size, 0)
+        self.pages, self.device = Pages(*at, n_layers, n_pages, page_tokens, n_kv_heads, head_size, 0), be.device
         self.at = C.addressof(self.pages)
+        self.buffers = [b for b in (self.codes, self.scales, refs) if isinstance(b, DeviceBuffer)]
 
     def free(self):
         """gives back the DeviceBuffers"""
-        for b in (self.codes, self.scales, self.refs):
-            if isinstance(b, DeviceBuffer):
-                b.free()
+        for b in self.buffers:
+            b.free()
 
 
 class CudaBackend:
@@ -585,6 +585,14 @@ class CudaBackend:
             raise PsCudaError(f"{what}: a contiguous array of capi.{name} records")
         return a.ctypes.data
 
+    def _cache(self, what: str, cache):
+        if not isinstance(cache, PagedCache) or cache.device != self.device:
+            raise PsCudaError(f"{what}: a PagedCache in the memory of device {self.device}")
+        for b in cache.buffers:
+            if not b.ptr:
+                raise PsCudaError(f"{what}: a cache whose memory has been given back")
+        return cache.at
+
     def _rows(self, what: str, a, need: int, io_type):
         """address of rows and their type: a tensor's own, else io_type (None: float32)"""
         torch = sys.modules.get("torch")
@@ -597,12 +605,12 @@ class CudaBackend:
         return _dev(what, a, self.device, (4 if t == F32 else 2) * need), t
 
     def _paged_rows(self, what: str, call, cache, layer, k, v, seqs, io_type):
-        at = self._records(what, seqs, PAGED_SEQ, "PAGED_SEQ")
+        cache_at, at = self._cache(what, cache), self._records(what, seqs, PAGED_SEQ, "PAGED_SEQ")
         n = int(seqs["n_tok"].sum()) * cache.n_kv_heads * cache.head_size
         (k_at, t), (v_at, t_v) = self._rows(what, k, n, io_type), self._rows(what, v, n, io_type)
         if t != t_v and k is not None and v is not None:
             raise PsCudaError(f"{what}: k and v of two types")
-        self._in_turn(call, cache.at, layer, k_at, v_at, t_v if k is None else t, at, seqs.size)
+        self._in_turn(call, cache_at, layer, k_at, v_at, t_v if k is None else t, at, seqs.size)
 
     def paged_store(self, cache, layer: int, k, v, seqs: np.ndarray, io_type: Optional[int] = None):
         """rows of K and V into the last n_tok slots of each sequence"""
@@ -614,7 +622,7 @@ class CudaBackend:
 
     def paged_attn(self, cache, layer: int, out, q, seqs: np.ndarray, n_heads: int, scale: float, tree_mask=None, io_type: Optional[int] = None):
         """attention of a step's tokens over the sequences' pages"""
-        at = self._records("paged_attn", seqs, PAGED_SEQ, "PAGED_SEQ")
+        cache_at, at = self._cache("paged_attn", cache), self._records("paged_attn", seqs, PAGED_SEQ, "PAGED_SEQ")
         tok = seqs["n_tok"]
         n = int(tok.sum()) * max(n_heads, 0) * cache.head_size
         q_at, t = self._rows("paged_attn: q", q, n, io_type)
@@ -622,16 +630,16 @@ class CudaBackend:
         if t != t_out:
             raise PsCudaError("paged_attn: q and out of two types")
         mask = None if tree_mask is None else _dev("paged_attn: tree_mask", tree_mask, self.device, int((tok.astype(np.int64) ** 2).sum()), ["uint8", "bool", "int8"])
-        self._in_turn(self.L.ps_cuda_paged_attn, cache.at, layer, out_at, q_at, t, at, seqs.size, n_heads, mask, scale)
+        self._in_turn(self.L.ps_cuda_paged_attn, cache_at, layer, out_at, q_at, t, at, seqs.size, n_heads, mask, scale)
 
     def paged_edit(self, cache, edits: np.ndarray, held=None):
         """sequences fork, grow, shrink and end (PAGE_EDIT records); held: int32 on the device, the tokens that each has room for then"""
-        at = self._records("paged_edit", edits, PAGE_EDIT, "PAGE_EDIT")
-        self._in_turn(self.L.ps_cuda_paged_edit, cache.at, at, edits.size, _dev("paged_edit: held", held, self.device, 4 * edits.size, ["int32"]))
+        cache_at, at = self._cache("paged_edit", cache), self._records("paged_edit", edits, PAGE_EDIT, "PAGE_EDIT")
+        self._in_turn(self.L.ps_cuda_paged_edit, cache_at, at, edits.size, _dev("paged_edit: held", held, self.device, 4 * edits.size, ["int32"]))
 
     def paged_compact(self, cache, moves: np.ndarray):
         """kept slots move together, in all layers (PAGE_MOVE records)"""
-        self._in_turn(self.L.ps_cuda_paged_compact, cache.at, self._records("paged_compact", moves, PAGE_MOVE, "PAGE_MOVE"), moves.size)
+        self._in_turn(self.L.ps_cuda_paged_compact, self._cache("paged_compact", cache), self._records("paged_compact", moves, PAGE_MOVE, "PAGE_MOVE"), moves.size)
 
     def verify(self, ids, path, n_path, n_nodes, parents, tokens, logits, vocab: int, samplers, u, draft_logits=None, draft_samplers=None, row_stride: Optional[int] = None):
         """drafted tokens are accepted or rejected, the next ones drawn (all arrays on the device but n_nodes); row_stride: floats from row to row of both matrices (None: as the target's says)"""

@@ -261,3 +261,28 @@ def test_arguments_that_python_refuses():
     names = [n for n, _ in be.calls]
     assert names == ["ps_cuda_paged_store", "ps_cuda_paged_load", "ps_cuda_paged_attn", "ps_cuda_verify"]
     assert be.calls[0][1][2:5] == (16, 32, capi.BF16) and be.calls[1][1][2:5] == (None, 32, capi.F32)
+
+
+def test_caches_that_are_not_this_devices_or_have_no_memory():
+    be, other = _NoDevice(), _NoDevice()
+    other.device = 1
+    mine, theirs = (capi.PagedCache(b, 1, 4, 16, 2, 64, codes=4096, scales=8192, refs=12288) for b in (be, other))
+    seqs = np.zeros(1, capi.PAGED_SEQ)
+    calls = [lambda c: be.paged_store(c, 0, 16, 16, seqs), lambda c: be.paged_load(c, 0, 16, 16, seqs), lambda c: be.paged_attn(c, 0, 16, 16, seqs, 4, 1.0), lambda c: be.paged_edit(c, np.zeros(1, capi.PAGE_EDIT)),
+             lambda c: be.paged_compact(c, np.zeros(1, capi.PAGE_MOVE))]
+    for call in calls:
+        for bad in (theirs, None, 4096, mine.pages):
+            with pytest.raises(capi.PsCudaError, match="a PagedCache in the memory of device 0"):
+                call(bad)
+    for which in ("codes", "scales", "refs"):       # a buffer that was freed, by the cache or beside it
+        gone = capi.DeviceBuffer.__new__(capi.DeviceBuffer)
+        gone.be, gone.nbytes, gone.ptr = be, 1 << 20, 4096
+        cache = capi.PagedCache(be, 1, 4, 16, 2, 64, **{**dict(codes=4096, scales=8192, refs=12288), which: gone})
+        gone.ptr = None
+        for call in calls:
+            with pytest.raises(capi.PsCudaError, match="given back"):
+                call(cache)
+    assert not be.calls
+    for call in calls:
+        call(mine)
+    assert len(be.calls) == 5
