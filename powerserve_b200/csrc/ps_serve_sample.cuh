@@ -153,25 +153,23 @@ template <bool LIST, typename F> PS_D void sv_each(const SvSmpRow &r, const SvSm
         if (LIST || v > -INFINITY) f(v, sv_key(v, r.i0 + at));
     }
 }
+// A weight by a float32 exponential, as a whole number: so that sums of them do not depend on who adds them up.  rs: log2 e / temperature (beside an infinite logit, where all others weigh nothing, 1)
+PS_D unsigned long long sv_rough(float v, float top, float rs) {
+    float w;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(v == top ? 0.f : (v - top) * rs));
+    return v > -INFINITY ? (unsigned long long)(w * (float)SV_ONE) : 0;
+}
 // The mass of all tokens of the warp.  ROUGH: by float32 exponentials, off by less than 2^-21 of itself, for those that compare it with a test's random number: a bit of 2^-44 decides a draw among 100 000 tokens, but
-// not whether p(c) / q(c) is above u
+// not whether p(c) / q(c) is above u.  (Sums of the floats took as long, but differed by who added them up, and with them the border of a top-p among thousands of tokens.)
 template <bool ROUGH> PS_D unsigned long long sv_all(const SvSmpRow &r, const SvSmpShared &sh, const float *x) {
     unsigned long long sum = 0;
     if (ROUGH) {
-        const float rs = r.log2w.top == INFINITY ? 1.f : (float)r.log2w.s; // (beside an infinite logit all others weigh nothing)
-        float part[4] = {};
-        double all = 0.0;
-        for (int i = r.w0 + (threadIdx.x & 31), k = 0; i < r.w1; i += 128, k++) {
+        const float rs = r.log2w.top == INFINITY ? 1.f : (float)r.log2w.s;
+        for (int i = r.w0 + (threadIdx.x & 31); i < r.w1; i += 128) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float v = i + 32 * e < r.w1 ? x[i + 32 * e] : -INFINITY;
-                float w;
-                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(v == r.log2w.top ? 0.f : (v - r.log2w.top) * rs));
-                part[e] += v > -INFINITY ? w : 0.f;
-            }
+            for (int e = 0; e < 4; e++) sum += sv_rough(i + 32 * e < r.w1 ? x[i + 32 * e] : -INFINITY, r.log2w.top, rs);
         }
-        all = ((double)part[0] + (double)part[1]) + ((double)part[2] + (double)part[3]);
-        return (unsigned long long)(all * (double)SV_ONE);
+        return sum;
     }
     for (int i = r.w0 + (threadIdx.x & 31); i < r.w1; i += 128) {
         unsigned long long w[4];

@@ -141,19 +141,15 @@ __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_rows(const __grid_cons
     const bool filters = r.use_k || r.use_p || r.min_w, last = r.min_w >= SV_ONE >> (int)SV_SMP_SPAN; // last: min-p takes out all that is not listed
     const bool mass = !filters || (r.use_p && !r.use_k);
     const float rs = r.log2w.top == INFINITY ? 1.f : (float)r.log2w.s;
-    float sum = 0.f;
+    unsigned long long whole = 0;
     each([&](float v, int i) {
         if (filters && v >= r.cut && v > -INFINITY) {
             const uint32_t n = atomicAdd(&sh.n_list, 1u);
             if (n < SV_SMP_BINS) sh.list[n] = sv_key(v, i);
         }
-        if (mass) {
-            float w;
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(v == r.log2w.top ? 0.f : (v - r.log2w.top) * rs)); // (as sv_all's rough ones)
-            sum += v > -INFINITY ? w : 0.f;
-        }
+        if (mass) whole += sv_rough(v, r.log2w.top, rs);
     });
-    unsigned long long whole = mass ? sv_block<false>(sh, (unsigned long long)((double)sum * (double)SV_ONE)) : 0;
+    whole = sv_block<false>(sh, mass ? whole : 0);
     __syncthreads();
     if (!filters) {
         if (tid == 0) *to = SvRowStats{0, whole, r.log2w.top, 0};

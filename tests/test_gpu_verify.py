@@ -222,3 +222,20 @@ def test_sampling_is_what_it_was(be):  # noqa: F811
     assert np.array_equal(want.numpy(np.int32), ids) and (n_path == 1).all() and (path == 0).all()
     for b in up + [want]:
         b.free()
+
+
+def test_a_row_alone_and_among_many(be):  # noqa: F811
+    """Rows of nearly equal logits that fall with the token's number, and a random number that asks for the last token of what top-p leaves: the border is the same one whatever the call's other rows are"""
+    V, n = 100001, 48
+    r = np.random.default_rng(32)
+    logits = -np.sort((r.random((n, V)) * 0.2).astype(np.float32), axis=1)
+    kinds = [(1.0, 0, 0.7, 0.0), (1.0, 0, 1.0, 0.0), (0.7, 0, 0.6, 2.0 ** -10), (1.3, 60000, 0.9, 0.0), (1.1, 0, 0.35, 0.0)]
+    sets = S.settings([kinds[i % len(kinds)] for i in range(n)])
+    u = np.full(n, 1.0 - 2.0 ** -24, np.float32)
+    minus, zero = np.full(n, -1, np.int32), np.zeros(n, np.int32)
+    ids = run(be, V, [1] * n, minus, zero, u, logits, sets)[0]
+    assert len(set(ids.tolist())) > n // 2
+    for size in (1, 8, 20):
+        for i in range(0, n - size + 1, size):
+            e = slice(i, i + size)
+            assert np.array_equal(run(be, V, [1] * size, minus[e], zero[e], u[e], logits[e], sets[e])[0], ids[e]), (size, i)
