@@ -227,7 +227,7 @@ typedef struct {                /* one table's change */
  * n_new > n_old take pages in the order of the edits, the free pages of the lowest numbers first.  A sequence that grows is going to be written: where its last page is not full and another table holds it too, it takes a
  * page for itself, into which the filled blocks of all layers are copied (of several that grow from one page nobody else holds, the last one keeps it).  held [n] (device, may be NULL): the tokens that each table
  * holds now - n_new, or n_old for the first edit that finds too few free pages and those behind it that need one (or share a page with one before).
- * A table may appear once (as `from` as often as one likes, not as its own).  A page given back that nobody holds stays free, and ps_cuda_sync reports it.  At most PS_CUDA_EDITS edits. */
+ * A table may appear once (as `from` as often as one likes, but not its own, nor one that has a `from` in the same call).  A page given back that nobody holds stays free, and ps_cuda_sync reports it.  At most PS_CUDA_EDITS edits. */
 int ps_cuda_paged_edit(ps_cuda_ctx *ctx, const ps_cuda_pages *pages, const ps_cuda_page_edit *edits, int n, int32_t *held);
 typedef struct {                /* slots of one sequence that move together */
     const int32_t *table;

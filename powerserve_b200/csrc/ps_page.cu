@@ -249,7 +249,7 @@ int ps_serve_paged_edit(PsServeCall *c, const ps_cuda_pages *pages, const ps_cud
     const int P = pages->page_tokens;
     int64_t most = 0;
     int copies = 0;
-    std::vector<const void *> tables;
+    std::vector<const void *> tables, begun; // begun: those that share from now on
     for (int i = 0; i < n; i++) {
         const ps_cuda_page_edit &e = edits[i];
         if (e.n_old < 0 || e.n_new < 0 || e.n_old > 1 << 30 || e.n_new > 1 << 30) return fail(c, PS_CUDA_ERR_INVALID, "paged_edit: edit %d: from %d to %d tokens", i, e.n_old, e.n_new);
@@ -259,6 +259,7 @@ int ps_serve_paged_edit(PsServeCall *c, const ps_cuda_pages *pages, const ps_cud
         if (e.from && e.from == e.table) return fail(c, PS_CUDA_ERR_INVALID, "paged_edit: edit %d: a table that begins as itself", i);
         if ((need && !e.table) || !aligned(e.table, 4) || !aligned(e.from, 4)) return fail(c, PS_CUDA_ERR_INVALID, "paged_edit: edit %d has no table, or one that is not aligned to its elements", i);
         if (e.table) tables.push_back(e.table);
+        if (e.from && e.table) begun.push_back(e.table);
         a.op[i] = PgEditOp{e.table, e.from, e.n_old, e.n_new};
         if (e.n_new > e.n_old) {
             const bool part = e.n_old % P != 0;
@@ -268,6 +269,10 @@ int ps_serve_paged_edit(PsServeCall *c, const ps_cuda_pages *pages, const ps_cud
     }
     std::sort(tables.begin(), tables.end());
     if (std::adjacent_find(tables.begin(), tables.end()) != tables.end()) return fail(c, PS_CUDA_ERR_INVALID, "paged_edit: two edits of one table");
+    std::sort(begun.begin(), begun.end());
+    for (int i = 0; i < n && !begun.empty(); i++) // (all `from` are read while those tables are written)
+        if (edits[i].from && std::binary_search(begun.begin(), begun.end(), static_cast<const void *>(edits[i].from)))
+            return fail(c, PS_CUDA_ERR_INVALID, "paged_edit: edit %d begins as a table that begins anew in the same call", i);
     if (most > INT32_MAX / 8) return fail(c, PS_CUDA_ERR_UNSUPPORTED, "paged_edit: %lld pages in one call", (long long)most);
     void *mem = nullptr;
     const size_t list = up(sizeof(int4) * (size_t)n);

@@ -119,6 +119,13 @@ int main() {
     {
         ps_cuda_page_edit two[2] = {grow, grow};
         expect("a table twice", I, "one table", [&](PsServeCall *c) { return ps_serve_paged_edit(c, &good, two, 2, nullptr); });
+        ps_cuda_page_edit chain[3] = {grow, grow, grow}; // a table begins as one that begins as a third
+        for (int i = 0; i < 3; i++) { chain[i].table = reinterpret_cast<int32_t *>(mem) + 64 * (i + 1); chain[i].from = reinterpret_cast<int32_t *>(mem); }
+        expect("three begin as one", PS_CUDA_ERR_OOM, nullptr, [&](PsServeCall *c) { return ps_serve_paged_edit(c, &good, chain, 3, nullptr); });
+        for (int by : {0, 2}) {
+            chain[1].from = chain[by].table;
+            expect("a chain", I, "begins anew", [&](PsServeCall *c) { return ps_serve_paged_edit(c, &good, chain, 3, nullptr); });
+        }
         ps_cuda_pages p = good;
         p.refs = nullptr;
         expect("no counts", I, "without refs", [&](PsServeCall *c) { return ps_serve_paged_edit(c, &p, two, 1, nullptr); });
