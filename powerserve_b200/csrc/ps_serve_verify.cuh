@@ -7,7 +7,7 @@
 // sv_k_stats finds for every row what its settings leave of it (ps_serve_sample.cuh): a border and a mass.  (Rows that were looked at only when the walk came to them, by the cluster of the walk: 780 us for 64 sequences of
 // five nodes, of whose rows two thirds are looked at, where 580 took all of them at once.)  Then sv_k_verify: a cluster a sequence walks its tree - every CTA the same walk, whose tests ask for a few weights - and meets
 // for the passes: a sum for each rejection that a sibling or the draw asks about, and the draw.  Weights and sums are whole numbers, as there, so what is accepted does not depend on the launch.
-// 64 sequences of five nodes, rows and drafts' rows of 128 256 with mixed settings: 84 us for rows by a CTA each, 272 for those left to clusters (a row a microsecond, bound by the cluster's exchanges), 81 for the walks.
+// 64 sequences of five nodes, rows and drafts' rows of 128 256 with mixed settings: 86 us for rows by a CTA each, 272 for those left to clusters (a row a microsecond, bound by the cluster's exchanges), 81 for the walks.
 #pragma once
 #include "ps_serve_sample.cuh"
 
