@@ -216,6 +216,7 @@ __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_verify(const __grid_co
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = cl.block_rank(), C = cl.num_blocks();
     const int seq = blockIdx.x / C, base = a.first[seq], n = a.first[seq + 1] - base;
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     int turn = 0;
     if (tid < 32) pow2[tid] = exp2(tid / 32.0);
     __syncthreads();
@@ -315,6 +316,7 @@ __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_verify(const __grid_co
         cl.sync();
         return mail[turn];
     };
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); // (all CTAs are there, so `meet` may write to them)
     for (int i = 1; i < n; i++) {
         const int c = s_token[i];
         if (s_parent[i] != cur || c < 0) continue;

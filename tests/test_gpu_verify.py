@@ -239,3 +239,15 @@ def test_a_row_alone_and_among_many(be):  # noqa: F811
         for i in range(0, n - size + 1, size):
             e = slice(i, i + size)
             assert np.array_equal(run(be, V, [1] * size, minus[e], zero[e], u[e], logits[e], sets[e])[0], ids[e]), (size, i)
+
+
+@pytest.mark.parametrize("n", [1, 30, 700])
+def test_clusters_meet_soon_after_they_begin(be, n):  # noqa: F811
+    """sequences of their last tokens alone: nothing lies between a cluster's beginning and its first exchange but a row's record.  In few clusters, and in more than run at a time"""
+    r = np.random.default_rng(40 + n)
+    V = 3000
+    logits = (r.standard_normal((n, V)) * 3).astype(np.float32)
+    sets = S.settings([KINDS[i % len(KINDS)] for i in range(n)])
+    args = np.full(n, -1, np.int32), np.zeros(n, np.int32), r.random(n).astype(np.float32), logits, sets
+    for _ in range(3):
+        check(be, V, [1] * n, *args)
