@@ -53,10 +53,10 @@ struct SvVerify {
     int first[SV_VERIFY_SEQS + 1];
 };
 
-// settings whose rows a CTA alone hardly ever decides: many tokens, or the border of a mass that thousands of tokens share
+// settings whose rows a CTA alone hardly ever decides: many tokens, the border of a mass that thousands of tokens share, or a min-p that leaves tokens which are not listed
 PS_D bool sv_hard(const ps_cuda_sampler &p, int vocab) {
     const bool use_k = p.top_k > 0 && p.top_k < vocab;
-    return p.temperature > 0.f && (use_k ? p.top_k > SV_SMP_THREADS / 2 : p.top_p < 1.f && !(p.min_p >= 0x1p-16f));
+    return p.temperature > 0.f && (use_k ? p.top_k > SV_SMP_THREADS / 2 : (p.top_p < 1.f || p.min_p > 0.f) && !(p.min_p >= 0x1p-16f));
 }
 // a cluster a row.  Where sv_k_rows runs before it, its end overlaps this one's start: what it leaves for certain is not waited for
 __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_stats(const __grid_constant__ SvStats a) {
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_rows(const __grid_cons
         return;
     }
     const int n = (int)min(sh.n_list, (uint32_t)SV_SMP_BINS + 1);
-    bool known = n <= SV_SMP_BINS && (r.use_k ? n >= r.p.top_k || (last && !r.use_p) : true);
+    bool known = n <= SV_SMP_BINS && (r.use_k ? n >= r.p.top_k || (last && !r.use_p) : last);
     if (known && r.use_p && !r.use_k && !last) { // does the border lie among the listed?
         unsigned long long in = 0;
         for (int i = tid; i < n; i += SV_SMP_THREADS) in += sv_weight(sh, r.log2w(sv_logit(sh.list[i])));

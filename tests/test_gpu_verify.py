@@ -251,3 +251,29 @@ def test_clusters_meet_soon_after_they_begin(be, n):  # noqa: F811
     args = np.full(n, -1, np.int32), np.zeros(n, np.int32), r.random(n).astype(np.float32), logits, sets
     for _ in range(3):
         check(be, V, [1] * n, *args)
+
+
+@pytest.mark.parametrize("sizes", [[2] * 10, [2] * 24, [5] * 4, [5] * 12, [1] * 48])
+@pytest.mark.parametrize("min_p", [1e-5, 1e-7])
+@pytest.mark.parametrize("draft", [False, True])
+def test_a_min_p_below_what_is_listed(be, sizes, min_p, draft):  # noqa: F811
+    """One likely token and tens of thousands whose weights lie between min-p and 2^-16, which together hold about as much, and as many below min-p: few rows and many"""
+    V, n = 80000, sum(sizes)
+    r = np.random.default_rng([41, n, draft])
+
+    def rows():
+        least = np.log(min_p * 1.01)
+        x = r.uniform(max(least, np.log(1.15e-5)), np.log(1.5e-5), (n, V))
+        x[:, 1::2] = r.uniform(least, np.log(1.5e-5), (n, V // 2))
+        x[:, ::5] = np.log(min_p) - r.uniform(0.01, 8.0, x[:, ::5].shape)
+        x[:, 77] = 0.0
+        return (x + r.uniform(-3, 3, (n, 1))).astype(np.float32)
+    logits, guess = rows(), rows() if draft else None
+    sets = S.settings([(1.0, 0, 1.0, min_p)] * n)
+    u = r.random(n).astype(np.float32)
+    parents, tokens = np.concatenate([np.arange(m) - 1 for m in sizes]).astype(np.int32), np.full(n, 77, np.int32)
+    if draft:                               # (drafted tokens of p < q and of p > q)
+        guess[::3, 77] -= 0.7
+        tokens[::4] = r.integers(0, V // 2, len(tokens[::4])) * 2 + 1
+    n_path = check(be, V, sizes, parents, tokens, u, logits, sets, guess, sets if draft else None)
+    assert draft or sizes[0] == 1 or len(set(n_path.tolist())) > 1     # (the likely token's own share decides)
