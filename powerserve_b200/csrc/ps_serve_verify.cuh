@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_stats(const __grid_con
     ps_grid_dep_wait(); // (who comes after this kernel comes after the one before, too)
 }
 
-// A CTA a row, for many rows: the row is read twice, once from memory and once from L2, and only the likely tokens are kept.  What they do not decide (more than 1 024 of them, or fewer than top_k or top_p asks for) is left
+// A CTA a row, for many rows: the row is read twice, once from memory and once from L2, and only the likely tokens are kept.  What they do not decide (more than 1 024 of them, or fewer than top_k asks for) is left
 // to the clusters, which keep the row: those have 37 rows under way at a time, this 296
 __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_rows(const __grid_constant__ SvStats a) {
     __shared__ SvSmpShared sh;
@@ -156,14 +156,8 @@ __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_rows(const __grid_cons
         return;
     }
     const int n = (int)min(sh.n_list, (uint32_t)SV_SMP_BINS + 1);
-    bool known = n <= SV_SMP_BINS && (r.use_k ? n >= r.p.top_k || (last && !r.use_p) : last);
-    if (known && r.use_p && !r.use_k && !last) { // does the border lie among the listed?
-        unsigned long long in = 0;
-        for (int i = tid; i < n; i += SV_SMP_THREADS) in += sv_weight(sh, r.log2w(sv_logit(sh.list[i])));
-        in = sv_block<false>(sh, in);
-        known = in >= max(1ull, (unsigned long long)ceil((double)fmaxf(r.p.top_p, 0.f) * (double)whole));
-        __syncthreads();
-    }
+    // (beside a smaller min-p, top-p without top-k is not asked here: sv_hard)
+    const bool known = n <= SV_SMP_BINS && (r.use_k ? n >= r.p.top_k || (last && !r.use_p) : last);
     if (!known) {
         if (tid == 0) a.todo[blockIdx.x] = 1;
         return;
