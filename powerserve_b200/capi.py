@@ -642,12 +642,16 @@ class CudaBackend:
         self._in_turn(self.L.ps_cuda_paged_compact, self._cache("paged_compact", cache), self._records("paged_compact", moves, PAGE_MOVE, "PAGE_MOVE"), moves.size)
 
     def verify(self, ids, path, n_path, n_nodes, parents, tokens, logits, vocab: int, samplers, u, draft_logits=None, draft_samplers=None, row_stride: Optional[int] = None):
-        """drafted tokens are accepted or rejected, the next ones drawn (all arrays on the device but n_nodes); row_stride: floats from row to row of both matrices (None: as the target's says)"""
+        """drafted tokens are accepted or rejected, the next ones drawn (all arrays on the device but n_nodes); row_stride: floats from row to row of both matrices (None: as the target's says; a draft whose rows are padded otherwise is refused)"""
         n_nodes = np.ascontiguousarray(n_nodes, np.int32).reshape(-1)
         n, S = sum(n_nodes.tolist()), n_nodes.size
         if row_stride is None:
             row_stride = logits.stride(0) if not isinstance(logits, DeviceBuffer) and hasattr(logits, "stride") and logits.dim() == 2 and logits.shape[0] > 1 else vocab
         last = 4 * ((n - 1) * row_stride + vocab) if n > 0 and 0 < vocab <= min(row_stride, 1 << 18) else 0
+        torch = sys.modules.get("torch")
+        for w, a in (("logits", logits), ("draft_logits", draft_logits)):   # (where elements follow one another _dev asks for their number alone; a matrix of as many in another shape will do)
+            if torch is not None and isinstance(a, torch.Tensor) and a.dim() >= 2 and a.is_contiguous() and a.shape[-1] not in (row_stride, a.numel()) and a.numel() != n * row_stride:
+                raise PsCudaError(f"verify: {w}: rows {a.shape[-1]} floats apart, those of the call are {row_stride}")
         ints = [_dev(f"verify: {w}", a, self.device, 4 * k, ["int32"]) for w, a, k in (("ids", ids, S), ("path", path, n), ("n_path", n_path, S), ("parents", parents, n), ("tokens", tokens, n))]
         rows = [_dev(f"verify: {w}", a, self.device, last, ["float32"], row_stride) for w, a in (("logits", logits), ("draft_logits", draft_logits))]
         sets = [_dev(f"verify: {w}", a, self.device, SAMPLER.itemsize * n) for w, a in (("samplers", samplers), ("draft_samplers", draft_samplers))]

@@ -152,3 +152,33 @@ def test_calls_that_the_library_refuses_reach_it(be):
     attend(be, caches(13))
     attend(be, caches(-1))
     assert len(be.L.calls) == 8
+
+
+def verify(be, **change):
+    a = dict(ids=on_device(torch.zeros(2, dtype=torch.int32)), path=on_device(torch.zeros(5, dtype=torch.int32)), n_path=on_device(torch.zeros(2, dtype=torch.int32)), n_nodes=[2, 3],
+             parents=on_device(torch.zeros(5, dtype=torch.int32)), tokens=on_device(torch.zeros(5, dtype=torch.int32)), logits=on_device(torch.zeros(5, 10)), vocab=10, samplers=on_device(torch.zeros(5, 4)),
+             u=on_device(torch.zeros(5)), draft_logits=on_device(torch.zeros(5, 10)), draft_samplers=on_device(torch.zeros(5, 4))) | change
+    be.verify(**a)
+
+
+def test_verified_rows_that_lie_as_the_call_says(be):
+    """both matrices' rows are one distance apart: wider tensors and parts of them, buffers, and the same numbers in another shape"""
+    wide = on_device(torch.zeros(5, 16))
+    for strides in ({}, dict(logits=buffer(200)), dict(draft_logits=buffer(200)), dict(draft_logits=None, draft_samplers=None), dict(logits=on_device(torch.zeros(50))), dict(logits=on_device(torch.zeros(1, 5, 10))),
+                    dict(draft_logits=on_device(torch.zeros(10, 5)))):
+        verify(be, **strides)
+        assert be.L.calls.pop()[1][9] == 10
+    for strides in (dict(logits=wide, draft_logits=wide), dict(logits=wide[:, :10], draft_logits=wide[:, 6:]), dict(logits=wide, draft_logits=buffer(320)), dict(logits=buffer(320), draft_logits=wide, row_stride=16)):
+        verify(be, **strides)
+        assert be.L.calls.pop()[1][9] == 16
+
+
+@pytest.mark.parametrize("change", [
+    dict(draft_logits=on_device(torch.zeros(5, 16))), dict(draft_logits=on_device(torch.zeros(5, 16))[:, :10]), dict(logits=on_device(torch.zeros(5, 16))), dict(logits=on_device(torch.zeros(5, 16)), draft_logits=on_device(torch.zeros(9, 10))),
+    dict(logits=buffer(200), draft_logits=on_device(torch.zeros(5, 16))), dict(logits=on_device(torch.zeros(50)), draft_logits=on_device(torch.zeros(5, 16))), dict(logits=on_device(torch.zeros(1, 5, 16))),
+    dict(logits=on_device(torch.zeros(9, 10)), draft_logits=on_device(torch.zeros(9, 16)), row_stride=16), dict(draft_logits=on_device(torch.zeros(2, 5, 16)))])
+def test_verified_rows_that_lie_otherwise(be, change):
+    """a draft's rows that are padded further than the target's, or the other way: they would be read from the wrong places"""
+    with pytest.raises(capi.PsCudaError, match="verify: (draft_)?logits"):
+        verify(be, **change)
+    assert not be.L.calls
