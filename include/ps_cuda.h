@@ -214,7 +214,7 @@ int ps_cuda_paged_load(ps_cuda_ctx *ctx, const ps_cuda_pages *pages, int layer, 
 /* ps_cuda_attn_tree's attention over such a cache: out[t][h] = sum_j p_j v_j, p = soft-max of scale * q[t][h] . k_j over the slots that the token sees (tree_mask and hidden as there, n_tok <= 256, at most
  * 32 heads a kv head).  A token that sees nothing gets zeros, one with a query that holds no number or an infinite one, or with a score above float32's range, NaN.  out may be q.  Tables may share pages.
  * Precision: a query is held to 2^-23 of its row's largest number, its products with codes and their sums are exact; soft-max and sums have 32 bits, a weight (times its block's V scale) is held to
- * 2^-22 of the largest one of its row (times the largest V scale of 128 slots). */
+ * 2^-23 of the largest one that its row has in the same 128 slots (times their largest V scale), so what rounding leaves does not grow with the cache. */
 int ps_cuda_paged_attn(ps_cuda_ctx *ctx, const ps_cuda_pages *pages, int layer, void *out, const void *q, int io_type, const ps_cuda_paged_seq *seqs, int n_seqs, int64_t n_heads,
                        const uint8_t *tree_mask, float scale);
 typedef struct {                /* one table's change */

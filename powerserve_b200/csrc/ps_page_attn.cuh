@@ -8,7 +8,7 @@
 //
 // The cache is the MMAs' M side: scores^T[128 slots][rows x digits] = K Q^T, then out^T[channels][rows x digits] = V^T P^T, a lane of tensor memory a slot, then a channel.  A thread of the soft-max has a slot,
 // so its scales are its own, the row's largest score is a reduction over the warp (redux) and over four warps (an atomic of shared memory); a weight's digits are three bytes stored.  A thread of the
-// output has a channel: it adds a tile's sums to what it holds, so the accumulator sees one tile alone and tiles may have factors and references of their own.
+// output has a channel: it adds a tile's sums to what it holds, so the accumulator sees one tile alone, and tiles have factors and references of their own.
 //
 // A CTA takes a run of tiles (128 slots of one kv head and up to RT of its query rows), from one sequence and head into the next: all CTAs have the same number of tiles, whatever the sequences' lengths.  A run that does
 // not have all tiles of its rows leaves the sums in the workspace, and pg_k_join joins them.  Rows above RT are other CTAs', which take the same tiles at the same time (L2).
@@ -234,8 +234,9 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG, OG>::THREADS, PgCfg<RT, MT, 
     __shared__ __align__(8) uint64_t k_full[PG_STAGES], v_full[PG_STAGES], k_free[PG_STAGES], v_free[PG_STAGES], s_full[SB], s_free[SB], p_full[SB], p_free[SB], o_full[2], o_free[2], q_full[2], fin[2], fin_free[2],
         meta_full[PG_META], meta_free[PG_META], done;
     __shared__ PgMeta s_meta[PG_META];
-    __shared__ int s_ref[SG][4][RT];                                    // largest score / row factor so far, in order of whole numbers
+    __shared__ int s_ref[SG][4][RT];                                    // a tile's largest score / row factor, in order of whole numbers: four tiles' places in turn
     __shared__ __align__(16) float s_row[SG * 4 + OG * 4][2][(RT + 3) / 4 * 4]; // a warp's numbers of the rows
+    __shared__ __align__(16) float s_share[SG * 4][RT % 8 == 0 ? RT : 1]; // a warp's numbers of the rows: what a tile's weights count for in the row's sum
     __shared__ float s_qs[2][RT], s_m[8][RT], s_vm[8], s_l[2][SG * 4][RT], s_mend[2][SG][RT];
     __shared__ uint32_t s_tmem;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, D = a.pool.hs, stage = PG_TILE * D;
@@ -517,7 +518,7 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG, OG>::THREADS, PgCfg<RT, MT, 
         // RT a multiple of eight: a lane has four slots, lane / 4 and every eighth of its warp's behind it, and of every eight rows two, 2 (lane % 4) and the next; five rows: a slot and all rows.  The numbers of a
         // row (its reference, its factor) are those of the lanes whose `own` it is
         constexpr bool FRAG = RT % 8 == 0;
-        constexpr int CG = FRAG ? RT / 8 : 1, NR = 2 * CG, NS = FRAG ? 4 : 1, NL = FRAG ? NR : RT; // eights of rows; rows, slots, sums of a lane
+        constexpr int CG = FRAG ? RT / 8 : 1, NR = 2 * CG, NS = FRAG ? 4 : 1; // eights of rows; rows, slots of a lane
         const int group = warp >> 2, w = warp & 3, bar = SG == 1 ? 1 : 1 + group, quad = 2 * (lane & 3);
         const int idx = (lane >> 2) / (FRAG ? 8 / NR : 1), own = FRAG ? idx / 2 * 8 + quad + (idx & 1) : min(lane, RT - 1);
         const bool owner = FRAG ? (lane >> 2) % (FRAG ? 8 / NR : 1) == 0 : lane < RT;
@@ -527,11 +528,13 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG, OG>::THREADS, PgCfg<RT, MT, 
         for (; walk.next(sg); n++) {
             const PgAttnSeq &s = a.seq[sg.s];
             const int rows = min(s.n_tok * a.R - r0, RT), past = s.n_kv - s.n_tok;
-            float run = PG_LOW, qs = 0.f; // row own's largest score over its factor, and the factor
-            float l[NL];
-            pg_f2 qs2[CG];
+            float M = PG_LOW, qs = 0.f; // row own's largest score so far, and its factor
+            float l[FRAG ? 1 : RT];
+            pg_f2 l2[CG], qs2[CG];
 #pragma unroll
-            for (int r = 0; r < NL; r++) l[r] = 0.f;
+            for (int r = 0; r < (FRAG ? 1 : RT); r++) l[r] = 0.f;
+#pragma unroll
+            for (int c = 0; c < CG; c++) l2[c] = 0ull;
             ok = ps_bar_all(bar, 128, ok); // (a run begins: nobody of the group reads the last one's numbers any more)
             if (!ok) break;
             if (w * 32 + lane < RT)
@@ -644,29 +647,37 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG, OG>::THREADS, PgCfg<RT, MT, 
                     }
                 }
                 int *ref = s_ref[group][turn & 3];
-                if (owner) atomicMax(&ref[own], pg_order(fmaxf(run, top)));
+                if (owner) atomicMax(&ref[own], pg_order(top));
                 ok = ps_bar_all(bar, 128, ok);
                 if (!ok) break;
-                const float was = run;
-                run = pg_unorder(ref[own]);
-                float z = run == PG_LOW ? 0.f : __fmul_ru(run, fmaxf(qs, 0x1p-126f)); // the reference, as the scores are: rounded up, so that no weight is above 1
-                if (fabsf(z) == INFINITY || (run != PG_LOW && qs != qs)) z = NAN;
+                // A tile has a reference of its own, its largest score (of the slots that the row sees), so a weight is rounded by what counts in its tile, however heavy another one's is; the row's sum has the largest so
+                // far.  (Weights under the largest so far: behind a slot that has nearly all of the mass the others lost their bits, and below 2^-24 left the output but not the sum: 22 % of the output for 12 000 such.)
+                const float here = pg_unorder(ref[own]);
+                float top_z = here == PG_LOW ? PG_LOW : __fmul_ru(here, fmaxf(qs, 0x1p-126f)); // as the scores are, and rounded up, so that no weight is above 1
+                if (fabsf(top_z) == INFINITY || (here != PG_LOW && qs != qs)) top_z = NAN;
+                const float was = M, z = here == PG_LOW ? 0.f : top_z;
+                M = fmaxf(was, top_z);
                 turn++;
+                if (w == 0 && owner) s_ref[group][(turn + 2) & 3][own] = pg_order(PG_LOW); // (the place of the tile before: all have passed a barrier since they read it, and pass another before it is used)
                 if (i >= SB && !wait(&p_free[i % SB], (i / SB - 1) & 1, 23)) continue; // (the weights of tile i - SB are used up, so outputs before it are taken, and of eight places for references this one is free)
+                const float share = pg_ex2(top_z - M);
                 if (w == 0 && owner) {
-                    s_m[i & 7][own] = run == PG_LOW ? PG_LOW : z;
+                    s_m[i & 7][own] = top_z;
                     if (own == 0) s_vm[i & 7] = vmax;
                 }
-                if (__any_sync(0xffffffffu, run > was)) { // sums so far follow their references
-                    if (owner) mine[own] = pg_ex2((was == PG_LOW ? PG_LOW : __fmul_ru(was, fmaxf(qs, 0x1p-126f))) - z);
+                if (__any_sync(0xffffffffu, M > was)) { // sums so far follow their references
+                    if (owner) mine[own] = pg_ex2(was - M);
                     __syncwarp();
                     if constexpr (FRAG) {
 #pragma unroll
-                        for (int r = 0; r < NR; r++) l[r] *= mine[r / 2 * 8 + quad + (r & 1)];
+                        for (int c = 0; c < CG; c++) l2[c] = pg_mul2(l2[c], *reinterpret_cast<const pg_f2 *>(mine + 8 * c + quad));
                     } else pg_rows<RT>(mine, [&](int r, float f) { l[r] *= f; });
                     __syncwarp();
                 }
-                if (owner) mine[own] = -z;
+                if (owner) {
+                    mine[own] = -z;
+                    if (FRAG) s_share[warp][own] = share;
+                }
                 __syncwarp();
                 // weights 2^23 + p, whose lower three bytes are the digits
                 const uint32_t to = ps_smem_u32(sm_p) + i % SB * C::P_BYTES;
@@ -686,9 +697,9 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG, OG>::THREADS, PgCfg<RT, MT, 
                             for (int b = 0; b < 2; b++) {
                                 float x0, x1;
                                 pg_one(pg_fma2(y2[h][b][c], qs2[c], z2[c]), x0, x1);
-                                x0 = pg_ex2(x0); x1 = pg_ex2(x1); // (a slot that is not seen: -inf)
-                                l[2 * c] += x0; l[2 * c + 1] += x1;
-                                pg_one(pg_fma2(pg_two(x0, x1), vq, one), x0, x1);
+                                const pg_f2 p = pg_two(pg_ex2(x0), pg_ex2(x1)); // (a slot that is not seen: -inf)
+                                l2[c] = pg_fma2(p, *reinterpret_cast<const pg_f2 *>(s_share[warp] + 8 * c + quad), l2[c]);
+                                pg_one(pg_fma2(p, vq, one), x0, x1);
                                 d[2 * b] = __float_as_uint(x0); d[2 * b + 1] = __float_as_uint(x1);
                             }
                             const uint32_t lo = __byte_perm(d[0], d[1], 0x5140), hi = __byte_perm(d[2], d[3], 0x5140);
@@ -710,7 +721,7 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG, OG>::THREADS, PgCfg<RT, MT, 
 #pragma unroll
                     for (int r = 0; r < RT; r++) {
                         const float p = pg_ex2(fmaf(y[r], f[r], zs[r]));
-                        l[r] += p;
+                        l[r] = fmaf(p, __shfl_sync(0xffffffffu, share, r), l[r]);
                         const uint32_t d = __float_as_uint(fmaf(p, vq0, 8388608.f));
 #pragma unroll
                         for (int k = 0; k < 3; k++) {
@@ -726,7 +737,10 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG, OG>::THREADS, PgCfg<RT, MT, 
             // the run's sums
             if (!ok || (n >= 2 && !wait(&fin_free[n & 1], ((n >> 1) - 1) & 1, 24))) continue;
             if constexpr (FRAG) {
-                const float x = pg_across<NR>(l, [](float x0, float x1) { return x0 + x1; });
+                float sums[NR];
+#pragma unroll
+                for (int c = 0; c < CG; c++) pg_one(l2[c], sums[2 * c], sums[2 * c + 1]);
+                const float x = pg_across<NR>(sums, [](float x0, float x1) { return x0 + x1; });
                 if (owner) s_l[n & 1][warp][own] = x;
             } else {
 #pragma unroll
@@ -737,7 +751,7 @@ __global__ void __launch_bounds__(PgCfg<RT, MT, SG, OG>::THREADS, PgCfg<RT, MT, 
                     if (lane == r) s_l[n & 1][warp][r] = x;
                 }
             }
-            if (w == 0 && owner) s_mend[n & 1][group][own] = run == PG_LOW ? PG_LOW : __fmul_ru(run, fmaxf(qs, 0x1p-126f));
+            if (w == 0 && owner) s_mend[n & 1][group][own] = M;
             __syncwarp();
             if (lane == 0) ps_mbar_arrive(&fin[n & 1]);
         }

@@ -212,3 +212,58 @@ def test_the_same_bits_every_time(be):  # noqa: F811
             _, b = run(be, c, toks, 16)
             assert np.array_equal(a.view(np.uint32), b.view(np.uint32))
     c.free()
+
+
+@pytest.mark.parametrize("tok,R,many", [(1, 4, 50), (1, 8, 50), (2, 8, 30), (8, 4, 18)])
+@pytest.mark.parametrize("D", [64, 160])
+@pytest.mark.parametrize("at,spread", [(0, 0.0), (0, 1.0), (100, 0.0), (5000, 0.3), (11990, 0.0)])
+def test_one_heavy_slot_and_a_long_tail(be, tok, R, many, D, at, spread):  # noqa: F811
+    """A slot that has nearly all of the mass, and twelve thousand whose weights are 2^-24 of it or less and together up to a thousandth; the heavy one's V is zero, so that the output is theirs.  Sequences share the pages,
+    so many that a CTA takes all tiles of one.
+
+    The bound, with e = 2^-24: a score is off by e (2 D M + 6 Z) as elsewhere, and by 6 Z e more for the difference of its tile's reference and the row's (all in units of e^x: numerator and denominator);
+    exponentials, factors and the digits' sums by 40 e twice.  A weight is rounded by e of its tile's largest, so a tile's 128 slots by 128 e of that one, and the tiles' largest are at most the whole mass: 130 e max|v|.
+    The numerator is one addition a tile, n / 128; the denominator in a lane four a tile at most, n / 32, and a factor a tile: n / 8 e for both."""
+    n, G = 12000, 8
+    c = P.Cache(be, [n], G, D, P=64, layers=1, seed=51, junk=False)
+    r = np.random.default_rng([52, D, at])
+    j = np.arange(n)
+    page, slot = c.tables[0][j // 64], j % 64
+    k, v = r.integers(-100, 101, (n, G, D)), r.integers(100, 128, (n, G, D))
+    k[at], v[at] = 127, 0
+    for kv, x in enumerate((k, v)):
+        c.codes[0, page[:, None, None], np.arange(G)[None, :, None], kv, c.index[kv][slot][:, None, :]] = x
+    sk, sv = np.full((n // 16, G), 0.01 * spread / np.sqrt(D)), 0.01 * (1 + r.random((n // 16, G)))
+    sk[at // 16], k16 = 0.01, at // 16 * 16
+    k[k16:k16 + 16][np.arange(k16, k16 + 16) != at] = 0
+    c.codes[0, page[k16:k16 + 16, None, None], np.arange(G)[None, :, None], 0, c.index[0][slot[k16:k16 + 16]][:, None, :]] = k[k16:k16 + 16]
+    b = np.arange(n // 16) * 16
+    for kv, s in enumerate((sk, sv)):
+        c.scales[0, c.tables[0][b // 64], :, kv, b % 64 // 16] = s
+    c.cache.codes.free(), c.cache.scales.free()
+    cache = capi.PagedCache(be, 1, c.n_pages, 64, G, D, codes=be.upload(c.codes), scales=be.upload(c.scales), refs=c.cache.refs)
+    seqs = np.zeros(many, capi.PAGED_SEQ)
+    seqs["table"], seqs["n_kv"], seqs["n_tok"], seqs["n_table"] = c.dev[0].ptr, n, tok, len(c.tables[0])
+    H, rows = G * R, many * tok
+    top = np.log(2.0) * r.choice([24.02, 24.05, 24.4, 25.0, 22.0], (rows, H))
+    q = np.repeat((top / (127 * 0.01 * D))[..., None], D, 2)
+    q = q.astype(np.float32).reshape(rows, H * D)
+    out = be.upload(np.full((rows, H * D), 7, np.float32))
+    up = be.upload(q)
+    mask = be.upload(np.ones((many, tok, tok), np.uint8))
+    be.paged_attn(cache, 0, out, up, seqs, H, 1.0, tree_mask=mask)
+    got = out.numpy(np.float32, (rows, H, D)).astype(np.float64)
+    kk, vv = c.values(0, 0), c.values(0, 1)
+    for h in range(H):
+        z = q[:, h * D:(h + 1) * D].astype(np.float64) @ kk[:, h // R].T
+        p = np.exp(z - z.max(-1, keepdims=True))
+        want = p @ vv[:, h // R] / p.sum(-1, keepdims=True)
+        M = np.abs(q[:, h * D:(h + 1) * D]).max(-1) * np.abs(kk[:, h // R]).max()
+        bound = S.EPS * (2 * (2 * D * M + 12 * np.abs(z).max(-1)) + 80 + 130 + n / 8) * np.abs(vv[:, h // R]).max()
+        off = np.abs(got[:, h] - want).max(-1)
+        assert (off <= bound).all(), (h, (off / bound).max(), off.max() / np.abs(want).max())
+    for x in (out, up, mask, cache.codes, cache.scales):
+        x.free()
+    c.cache.refs.free()
+    for d in c.dev:
+        d.free()
