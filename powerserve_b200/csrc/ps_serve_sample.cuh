@@ -153,24 +153,9 @@ template <bool LIST, typename F> PS_D void sv_each(const SvSmpRow &r, const SvSm
         if (LIST || v > -INFINITY) f(v, sv_key(v, r.i0 + at));
     }
 }
-// A weight by a float32 exponential, as a whole number: so that sums of them do not depend on who adds them up.  rs: log2 e / temperature (beside an infinite logit, where all others weigh nothing, 1)
-PS_D unsigned long long sv_rough(float v, float top, float rs) {
-    float w;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(v == top ? 0.f : (v - top) * rs));
-    return v > -INFINITY ? (unsigned long long)(w * (float)SV_ONE) : 0;
-}
-// The mass of all tokens of the warp.  ROUGH: by float32 exponentials, off by less than 2^-21 of itself, for those that compare it with a test's random number: a bit of 2^-44 decides a draw among 100 000 tokens, but
-// not whether p(c) / q(c) is above u.  (Sums of the floats took as long, but differed by who added them up, and with them the border of a top-p among thousands of tokens.)
-template <bool ROUGH> PS_D unsigned long long sv_all(const SvSmpRow &r, const SvSmpShared &sh, const float *x) {
+// the mass of all tokens of the warp
+PS_D unsigned long long sv_all(const SvSmpRow &r, const SvSmpShared &sh, const float *x) {
     unsigned long long sum = 0;
-    if (ROUGH) {
-        const float rs = r.log2w.top == INFINITY ? 1.f : (float)r.log2w.s;
-        for (int i = r.w0 + (threadIdx.x & 31); i < r.w1; i += 128) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) sum += sv_rough(i + 32 * e < r.w1 ? x[i + 32 * e] : -INFINITY, r.log2w.top, rs);
-        }
-        return sum;
-    }
     for (int i = r.w0 + (threadIdx.x & 31); i < r.w1; i += 128) {
         unsigned long long w[4];
 #pragma unroll
@@ -368,7 +353,7 @@ template <bool LIST, bool STATS> PS_D void sv_pick(const SvSample &a, int64_t ro
         return w >= r.min_w ? w : 0;
     };
     unsigned long long mine = 0;
-    if (!LIST && !filters) mine = sv_all<STATS>(r, sh, x);
+    if (!LIST && !filters) mine = sv_all(r, sh, x);
     else sv_each<LIST>(r, sh, x, [&](float v, unsigned long long key) { mine += mass_of(v, key); });
 #pragma unroll
     for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
@@ -629,7 +614,7 @@ template <bool STATS> PS_D void sv_sample(const SvSample &a, int64_t row) {
         const bool exactly = r.use_p && !r.use_k && !least;
         const float rs = (float)r.log2w.s;
         float rough = 0.f, rough_in = 0.f;
-        if (exactly) whole = sv_block<false>(sh, sv_all<STATS>(r, sh, x));
+        if (exactly) whole = sv_block<false>(sh, sv_all(r, sh, x));
         for (int i = r.w0; i < r.w1; i += 128) {
             float v[4];
 #pragma unroll
@@ -684,7 +669,7 @@ template <bool STATS> PS_D void sv_sample(const SvSample &a, int64_t row) {
             if (roughly) {
                 if (1.002 * (double)all_in < (double)fmaxf(r.p.top_p, 0.f) * (double)whole) r.use_p = false;
                 else {
-                    const unsigned long long mine = sv_block<false>(sh, sv_all<STATS>(r, sh, x));
+                    const unsigned long long mine = sv_block<false>(sh, sv_all(r, sh, x));
                     const unsigned long long(*n)[16] = mail.post(mine);
                     whole = 0;
                     for (int o = 0; o < C; o++) whole += n[0][o];

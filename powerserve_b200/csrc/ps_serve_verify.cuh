@@ -7,7 +7,8 @@
 // sv_k_stats finds for every row what its settings leave of it (ps_serve_sample.cuh): a border and a mass.  (Rows that were looked at only when the walk came to them, by the cluster of the walk: 780 us for 64 sequences of
 // five nodes, of whose rows two thirds are looked at, where 580 took all of them at once.)  Then sv_k_verify: a cluster a sequence walks its tree - every CTA the same walk, whose tests ask for a few weights - and meets
 // for the passes: a sum for each rejection that a sibling or the draw asks about, and the draw.  Weights and sums are whole numbers, as there, so what is accepted does not depend on the launch.
-// 64 sequences of five nodes, rows and drafts' rows of 128 256 with mixed settings: 86 us for rows by a CTA each, 272 for those left to clusters (a row a microsecond, bound by the cluster's exchanges), 81 for the walks.
+// 64 sequences of five nodes, rows and drafts' rows of 128 256 with mixed settings: 95 us for rows by a CTA each, 283 for those left to clusters (a row a microsecond, bound by the cluster's exchanges), 81 for the walks.
+// Masses of whole rows are sums of the weights that a draw sees, of 2^-44: p sums to one, and a top-p has the border that ps_cuda_sample finds.  (By float32 exponentials, off by 2^-20: 86 and 272 us.)
 #pragma once
 #include "ps_serve_sample.cuh"
 
@@ -140,16 +141,22 @@ __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_rows(const __grid_cons
     sv_settings(r, sv_unrank(worst), reach);
     const bool filters = r.use_k || r.use_p || r.min_w, last = r.min_w >= SV_ONE >> (int)SV_SMP_SPAN; // last: min-p takes out all that is not listed
     const bool mass = !filters || (r.use_p && !r.use_k);
-    const float rs = r.log2w.top == INFINITY ? 1.f : (float)r.log2w.s;
     unsigned long long whole = 0;
-    each([&](float v, int i) {
-        if (filters && v >= r.cut && v > -INFINITY) {
+    auto list = [&](float v, int i) {
+        if (v >= r.cut && v > -INFINITY) {
             const uint32_t n = atomicAdd(&sh.n_list, 1u);
             if (n < SV_SMP_BINS) sh.list[n] = sv_key(v, i);
         }
-        if (mass) whole += sv_rough(v, r.log2w.top, rs);
-    });
-    whole = sv_block<false>(sh, mass ? whole : 0);
+    };
+    auto weigh = [&](float v) {
+        const unsigned long long w = sv_weight(sh, r.log2w(v));
+        whole += v > -INFINITY ? w : 0;
+    };
+    // (a loop for each case, so that several weights are under way at once)
+    if (!filters) each([&](float v, int) { weigh(v); });
+    else if (!mass) each(list);
+    else each([&](float v, int i) { list(v, i); weigh(v); });
+    whole = sv_block<false>(sh, whole);
     __syncthreads();
     if (!filters) {
         if (tid == 0) *to = SvRowStats{0, whole, r.log2w.top, 0};

@@ -277,3 +277,50 @@ def test_a_min_p_below_what_is_listed(be, sizes, min_p, draft):  # noqa: F811
         tokens[::4] = r.integers(0, V // 2, len(tokens[::4])) * 2 + 1
     n_path = check(be, V, sizes, parents, tokens, u, logits, sets, guess, sets if draft else None)
     assert draft or sizes[0] == 1 or len(set(n_path.tolist())) > 1     # (the likely token's own share decides)
+
+
+@pytest.mark.parametrize("sizes", [[2] * 15, [2] * 40])
+@pytest.mark.parametrize("draft", [False, True])
+def test_random_numbers_beside_the_border(be, sizes, draft):  # noqa: F811
+    """Rows without filters: one likely token, and a tail of equal ones that together hold from a hundredth to nine tenths; the likely one's test is 2^-22 of p(c) / q(c) above it or below.  (Masses are sums of whole numbers
+    of 2^-44, each off by half a one at most: 128 255 of them by 2^-28 of the mass; a random number of float32 by 2^-24.)"""
+    V, n = 128256, sum(sizes)
+    r = np.random.default_rng([42, n, draft])
+
+    def rows():
+        x = np.repeat(r.uniform(-12.5, -9.5, (n, 1)).astype(np.float32), V, 1)
+        x[:, 1001] = 0.0
+        return x + r.uniform(-2, 2, (n, 1)).astype(np.float32)
+    logits, guess = rows(), rows() if draft else None
+    sets = S.settings([(float(np.float32(t)), 0, 1.0, 0.0) for t in r.uniform(0.95, 1.1, n)])
+    parents, tokens, u = np.tile(np.array([-1, 0], np.int32), len(sizes)), np.full(n, 1001, np.int32), r.random(n).astype(np.float32)
+    side = np.where(np.arange(len(sizes)) % 2, 1, -1)
+    for s in range(len(sizes)):
+        p = P.distribution(logits[2 * s], *sets[2 * s].tolist())[1001]
+        q = P.distribution(guess[2 * s], *sets[2 * s].tolist())[1001] if draft else 1.0
+        u[2 * s + 1] = p / q * (1 + side[s] * 2.0 ** -22)
+    n_path = check(be, V, sizes, parents, tokens, u, logits, sets, guess, sets if draft else None)
+    assert (n_path[side < 0] == 2).all() and ((n_path[side > 0] == 1) | (u[1::2][side > 0] > 1)).all()
+
+
+def test_the_same_border_as_samplings(be):  # noqa: F811
+    """top-p over one likely token and a tail of equal ones: the last token that is left is the one that ps_cuda_sample draws, in few rows and in many"""
+    V, n = 128256, 240
+    r = np.random.default_rng(43)
+    logits = np.repeat(r.uniform(-11.5, -9.0, (n, 1)).astype(np.float32), V, 1)
+    logits[:, 7] = 0.0
+    sets = S.settings([(1.0, 0, float(p), 0.0) for p in r.uniform(0.6, 0.99, n)])
+    sets["min_p"][::3] = 2.0 ** -18
+    sets["min_p"][1::9] = 2.0 ** -17
+    u, minus, zero = np.full(n, 1.0 - 2.0 ** -24, np.float32), np.full(n, -1, np.int32), np.zeros(n, np.int32)
+    up = [be.upload(a) for a in (logits, sets, u)]
+    want = be.upload(np.zeros(n, np.int32))
+    be.sample(want, None, up[0], V, n, up[1], up[2])
+    ids = want.numpy(np.int32)
+    assert len(set(ids.tolist())) > n // 2
+    assert np.array_equal(run(be, V, [1] * n, minus, zero, u, logits, sets)[0], ids)
+    for i in range(0, n, 20):
+        e = slice(i, i + 20)
+        assert np.array_equal(run(be, V, [1] * 20, minus[e], zero[e], u[e], logits[e], sets[e])[0], ids[e]), i
+    for b in up + [want]:
+        b.free()
