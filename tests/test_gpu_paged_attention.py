@@ -267,3 +267,39 @@ def test_one_heavy_slot_and_a_long_tail(be, tok, R, many, D, at, spread):  # noq
     c.cache.refs.free()
     for d in c.dev:
         d.free()
+
+
+@pytest.mark.parametrize("tok,R", [(1, 4), (1, 8), (4, 4), (8, 4), (20, 4)])
+@pytest.mark.parametrize("D", [64, 160])
+@pytest.mark.parametrize("block,q_scale,k_scale,rest", [(3, 1.0, 1e37, 1e-3), (20, 1e30, 1e8, 1e-33), (39, 1e30, 1e8, 1e-33)])
+def test_scores_outside_float32_in_one_tile(be, tok, R, D, block, q_scale, k_scale, rest):  # noqa: F811
+    """sixteen of 640 slots with scores above float32's range: no number; below it: the others are what there is.  In the first tile, inside, in the last one"""
+    n, G = 640, 2
+    for above in (True, False):
+        c = P.Cache(be, [n, n], G, D, P=32, layers=1, seed=61, junk=False)
+        for i in range(2):
+            page, o = c.tables[i][block * 16 // 32], block * 16 % 32
+            c.scales[0, c.tables[i][:n // 32], :, 0] = rest
+            c.scales[0, page, :, 0, o // 16] = k_scale
+            for s in range(16):
+                c.codes[0, page[None], np.arange(G)[:, None], 0, c.index[0][o + s]] = 100 if above else -100
+        q = np.abs(np.random.default_rng(62).standard_normal((2 * tok, G * R * D)) + 2.0).astype(np.float32) * np.float32(q_scale)
+        hidden = np.zeros(n, np.uint8)
+        if not above:
+            hidden[block * 16:block * 16 + 16] = 1
+        masks = [np.ones((tok, tok), np.uint8)] * 2
+        if not above:
+            c2 = P.Cache(be, [n, n], G, D, P=32, layers=1, seed=61, junk=False)
+            c2.codes, c2.scales = c.codes.copy(), c.scales.copy()
+            for i in range(2):
+                c2.scales[0, c2.tables[i][block * 16 // 32], :, 0, block * 16 % 32 // 16] = rest
+            want, bound = P.attention(q, c2, [tok, tok], G * R, 1.0, masks, [hidden, hidden])
+            c2.free()
+        c.cache.free()
+        c.cache = capi.PagedCache(be, 1, c.n_pages, 32, G, D, codes=be.upload(c.codes), scales=be.upload(c.scales), refs=be.upload(c.refs))
+        _, out = run(be, c, [tok, tok], G * R, masks, scale=1.0, q=q)
+        if above:
+            assert np.isnan(out).all()
+        else:
+            assert (np.abs(out - want) <= bound[:, None]).all(), (np.abs(out - want).max(), bound.max())
+        c.free()
