@@ -244,7 +244,8 @@ int ps_cuda_paged_compact(ps_cuda_ctx *ctx, const ps_cuda_pages *pages, const ps
 /* Drafted tokens against the target's distribution p and the draft's q (each what its row of logits leaves by its ps_cuda_sampler, as ps_cuda_sample draws from it;
  * no result depends on what else is in the call).  A sequence has n_nodes[s] nodes (HOST array; 1 .. 256):
  * node 0 is its last token, node i > 0 the drafted token tokens[i], a child of parents[i] < i (numbers within the sequence); row i of the logits is the target's after node i, row i of draft_logits the
- * draft's that the children of node i were drawn from (rows of childless nodes are not read).  Beginning at node 0, the children of the last accepted node are asked in order: child i with token c is accepted where u[i] < p(c) / q(c);
+ * draft's that the children of node i were drawn from, each of them on its own (siblings drawn without replacement have another distribution: they are verified with draft_logits NULL, which asks nothing of where
+ * tokens come from; rows of childless nodes are not read).  Beginning at node 0, the children of the last accepted node are asked in order: child i with token c is accepted where u[i] < p(c) / q(c);
  * where it is not, p becomes max(p - q, 0), normalised (p stays where nothing is left), for its siblings and the last draw.  draft_logits NULL: the drafted tokens are nobody's draws, q is 1 at c: p loses c.  What is drawn then
  * is distributed as if the target had drawn every token.  ids[s]: the next token, drawn with u[0] from what p has become at the last accepted node (-1: its row has no number above -inf);
  * path: the accepted nodes of each sequence, node 0 first, -1 behind them; n_path[s] their number.  A token outside the vocabulary is never accepted and changes nothing.

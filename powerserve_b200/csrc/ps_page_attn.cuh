@@ -14,7 +14,9 @@
 // not have all tiles of its rows leaves the sums in the workspace, and pg_k_join joins them.  Rows above RT are other CTAs', which take the same tiles at the same time (L2).
 // Roles: soft-max (SG groups of four warps, tiles in turn), output (OG groups of four, likewise), and a warp each for copies (a page's K or V of a head is one run of bytes), the MMAs of either product, scales and live
 // slots, and queries.  One row a head: 64 sequences of up to 2 040 slots, 8 heads of 128, 33 us + 6 of pg_k_join: 5.5 TB/s while tiles stream, the rest is the CTAs' start and end.  32 rows: 2 x 32 tokens over 32 700 slots
-// 108 + 6: bound by the soft-max's instructions and waits (1 600 cycles for 128 slots x 32 rows), matrix pipe 23 %; three soft-max and two output groups 114, two and one 125, either one alone no better.
+// 112 + 6: bound by the soft-max's instructions and waits (1 650 cycles for 128 slots x 32 rows), matrix pipe 22 %; three soft-max and two output groups, two and one take a tenth more, either one alone no better.  (At the
+// 72 registers of 32 rows, 24 bytes a thread lie in local memory.)
+// Weights under a tile's own reference cost 4 us of the 112, against those under the row's largest score so far, which lose bits behind a heavy slot.
 #pragma once
 #include "ps_page.cuh"
 

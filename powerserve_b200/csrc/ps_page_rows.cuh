@@ -3,7 +3,9 @@
 //   scale' = max(scale, where earlier slots lie in the block; max |x| / 127),   code = rint(x / scale'),   earlier codes rint(code * (scale / scale'))
 //
 // store: a CTA takes a block of sixteen slots of one head's K or V, a thread sixteen of its numbers, which are read once: a slot's sixteen channels (K), a channel's sixteen slots (V), so that sixteen bytes a lane go to
-// memory lane after lane.  Bound by memory for prompts, by latency (a chain of table, numbers, the CTA's largest) for single tokens.  (A warp a block, 64 numbers a lane: 4 600 tokens 55 us, for few warps an SM; 33 now.)
+// memory lane after lane.  Bound by instructions (the SMs issue 47 % of the time) and latency for prompts: 6 385 tokens of 8 heads of 128 in bfloat16 33 us, 1.2 TB/s;
+// by latency (a chain of table, numbers, the CTA's largest) for single tokens.  (A warp a block, 64 numbers a lane: 55 us, for few warps an SM.  At 64 registers, which heads of 256 need for four CTAs an SM, 72 bytes a thread
+// of numbers whose codes are asked again lie in local memory.)
 // load: a warp a block.
 #pragma once
 #include "ps_page.cuh"
