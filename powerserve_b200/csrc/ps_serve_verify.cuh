@@ -207,6 +207,17 @@ struct SvDist {
     }
 };
 
+// how many of the warp's tokens come before token c.  (Hardly ever asked for: no registers of the walk's are kept for it)
+__device__ __noinline__ unsigned sv_above(const float *row, int c, int w0, int w1) {
+    const unsigned long long key = sv_key(row[c], c);
+    unsigned above = 0;
+    for (int i = w0 + (threadIdx.x & 31); i < w1; i += 32) {
+        const float v = row[i];
+        above += v > -INFINITY && sv_key(v, i) > key;
+    }
+    return __reduce_add_sync(0xffffffffu, above);
+}
+
 __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_verify(const __grid_constant__ SvVerify a) {
     namespace cg = cooperative_groups;
     constexpr int WARPS = SV_SMP_THREADS / 32;
@@ -334,6 +345,15 @@ __global__ void __launch_bounds__(SV_SMP_THREADS, 2) sv_k_verify(const __grid_co
                 n_gone++;
                 left -= w;
                 __syncthreads();
+            }
+        }
+        if (yes && s_w[i] == 0) { // a token below 2^-46 of the likeliest, by u = 0 or a q as small: where the border of a top-k lies down there, the row's record leaves all of them in (no draw asks)
+            const ps_cuda_sampler &set = a.samplers[base + cur];
+            if (set.top_k > 0 && set.top_k < a.vocab) {
+                const unsigned long long *m = meet(sv_above(a.logits + (int64_t)(base + cur) * a.row_stride, c, w0, w1));
+                unsigned long long rank_c = 0;
+                for (int o = 0; o < C; o++) rank_c += m[o];
+                yes = rank_c < (unsigned long long)set.top_k;
             }
         }
         if (yes) {

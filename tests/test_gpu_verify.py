@@ -324,3 +324,26 @@ def test_the_same_border_as_samplings(be):  # noqa: F811
         assert np.array_equal(run(be, V, [1] * 20, minus[e], zero[e], u[e], logits[e], sets[e])[0], ids[e]), i
     for b in up + [want]:
         b.free()
+
+
+@pytest.mark.parametrize("V,k", [(60, 3), (60, 50), (5000, 40), (5000, 600), (30000, 3000)])
+@pytest.mark.parametrize("sizes", [[2] * 6, [2] * 50])
+@pytest.mark.parametrize("draft", [False, True])
+def test_a_top_k_whose_border_weighs_nothing(be, V, k, sizes, draft):  # noqa: F811
+    """Peaked rows, in which all tokens but one lie below 2^-46 of it, those around the border of top-k too: at u = 0, or where the draft holds them for less likely still, the ones inside are accepted and no other one"""
+    n, r = sum(sizes), np.random.default_rng([44, V, k])
+    logits = (np.stack([r.permutation(V) for _ in range(n)]) * (-10.0 / V) - 40).astype(np.float32)
+    best = r.integers(0, V, n)
+    logits[np.arange(n), best] = 0.0
+    order = np.argsort(-logits, 1, kind="stable")
+    guess = None
+    if draft:
+        guess = np.full((n, V), -60, np.float32)
+        guess[np.arange(n), (best + 1) % V] = 0.0
+    sets = S.settings([(1.0, k, 1.0, 0.0)] * n)
+    parents, tokens, u = np.tile(np.array([-1, 0], np.int32), len(sizes)), np.zeros(n, np.int32), r.random(n).astype(np.float32)
+    rank = np.resize([1, k - 1, k, k + 1, V - 1], n // 2)
+    tokens[1::2] = order[::2][np.arange(n // 2), rank]
+    u[1::2][::2] = 0
+    n_path = check(be, V, sizes, parents, tokens, u, logits, sets, guess, S.settings([(1.0, 0, 1.0, 0.0)] * n) if draft else None)
+    assert (n_path[rank >= k] == 1).all() and (n_path == 2).any()
